@@ -323,6 +323,58 @@ int l8_rmsnorm_bwd_as(const void *gy, const void *x, const void *w, int w_is_f32
                       int64_t R, int64_t C, int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_is_f32,
                       void *workspace, int64_t workspace_bytes, void *stream);
 
+/* The norm of a residual sum (lingua/transformer.py:497-543: h = x + attention(...), ffn_norm(h)) with the sum:
+ *   h = bf16(f32(x) + f32(residual))   [R,C] (ldh), always written
+ *   y, q, scale, rstd, col_amax: as l8_rmsnorm_cast_rowwise leaves them for h
+ * x, residual, h and y must not overlap, but x and residual may be one tensor.  Requirements and workspace as there. */
+int l8_add_rmsnorm_cast_rowwise(const void *x, const void *residual, const void *w, int w_is_f32, int64_t R, int64_t C,
+                                int64_t ldx, int64_t ldr, float eps, void *h, int64_t ldh, void *y, int64_t ldy, void *q,
+                                int64_t ldq, float *scale, float *rstd, float *col_amax, void *workspace,
+                                int64_t workspace_bytes, void *stream);
+/* Its backward: with gy the gradient of y and gh that of h, gx = bf16(f32(gh) + what l8_rmsnorm_bwd finds before its rounding), the
+ * gradient of x and of residual alike; gw as l8_rmsnorm_bwd_as.  Requirements and workspace as there. */
+int l8_add_rmsnorm_bwd(const void *gy, const void *gh, const void *h, const void *w, int w_is_f32, const float *rstd, int64_t R,
+                       int64_t C, int64_t ldgy, int64_t ldgh, int64_t ldh, void *gx, int64_t ldgx, void *gw, int gw_is_f32,
+                       void *workspace, int64_t workspace_bytes, void *stream);
+
+/* Rotary positions of queries and keys (apply_rotary_emb of lingua/transformer.py), both in one launch:
+ *   y[b,s,h,:] = x[b,s,h,:] with its first `rot` columns turned: pair i = columns (2 i, 2 i + 1), or with in_halves
+ *   (i, i + rot / 2), (a, c) -> (a cos - c sin, a sin + c cos) in fp32, rounded once; the other columns are copied.
+ *   x bf16 [B,S,heads,D], strides of the first three dimensions in elements; y bf16, dense.  heads may be 0.
+ *   cos, sin fp32 [length, rot / 2], strides table_row and table_col
+ *   positions int64 or (positions_i32) int32, element (b,s) at b * pos_b + s * pos_s; NULL: s.  A token at a position outside
+ *   [0, length) becomes NaN.
+ *   inverse: the transposed rotation, which is the backward pass.
+ * Requires D even, at most 512, rot even and at least 2, fewer than 2^24 tokens.  x and y may not overlap. */
+typedef struct {
+  const void *x;
+  void *y;
+  int64_t heads, ldb, lds, ldh;
+} l8_rotary_operand;
+int l8_rotary(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, int64_t rot, int in_halves, int inverse,
+              const float *cos, const float *sin, int64_t table_row, int64_t table_col, int64_t length,
+              const void *positions, int positions_i32, int64_t pos_b, int64_t pos_s, void *stream);
+
+/* MXFP4 (OCP Microscaling formats 1.0): e2m1 codes in blocks of 32, the last block of a row possibly shorter, with an e8m0 scale each.
+ *   byte = max(E - 2, 0), E the biased exponent of the block's amax; 255 (NaN), with codes 0, for a block with an inf or NaN
+ *   code = e2m1(x * 2^(127 - byte)), nearest even, saturating at 6
+ * A row of C elements is ceil(C / 32) * 16 bytes of codes (the first of two in the low half; zeros behind column C) and
+ * ceil(C / 32) scales.
+ *   x       bf16 [R,C] (ldx, elements)
+ *   q, s    codes and scales of the rows; qt, st of the columns (that is, of x transposed: [C,R]); either pair may be NULL
+ *   ldq, lds, ldqt, ldst   bytes from row to row: multiples of 16 for codes and of 4 for scales, pointers aligned alike
+ * Requires C % 8 == 0, ldx % 8 == 0, 16-byte aligned x, R <= 1048560. */
+int l8_cast_mxfp4(const void *x, int64_t R, int64_t C, int64_t ldx, void *q, int64_t ldq, void *s, int64_t lds,
+                  void *qt, int64_t ldqt, void *st, int64_t ldst, void *stream);
+/* Back to bf16 [R,C] (ldy, elements): exact, but infinite from 6 * 2^126 on; a block of scale 255 is NaN. */
+int l8_mxfp4_to_bf16(const void *q, int64_t ldq, const void *s, int64_t lds, int64_t R, int64_t C, void *y, int64_t ldy, void *stream);
+
+/* C [M,N] bf16 (ldc) = A [M,K] . B [N,K]^T + bias, both operands MXFP4 as above, summed in fp32 and rounded once; bias bf16 [N] or NULL.
+ * Leading dimensions of codes and scales in bytes, multiples of 16 below 2^23, pointers 16-byte aligned.  K < 2^24; what lies
+ * behind the last block of a row is not used. */
+int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, const void *sb, int64_t M, int64_t N, int64_t K, int64_t lda,
+                     int64_t ldsa, int64_t ldb, int64_t ldsb, const void *bias, void *C, int64_t ldc, void *stream);
+
 int l8_gemm_algo_count(void);
 /* human-readable description of tile configuration `algo` (1-based), or NULL */
 const char *l8_gemm_algo_name(int algo);

@@ -61,6 +61,12 @@ SIGNATURES = {
     "l8_rmsnorm_bwd": [_p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _i64, _p],
     "l8_rmsnorm_bwd_workspace": [_i64, _i64],
     "l8_rmsnorm_bwd_as": [_p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _i64, _p],
+    "l8_add_rmsnorm_cast_rowwise": [_p, _p, _p, _int, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p],
+    "l8_add_rmsnorm_bwd": [_p, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _i64, _p],
+    "l8_rotary": [_p, _i64, _i64, _i64, _i64, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _p],
+    "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+    "l8_mxfp4_to_bf16": [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
+    "l8_gemm_mxfp4_nt": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p],
     "l8_linear_fwd": [ctypes.c_char_p],
     "l8_linear_fwd_workspace": [ctypes.c_char_p],
     "l8_linear_fwd_rows": [ctypes.c_char_p, _i64, _i64],

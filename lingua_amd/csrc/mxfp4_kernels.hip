@@ -1,0 +1,243 @@
+// MXFP4 casts: bf16 to e2m1 codes in blocks of 32 with one power-of-two scale (e8m0) each, along the rows of a matrix, along its
+// columns (written transposed), or both from one read; and back to bf16.  The format is the OCP Microscaling one (version 1.0):
+//
+//   byte = max(E - 2, 0)   E the biased exponent of the block's amax: 2^(byte - 127) = 2^(floor(log2 amax) - 2)
+//   code = e2m1(x * 2^(127 - byte))   nearest even, saturating at 6, sign kept
+//   a block that holds an infinity or a NaN: byte 255 (NaN), codes 0
+//
+// All of it is integer work on the exponent and one conversion instruction (v_cvt_scalef32_pk_fp4_bf16), exact by definition: no
+// rounding but the format's own.
+//
+// Bound by memory: 2 bytes read and 17/32 written per element and direction.
+//   * rows: a lane takes 8 columns (16 bytes), four neighbours share a block: its amax takes two DPP steps, the four lanes' codes
+//     leave as 16 bytes side by side;
+//   * columns: a workgroup passes a tile of 256 rows x 128 columns through LDS, so that rows are read in 256-byte pieces and the
+//     transposed copy is written in whole 128-byte lines: 8 lanes side by side take the 8 blocks of one pair of columns.  The
+//     block index shifts a lane's LDS address by 8 banks, so the 64 lanes of a read touch every bank once.
+#include "l8_common.h"
+
+namespace l8 {
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kMxBlock = 32;                 // elements per scale
+constexpr int kMxTileR = 256, kMxTileC = 128;
+constexpr int kMxThreads = 512;
+// LDS image of a tile: 32-row blocks of rows of 64 dwords, a block padded by 8 dwords
+constexpr int kMxBandDwords = kMxBlock * (kMxTileC / 2) + 8;
+constexpr int kMxLds = (kMxTileR / kMxBlock) * kMxBandDwords * 4;
+
+struct MxCastArgs {
+  const uint16_t *x;
+  int64_t R, C, ldx;
+  uint8_t *q, *s, *qt, *st;                  // row-wise copy and its scales, transposed copy and its scales (NULL: not wanted)
+  int64_t ldq, lds, ldqt, ldst;              // bytes
+};
+
+#if defined(__HIP_DEVICE_COMPILE__)
+// byte of a block whose largest magnitude has the bf16 bits `amax`
+L8_DEV uint32_t mx_byte(uint32_t amax) {
+  const uint32_t e = amax >> 7;
+  return e == 255u ? 255u : (e < 2u ? 0u : e - 2u);
+}
+// 2^(byte - 127) as fp32: what the conversion divides by (byte 0 is the subnormal 2^-127)
+L8_DEV float mx_scale(uint32_t byte) { return __uint_as_float(byte == 0u ? 0x00400000u : byte << 23); }
+
+// eight bf16 (four packed pairs) -> eight codes, the first in the low nibble
+L8_DEV uint32_t mx_codes8(uint32_t p0, uint32_t p1, uint32_t p2, uint32_t p3, float scale) {
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, p0), scale, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, p1), scale, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, p2), scale, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2, p3), scale, 3);
+  return r;
+}
+L8_DEV uint32_t amax8(v4i v) {
+  uint32_t m = pk_absmax_u16(0, (uint32_t)v[0]);
+#pragma unroll
+  for (int k = 1; k < 4; ++k) m = pk_absmax_u16(m, (uint32_t)v[k]);
+  return max(m & 0xffffu, m >> 16);
+}
+template <int CTRL>
+L8_DEV uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true); }
+// maximum over the four lanes of a quad
+L8_DEV uint32_t quad_max(uint32_t v) {
+  v = max(v, dpp<0xB1>(v));    // quad_perm [1,0,3,2]
+  return max(v, dpp<0x4E>(v)); // quad_perm [2,3,0,1]
+}
+
+// Eight columns of a row from c on (a lane; zeros beyond C): the block's codes and scale.  `whole`: the row's four scale
+// bytes of 16 lanes leave as one dword.
+L8_DEV void cast_row_piece(const MxCastArgs &p, v4i v, int64_t r, int64_t c) {
+  const uint32_t byte = mx_byte(quad_max(amax8(v)));
+  const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], mx_scale(byte));
+  const int64_t padded = (p.C + kMxBlock - 1) / kMxBlock * kMxBlock;
+  // lanes 0, 4, 8, 12 of a row of 16 hold the four bytes of 128 columns
+  const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
+  if (r >= p.R || c >= padded) return;
+  *(uint32_t *)(p.q + r * p.ldq + c / 2) = codes;
+  const int lane16 = threadIdx.x & 15;
+  if (c - lane16 * 8 + 128 <= padded) {
+    if (lane16 == 0) *(uint32_t *)(p.s + r * p.lds + c / kMxBlock) = four;
+  } else if ((lane16 & 3) == 0) {
+    p.s[r * p.lds + c / kMxBlock] = (uint8_t)byte;
+  }
+}
+#endif
+
+// Rows alone: a wave takes 512 columns of a row at a time, UNROLL rows requested together.
+template <int UNROLL>
+__global__ __launch_bounds__(256) void mxfp4_rows_kernel(const MxCastArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t c = (int64_t)blockIdx.x * 512 + lane * 8;
+  const int64_t r0 = ((int64_t)blockIdx.y * 4 + wave) * UNROLL;
+  v4i v[UNROLL];
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) {
+    v[i] = v4i{0, 0, 0, 0};
+    if (r0 + i < p.R && c < p.C) v[i] = *(const v4i *)(p.x + (r0 + i) * p.ldx + c);
+  }
+#pragma unroll
+  for (int i = 0; i < UNROLL; ++i) cast_row_piece(p, v[i], r0 + i, c);
+#endif
+}
+
+// Columns, and rows from the same read where ROWS.
+template <bool ROWS>
+__global__ __launch_bounds__(kMxThreads) void mxfp4_tile_kernel(const MxCastArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __shared__ __attribute__((aligned(16))) uint32_t tile[kMxLds / 4];
+  const int64_t r0 = (int64_t)blockIdx.y * kMxTileR, c0 = (int64_t)blockIdx.x * kMxTileC;
+  constexpr int kLanes = kMxTileC / 8, kStep = kMxThreads / kLanes, kLoads = kMxTileR / kStep;   // 16 lanes a row, 32 rows a load
+  static_assert(kStep == kMxBlock, "a load fills one band of the tile");
+  const int lr = threadIdx.x / kLanes, lc = (threadIdx.x % kLanes) * 8;
+  v4i v[kLoads];
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) {
+    const int64_t r = r0 + i * kStep + lr;
+    v[i] = v4i{0, 0, 0, 0};
+    if (r < p.R && c0 + lc < p.C) v[i] = *(const v4i *)(p.x + r * p.ldx + c0 + lc);
+  }
+#pragma unroll
+  for (int i = 0; i < kLoads; ++i) *(v4i *)(tile + i * kMxBandDwords + lr * (kMxTileC / 2) + lc / 2) = v[i];
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) cast_row_piece(p, v[i], r0 + i * kStep + lr, c0 + lc);
+  }
+  __syncthreads();
+  const int64_t bands = (p.R + kMxBlock - 1) / kMxBlock;
+  const int band = threadIdx.x & 7, pair = threadIdx.x >> 3;   // this thread's block of 32 rows, its two columns
+  const int64_t gb = r0 / kMxBlock + band, col = c0 + pair * 2;
+  uint32_t w[kMxBlock], m = 0;
+#pragma unroll
+  for (int i = 0; i < kMxBlock; ++i) {
+    w[i] = tile[band * kMxBandDwords + i * (kMxTileC / 2) + pair];
+    m = pk_absmax_u16(m, w[i]);
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const uint32_t byte = mx_byte(half ? m >> 16 : m & 0xffffu);
+    const float scale = mx_scale(byte);
+    v4i codes;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t pr[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)   // this column of two neighbouring rows
+        pr[j] = __builtin_amdgcn_perm(w[k * 8 + 2 * j + 1], w[k * 8 + 2 * j], half ? 0x07060302u : 0x05040100u);
+      codes[k] = byte == 255u ? 0 : (int)mx_codes8(pr[0], pr[1], pr[2], pr[3], scale);
+    }
+    const uint32_t four = byte | dpp<0x101>(byte) << 8 | dpp<0x102>(byte) << 16 | dpp<0x103>(byte) << 24;   // of four bands side by side
+    if (col + half < p.C && gb < bands) {
+      *(v4i *)(p.qt + (col + half) * p.ldqt + gb * 16) = codes;
+      if ((gb & ~(int64_t)3) + 4 <= bands) {
+        if ((band & 3) == 0) *(uint32_t *)(p.st + (col + half) * p.ldst + gb) = four;
+      } else {
+        p.st[(col + half) * p.ldst + gb] = (uint8_t)byte;
+      }
+    }
+  }
+#endif
+}
+
+// Back to bf16: the products of codes and scales are exact but for scales beyond 2^125 (6 * 2^126 and more are infinite).
+__global__ __launch_bounds__(256) void mxfp4_to_bf16_kernel(const uint8_t *__restrict__ q, int64_t ldq, const uint8_t *__restrict__ s, int64_t lds,
+                                                            int64_t R, int64_t C, uint16_t *__restrict__ y, int64_t ldy) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  const int64_t r = blockIdx.y;
+  if (c >= C) return;
+  const uint32_t codes = *(const uint32_t *)(q + r * ldq + c / 2);
+  const uint32_t byte = s[r * lds + c / kMxBlock];
+  const float scale = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale(byte);
+  uint32_t out[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint32_t lohi[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t code = codes >> (8 * k + 4 * h) & 15u, mag = code & 7u;
+      // 0, 0.5, 1, 1.5, 2, 3, 4, 6: the values at twice their size fit a byte each
+      const float v = 0.5f * (float)((mag < 4u ? 0x03020100u >> (8u * mag) : 0x0c080604u >> (8u * (mag - 4u))) & 255u);
+      lohi[h] = bf16_rne_bits((code & 8u ? -v : v) * scale);
+    }
+    out[k] = lohi[0] | lohi[1] << 16;
+  }
+  if (c + 8 <= C && ((uintptr_t)(y + r * ldy + c) % 16) == 0) {
+    *(v4i *)(y + r * ldy + c) = v4i{(int)out[0], (int)out[1], (int)out[2], (int)out[3]};
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < C) y[r * ldy + c + k] = (uint16_t)(k & 1 ? out[k / 2] >> 16 : out[k / 2] & 0xffffu);
+  }
+#endif
+}
+
+}  // namespace l8
+
+using namespace l8;
+
+extern "C" int l8_cast_mxfp4(const void *x, int64_t R, int64_t C, int64_t ldx, void *q, int64_t ldq, void *s, int64_t lds, void *qt,
+                             int64_t ldqt, void *st, int64_t ldst, void *stream) {
+  L8_REQUIRE(R >= 0 && C >= 0, "l8_cast_mxfp4: negative shape R=%lld C=%lld", (long long)R, (long long)C);
+  if (R == 0 || C == 0) return L8_OK;
+  L8_REQUIRE((q == nullptr) == (s == nullptr) && (qt == nullptr) == (st == nullptr) && (q || qt), "l8_cast_mxfp4: a copy comes with its scales, and one copy at least");
+  const int64_t blocks = (C + 31) / 32, bands = (R + 31) / 32;
+  L8_REQUIRE(x && C % 8 == 0 && ldx % 8 == 0 && ldx >= C && ((uintptr_t)x % 16) == 0,
+             "l8_cast_mxfp4: C=%lld and ldx must be multiples of 8 with ldx >= C, x 16-byte aligned", (long long)C);
+  L8_REQUIRE(!q || (ldq % 16 == 0 && ldq >= blocks * 16 && ((uintptr_t)q % 16) == 0 && lds % 4 == 0 && lds >= blocks && ((uintptr_t)s % 4) == 0),
+             "l8_cast_mxfp4: rows of 16 bytes per block on 16-byte lines and of a scale per block on 4-byte lines are wanted");
+  L8_REQUIRE(!qt || (ldqt % 16 == 0 && ldqt >= bands * 16 && ((uintptr_t)qt % 16) == 0 && ldst % 4 == 0 && ldst >= bands && ((uintptr_t)st % 4) == 0),
+             "l8_cast_mxfp4: transposed rows of 16 bytes per block on 16-byte lines and of a scale per block on 4-byte lines are wanted");
+  L8_REQUIRE(R <= (int64_t)65535 * 16 && C <= (int64_t)1 << 30, "l8_cast_mxfp4: R=%lld exceeds %d or C=%lld 2^30", (long long)R, 65535 * 16, (long long)C);
+  const MxCastArgs a = {(const uint16_t *)x, R, C, ldx, (uint8_t *)q, (uint8_t *)s, (uint8_t *)qt, (uint8_t *)st, ldq, lds, ldqt, ldst};
+  hipStream_t hs = (hipStream_t)stream;
+  if (!qt) {
+    constexpr int U = 4;
+    hipLaunchKernelGGL((mxfp4_rows_kernel<U>), dim3((unsigned)((C + 511) / 512), (unsigned)((R + 4 * U - 1) / (4 * U))), dim3(256), 0, hs, a);
+  } else {
+    const dim3 grid((unsigned)((C + kMxTileC - 1) / kMxTileC), (unsigned)((R + kMxTileR - 1) / kMxTileR));
+    if (q) hipLaunchKernelGGL((mxfp4_tile_kernel<true>), grid, dim3(kMxThreads), 0, hs, a);
+    else hipLaunchKernelGGL((mxfp4_tile_kernel<false>), grid, dim3(kMxThreads), 0, hs, a);
+  }
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+extern "C" int l8_mxfp4_to_bf16(const void *q, int64_t ldq, const void *s, int64_t lds, int64_t R, int64_t C, void *y, int64_t ldy, void *stream) {
+  L8_REQUIRE(R >= 0 && C >= 0, "l8_mxfp4_to_bf16: negative shape R=%lld C=%lld", (long long)R, (long long)C);
+  if (R == 0 || C == 0) return L8_OK;
+  const int64_t blocks = (C + 31) / 32;
+  L8_REQUIRE(q && s && y, "l8_mxfp4_to_bf16: null pointer");
+  L8_REQUIRE(ldq % 4 == 0 && ldq >= blocks * 16 && ((uintptr_t)q % 4) == 0 && lds >= blocks && ldy >= C,
+             "l8_mxfp4_to_bf16: rows of 16 bytes and a scale per block of 32 columns are wanted, the codes on 4-byte lines");
+  L8_REQUIRE(R <= 65535 * (int64_t)16 && C <= (int64_t)1 << 30, "l8_mxfp4_to_bf16: R=%lld exceeds %d or C=%lld 2^30", (long long)R, 65535 * 16, (long long)C);
+  for (int64_t r = 0; r < R; r += 65535) {   // (rows are the grid's second dimension)
+    const int64_t n = R - r < 65535 ? R - r : 65535;
+    hipLaunchKernelGGL(mxfp4_to_bf16_kernel, dim3((unsigned)((C + 2047) / 2048), (unsigned)n), dim3(256), 0, (hipStream_t)stream,
+                       (const uint8_t *)q + r * ldq, ldq, (const uint8_t *)s + r * lds, lds, n, C, (uint16_t *)y + r * ldy, ldy);
+  }
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}

@@ -83,16 +83,46 @@ L8_DEV void store16_nt(__amdgpu_buffer_rsrc_t rs, uint32_t voff, v4i data) {
 L8_DEV void store8_nt(__amdgpu_buffer_rsrc_t rs, uint32_t voff, v2i data) {
   __builtin_amdgcn_raw_buffer_store_b64(data, rs, (int)voff, 0, 2 /* non-temporal */);
 }
+// Eight bf16 plus eight bf16, each sum rounded to nearest even.
+L8_DEV v4i sum_bf16x8(v4i a, v4i b) {
+  v4i out;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float lo = __uint_as_float((uint32_t)a[k] << 16) + __uint_as_float((uint32_t)b[k] << 16);
+    const float hi = __uint_as_float((uint32_t)a[k] & 0xffff0000u) + __uint_as_float((uint32_t)b[k] & 0xffff0000u);
+    out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
+  }
+  return out;
+}
+// The row of x becomes the row of h = bf16(x + residual), which is also written: the norm is that of the sum as it is kept.
+template <int N, typename ColOf>
+L8_DEV void add_residual(v4i (&cur)[N], const v4i (&res)[N], uint16_t *h, int64_t r, int64_t ldh, int C, ColOf col_of) {
+  const __amdgpu_buffer_rsrc_t rsH = make_rsrc(h + r * ldh, (uint32_t)C * 2u);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    cur[j] = sum_bf16x8(cur[j], res[j]);
+    store16_nt(rsH, (uint32_t)col_of(j) * 2u, cur[j]);
+  }
+}
 #endif
+
+// The residual stream of a block (lingua/transformer.py:497-543: h = x + attention(..), then ffn_norm(h)): kernels with ADD
+// read a second operand of x's shape, write the sum and normalise it.
+struct Residual {
+  const uint16_t *x;
+  int64_t ldx;
+  uint16_t *h;
+  int64_t ldh;
+};
 
 // Short rows (C <= NCH * 512): one wavefront owns a row, so neither the sum of squares nor the row amax crosses waves
 // and there is no barrier; the next row is requested before the current one is touched (loads through descriptors
 // without branches, as in the row-wise cast).  HBM-bound: 5 bytes per element.
-template <int NCH, bool COLMAX, bool W_F32>
+template <int NCH, bool COLMAX, bool W_F32, bool ADD>
 __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_wave_kernel(
     const uint16_t *__restrict__ x, const void *__restrict__ w, int64_t R, int C, int64_t ldx, float eps,
     uint16_t *__restrict__ y, int64_t ldy, uint8_t *__restrict__ q, int64_t ldq, float *__restrict__ scale,
-    float *__restrict__ rstd, uint16_t *__restrict__ col_partials, int scale_rule) {
+    float *__restrict__ rstd, uint16_t *__restrict__ col_partials, int scale_rule, const Residual res) {
 #if defined(__HIP_DEVICE_COMPILE__)  // buffer descriptors exist in the device pass only
   extern __shared__ __attribute__((aligned(16))) uint8_t dyn_lds[];  // [C] bf16 when COLMAX
   const int lane = threadIdx.x & 63;
@@ -109,10 +139,16 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_wave_kerne
   const int64_t stride = (int64_t)gridDim.x * kNormWaves;
   int64_t r = (int64_t)blockIdx.x * kNormWaves + wave;
   v4i cur[NCH], nxt[NCH];
+  [[maybe_unused]] v4i rnxt[NCH];
   load_norm_row<NCH>(cur, x, r, R, ldx, C, [&](int j) { return col_of(j); });
+  if constexpr (ADD) load_norm_row<NCH>(rnxt, res.x, r, R, res.ldx, C, [&](int j) { return col_of(j); });
   while (r < R) {
     const int64_t rn = r + stride;
     load_norm_row<NCH>(nxt, x, rn, R, ldx, C, [&](int j) { return col_of(j); });
+    if constexpr (ADD) {
+      add_residual<NCH>(cur, rnxt, res.h, r, res.ldh, C, [&](int j) { return col_of(j); });
+      load_norm_row<NCH>(rnxt, res.x, rn, R, res.ldx, C, [&](int j) { return col_of(j); });
+    }
     // each chunk of 512 columns is summed for itself and the chunks are added in order, as the waves of a workgroup that
     // shares a row add theirs: one order of summation, hence one result, in both layouts
     float tot = 0.0f;
@@ -190,11 +226,11 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_wave_kerne
 
 // Longer rows: one workgroup per row (a wave-per-row kernel would need more than 256 registers), the next row requested
 // ahead of the two barriers of the current one.
-template <int NCHW, bool COLMAX, bool W_F32>
+template <int NCHW, bool COLMAX, bool W_F32, bool ADD>
 __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_kernel(
     const uint16_t *__restrict__ x, const void *__restrict__ w, int64_t R, int C, int64_t ldx, float eps,
     uint16_t *__restrict__ y, int64_t ldy, uint8_t *__restrict__ q, int64_t ldq, float *__restrict__ scale,
-    float *__restrict__ rstd, uint16_t *__restrict__ col_partials, int scale_rule) {
+    float *__restrict__ rstd, uint16_t *__restrict__ col_partials, int scale_rule, const Residual res) {
 #if defined(__HIP_DEVICE_COMPILE__)  // buffer descriptors exist in the device pass only
   __shared__ float red_ss[2][kNormWaves];
   __shared__ uint32_t red_mx[2][kNormWaves];
@@ -210,10 +246,16 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_kernel(
   wt.load(w, C, [&](int j) { return col_of(j); });
   const float inv_c = 1.0f / (float)C;
   v4i cur[NCHW], nxt[NCHW];
+  [[maybe_unused]] v4i rnxt[NCHW];
   load_norm_row<NCHW>(cur, x, blockIdx.x, R, ldx, C, [&](int j) { return col_of(j); });
+  if constexpr (ADD) load_norm_row<NCHW>(rnxt, res.x, blockIdx.x, R, res.ldx, C, [&](int j) { return col_of(j); });
   int it = 0;
   for (int64_t r = blockIdx.x; r < R; r += gridDim.x, ++it) {
     load_norm_row<NCHW>(nxt, x, r + gridDim.x, R, ldx, C, [&](int j) { return col_of(j); });
+    if constexpr (ADD) {
+      add_residual<NCHW>(cur, rnxt, res.h, r, res.ldh, C, [&](int j) { return col_of(j); });
+      load_norm_row<NCHW>(rnxt, res.x, r + gridDim.x, R, res.ldx, C, [&](int j) { return col_of(j); });
+    }
     float ss = 0.0f;
 #pragma unroll
     for (int j = 0; j < NCHW; ++j)
@@ -284,6 +326,8 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_kernel(
 // Backward of the norm: with xhat = x * r and gh = gy * w,
 //   gx = (gh - xhat * mean(gh * xhat)) * r        (bf16)
 //   gw = sum over rows of gy * xhat               (fp32)
+// and with ADD, for the norm of a sum whose own gradient gh arrives beside gy,
+//   gx = gh + the above, rounded once: the gradient of either operand of the sum.
 // One workgroup per row, also for short rows; the row products for gw are
 // accumulated in registers over all rows a workgroup sees and leave as one row
 // of fp32 partial sums per workgroup, which rmsnorm_gw_fold_kernel adds up column
@@ -291,11 +335,11 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_cast_rowwise_kernel(
 // on the number of rows alone (no atomics: the result does not depend on timing).
 // Rows are requested AHEAD - 1 rows before they are used: a row of one chunk per
 // lane (up to 2048 columns) is too few bytes in flight for one row ahead.
-template <int NCHW, int AHEAD, bool W_F32>
+template <int NCHW, int AHEAD, bool W_F32, bool ADD>
 __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_bwd_kernel(
     const uint16_t *__restrict__ gy, const uint16_t *__restrict__ x, const void *__restrict__ w,
     const float *__restrict__ rstd, int64_t R, int C, int64_t ldg, int64_t ldx, uint16_t *__restrict__ gx, int64_t ldgx,
-    float *__restrict__ gw_partials) {
+    float *__restrict__ gw_partials, const uint16_t *__restrict__ gh, int64_t ldgh) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(AHEAD % 2 == 0, "a buffer meets the same half of `red` every time");
   __shared__ float red[2][kNormWaves];
@@ -311,11 +355,15 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_bwd_kernel(
     for (int e = 0; e < 8; ++e) gwacc[j][e] = 0.0f;
   const float inv_c = 1.0f / (float)C;
   v4i xb[AHEAD][NCHW], gb[AHEAD][NCHW];
+  // gh is needed last of the three: the longest rows, which fill the registers, request it in front of their barrier
+  constexpr int H_AHEAD = NCHW == 4 ? 1 : AHEAD;
+  [[maybe_unused]] v4i hb[H_AHEAD][NCHW];
   float rb[AHEAD];
   auto request = [&](int a, int64_t r) {  // a row beyond R: zeros, nothing is read
     rb[a] = rstd[r < R ? r : 0];
     load_norm_row<NCHW>(xb[a], x, r, R, ldx, C, [&](int j) { return col_of(j); });
     load_norm_row<NCHW>(gb[a], gy, r, R, ldg, C, [&](int j) { return col_of(j); });
+    if constexpr (ADD && H_AHEAD > 1) load_norm_row<NCHW>(hb[a], gh, r, R, ldgh, C, [&](int j) { return col_of(j); });
   };
 #pragma unroll
   for (int a = 0; a < AHEAD - 1; ++a) request(a, blockIdx.x + a * (int64_t)gridDim.x);
@@ -344,6 +392,7 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_bwd_kernel(
           gwacc[j][e] += ge * xh;
           dot += (ge * wt.get(j, e)) * xh;
         }
+      if constexpr (ADD && H_AHEAD == 1) load_norm_row<NCHW>(hb[0], gh, r, R, ldgh, C, [&](int j) { return col_of(j); });
       dot = wave_sum_f32(dot);
       if (lane == 0) red[a & 1][wave] = dot;
       __syncthreads();
@@ -351,15 +400,23 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_bwd_kernel(
 #pragma unroll
       for (int wv = 0; wv < kNormWaves; ++wv) tot += red[a & 1][wv];
       const float c1 = tot * inv_c;
+      if constexpr (ADD && H_AHEAD == 1) {  // the row stays packed across the barrier: unpacked it would spill
+#pragma unroll
+        for (int j = 0; j < NCHW; ++j) asm volatile("" : "+v"(xb[a][j]), "+v"(gb[a][j]));
+      }
       const __amdgpu_buffer_rsrc_t rsG = make_rsrc(gx + r * ldgx, (uint32_t)C * 2u);
 #pragma unroll
       for (int j = 0; j < NCHW; ++j) {
         v4i out;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t lo = bf16_rne_bits((grad(j, 2 * k) * wt.get(j, 2 * k) - xhat(j, 2 * k) * c1) * rinv);
-          const uint32_t hi = bf16_rne_bits((grad(j, 2 * k + 1) * wt.get(j, 2 * k + 1) - xhat(j, 2 * k + 1) * c1) * rinv);
-          out[k] = (int)(lo | (hi << 16));
+          float glo = (grad(j, 2 * k) * wt.get(j, 2 * k) - xhat(j, 2 * k) * c1) * rinv;
+          float ghi = (grad(j, 2 * k + 1) * wt.get(j, 2 * k + 1) - xhat(j, 2 * k + 1) * c1) * rinv;
+          if constexpr (ADD) {
+            glo += __uint_as_float((uint32_t)hb[a % H_AHEAD][j][k] << 16);
+            ghi += __uint_as_float((uint32_t)hb[a % H_AHEAD][j][k] & 0xffff0000u);
+          }
+          out[k] = (int)(bf16_rne_bits(glo) | (bf16_rne_bits(ghi) << 16));
         }
         store16_nt(rsG, (uint32_t)col_of(j) * 2u, out);
       }
@@ -447,31 +504,31 @@ constexpr int64_t kNormMaxC = 4 * kNormWaves * 512;  // 8192: the weights of a t
 static int64_t norm_wave_blocks(int64_t R) { return norm_blocks((R + kNormWaves - 1) / kNormWaves); }
 
 // N = chunks of 512 columns per wave (WAVE) or of 2048 per workgroup
-template <bool WAVE, int N, bool W_F32>
+template <bool WAVE, int N, bool W_F32, bool ADD>
 static int launch_norm(const void *x, const void *w, int64_t R, int64_t C, int64_t ldx, float eps, void *y, int64_t ldy,
-                       void *q, int64_t ldq, float *scale, float *rstd, float *col_amax, void *ws, hipStream_t st) {
+                       void *q, int64_t ldq, float *scale, float *rstd, float *col_amax, void *ws, const Residual &res, hipStream_t st) {
   const int64_t blocks = WAVE ? norm_wave_blocks(R) : norm_blocks(R);
   auto go = [&](auto kernel, size_t lds) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kNormBlock), lds, st, (const uint16_t *)x, w, R, (int)C, ldx, eps,
-                       (uint16_t *)y, ldy, (uint8_t *)q, ldq, scale, rstd, (uint16_t *)ws, l8::scale_rule());
+                       (uint16_t *)y, ldy, (uint8_t *)q, ldq, scale, rstd, (uint16_t *)ws, l8::scale_rule(), res);
   };
   if constexpr (WAVE) {
-    if (col_amax) go(rmsnorm_cast_rowwise_wave_kernel<N, true, W_F32>, (size_t)C * 2);
-    else go(rmsnorm_cast_rowwise_wave_kernel<N, false, W_F32>, 0);
+    if (col_amax) go(rmsnorm_cast_rowwise_wave_kernel<N, true, W_F32, ADD>, (size_t)C * 2);
+    else go(rmsnorm_cast_rowwise_wave_kernel<N, false, W_F32, ADD>, 0);
   } else {
-    if (col_amax) go(rmsnorm_cast_rowwise_kernel<N, true, W_F32>, 0);
-    else go(rmsnorm_cast_rowwise_kernel<N, false, W_F32>, 0);
+    if (col_amax) go(rmsnorm_cast_rowwise_kernel<N, true, W_F32, ADD>, 0);
+    else go(rmsnorm_cast_rowwise_kernel<N, false, W_F32, ADD>, 0);
   }
   L8_HIP(hipGetLastError());
   return col_amax ? fold_colmax(ws, blocks, C, col_amax, st) : L8_OK;
 }
 
-template <int N, bool W_F32>
+template <int N, bool W_F32, bool ADD>
 static int launch_norm_bwd(const void *gy, const void *x, const void *w, const float *rstd, int64_t R, int64_t C,
-                           int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_f32, void *ws, hipStream_t st) {
+                           int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_f32, const void *gh, int64_t ldgh, void *ws, hipStream_t st) {
   const int64_t blocks = norm_blocks(R);
-  hipLaunchKernelGGL((rmsnorm_bwd_kernel<N, N == 1 ? 4 : 2, W_F32>), dim3((unsigned)blocks), dim3(kNormBlock), 0, st, (const uint16_t *)gy,
-                     (const uint16_t *)x, w, rstd, R, (int)C, ldg, ldx, (uint16_t *)gx, ldgx, (float *)ws);
+  hipLaunchKernelGGL((rmsnorm_bwd_kernel<N, N == 1 ? 4 : 2, W_F32, ADD>), dim3((unsigned)blocks), dim3(kNormBlock), 0, st, (const uint16_t *)gy,
+                     (const uint16_t *)x, w, rstd, R, (int)C, ldg, ldx, (uint16_t *)gx, ldgx, (float *)ws, (const uint16_t *)gh, ldgh);
   L8_HIP(hipGetLastError());
   hipLaunchKernelGGL(rmsnorm_gw_fold_kernel, dim3((unsigned)((C + kGwCols - 1) / kGwCols)), dim3(kGwThreads), 0, st,
                      (const float *)ws, (int)blocks, (int)C, gw, gw_f32);
@@ -494,31 +551,38 @@ extern "C" int l8_rmsnorm_bwd(const void *gy, const void *x, const void *w, int 
   return l8_rmsnorm_bwd_as(gy, x, w, w_is_f32, rstd, R, C, ldg, ldx, gx, ldgx, gw, 1, workspace, workspace_bytes, stream);
 }
 
-extern "C" int l8_rmsnorm_bwd_as(const void *gy, const void *x, const void *w, int w_is_f32, const float *rstd, int64_t R,
-                                 int64_t C, int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_is_f32, void *workspace,
-                                 int64_t workspace_bytes, void *stream) {
-  L8_REQUIRE(R >= 0 && C >= 0, "l8_rmsnorm_bwd: negative shape R=%lld C=%lld", (long long)R, (long long)C);
+namespace l8 {
+
+// Both backward entries; gh NULL: no gradient of the normalised sum itself.
+static int rmsnorm_bwd_impl(const char *who, const void *gy, const void *x, const void *w, int w_is_f32, const float *rstd, int64_t R,
+                            int64_t C, int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_is_f32, const void *gh, int64_t ldgh,
+                            void *workspace, int64_t workspace_bytes, void *stream) {
+  L8_REQUIRE(R >= 0 && C >= 0, "%s: negative shape R=%lld C=%lld", who, (long long)R, (long long)C);
   if (C == 0) return L8_OK;
-  L8_REQUIRE(gw, "l8_rmsnorm_bwd: null pointer");
+  L8_REQUIRE(gw, "%s: null pointer", who);
   if (R == 0) {  // no rows: gw = 0, written by the fold kernel over zero partial rows
     hipLaunchKernelGGL(rmsnorm_gw_fold_kernel, dim3((unsigned)((C + kGwCols - 1) / kGwCols)), dim3(kGwThreads), 0, (hipStream_t)stream,
                        (const float *)nullptr, 0, (int)C, gw, gw_is_f32);
     L8_HIP(hipGetLastError());
     return L8_OK;
   }
-  L8_REQUIRE(gy && x && w && rstd && gx, "l8_rmsnorm_bwd: null pointer");
-  L8_REQUIRE(C % 8 == 0 && ldg % 8 == 0 && ldx % 8 == 0 && ldgx % 8 == 0 && ldg >= C && ldx >= C && ldgx >= C,
-             "l8_rmsnorm_bwd: C=%lld and the leading dimensions must be multiples of 8 with ld >= C", (long long)C);
-  L8_REQUIRE(((uintptr_t)gy % 16) == 0 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)gx % 16) == 0,
-             "l8_rmsnorm_bwd: gy, x and gx must be 16-byte aligned");
-  L8_REQUIRE(C <= kNormMaxC, "l8_rmsnorm_bwd: C=%lld exceeds %lld", (long long)C, (long long)kNormMaxC);
+  L8_REQUIRE(gy && x && w && rstd && gx, "%s: null pointer", who);
+  L8_REQUIRE(C % 8 == 0 && ldg % 8 == 0 && ldx % 8 == 0 && ldgx % 8 == 0 && ldg >= C && ldx >= C && ldgx >= C && (!gh || (ldgh % 8 == 0 && ldgh >= C)),
+             "%s: C=%lld and the leading dimensions must be multiples of 8 with ld >= C", who, (long long)C);
+  L8_REQUIRE(((uintptr_t)gy % 16) == 0 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)gx % 16) == 0 && ((uintptr_t)gh % 16) == 0,
+             "%s: gy, x, gx and gh must be 16-byte aligned", who);
+  L8_REQUIRE(C <= kNormMaxC, "%s: C=%lld exceeds %lld", who, (long long)C, (long long)kNormMaxC);
   const int64_t need = l8_rmsnorm_bwd_workspace(R, C);
-  L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0,
-             "l8_rmsnorm_bwd: needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+  L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
   hipStream_t st = (hipStream_t)stream;
-#define L8_NORM_BWD(N)                                                                                               \
-  return w_is_f32 ? launch_norm_bwd<N, true>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, workspace, st)  \
-                  : launch_norm_bwd<N, false>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, workspace, st)
+#define L8_NORM_BWD(N)                                                                                                          \
+  do {                                                                                                                          \
+    if (gh)                                                                                                                     \
+      return w_is_f32 ? launch_norm_bwd<N, true, true>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, gh, ldgh, workspace, st)    \
+                      : launch_norm_bwd<N, false, true>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, gh, ldgh, workspace, st);  \
+    return w_is_f32 ? launch_norm_bwd<N, true, false>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, gh, ldgh, workspace, st)     \
+                    : launch_norm_bwd<N, false, false>(gy, x, w, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, gh, ldgh, workspace, st);   \
+  } while (0)
   const int64_t nchw = ((C + 511) / 512 + kNormWaves - 1) / kNormWaves;
   if (nchw <= 1) L8_NORM_BWD(1);
   if (nchw <= 2) L8_NORM_BWD(2);
@@ -526,37 +590,80 @@ extern "C" int l8_rmsnorm_bwd_as(const void *gy, const void *x, const void *w, i
 #undef L8_NORM_BWD
 }
 
+}  // namespace l8
+
+extern "C" int l8_rmsnorm_bwd_as(const void *gy, const void *x, const void *w, int w_is_f32, const float *rstd, int64_t R,
+                                 int64_t C, int64_t ldg, int64_t ldx, void *gx, int64_t ldgx, void *gw, int gw_is_f32, void *workspace,
+                                 int64_t workspace_bytes, void *stream) {
+  return rmsnorm_bwd_impl("l8_rmsnorm_bwd", gy, x, w, w_is_f32, rstd, R, C, ldg, ldx, gx, ldgx, gw, gw_is_f32, nullptr, 0, workspace,
+                          workspace_bytes, stream);
+}
+
+extern "C" int l8_add_rmsnorm_bwd(const void *gy, const void *gh, const void *h, const void *w, int w_is_f32, const float *rstd, int64_t R,
+                                  int64_t C, int64_t ldgy, int64_t ldgh, int64_t ldh, void *gx, int64_t ldgx, void *gw, int gw_is_f32,
+                                  void *workspace, int64_t workspace_bytes, void *stream) {
+  L8_REQUIRE(gh || R <= 0 || C <= 0, "l8_add_rmsnorm_bwd: null pointer");
+  return rmsnorm_bwd_impl("l8_add_rmsnorm_bwd", gy, h, w, w_is_f32, rstd, R, C, ldgy, ldh, gx, ldgx, gw, gw_is_f32, gh, ldgh, workspace,
+                          workspace_bytes, stream);
+}
+
 extern "C" int64_t l8_rmsnorm_workspace(int64_t R, int64_t C) {
   if (R <= 0 || C <= 0) return 0;
   return norm_blocks(R) * C * (int64_t)sizeof(uint16_t);
 }
 
-extern "C" int l8_rmsnorm_cast_rowwise(const void *x, const void *w, int w_is_f32, int64_t R, int64_t C, int64_t ldx, float eps,
-                                       void *y, int64_t ldy, void *q, int64_t ldq, float *scale, float *rstd,
-                                       float *col_amax, void *workspace, int64_t workspace_bytes, void *stream) {
-  L8_REQUIRE(R >= 0 && C >= 0, "l8_rmsnorm_cast_rowwise: negative shape R=%lld C=%lld", (long long)R, (long long)C);
+namespace l8 {
+
+// Both forward entries; res.h NULL: the norm of x alone.
+static int rmsnorm_cast_impl(const char *who, const void *x, const void *w, int w_is_f32, int64_t R, int64_t C, int64_t ldx, float eps,
+                             void *y, int64_t ldy, void *q, int64_t ldq, float *scale, float *rstd, float *col_amax, void *workspace,
+                             int64_t workspace_bytes, bool add, const Residual &res, void *stream) {
+  L8_REQUIRE(R >= 0 && C >= 0, "%s: negative shape R=%lld C=%lld", who, (long long)R, (long long)C);
   if (R == 0 || C == 0) return empty_col_amax(col_amax, C, (hipStream_t)stream);
-  L8_REQUIRE(x && w && y, "l8_rmsnorm_cast_rowwise: null pointer");
-  L8_REQUIRE((q == nullptr) == (scale == nullptr), "l8_rmsnorm_cast_rowwise: pass q and scale together");
-  L8_REQUIRE(C % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && ldx >= C && ldy >= C && (!q || (ldq % 8 == 0 && ldq >= C)),
-             "l8_rmsnorm_cast_rowwise: C=%lld and the leading dimensions must be multiples of 8 with ld >= C", (long long)C);
-  L8_REQUIRE(((uintptr_t)x % 16) == 0 && ((uintptr_t)y % 16) == 0 && ((uintptr_t)q % 8) == 0,
-             "l8_rmsnorm_cast_rowwise: x and y must be 16-byte aligned and q 8-byte aligned");
-  L8_REQUIRE(C <= kNormMaxC, "l8_rmsnorm_cast_rowwise: C=%lld exceeds %lld", (long long)C, (long long)kNormMaxC);
-  L8_REQUIRE(!col_amax || q, "l8_rmsnorm_cast_rowwise: column amaxes come with the cast");
+  L8_REQUIRE(x && w && y && (!add || (res.x && res.h)), "%s: null pointer", who);
+  L8_REQUIRE((q == nullptr) == (scale == nullptr), "%s: pass q and scale together", who);
+  L8_REQUIRE(C % 8 == 0 && ldx % 8 == 0 && ldy % 8 == 0 && ldx >= C && ldy >= C && (!q || (ldq % 8 == 0 && ldq >= C)) &&
+                 (!add || (res.ldx % 8 == 0 && res.ldh % 8 == 0 && res.ldx >= C && res.ldh >= C)),
+             "%s: C=%lld and the leading dimensions must be multiples of 8 with ld >= C", who, (long long)C);
+  L8_REQUIRE(((uintptr_t)x % 16) == 0 && ((uintptr_t)y % 16) == 0 && ((uintptr_t)q % 8) == 0 && ((uintptr_t)res.x % 16) == 0 && ((uintptr_t)res.h % 16) == 0,
+             "%s: the bf16 operands must be 16-byte aligned and q 8-byte aligned", who);
+  L8_REQUIRE(C <= kNormMaxC, "%s: C=%lld exceeds %lld", who, (long long)C, (long long)kNormMaxC);
+  L8_REQUIRE(!col_amax || q, "%s: column amaxes come with the cast", who);
   if (col_amax) {
     const int64_t need = l8_rmsnorm_workspace(R, C);
     L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0,
-               "l8_rmsnorm_cast_rowwise: col_amax needs a 16-byte aligned workspace of %lld bytes", (long long)need);
+               "%s: col_amax needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
   }
   hipStream_t st = (hipStream_t)stream;
 #define L8_NORM(WAVE, N)                                                                                                        \
-  return w_is_f32 ? launch_norm<WAVE, N, true>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, st)      \
-                  : launch_norm<WAVE, N, false>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, st)
+  do {                                                                                                                          \
+    if (add)                                                                                                                    \
+      return w_is_f32 ? launch_norm<WAVE, N, true, true>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, res, st)   \
+                      : launch_norm<WAVE, N, false, true>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, res, st); \
+    return w_is_f32 ? launch_norm<WAVE, N, true, false>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, res, st)    \
+                    : launch_norm<WAVE, N, false, false>(x, w, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace, res, st);  \
+  } while (0)
   const int64_t nch = (C + 511) / 512, nchw = (nch + kNormWaves - 1) / kNormWaves;
   if (nch <= 4 && R > norm_blocks(R)) L8_NORM(true, 4);
   if (nchw <= 1) L8_NORM(false, 1);
   if (nchw <= 2) L8_NORM(false, 2);
   L8_NORM(false, 4);
 #undef L8_NORM
+}
+
+}  // namespace l8
+
+extern "C" int l8_rmsnorm_cast_rowwise(const void *x, const void *w, int w_is_f32, int64_t R, int64_t C, int64_t ldx, float eps,
+                                       void *y, int64_t ldy, void *q, int64_t ldq, float *scale, float *rstd,
+                                       float *col_amax, void *workspace, int64_t workspace_bytes, void *stream) {
+  return rmsnorm_cast_impl("l8_rmsnorm_cast_rowwise", x, w, w_is_f32, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace,
+                           workspace_bytes, false, Residual{nullptr, 0, nullptr, 0}, stream);
+}
+
+extern "C" int l8_add_rmsnorm_cast_rowwise(const void *x, const void *residual, const void *w, int w_is_f32, int64_t R, int64_t C,
+                                           int64_t ldx, int64_t ldr, float eps, void *h, int64_t ldh, void *y, int64_t ldy, void *q,
+                                           int64_t ldq, float *scale, float *rstd, float *col_amax, void *workspace,
+                                           int64_t workspace_bytes, void *stream) {
+  return rmsnorm_cast_impl("l8_add_rmsnorm_cast_rowwise", x, w, w_is_f32, R, C, ldx, eps, y, ldy, q, ldq, scale, rstd, col_amax, workspace,
+                           workspace_bytes, true, Residual{(const uint16_t *)residual, ldr, (uint16_t *)h, ldh}, stream);
 }

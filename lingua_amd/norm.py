@@ -10,6 +10,12 @@ over through the memo of ``lingua_amd.float8`` that already lets such linears
 share one cast, so nothing changes in the attention / MLP modules.
 
 Opt-in: ``fuse_rmsnorm(model)`` after (or before) ``convert_linears_to_fp8``.
+
+``add_rmsnorm`` is the norm of a residual sum together with the sum, as the
+second half of a block computes it (lingua/transformer.py:497-543:
+``h = x + attention(...)``, then ``ffn_norm(h)``): one pass over both operands
+forward, and one backward that adds the two gradients of the sum.
+``fuse_residual_norm(model)`` has the blocks of a model call it.
 """
 import re
 
@@ -51,6 +57,52 @@ class Fp8RMSNormFn(torch.autograd.Function):
         return gx, (gw if ctx.needs_input_grad[1] else None), None, None
 
 
+class Fp8AddRMSNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, training):
+        if x.dtype != torch.bfloat16 or residual.dtype != torch.bfloat16:
+            raise RuntimeError(f"add_rmsnorm: bf16 activations required, got {x.dtype} and {residual.dtype}")
+        if x.shape != residual.shape:
+            raise RuntimeError(f"add_rmsnorm: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
+        want_col = bool(training and f8.config.fp8_wgrad)
+        x2d, r2d = x.flatten(end_dim=-2), residual.flatten(end_dim=-2)
+        col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
+        h2d, y2d, q, s, rstd = ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True)
+        if f8.config.share_input_casts:
+            f8._fwd_cast.put(y2d, (q, s, col), "rmsnorm")
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(h2d, weight, rstd)
+        ctx.x_shape = x.shape
+        return h2d.unflatten(0, x.shape[:-1]), y2d.unflatten(0, x.shape[:-1])
+
+    @staticmethod
+    def backward(ctx, gh, gy):
+        h2d, weight, rstd = ctx.saved_tensors
+        for g in (gh, gy):
+            if g is not None and g.dtype != torch.bfloat16:
+                raise RuntimeError(f"add_rmsnorm backward: bf16 gradients required, got {g.dtype}")
+        gx = gw = None
+        if gy is None:   # only the sum was used
+            gx = gh
+        else:
+            gy2d = gy.flatten(end_dim=-2)
+            if gh is None:
+                gx2d, gw = ops.rmsnorm_bwd(gy2d, h2d, weight, rstd, gw_dtype=weight.dtype)
+            else:
+                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh.flatten(end_dim=-2), h2d, weight, rstd, gw_dtype=weight.dtype)
+            gx = gx2d.reshape(ctx.x_shape)
+        need = ctx.needs_input_grad
+        return gx if need[0] else None, gx if need[1] else None, gw if need[2] else None, None, None
+
+
+def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float):
+    """``h = x + residual`` (rounded to bf16) and ``y = rmsnorm(h) * weight``: returns ``(h, y)``, shaped like x [..., C].  The fp8
+    linears that are called on ``y`` find it quantised, as behind an ``Fp8RMSNorm``."""
+    if x.dim() < 2:
+        raise RuntimeError(f"add_rmsnorm: expected [..., C] with at least one leading dimension, got {tuple(x.shape)}")
+    return Fp8AddRMSNormFn.apply(x, residual, weight, eps, torch.is_grad_enabled())
+
+
 class Fp8RMSNorm(torch.nn.Module):
     """Same parameters and state-dict keys as the reference's RMSNorm (``weight``; ``eps`` attribute)."""
 
@@ -62,6 +114,10 @@ class Fp8RMSNorm(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         # grad mode is read here: inside an autograd Function's forward it is always off
         return Fp8RMSNormFn.apply(x, self.weight, self.eps, torch.is_grad_enabled())
+
+    def add(self, x: torch.Tensor, residual: torch.Tensor):
+        """``(x + residual, this norm of it)`` in one pass."""
+        return add_rmsnorm(x, residual, self.weight, self.eps)
 
     def reset_parameters(self):
         torch.nn.init.ones_(self.weight)
@@ -83,3 +139,31 @@ def fuse_rmsnorm(root_module: torch.nn.Module, filter: str = r"(attention_norm|f
         return Fp8RMSNorm(w.numel(), float(module.eps), weight=w)
 
     return f8.named_replace(replace, root_module)
+
+
+class _ResidualNormForward:
+    """``forward`` of a block whose second norm takes the residual sum with it (lingua/transformer.py:497-543: ``h = x +
+    attention(attention_norm(x), ...)``, ``h + feed_forward(ffn_norm(h))``)."""
+
+    def forward(self, x, *args, **kwargs):
+        h, y = self.ffn_norm.add(x, self.attention(self.attention_norm(x), *args, **kwargs))
+        return h + self.feed_forward(y)
+
+
+def fuse_residual_norm(root_module: torch.nn.Module, filter: str = r"layers\.[0-9]+$") -> torch.nn.Module:
+    """In every module whose dotted name matches ``filter`` and whose children are exactly ``attention``, ``feed_forward``,
+    ``attention_norm`` and an ``Fp8RMSNorm`` ``ffn_norm`` (the reference's TransformerBlock, lingua/transformer.py:497-543, after
+    ``fuse_rmsnorm``), the residual sum in front of ``ffn_norm`` becomes part of it.  The caller vouches that the module computes
+    ``h = x + attention(attention_norm(x), ...)``, ``h + feed_forward(ffn_norm(h))``; modules, parameters and state-dict keys stay."""
+    filter_re = re.compile(filter)
+    for name, module in root_module.named_modules():
+        if not filter_re.search(name) or isinstance(module, _ResidualNormForward):
+            continue
+        children = dict(module.named_children())
+        if (set(children) != {"attention", "feed_forward", "attention_norm", "ffn_norm"} or not isinstance(children["ffn_norm"], Fp8RMSNorm) or
+                list(module.parameters(recurse=False))):
+            raise RuntimeError(f"fuse_residual_norm: {name!r} ({type(module).__name__}) is not a block of attention, feed_forward, "
+                               "attention_norm and an Fp8RMSNorm ffn_norm (run fuse_rmsnorm first)")
+        cls = type(module)
+        module.__class__ = type(cls.__name__, (_ResidualNormForward, cls), {"__module__": cls.__module__})
+    return root_module

@@ -763,3 +763,240 @@ def rmsnorm_bwd(gy: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, rstd: t
                                              int(gw_dtype == torch.float32), ws.data_ptr(), ws_bytes, st)
     _lib.check(code, "l8_rmsnorm_bwd")
     return gx, gw
+
+
+def add_rmsnorm_cast_rowwise(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float, want_q: bool = True,
+                             col_amax: Optional[torch.Tensor] = None, want_rstd: bool = True, on_lines: bool = False):
+    """h = bf16(x + residual) and ``rmsnorm_cast_rowwise`` of it in one pass.
+    Returns (h [R,C] bf16, y [R,C] bf16, q [R,C] fp8 | None, scale [R,1] fp32 | None, rstd [R,1] fp32 | None)."""
+    what = "add_rmsnorm_cast_rowwise"
+    x = _rows_2d(x, torch.bfloat16, what)
+    residual = _rows_2d(residual, torch.bfloat16, what)
+    if x.shape != residual.shape or x.device != residual.device:
+        raise RuntimeError(f"{what}: x and residual must have the same shape and device, got {tuple(x.shape)} and {tuple(residual.shape)}")
+    st = _prep(x, what)
+    R, C = x.shape
+    dev = x.device
+    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.numel() != C or weight.device != dev:
+        raise RuntimeError(f"{what}: weight must be bf16 or fp32 with C elements on the same device")
+    weight = weight.contiguous()
+    if col_amax is not None and (not want_q or col_amax.dtype != torch.float32 or col_amax.numel() != C or not col_amax.is_contiguous()):
+        raise RuntimeError(f"{what}: col_amax needs the cast and must be a contiguous fp32 tensor with C elements")
+    h, y = (torch.empty((R, C), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    q = _empty_fp8(R, C, dev, on_lines) if want_q else None
+    scale = torch.empty((R, 1), dtype=torch.float32, device=dev) if want_q else None
+    rstd = torch.empty((R, 1), dtype=torch.float32, device=dev) if want_rstd else None
+    with _timed("add_rmsnorm_cast_rowwise", R * C * (8 + (1 if want_q else 0)) + 8 * R, dev):
+        ws_bytes = _lib.load().l8_rmsnorm_workspace(R, C) if col_amax is not None else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        code = _lib.load().l8_add_rmsnorm_cast_rowwise(
+            x.data_ptr(), residual.data_ptr(), weight.data_ptr(), int(weight.dtype == torch.float32), R, C, _ld(x), _ld(residual), float(eps),
+            h.data_ptr(), C, y.data_ptr(), C, q.data_ptr() if want_q else None, _ld(q) if want_q else C, scale.data_ptr() if want_q else None,
+            rstd.data_ptr() if want_rstd else None, col_amax.data_ptr() if col_amax is not None else None,
+            ws.data_ptr() if ws is not None else None, ws_bytes, st)
+    _lib.check(code, "l8_add_rmsnorm_cast_rowwise")
+    return h, y, q, scale, rstd
+
+
+def add_rmsnorm_bwd(gy: torch.Tensor, gh: torch.Tensor, h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor,
+                    gw_dtype: torch.dtype = torch.float32):
+    """Backward of the norm of a sum: returns (gx [R,C] bf16, the gradient of either operand, gw [C] of ``gw_dtype``) from the
+    gradients gy of the norm and gh of the sum, the sum h (bf16 [R,C]), weight [C], rstd [R,1] fp32."""
+    what = "add_rmsnorm_bwd"
+    gy, gh, h = (_rows_2d(t, torch.bfloat16, f"{what}({n})") for t, n in ((gy, "gy"), (gh, "gh"), (h, "h")))
+    if gy.shape != h.shape or gh.shape != h.shape or gy.device != h.device or gh.device != h.device:
+        raise RuntimeError(f"{what}: gy, gh and h must have the same shape and device")
+    st = _prep(h, what)
+    R, C = h.shape
+    dev = h.device
+    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.numel() != C or weight.device != dev:
+        raise RuntimeError(f"{what}: weight must be bf16 or fp32 with C elements on the same device")
+    if rstd.dtype != torch.float32 or rstd.numel() != R or rstd.device != dev:
+        raise RuntimeError(f"{what}: rstd must be fp32 with R elements on the same device")
+    if gw_dtype not in (torch.bfloat16, torch.float32):
+        raise RuntimeError(f"{what}: gw_dtype must be bf16 or fp32")
+    weight, rstd = weight.contiguous(), rstd.contiguous()
+    gx = torch.empty((R, C), dtype=torch.bfloat16, device=dev)
+    gw = torch.empty((C,), dtype=gw_dtype, device=dev)
+    with _timed("add_rmsnorm_bwd", R * C * 8 + 4 * R, dev):
+        ws_bytes = _lib.load().l8_rmsnorm_bwd_workspace(R, C)
+        ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=dev)
+        code = _lib.load().l8_add_rmsnorm_bwd(gy.data_ptr(), gh.data_ptr(), h.data_ptr(), weight.data_ptr(), int(weight.dtype == torch.float32),
+                                              rstd.data_ptr(), R, C, _ld(gy), _ld(gh), _ld(h), gx.data_ptr(), C, gw.data_ptr(),
+                                              int(gw_dtype == torch.float32), ws.data_ptr(), ws_bytes, st)
+    _lib.check(code, "l8_add_rmsnorm_bwd")
+    return gx, gw
+
+
+def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+           positions: Optional[torch.Tensor] = None, in_halves: bool = False, inverse: bool = False):
+    """Rotary positions of xq [B,S,Hq,D] and xk [B,S,Hk,D] (bf16, either may be None) by the angles whose cosines and sines are
+    cos, sin (fp32 [P, rot / 2]); positions int32 or int64, broadcastable to [B,S] (None: 0 .. S - 1).  ``inverse``: the transposed
+    rotation.  Returns dense tensors of the same shapes.  A token at a position outside [0, P) becomes NaN."""
+    what = "rotary"
+    xs = [t for t in (xq, xk) if t is not None]
+    if not xs:
+        raise RuntimeError(f"{what}: xq or xk is needed")
+    for t in xs:
+        if t.dtype != torch.bfloat16 or t.dim() != 4:
+            raise RuntimeError(f"{what}: expected bf16 [B,S,H,D] tensors, got {t.dtype} {tuple(t.shape)}")
+        if t.device != xs[0].device or t.shape[:2] != xs[0].shape[:2] or t.shape[3] != xs[0].shape[3]:
+            raise RuntimeError(f"{what}: xq and xk must agree in batch, tokens, head size and device, got {tuple(xs[0].shape)} and {tuple(t.shape)}")
+    st = _prep(xs[0], what)
+    dev = xs[0].device
+    B, S, _, D = xs[0].shape
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.device != dev:
+            raise RuntimeError(f"{what}: cos and sin must be fp32 [P, rot / 2] tensors of one shape on the inputs' device")
+    if cos.stride() != sin.stride():
+        cos, sin = cos.contiguous(), sin.contiguous()
+    P, rot = cos.shape[0], 2 * cos.shape[1]
+    if rot < 2 or rot > D:
+        raise RuntimeError(f"{what}: tables for {rot} columns do not fit heads of {D}")
+    pos_ptr, pos_i32, pos_b, pos_s = None, 0, 0, 0
+    if positions is not None:
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+            raise RuntimeError(f"{what}: positions must be int32 or int64 on the inputs' device")
+        try:
+            positions = positions.expand(B, S)
+        except RuntimeError:
+            raise RuntimeError(f"{what}: positions {tuple(positions.shape)} do not broadcast to [{B}, {S}]") from None
+        pos_ptr, pos_i32, (pos_b, pos_s) = positions.data_ptr(), int(positions.dtype == torch.int32), positions.stride()
+    elif S > P:
+        raise RuntimeError(f"{what}: {S} tokens, the tables hold {P} positions")
+    outs, items, keep = [], [], []
+    for t in (xq, xk):
+        if t is None:
+            outs.append(None)
+            items += [0] * 6
+            continue
+        if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 2):
+            t = t.contiguous()
+        y = torch.empty(t.shape, dtype=torch.bfloat16, device=dev)
+        keep.append(t)
+        outs.append(y)
+        items += [t.data_ptr(), y.data_ptr(), t.shape[2], t.stride(0), t.stride(1), t.stride(2)]
+    with _timed("rotary", sum(4 * t.numel() for t in xs) + 4 * B * S * rot, dev):
+        code = _lib.load().l8_rotary(struct.pack("12q", *items), B, S, D, rot, int(in_halves), int(inverse), cos.data_ptr(), sin.data_ptr(),
+                                     cos.stride(0), cos.stride(1), P, pos_ptr, pos_i32, pos_b, pos_s, st)
+    _lib.check(code, "l8_rotary")
+    return tuple(outs)
+
+
+# ---- MXFP4: e2m1 codes, two a byte, in blocks of 32 along a row, with an e8m0 scale each ----
+
+MX_BLOCK = 32
+
+
+def _empty_mxfp4(rows: int, cols: int, device, on_lines: bool):
+    """Codes and scales of a matrix; rows of scales on 16-byte lines, and with ``on_lines`` those of codes on 128-byte lines where that
+    adds at most an eighth."""
+    blocks = (cols + MX_BLOCK - 1) // MX_BLOCK
+    nbytes = blocks * 16
+    ld = (nbytes + 127) // 128 * 128 if on_lines and keeps_on_lines(nbytes) else nbytes
+    q = torch.empty_strided((rows, nbytes), (ld, 1), dtype=torch.uint8, device=device)
+    s = torch.empty_strided((rows, blocks), ((blocks + 15) // 16 * 16, 1), dtype=torch.uint8, device=device)
+    return q.view(torch.float4_e2m1fn_x2), s.view(torch.float8_e8m0fnu)
+
+
+def _mx_operand(q: torch.Tensor, s: torch.Tensor, what: str):
+    """Codes [R, 16 * blocks] and scales [R, blocks] of one matrix as bytes, each row dense."""
+    if q.dtype not in (torch.float4_e2m1fn_x2, torch.uint8) or s.dtype not in (torch.float8_e8m0fnu, torch.uint8) or q.dim() != 2 or s.dim() != 2:
+        raise RuntimeError(f"{what}: expected 2-D codes (float4_e2m1fn_x2 or uint8) and scales (float8_e8m0fnu or uint8), got {q.dtype} {tuple(q.shape)} "
+                           f"and {s.dtype} {tuple(s.shape)}")
+    if q.shape[0] != s.shape[0] or q.shape[1] != 16 * s.shape[1] or q.device != s.device:
+        raise RuntimeError(f"{what}: codes {tuple(q.shape)} and scales {tuple(s.shape)} are not 16 bytes and one scale per block of 32 on one device")
+    q, s = q.view(torch.uint8), s.view(torch.uint8)
+    return (q if _rows_apart(q) else q.contiguous()), (s if _rows_apart(s) else s.contiguous())
+
+
+def _on_16_bytes(t: torch.Tensor) -> torch.Tensor:
+    """Rows of bytes that start on 16-byte lines: ``t`` where they do, else a copy."""
+    if t.data_ptr() % 16 == 0 and (_ld(t) % 16 == 0 or t.shape[0] <= 1):
+        return t
+    out = torch.empty_strided(t.shape, ((t.shape[1] + 15) // 16 * 16, 1), dtype=torch.uint8, device=t.device)
+    return out.copy_(t)
+
+
+def _ld16(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def cast_mxfp4(x: torch.Tensor, rowwise: bool = True, transposed: bool = False, on_lines: bool = False):
+    """x [R,C] bf16 in MXFP4, blocks of 32 along its rows and / or along its columns (the copy of x.t()), from one read.
+    Returns ((codes [R, 16 * ceil(C / 32)] float4_e2m1fn_x2, scales [R, ceil(C / 32)] float8_e8m0fnu) | None, the same of x.t() | None).
+    Codes behind the last column are zeros.  ``on_lines``: codes have their rows on 128-byte lines where that adds little."""
+    x = _rows_2d(x, torch.bfloat16, "cast_mxfp4")
+    st = _prep(x, "cast_mxfp4")
+    if not rowwise and not transposed:
+        raise RuntimeError("cast_mxfp4: rowwise or transposed, or both")
+    R, C = x.shape
+    rows = _empty_mxfp4(R, C, x.device, on_lines) if rowwise else None
+    cols = _empty_mxfp4(C, R, x.device, on_lines) if transposed else None
+    args = []
+    for pair in (rows, cols):
+        args += [None, 0, None, 0] if pair is None else [pair[0].data_ptr(), pair[0].stride(0), pair[1].data_ptr(), pair[1].stride(0)]
+    with _timed("cast_mxfp4", R * C * 2 + (R * C * 17 // 32) * (int(rowwise) + int(transposed)), x.device):
+        code = _lib.load().l8_cast_mxfp4(x.data_ptr(), R, C, _ld(x), *args, st)
+    _lib.check(code, "l8_cast_mxfp4")
+    return rows, cols
+
+
+def mxfp4_to_bf16(q: torch.Tensor, s: torch.Tensor, cols: int) -> torch.Tensor:
+    """bf16 [R, cols] values of MXFP4 codes and scales as ``cast_mxfp4`` makes them (or the same as uint8)."""
+    q, s = _mx_operand(q, s, "mxfp4_to_bf16")
+    st = _prep(q, "mxfp4_to_bf16")
+    if not 0 <= cols <= MX_BLOCK * s.shape[1]:
+        raise RuntimeError(f"mxfp4_to_bf16: {s.shape[1]} blocks of {MX_BLOCK} do not hold {cols} columns")
+    if q.data_ptr() % 4 or (q.shape[0] > 1 and _ld(q) % 4):
+        q = _on_16_bytes(q)
+    y = torch.empty((q.shape[0], cols), dtype=torch.bfloat16, device=q.device)
+    with _timed("mxfp4_to_bf16", y.numel() * 2 + q.numel() + s.numel(), q.device):
+        code = _lib.load().l8_mxfp4_to_bf16(q.data_ptr(), _ld16(q), s.data_ptr(), _ld(s), q.shape[0], cols, y.data_ptr(), max(cols, 1), st)
+    _lib.check(code, "l8_mxfp4_to_bf16")
+    return y
+
+
+def _mx_bias(bias, N, device, what):
+    if bias is None:
+        return None
+    if bias.dtype != torch.bfloat16 or bias.numel() != N or bias.device != device:
+        raise RuntimeError(f"{what}: bias must be bf16 with N elements on the operands' device")
+    return bias.contiguous()
+
+
+def gemm_mxfp4_nt(qa: torch.Tensor, qb: torch.Tensor, sa: torch.Tensor, sb: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 [M,N] product of MXFP4 operands, codes qa [M, 16 * blocks] and qb [N, 16 * blocks] with scales sa, sb [.., blocks], plus
+    bias; summed in fp32 and rounded once."""
+    what = "gemm_mxfp4_nt"
+    qa, sa = _mx_operand(qa, sa, f"{what}(A)")
+    qb, sb = _mx_operand(qb, sb, f"{what}(B)")
+    st = _prep(qa, what)
+    if qa.shape[1] != qb.shape[1] or qa.device != qb.device:
+        raise RuntimeError(f"{what}: reduction dims or devices differ ({2 * qa.shape[1]} on {qa.device}, {2 * qb.shape[1]} on {qb.device})")
+    M, N, K = qa.shape[0], qb.shape[0], MX_BLOCK * sa.shape[1]
+    bias = _mx_bias(bias, N, qa.device, what)
+    qa, sa, qb, sb = (_on_16_bytes(t) for t in (qa, sa, qb, sb))
+    user_out = out is not None
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=qa.device)
+    elif out.dtype != torch.bfloat16 or out.shape != (M, N) or out.device != qa.device or (out.numel() and (out.stride(1) != 1 or (M > 1 and out.stride(0) < N))):
+        raise RuntimeError(f"{what}: out must be bf16 [M,N] with unit column stride on the operands' device")
+    with _timed("gemm_mxfp4_nt", 2 * M * N * K, qa.device):
+        code = _lib.load().l8_gemm_mxfp4_nt(qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), M, N, K, _ld16(qa), _ld16(sa), _ld16(qb), _ld16(sb),
+                                            bias.data_ptr() if bias is not None else None, out.data_ptr(), _ld(out) if M > 1 else max(N, 1), st)
+    _lib.check(code, "l8_gemm_mxfp4_nt")
+    if user_out:
+        _wrote_into(out)
+    return out
+
+
+def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 [M,N]: x [M,K] bf16 quantised along its rows times a weight kept in MXFP4 (codes [N, 16 * ceil(K / 32)] and scales), plus
+    bias."""
+    x = _rows_2d(x, torch.bfloat16, "mxfp4_linear_fwd")
+    if sw.dim() != 2 or (x.shape[1] + MX_BLOCK - 1) // MX_BLOCK != sw.shape[1]:
+        raise RuntimeError(f"mxfp4_linear_fwd: x {tuple(x.shape)} and a weight of scales {tuple(sw.shape)} do not fit")
+    (qx, sx), _ = cast_mxfp4(x, on_lines=True)
+    return gemm_mxfp4_nt(qx, qw, sx, sw, bias)
