@@ -17,6 +17,9 @@
 //   * rows beyond M / N and chunks beyond K lie outside the buffers' ranges: zeros.  Scale bytes beyond K are cleared when they are
 //     read (what lies behind a row's end may be a NaN);
 //   * workgroups are dealt to the 8 XCDs in contiguous ranges of a grouped tile order, so that an XCD's share panels in its L2.
+#include <type_traits>
+#include <utility>
+
 #include "l8_common.h"
 
 namespace l8 {
@@ -199,6 +202,344 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
 #endif
 }
 
+// ---------------------------------------------------------------------------
+// Large products: one workgroup per compute unit walks a list of 256 x 256 tiles, and the stream of panels (one operand's 256 rows of
+// a stage, 32 KiB) runs on from the last stage of a tile into the first of the next, so that only a workgroup's first tile waits for
+// its operands.  Four waves, 128 x 128 each: the least LDS traffic per flop.
+//
+//   * LDS is a ring of five panels, 2.5 stages; a trip (one stage, 128 matrix instructions of 16 cycles) requests one panel in front of
+//     its barrier, into the slot that the barrier before released, and one behind it, into the slot that this stage's A panel left;
+//   * the barrier stands between a stage's two halves of 128 codes.  While a half is multiplied, the eight A and eight B fragments of
+//     the next one are read: 16 KiB of LDS to 64 matrix instructions, and never more than two sets in registers.  Each group of two
+//     matrix instructions carries at most one LDS read and one load, and fences keep it so: the matrix cores want an instruction
+//     every 16 cycles, four issue slots;
+//   * the LDS is full, so scales stay in registers: a lane loads the 16 scale bytes of one row (two stages) for 64 rows at a time,
+//     two stages ahead; byte permutes and lane-group swaps turn those four registers into four of the layout that the
+//     instruction wants (lane group g: the bytes of blocks 2 g, 2 g + 1 of both stages, picked by its op_sel) -- 32 vector
+//     instructions to 256 matrix instructions;
+//   * C leaves straight from the accumulators, 16 bytes a lane, under the next tile's first panels.
+// ---------------------------------------------------------------------------
+#if defined(__HIP_DEVICE_COMPILE__)
+// A 16-byte buffer store with a register offset, and two wait states: a write to its data registers right behind it may overtake it.
+L8_DEV void store16_streaming(v4i data, __amdgpu_buffer_rsrc_t rs, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_buffer_store_b128(data, rs, (int)voff, soff, 2);
+  asm volatile("s_nop 1" : : "v"(data));
+}
+// Scales of 64 rows, a row a lane (16 bytes: two stages of 8 blocks), to out[q]: of rows 16 q + (lane & 15), lane group g holding the
+// bytes of blocks 2 g and 2 g + 1 of the first stage and of the second.
+L8_DEV void turn_scales(v4i d, uint32_t (&out)[4]) {
+  uint32_t e[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    e[2 * h] = __builtin_amdgcn_perm((uint32_t)d[2 + h], (uint32_t)d[h], 0x05040100u);
+    e[2 * h + 1] = __builtin_amdgcn_perm((uint32_t)d[2 + h], (uint32_t)d[h], 0x07060302u);
+  }
+  // a 4 x 4 transposition of registers and groups of 16 lanes
+  const auto a = __builtin_amdgcn_permlane32_swap(e[0], e[2], false, false), b = __builtin_amdgcn_permlane32_swap(e[1], e[3], false, false);
+  const auto lo = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), hi = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
+  out[0] = lo[0], out[1] = lo[1], out[2] = hi[0], out[3] = hi[1];
+}
+#endif
+
+// f(0), f(1), .. as straight code, each with its number as a constant
+template <typename F, int... I>
+L8_DEV void in_turn(std::integer_sequence<int, I...>, F &&f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <bool HAS_BIAS>
+__global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  constexpr int BM = 256, BN = 256, TM = 8, TN = 8, GROUP = 4, R = 5, UNIT = 256 * 128;
+  constexpr int NL = 8;                 // wave loads (8 rows) of a panel per wave
+  constexpr int NSC = 4;                // scale loads of a window per wave
+  constexpr int N_STORES = TM * 4;      // of a C tile per wave
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+
+  // ---- this workgroup's tiles: first + loc, + W, + 2 W, ... of the grouped order ----
+  const int nb = p.tiles_m * p.tiles_n;
+  const int xcd = blockIdx.x & 7, loc = blockIdx.x >> 3, W = gridDim.x >> 3;
+  const int q = nb >> 3, rem = nb & 7;
+  const int first = (xcd < rem) ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q;
+  const int cnt = q + (xcd < rem ? 1 : 0);
+  const int KT = (p.blocks + 7) / 8;    // at least 2 (the host sees to it)
+  const int n_seg = loc < cnt ? (cnt - loc + W - 1) / W : 0;
+  if (n_seg == 0) return;
+  const int per_group = GROUP * p.tiles_n;
+  struct Cursor { int grp, in_grp; };   // one for the loader, one for the multiplying side: a tile's origin without a division
+  Cursor cur_mul, cur_ld;
+  cur_mul.grp = (first + loc) / per_group;
+  cur_mul.in_grp = first + loc - cur_mul.grp * per_group;
+  cur_ld = cur_mul;
+  auto origin = [&](const Cursor &c, int &m0, int &n0) {
+    const int first_m = c.grp * GROUP, left = p.tiles_m - first_m;
+    if (left >= GROUP) {
+      m0 = (first_m + (c.in_grp & (GROUP - 1))) * BM;
+      n0 = (c.in_grp / GROUP) * BN;
+    } else {
+      m0 = (first_m + c.in_grp % left) * BM;
+      n0 = (c.in_grp / left) * BN;
+    }
+  };
+  auto step = [&](Cursor &c) {
+    c.in_grp += W;
+    while (c.in_grp >= per_group) {
+      c.in_grp -= per_group;
+      ++c.grp;
+    }
+  };
+
+  // ---- loads ----
+  const int kbytes = p.blocks * 16;
+  const int lrow = lane >> 3, lpos = lane & 7;
+  const int chunk[2] = {(lpos ^ lrow) * 16, (lpos ^ lrow ^ 1) * 16};
+  const uint32_t a_voff[2] = {(uint32_t)(lrow * (int)p.lda + chunk[0]), (uint32_t)(lrow * (int)p.lda + chunk[1])};
+  const uint32_t b_voff[2] = {(uint32_t)(lrow * 8 * (int)p.ldb + chunk[0]), (uint32_t)(lrow * 8 * (int)p.ldb + chunk[1])};
+  const uint32_t sa_voff = (uint32_t)((wm * 128 + lane) * (int)p.ldsa);
+  const uint32_t sb_voff = (uint32_t)((wn * 128 + 8 * (lane & 15) + (lane >> 4)) * (int)p.ldsb);
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
+  auto wrap = [](int slot) { return slot >= R ? slot - R : slot; };
+  auto range = [](int64_t n) { return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu; };
+  int ld_seg = 0, ld_kt = 0;
+  __amdgpu_buffer_rsrc_t ld_rsA, ld_rsB, ld_rsSa, ld_rsSb;
+  auto ld_open = [&](int seg) {
+    if (seg < n_seg) {
+      int m0, n0;
+      origin(cur_ld, m0, n0);
+      step(cur_ld);
+      ld_rsA = make_rsrc(p.A + (int64_t)m0 * p.lda, range((int64_t)(p.M - m0 - 1) * p.lda + kbytes));
+      ld_rsB = make_rsrc(p.B + (int64_t)n0 * p.ldb, range((int64_t)(p.N - n0 - 1) * p.ldb + kbytes));
+      ld_rsSa = make_rsrc(p.sa + (int64_t)m0 * p.ldsa, range((int64_t)(p.M - m0 - 1) * p.ldsa + (p.blocks + 3) / 4 * 4));
+      ld_rsSb = make_rsrc(p.sb + (int64_t)n0 * p.ldsb, range((int64_t)(p.N - n0 - 1) * p.ldsb + (p.blocks + 3) / 4 * 4));
+    } else {   // past the last tile: zeros
+      ld_rsA = make_rsrc(p.A, 0);
+      ld_rsB = make_rsrc(p.B, 0);
+      ld_rsSa = make_rsrc(p.sa, 0);
+      ld_rsSb = make_rsrc(p.sb, 0);
+    }
+  };
+  auto ld_advance = [&]() {
+    if (++ld_kt == KT) {
+      ld_kt = 0;
+      ld_open(++ld_seg);
+    }
+  };
+  // i-th wave load of the loader's A or B panel into the panel at LDS offset `at`.  A load's row offset is formed from the one before
+  // (kept in scalar registers, all sixteen would spill).
+  int ld_off = 0, step_a = 8 * (int)p.lda, step_b = 64 * (int)p.ldb, back_b = -63 * (int)p.ldb;
+  int a0_off = wave * NL * 8 * (int)p.lda, b0_off = ((wave >> 1) * 128 + (wave & 1) * 4) * (int)p.ldb;
+  asm volatile("" : "+s"(step_a), "+s"(step_b), "+s"(back_b), "+s"(a0_off), "+s"(b0_off));
+  auto load_one = [&](bool is_b, int at, int i) __attribute__((always_inline)) {
+    const int k0 = ld_kt * 128;
+    const uint32_t off = (k0 + chunk[i & 1] < kbytes) ? 0u : kBeyond;
+    const uint32_t dst = lds0 + at + (wave * NL + i) * 1024;
+    if (!is_b) {
+      ld_off = i == 0 ? k0 + a0_off : ld_off + step_a;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ld_rsA, reinterpret_cast<lds_void_ptr>(dst), 16, a_voff[i & 1] | off, ld_off, 0, 0);
+    } else {   // LDS rows 8 g .. 8 g + 7 of a span of 128: rows g / 2 + 64 (g % 2) + 0, 8, .. 56 of it
+      ld_off = i == 0 ? k0 + b0_off : ld_off + (i & 1 ? step_b : back_b);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(ld_rsB, reinterpret_cast<lds_void_ptr>(dst), 16, b_voff[i & 1] | off, ld_off, 0, 0);
+    }
+  };
+  // scales of the window that the loader's stage lies in: A rows 0 .. 63 and 64 .. 127 of the wave's share, and B rows
+  v4i sc_in[NSC];
+  int sc_left = 0;   // blocks from that window on
+  auto load_scales = [&]() __attribute__((always_inline)) {
+    const int w16 = (ld_kt >> 1) * 16;
+    sc_left = p.blocks - w16;
+    sc_in[0] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, (int)sa_voff, w16, 0);
+    sc_in[1] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, (int)sa_voff, w16 + 64 * (int)p.ldsa, 0);
+    sc_in[2] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, (int)sb_voff, w16, 0);
+    sc_in[3] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, (int)sb_voff, w16 + 4 * (int)p.ldsb, 0);
+  };
+  uint32_t asc[TM], bsc[TN];
+  auto turn_all = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      uint32_t t[4];
+      turn_scales(sc_in[s], t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asc[s * 4 + i] = t[i];
+      turn_scales(sc_in[2 + s], t);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bsc[s * 4 + i] = t[i];
+    }
+    if (sc_left < 16) {   // behind a row's end: whatever lies there, the codes are zeros and must not meet a NaN
+      int l = lane;   // (opaque: what follows from it is not kept in registers)
+      asm volatile("" : "+v"(l));
+      const int g2 = 2 * (l >> 4);
+      uint32_t mask = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) mask |= ((k >> 1) * 8 + g2 + (k & 1) < sc_left ? 0xffu : 0u) << (8 * k);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) asc[i] &= mask, bsc[i] &= mask;
+    }
+  };
+
+  // ---- fragments ----
+  const int frow = lane & 15, fg = lane >> 4;
+  const int fr = (frow & 7) ^ (frow >> 3);
+  const uint32_t foff[2] = {(uint32_t)(frow * 128 + (((fg * 2) ^ fr) * 16)), (uint32_t)(frow * 128 + (((fg * 2 + 1) ^ fr) * 16))};
+  typedef const __attribute__((address_space(3))) v4i *lds_v4i;
+  auto frag_addrs = [&](int panel_a, int panel_b, uint32_t (&ad)[4]) {
+    const uint32_t a = lds0 + panel_a + wm * (128 * 128), b = lds0 + panel_b + wn * (128 * 128);
+    asm volatile("v_add_u32 %0, %1, %2" : "=v"(ad[0]) : "s"(a), "v"(foff[0]));
+    asm volatile("v_add_u32 %0, %1, %2" : "=v"(ad[1]) : "s"(a), "v"(foff[1]));
+    asm volatile("v_add_u32 %0, %1, %2" : "=v"(ad[2]) : "s"(b), "v"(foff[0]));
+    asm volatile("v_add_u32 %0, %1, %2" : "=v"(ad[3]) : "s"(b), "v"(foff[1]));
+  };
+  auto read_frag = [&](uint32_t at, int t) { return *reinterpret_cast<lds_v4i>(at + t * 2048); };
+  v4i fa[2][TM], fb[2][TN];   // of the stage's two halves
+  uint32_t ad[4];
+  // r-th read of half h: B0, A0, B1, .. in the order of their use (row by row of the wave's tiles)
+  auto read_next = [&](auto half, int r) __attribute__((always_inline)) {
+    constexpr int h = decltype(half)::value;
+    if (r == 0) fb[h][0] = read_frag(ad[2 + h], 0);
+    else if (r == 1) fa[h][0] = read_frag(ad[h], 0);
+    else if (r <= TN) fb[h][r - 1] = read_frag(ad[2 + h], r - 1);
+    else fa[h][r - TN] = read_frag(ad[h], r - TN);
+  };
+
+  v4f acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM * TN * 4; ++i) asm volatile("v_accvgpr_write_b32 %0, 0" : "=a"(acc[i / (4 * TN)][i / 4 % TN][i % 4]));
+  // One element, and zero in its place for the next tile: the 256 instructions pass under the stores, and every trip is the same code
+  // (one of its own for a tile's first stage, starting from constant zeros, spilled accumulators).
+  auto acc_take = [&](int tm, int tn, int e) -> float {
+    float x;
+    asm volatile("v_accvgpr_read_b32 %0, %1\n\tv_accvgpr_write_b32 %1, 0" : "=v"(x), "+a"(acc[tm][tn][e]));
+    return x;
+  };
+  [[maybe_unused]] v4i seg_bias = {0, 0, 0, 0};
+  [[maybe_unused]] const __amdgpu_buffer_rsrc_t rsBias = make_rsrc(HAS_BIAS ? (const void *)p.bias : (const void *)p.A, HAS_BIAS ? (uint32_t)p.N * 2u : 0u);
+  auto store_tile = [&](int m0, int n0) {
+    int ldc2 = (int)p.ldc * 2;
+    asm volatile("" : "+s"(ldc2));
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int col = wn * 128 + 8 * (l & 15);
+    const __amdgpu_buffer_rsrc_t rsC = make_rsrc(p.C + (int64_t)m0 * p.ldc + n0, range(((int64_t)(p.M - m0 - 1) * p.ldc + (p.N - n0)) * 2));
+    const uint32_t voff = (n0 + col < p.N) ? (uint32_t)(4 * (l >> 4) * ldc2 + col * 2) : kBeyond;
+#pragma unroll
+    for (int tm = 0; tm < TM; ++tm)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v4i out;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float lo = acc_take(tm, 2 * k, e), hi = acc_take(tm, 2 * k + 1, e);
+          if constexpr (HAS_BIAS) {
+            lo += __uint_as_float((uint32_t)seg_bias[k] << 16);
+            hi += __uint_as_float((uint32_t)seg_bias[k] & 0xffff0000u);
+          }
+          typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+          const bf2 b = {(__bf16)lo, (__bf16)hi};
+          out[k] = __builtin_bit_cast(int, b);
+        }
+        store16_streaming(out, rsC, voff, (wm * 128 + tm * 16 + e) * ldc2);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+
+  // ---- prologue: two stages and the first window of scales requested, stage 0 published, its first fragments read ----
+  ld_open(0);
+  load_scales();
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+#pragma unroll
+    for (int i = 0; i < NL; ++i) load_one(u & 1, u * UNIT, i);
+    if (u & 1) ld_advance();
+  }
+  MX_WAIT_VM(2 * NL);
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  frag_addrs(0, UNIT, ad);
+  constexpr std::integral_constant<int, 0> lower{};
+  constexpr std::integral_constant<int, 1> upper{};
+#pragma unroll
+  for (int r = 0; r < TM + TN; ++r) read_next(lower, r);
+  turn_all();
+  int s0 = 0;   // ring slot of this stage's A panel
+
+  constexpr int N_MMA = TM * TN;        // of a half
+  constexpr int SPREAD0 = 56, SPREAD1 = 60;   // instructions of the lower and the upper half over which the reads are spread
+  // `stores`: those of the tile before were issued since the panels that this trip's barrier waits for were requested.  They are
+  // younger than the panels and the counter retires in order, so the count allows for them.  ODD: the second stage of a window.
+  // The first stage of a window requests the scales of the next: the loader is two stages ahead, in that window already.
+  auto trip = [&](auto odd_tag, bool stores) __attribute__((always_inline)) {
+    constexpr int ODD = decltype(odd_tag)::value ? 1 : 0;
+    const int at1 = wrap(s0 + 4) * UNIT, at2 = s0 * UNIT;
+    if constexpr (!ODD) load_scales();
+    auto mma_one = [&](auto half, int i) __attribute__((always_inline)) {
+      constexpr int h = decltype(half)::value;
+      const int tm = i / TN, tn = i % TN;
+      const v4i x = fa[h][tm], y = fb[h][tn];
+      // fragments belong in ordinary registers: one among the accumulators' pushes an accumulator out to memory
+      if (tn == 0) asm volatile("" : : "v"(x));
+      if (tm == 0) asm volatile("" : : "v"(y));
+      const v8i a = {x[0], x[1], x[2], x[3], 0, 0, 0, 0}, b = {y[0], y[1], y[2], y[3], 0, 0, 0, 0};
+      acc[tm][tn] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[tm][tn], 4, 4, 2 * ODD + h, (int)asc[tm], 2 * ODD + h, (int)bsc[tn]);
+    };
+    in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
+      constexpr int i = decltype(number)::value;
+      mma_one(lower, i);
+#pragma unroll
+      for (int r = ((TM + TN) * i) / SPREAD0; i < SPREAD0 && r < ((TM + TN) * (i + 1)) / SPREAD0; ++r) read_next(upper, r);
+#pragma unroll
+      for (int j = (NL * i) / N_MMA; j < (NL * (i + 1)) / N_MMA; ++j) load_one(false, at1, j);
+      if (i & 1) __builtin_amdgcn_sched_barrier(0);
+    });
+    frag_addrs(wrap(s0 + 2) * UNIT, wrap(s0 + 3) * UNIT, ad);
+    constexpr int PEND = NL + (ODD ? 0 : NSC);
+    if (!ODD && stores) __builtin_amdgcn_s_waitcnt(((N_STORES + PEND) & 0xF) | (0x7 << 4) | (((N_STORES + PEND) >> 4) << 14));
+    else __builtin_amdgcn_s_waitcnt((PEND & 0xF) | (0x7 << 4) | ((PEND >> 4) << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
+      constexpr int i = decltype(number)::value;
+      mma_one(upper, i);
+#pragma unroll
+      for (int r = ((TM + TN) * i) / SPREAD1; i < SPREAD1 && r < ((TM + TN) * (i + 1)) / SPREAD1; ++r) read_next(lower, r);
+#pragma unroll
+      for (int j = (NL * i) / N_MMA; j < (NL * (i + 1)) / N_MMA; ++j) load_one(true, at2, j);
+      if (i & 1) __builtin_amdgcn_sched_barrier(0);
+    });
+    ld_advance();
+    s0 = wrap(s0 + 2);
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+#pragma unroll 1
+  for (int seg = 0; seg < n_seg; ++seg) {
+    int m0, n0;
+    origin(cur_mul, m0, n0);
+    step(cur_mul);
+    if constexpr (HAS_BIAS) {
+      int l = lane;
+      asm volatile("" : "+v"(l));
+      seg_bias = __builtin_amdgcn_raw_buffer_load_b128(rsBias, (wn * 128 + 8 * (l & 15)) * 2, n0 * 2, 0);
+    }
+#pragma unroll 1
+    for (int kt = 0; kt < KT; kt += 2) {
+      trip(no, kt == 0 && seg > 0);
+      if (kt + 1 < KT) trip(yes, false);
+      turn_all();
+    }
+    if constexpr (HAS_BIAS) asm volatile("" : : "v"(seg_bias));
+    store_tile(m0, n0);
+  }
+  // what was requested beyond the last tile (zeros) must have landed before the workgroup's LDS is released
+  MX_WAIT_VM(0);
+#else
+  (void)p;
+#endif
+}
+
 template <int WM, int WN, int TM, int TN, int NS>
 static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
   constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
@@ -212,6 +553,23 @@ static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
     if (slot >= 0) ready[slot] = true;
   }
   hipLaunchKernelGGL((gemm_mxfp4_kernel<WM, WN, TM, TN, NS>), dim3((unsigned)(a.tiles_m * a.tiles_n)), dim3(WM * WN * 64), lds, st, a);
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+// one workgroup per compute unit, a multiple of 8 of them (the hardware deals workgroups to the 8 XCDs in turn)
+template <bool HAS_BIAS>
+static int launch_gemm_mxfp4_stream(MxGemmArgs a, hipStream_t st) {
+  constexpr int lds = 5 * 256 * 128;
+  a.tiles_m = (a.M + 255) / 256, a.tiles_n = (a.N + 255) / 256;
+  static bool ready[kMaxDev];
+  const int slot = device_slot();
+  if (slot < 0 || !ready[slot]) {
+    L8_HIP(hipFuncSetAttribute((const void *)gemm_mxfp4_stream_kernel<HAS_BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+    if (slot >= 0) ready[slot] = true;
+  }
+  const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n, cus8 = (num_cus() / 8) * 8, want = (tiles + 7) / 8 * 8;
+  hipLaunchKernelGGL((gemm_mxfp4_stream_kernel<HAS_BIAS>), dim3((unsigned)(want < cus8 ? want : cus8)), dim3(256), lds, st, a);
   L8_HIP(hipGetLastError());
   return L8_OK;
 }
@@ -240,7 +598,12 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
   hipStream_t st = (hipStream_t)stream;
   L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");
   const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-  if (big >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 8, 8, 2>(a, st);
+  if (big >= num_cus() / 2) {
+    // the stores of the large kernel take eight columns at once, and its stream runs two stages ahead
+    if (blocks > 8 && N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && num_cus() >= 8)
+      return bias ? launch_gemm_mxfp4_stream<true>(a, st) : launch_gemm_mxfp4_stream<false>(a, st);
+    return launch_gemm_mxfp4<2, 2, 8, 8, 2>(a, st);
+  }
   if (mid >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 4, 4, 4>(a, st);
   return launch_gemm_mxfp4<2, 2, 2, 2, 8>(a, st);
 }
