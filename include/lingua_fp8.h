@@ -373,7 +373,11 @@ int l8_mxfp4_to_bf16(const void *q, int64_t ldq, const void *s, int64_t lds, int
  * Leading dimensions of codes and scales in bytes, multiples of 16 below 2^23, pointers 16-byte aligned.  K < 2^24; what lies
  * behind the last block of a row is not used. */
 int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, const void *sb, int64_t M, int64_t N, int64_t K, int64_t lda,
-                     int64_t ldsa, int64_t ldb, int64_t ldsb, const void *bias, void *C, int64_t ldc, void *stream);
+                     int64_t ldsa, int64_t ldb, int64_t ldsb, const void *bias, void *C, int64_t ldc, void *workspace,
+                     int64_t workspace_bytes, void *stream);
+/* Bytes of that workspace (the scales of large problems laid out for the matrix cores; 0 for others): 16-byte aligned, used by
+ * the call's own work alone. */
+int64_t l8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
 
 int l8_gemm_algo_count(void);
 /* human-readable description of tile configuration `algo` (1-based), or NULL */

@@ -213,10 +213,10 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
 //     the next one are read: 16 KiB of LDS to 64 matrix instructions, and never more than two sets in registers.  Each group of two
 //     matrix instructions carries at most one LDS read and one load, and fences keep it so: the matrix cores want an instruction
 //     every 16 cycles, four issue slots;
-//   * the LDS is full, so scales stay in registers: a lane loads the 16 scale bytes of one row (two stages) for 64 rows at a time,
-//     two stages ahead; byte permutes and lane-group swaps turn those four registers into four of the layout that the
-//     instruction wants (lane group g: the bytes of blocks 2 g, 2 g + 1 of both stages, picked by its op_sel) -- 32 vector
-//     instructions to 256 matrix instructions;
+//   * the LDS is full, so scales go straight to registers, in the layout that the instruction wants (lane group g: the bytes of
+//     blocks 2 g and 2 g + 1 of both stages of a window, picked by its op_sel).  A kernel of its own lays them out so beforehand, 1 KiB
+//     of consecutive bytes per load: it moves 1/16 of the operands' bytes.  (Loaded as they lie, 16 bytes of each of 64 rows, and
+//     turned in registers, they took 40 of 340 us.)
 //   * C leaves straight from the accumulators, 16 bytes a lane, under the next tile's first panels.
 // ---------------------------------------------------------------------------
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -225,21 +225,53 @@ L8_DEV void store16_streaming(v4i data, __amdgpu_buffer_rsrc_t rs, uint32_t voff
   __builtin_amdgcn_raw_buffer_store_b128(data, rs, (int)voff, soff, 2);
   asm volatile("s_nop 1" : : "v"(data));
 }
-// Scales of 64 rows, a row a lane (16 bytes: two stages of 8 blocks), to out[q]: of rows 16 q + (lane & 15), lane group g holding the
-// bytes of blocks 2 g and 2 g + 1 of the first stage and of the second.
-L8_DEV void turn_scales(v4i d, uint32_t (&out)[4]) {
-  uint32_t e[4];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    e[2 * h] = __builtin_amdgcn_perm((uint32_t)d[2 + h], (uint32_t)d[h], 0x05040100u);
-    e[2 * h + 1] = __builtin_amdgcn_perm((uint32_t)d[2 + h], (uint32_t)d[h], 0x07060302u);
-  }
-  // a 4 x 4 transposition of registers and groups of 16 lanes
-  const auto a = __builtin_amdgcn_permlane32_swap(e[0], e[2], false, false), b = __builtin_amdgcn_permlane32_swap(e[1], e[3], false, false);
-  const auto lo = __builtin_amdgcn_permlane16_swap(a[0], b[0], false, false), hi = __builtin_amdgcn_permlane16_swap(a[1], b[1], false, false);
-  out[0] = lo[0], out[1] = lo[1], out[2] = hi[0], out[3] = hi[1];
-}
 #endif
+
+// Scales as the kernel below loads them: for every 64 LDS rows of a panel and window of 16 blocks 64 lanes' 16 bytes, lane (g, r) = 16 g +
+// r holding, for q = 0 .. 3, the bytes of blocks 2 g, 2 g + 1, 8 + 2 g and 9 + 2 g of row 16 q + r.  Zeros for rows beyond the last and
+// blocks beyond K (the codes there are zeros and must not meet a NaN).  LDS row l of B is row 8 (l % 16) + l / 16 of its 128.
+struct MxScaleArgs {
+  const uint8_t *s[2];
+  uint8_t *t[2];
+  int64_t ld[2];
+  int rows[2], chunks[2];   // rows; groups of 64 of them, up to whole tiles
+  int blocks, windows;
+};
+__global__ __launch_bounds__(256) void mxfp4_lay_scales_kernel(const MxScaleArgs p) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  // a workgroup: 64 rows, 4 windows (64 bytes a row), in LDS as rows of 17 dwords
+  __shared__ uint32_t rows[64 * 17];
+  const bool is_b = (int)blockIdx.y >= p.chunks[0];
+  const int o = is_b ? 1 : 0, chunk = blockIdx.y - (is_b ? p.chunks[0] : 0), w0 = blockIdx.x * 4;
+  const int row = threadIdx.x >> 2, part = threadIdx.x & 3;   // this thread's row and window
+  const int l = (chunk & 1) * 64 + row;
+  const int src = (chunk >> 1) * 128 + (is_b ? 8 * (l & 15) + (l >> 4) : l);
+  const int first = (w0 + part) * 16;
+  uint32_t v[4] = {0, 0, 0, 0};
+  if (src < p.rows[o]) {
+    const uint8_t *at = p.s[o] + (int64_t)src * p.ld[o] + first;
+    if (first + 16 <= p.blocks) {
+      __builtin_memcpy(v, at, 16);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (first + k < p.blocks) v[k >> 2] |= (uint32_t)at[k] << (8 * (k & 3));
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) rows[row * 17 + part * 4 + k] = v[k];
+  __syncthreads();
+  const int win = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  if (w0 + win >= p.windows) return;
+  v4i out;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint32_t lo = rows[(16 * q + r) * 17 + win * 4 + (g >> 1)], hi = rows[(16 * q + r) * 17 + win * 4 + 2 + (g >> 1)];
+    out[q] = (int)__builtin_amdgcn_perm(hi, lo, g & 1 ? 0x07060302u : 0x05040100u);
+  }
+  *(v4i *)(p.t[o] + ((int64_t)chunk * p.windows + w0 + win) * 1024 + lane * 16) = out;
+#endif
+}
 
 // f(0), f(1), .. as straight code, each with its number as a constant
 template <typename F, int... I>
@@ -298,8 +330,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
   const int chunk[2] = {(lpos ^ lrow) * 16, (lpos ^ lrow ^ 1) * 16};
   const uint32_t a_voff[2] = {(uint32_t)(lrow * (int)p.lda + chunk[0]), (uint32_t)(lrow * (int)p.lda + chunk[1])};
   const uint32_t b_voff[2] = {(uint32_t)(lrow * 8 * (int)p.ldb + chunk[0]), (uint32_t)(lrow * 8 * (int)p.ldb + chunk[1])};
-  const uint32_t sa_voff = (uint32_t)((wm * 128 + lane) * (int)p.ldsa);
-  const uint32_t sb_voff = (uint32_t)((wn * 128 + 8 * (lane & 15) + (lane >> 4)) * (int)p.ldsb);
+  const int windows = (KT + 1) >> 1;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void_ptr)smem;
   auto wrap = [](int slot) { return slot >= R ? slot - R : slot; };
   auto range = [](int64_t n) { return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu; };
@@ -312,8 +343,8 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
       step(cur_ld);
       ld_rsA = make_rsrc(p.A + (int64_t)m0 * p.lda, range((int64_t)(p.M - m0 - 1) * p.lda + kbytes));
       ld_rsB = make_rsrc(p.B + (int64_t)n0 * p.ldb, range((int64_t)(p.N - n0 - 1) * p.ldb + kbytes));
-      ld_rsSa = make_rsrc(p.sa + (int64_t)m0 * p.ldsa, range((int64_t)(p.M - m0 - 1) * p.ldsa + (p.blocks + 3) / 4 * 4));
-      ld_rsSb = make_rsrc(p.sb + (int64_t)n0 * p.ldsb, range((int64_t)(p.N - n0 - 1) * p.ldsb + (p.blocks + 3) / 4 * 4));
+      ld_rsSa = make_rsrc(p.sa + (int64_t)(m0 / 64 + wm * 2) * windows * 1024, windows * 2048);
+      ld_rsSb = make_rsrc(p.sb + (int64_t)(n0 / 64 + wn * 2) * windows * 1024, windows * 2048);
     } else {   // past the last tile: zeros
       ld_rsA = make_rsrc(p.A, 0);
       ld_rsB = make_rsrc(p.B, 0);
@@ -344,39 +375,18 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
       __builtin_amdgcn_raw_ptr_buffer_load_lds(ld_rsB, reinterpret_cast<lds_void_ptr>(dst), 16, b_voff[i & 1] | off, ld_off, 0, 0);
     }
   };
-  // scales of the window that the loader's stage lies in: A rows 0 .. 63 and 64 .. 127 of the wave's share, and B rows
-  v4i sc_in[NSC];
-  int sc_left = 0;   // blocks from that window on
+  // scales of the window that the loader's stage lies in, of the wave's 128 rows of A and of B
+  v4i sc_in[NSC], sc[NSC];
   auto load_scales = [&]() __attribute__((always_inline)) {
-    const int w16 = (ld_kt >> 1) * 16;
-    sc_left = p.blocks - w16;
-    sc_in[0] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, (int)sa_voff, w16, 0);
-    sc_in[1] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, (int)sa_voff, w16 + 64 * (int)p.ldsa, 0);
-    sc_in[2] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, (int)sb_voff, w16, 0);
-    sc_in[3] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, (int)sb_voff, w16 + 4 * (int)p.ldsb, 0);
+    const int at = (ld_kt >> 1) * 1024;
+    sc_in[0] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, lane * 16, at, 0);
+    sc_in[1] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSa, lane * 16, at + windows * 1024, 0);
+    sc_in[2] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, lane * 16, at, 0);
+    sc_in[3] = __builtin_amdgcn_raw_buffer_load_b128(ld_rsSb, lane * 16, at + windows * 1024, 0);
   };
-  uint32_t asc[TM], bsc[TN];
-  auto turn_all = [&]() __attribute__((always_inline)) {
+  auto next_scales = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      uint32_t t[4];
-      turn_scales(sc_in[s], t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) asc[s * 4 + i] = t[i];
-      turn_scales(sc_in[2 + s], t);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) bsc[s * 4 + i] = t[i];
-    }
-    if (sc_left < 16) {   // behind a row's end: whatever lies there, the codes are zeros and must not meet a NaN
-      int l = lane;   // (opaque: what follows from it is not kept in registers)
-      asm volatile("" : "+v"(l));
-      const int g2 = 2 * (l >> 4);
-      uint32_t mask = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) mask |= ((k >> 1) * 8 + g2 + (k & 1) < sc_left ? 0xffu : 0u) << (8 * k);
-#pragma unroll
-      for (int i = 0; i < TM; ++i) asc[i] &= mask, bsc[i] &= mask;
-    }
+    for (int i = 0; i < NSC; ++i) sc[i] = sc_in[i];
   };
 
   // ---- fragments ----
@@ -462,7 +472,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
   constexpr std::integral_constant<int, 1> upper{};
 #pragma unroll
   for (int r = 0; r < TM + TN; ++r) read_next(lower, r);
-  turn_all();
+  next_scales();
   int s0 = 0;   // ring slot of this stage's A panel
 
   constexpr int N_MMA = TM * TN;        // of a half
@@ -482,7 +492,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
       if (tn == 0) asm volatile("" : : "v"(x));
       if (tm == 0) asm volatile("" : : "v"(y));
       const v8i a = {x[0], x[1], x[2], x[3], 0, 0, 0, 0}, b = {y[0], y[1], y[2], y[3], 0, 0, 0, 0};
-      acc[tm][tn] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[tm][tn], 4, 4, 2 * ODD + h, (int)asc[tm], 2 * ODD + h, (int)bsc[tn]);
+      acc[tm][tn] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[tm][tn], 4, 4, 2 * ODD + h, sc[tm / 4][tm % 4], 2 * ODD + h, sc[2 + tn / 4][tn % 4]);
     };
     in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
       constexpr int i = decltype(number)::value;
@@ -528,7 +538,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
     for (int kt = 0; kt < KT; kt += 2) {
       trip(no, kt == 0 && seg > 0);
       if (kt + 1 < KT) trip(yes, false);
-      turn_all();
+      next_scales();
     }
     if constexpr (HAS_BIAS) asm volatile("" : : "v"(seg_bias));
     store_tile(m0, n0);
@@ -557,9 +567,16 @@ static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
   return L8_OK;
 }
 
+// Do the large kernel's tiles fill half of the units?  Its stream runs two stages ahead.
+static bool takes_stream(int64_t M, int64_t N, int64_t blocks) {
+  return ((M + 255) / 256) * ((N + 255) / 256) >= num_cus() / 2 && blocks > 8 && num_cus() >= 8;
+}
+// bytes of one operand's laid-out scales: whole tiles of 256 rows, whole windows of 16 blocks
+static int64_t laid_bytes(int64_t rows, int64_t blocks) { return (rows + 255) / 256 * 4 * ((blocks + 15) / 16) * 1024; }
+
 // one workgroup per compute unit, a multiple of 8 of them (the hardware deals workgroups to the 8 XCDs in turn)
 template <bool HAS_BIAS>
-static int launch_gemm_mxfp4_stream(MxGemmArgs a, hipStream_t st) {
+static int launch_gemm_mxfp4_stream(MxGemmArgs a, uint8_t *workspace, hipStream_t st) {
   constexpr int lds = 5 * 256 * 128;
   a.tiles_m = (a.M + 255) / 256, a.tiles_n = (a.N + 255) / 256;
   static bool ready[kMaxDev];
@@ -568,6 +585,12 @@ static int launch_gemm_mxfp4_stream(MxGemmArgs a, hipStream_t st) {
     L8_HIP(hipFuncSetAttribute((const void *)gemm_mxfp4_stream_kernel<HAS_BIAS>, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
     if (slot >= 0) ready[slot] = true;
   }
+  const int windows = (a.blocks + 15) / 16;
+  uint8_t *const tb = workspace + laid_bytes(a.M, a.blocks);
+  const MxScaleArgs sc = {{a.sa, a.sb}, {workspace, tb}, {a.ldsa, a.ldsb}, {a.M, a.N}, {a.tiles_m * 4, a.tiles_n * 4}, a.blocks, windows};
+  hipLaunchKernelGGL(mxfp4_lay_scales_kernel, dim3((unsigned)((windows + 3) / 4), (unsigned)(sc.chunks[0] + sc.chunks[1])), dim3(256), 0, st, sc);
+  L8_HIP(hipGetLastError());
+  a.sa = workspace, a.sb = tb;
   const int64_t tiles = (int64_t)a.tiles_m * a.tiles_n, cus8 = (num_cus() / 8) * 8, want = (tiles + 7) / 8 * 8;
   hipLaunchKernelGGL((gemm_mxfp4_stream_kernel<HAS_BIAS>), dim3((unsigned)(want < cus8 ? want : cus8)), dim3(256), lds, st, a);
   L8_HIP(hipGetLastError());
@@ -578,8 +601,15 @@ static int launch_gemm_mxfp4_stream(MxGemmArgs a, hipStream_t st) {
 
 using namespace l8;
 
+extern "C" int64_t l8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0 || M >= (1 << 28) || N >= (1 << 28) || K >= (1 << 24)) return 0;
+  const int64_t blocks = (K + 31) / 32;
+  return takes_stream(M, N, blocks) ? laid_bytes(M, blocks) + laid_bytes(N, blocks) : 0;
+}
+
 extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, const void *sb, int64_t M, int64_t N, int64_t K, int64_t lda,
-                                int64_t ldsa, int64_t ldb, int64_t ldsb, const void *bias, void *C, int64_t ldc, void *stream) {
+                                int64_t ldsa, int64_t ldb, int64_t ldsb, const void *bias, void *C, int64_t ldc, void *workspace,
+                                int64_t workspace_bytes, void *stream) {
   L8_REQUIRE(M >= 0 && N >= 0 && K >= 0, "l8_gemm_mxfp4_nt: negative shape M=%lld N=%lld K=%lld", (long long)M, (long long)N, (long long)K);
   if (M == 0 || N == 0) return L8_OK;
   const int64_t blocks = (K + 31) / 32;
@@ -598,12 +628,15 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
   hipStream_t st = (hipStream_t)stream;
   L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");
   const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
-  if (big >= num_cus() / 2) {
-    // the stores of the large kernel take eight columns at once, and its stream runs two stages ahead
-    if (blocks > 8 && N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && num_cus() >= 8)
-      return bias ? launch_gemm_mxfp4_stream<true>(a, st) : launch_gemm_mxfp4_stream<false>(a, st);
-    return launch_gemm_mxfp4<2, 2, 8, 8, 2>(a, st);
+  if (takes_stream(M, N, blocks)) {
+    const int64_t need = l8_gemm_mxfp4_workspace(M, N, K);
+    L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "l8_gemm_mxfp4_nt: needs a 16-byte aligned workspace of %lld bytes",
+               (long long)need);
+    // (its stores take eight columns at once, and the groups of rows of its scales are a grid's second dimension)
+    if (N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && (M + 255) / 256 + (N + 255) / 256 < 16384)
+      return bias ? launch_gemm_mxfp4_stream<true>(a, (uint8_t *)workspace, st) : launch_gemm_mxfp4_stream<false>(a, (uint8_t *)workspace, st);
   }
+  if (big >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 8, 8, 2>(a, st);
   if (mid >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 4, 4, 4>(a, st);
   return launch_gemm_mxfp4<2, 2, 2, 2, 8>(a, st);
 }

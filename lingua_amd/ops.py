@@ -984,8 +984,10 @@ def gemm_mxfp4_nt(qa: torch.Tensor, qb: torch.Tensor, sa: torch.Tensor, sb: torc
     elif out.dtype != torch.bfloat16 or out.shape != (M, N) or out.device != qa.device or (out.numel() and (out.stride(1) != 1 or (M > 1 and out.stride(0) < N))):
         raise RuntimeError(f"{what}: out must be bf16 [M,N] with unit column stride on the operands' device")
     with _timed("gemm_mxfp4_nt", 2 * M * N * K, qa.device):
+        ws_bytes = _lib.load().l8_gemm_mxfp4_workspace(M, N, K)   # (it goes by the device's compute units)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=qa.device) if ws_bytes else None
         code = _lib.load().l8_gemm_mxfp4_nt(qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), M, N, K, _ld16(qa), _ld16(sa), _ld16(qb), _ld16(sb),
-                                            bias.data_ptr() if bias is not None else None, out.data_ptr(), _ld(out) if M > 1 else max(N, 1), st)
+                                            bias.data_ptr() if bias is not None else None, out.data_ptr(), _ld(out) if M > 1 else max(N, 1), ws.data_ptr() if ws is not None else None, ws_bytes, st)
     _lib.check(code, "l8_gemm_mxfp4_nt")
     if user_out:
         _wrote_into(out)
