@@ -68,6 +68,8 @@ SIGNATURES = {
     "l8_mxfp4_to_bf16": [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
     "l8_gemm_mxfp4_nt": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p],
     "l8_gemm_mxfp4_workspace": [_i64, _i64, _i64],
+    "l8_mxfp4_linear": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _p],
+    "l8_mxfp4_linear_workspace": [_i64, _i64, _i64],
     "l8_linear_fwd": [ctypes.c_char_p],
     "l8_linear_fwd_workspace": [ctypes.c_char_p],
     "l8_linear_fwd_rows": [ctypes.c_char_p, _i64, _i64],
@@ -81,7 +83,7 @@ SIGNATURES = {
 }
 _RETURNS_STR = {"l8_last_error", "l8_gemm_algo_name"}
 _RETURNS_I64 = {"l8_cast_rowwise_workspace", "l8_gemm_workspace", "l8_gemm_workspace_gave_up_offset", "l8_swiglu_workspace", "l8_rmsnorm_workspace", "l8_rmsnorm_bwd_workspace",
-                "l8_linear_fwd_workspace", "l8_linear_fwd_rows_workspace", "l8_col_sum_workspace", "l8_gemm_mxfp4_workspace"}
+                "l8_linear_fwd_workspace", "l8_linear_fwd_rows_workspace", "l8_col_sum_workspace", "l8_gemm_mxfp4_workspace", "l8_mxfp4_linear_workspace"}
 
 _lib = None
 _native = None    # the host extension, bound to the library's entries

@@ -30,7 +30,8 @@ struct Library {
   X(l8_cast_tensorwise) X(l8_cast_tensorwise_t_rows) X(l8_amax_reduce) X(l8_cast_colwise_transposed_pad) X(l8_cast_transposed_many) X(l8_col_amax) X(l8_col_sum) X(l8_col_sum_workspace) X(l8_gemm_nt) X(l8_linear_bwd_casts_bias) X(l8_linear_bwd_casts_pays)  \
   X(l8_cast_rowwise_many) X(l8_cast_rowwise_cols_many) X(l8_gemm_nt_multi) X(l8_gemm_nt_sum) X(l8_rmsnorm_cast_rowwise)            \
   X(l8_rmsnorm_workspace) X(l8_rmsnorm_bwd_as) X(l8_rmsnorm_bwd_workspace) X(l8_swiglu_cast_rowwise) X(l8_swiglu_workspace)        \
-  X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed)
+  X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed) X(l8_add_rmsnorm_cast_rowwise) X(l8_add_rmsnorm_bwd) X(l8_rotary)     \
+  X(l8_cast_mxfp4) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
   L8_ENTRIES(L8_ENTRY)
 #undef L8_ENTRY
 } lib;
@@ -692,6 +693,315 @@ PyObject *swiglu_bwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// add_rmsnorm_fwd(x, residual, weight, eps, want_q, want_col, want_rstd, on_lines) -> (h, y, q, scale, rstd, col amax) or None
+PyObject *add_rmsnorm_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) throw std::runtime_error("add_rmsnorm_fwd: 8 arguments");
+  if (!tensors(args, 3) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]), &res = THPVariable_Unpack(args[1]), &w = THPVariable_Unpack(args[2]);
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  const bool want_q = truth(args[4]), want_col = truth(args[5]), want_rstd = truth(args[6]), on_lines = truth(args[7]);
+  if (!x.is_cuda() || x.dim() != 2 || res.dim() != 2 || (want_col && !want_q)) Py_RETURN_NONE;
+  const int device = x.get_device();
+  Rows rx, rr;
+  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || rr.rows != rx.rows || rr.cols != rx.cols || c10::hip::current_device() != device) Py_RETURN_NONE;
+  const int64_t R = rx.rows, C = rx.cols;
+  const bool f32 = w.scalar_type() == at::kFloat;
+  if (!dense(w, f32 ? at::kFloat : at::kBFloat16, C, device)) Py_RETURN_NONE;
+  Tensor h, y, q, s, rstd, col;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const auto o = x.options();
+    h = at::empty({R, C}, o), y = at::empty({R, C}, o);
+    if (want_q) q = empty_fp8(R, C, o, on_lines), s = at::empty({R, 1}, o.dtype(at::kFloat));
+    if (want_rstd) rstd = at::empty({R, 1}, o.dtype(at::kFloat));
+    if (want_col) col = at::empty({C}, o.dtype(at::kFloat));
+    const int64_t ws_bytes = want_col ? lib.l8_rmsnorm_workspace(R, C) : 0;
+    const Space ws(x, ws_bytes);
+    check(lib.l8_add_rmsnorm_cast_rowwise(rx.p, rr.p, w.const_data_ptr(), f32, R, C, rx.ld, rr.ld, (float)eps, h.mutable_data_ptr(), C, y.mutable_data_ptr(), C,
+                                          want_q ? q.mutable_data_ptr() : nullptr, want_q ? q.stride(0) : C, want_q ? s.mutable_data_ptr<float>() : nullptr,
+                                          want_rstd ? rstd.mutable_data_ptr<float>() : nullptr, want_col ? col.mutable_data_ptr<float>() : nullptr, ws.p(), ws_bytes,
+                                          stream_of(device)), "l8_add_rmsnorm_cast_rowwise");
+  }
+  return tuple_of({h, y, q, s, rstd, col});
+  END_HANDLE_TH_ERRORS
+}
+
+// add_rmsnorm_bwd(gy, gh, h, weight, rstd) -> (gx, gw of the weight's type) or None
+PyObject *add_rmsnorm_bwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) throw std::runtime_error("add_rmsnorm_bwd: 5 arguments");
+  if (!tensors(args, 5)) Py_RETURN_NONE;
+  for (int i = 0; i < 5; ++i)
+    if (args[i] == Py_None) Py_RETURN_NONE;
+  const Tensor &gy = THPVariable_Unpack(args[0]), &gh = THPVariable_Unpack(args[1]), &h = THPVariable_Unpack(args[2]), &w = THPVariable_Unpack(args[3]),
+               &rstd = THPVariable_Unpack(args[4]);
+  if (!h.is_cuda()) Py_RETURN_NONE;
+  const int device = h.get_device();
+  Rows rg, ru, rh;
+  if (!as_rows(gy, device, rg) || !as_rows(gh, device, ru) || !as_rows(h, device, rh) || rg.rows != rh.rows || rg.cols != rh.cols || ru.rows != rh.rows ||
+      ru.cols != rh.cols || c10::hip::current_device() != device)
+    Py_RETURN_NONE;
+  const int64_t R = rh.rows, C = rh.cols;
+  const bool f32 = w.scalar_type() == at::kFloat;
+  if (!dense(w, f32 ? at::kFloat : at::kBFloat16, C, device) || !dense(rstd, at::kFloat, R, device)) Py_RETURN_NONE;
+  Tensor gx, gw;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const auto o = h.options();
+    gx = at::empty({R, C}, o), gw = at::empty({C}, w.options());
+    const int64_t ws_bytes = lib.l8_rmsnorm_bwd_workspace(R, C);
+    const Space ws(h, ws_bytes);
+    check(lib.l8_add_rmsnorm_bwd(rg.p, ru.p, rh.p, w.const_data_ptr(), f32, rstd.const_data_ptr<float>(), R, C, rg.ld, ru.ld, rh.ld, gx.mutable_data_ptr(), C,
+                                 gw.mutable_data_ptr(), f32, ws.p(), ws_bytes, stream_of(device)), "l8_add_rmsnorm_bwd");
+  }
+  return tuple_of({gx, gw});
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary(xq, xk, cos, sin, positions, in_halves, inverse) -> (yq, yk) or None; either of xq and xk may be None
+PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 7) throw std::runtime_error("rotary: 7 arguments");
+  if (!tensors(args, 5) || (args[0] == Py_None && args[1] == Py_None) || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
+  const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
+  const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]), &one = x[0].defined() ? x[0] : x[1];
+  const bool in_halves = truth(args[5]), inverse = truth(args[6]);
+  if (!one.is_cuda() || one.dim() != 4) Py_RETURN_NONE;
+  const int device = one.get_device();
+  const int64_t B = one.size(0), S = one.size(1), D = one.size(3);
+  if (c10::hip::current_device() != device) Py_RETURN_NONE;
+  for (const Tensor &t : x)
+    if (t.defined() && (t.scalar_type() != at::kBFloat16 || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || t.dim() != 4 || t.numel() < 1 ||
+                        t.size(0) != B || t.size(1) != S || t.size(3) != D || t.stride(3) != 1))
+      Py_RETURN_NONE;
+  for (const Tensor *t : {&cos, &sin})
+    if (t->scalar_type() != at::kFloat || t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device || t->dim() != 2 || t->sizes() != cos.sizes() ||
+        t->strides() != cos.strides())
+      Py_RETURN_NONE;
+  const int64_t P = cos.size(0), rot = 2 * cos.size(1);
+  if (rot < 2 || rot > D || (!pos.defined() && S > P)) Py_RETURN_NONE;
+  int64_t pos_b = 0, pos_s = 0;
+  if (pos.defined()) {   // [S], [1,S], [B,1] or [B,S]
+    if ((pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || pos.layout() != at::kStrided || !pos.is_cuda() || pos.get_device() != device ||
+        pos.dim() < 1 || pos.dim() > 2)
+      Py_RETURN_NONE;
+    const int64_t ps = pos.size(-1), pb = pos.dim() == 2 ? pos.size(0) : 1;
+    if ((ps != S && ps != 1) || (pb != B && pb != 1)) Py_RETURN_NONE;
+    pos_s = ps == 1 ? 0 : pos.stride(-1);
+    pos_b = pb == 1 ? 0 : pos.stride(0);
+  }
+  Tensor y[2];
+  {
+    pybind11::gil_scoped_release no_gil;
+    l8_rotary_operand two[2];
+    for (int i = 0; i < 2; ++i) {
+      two[i] = {nullptr, nullptr, 0, 0, 0, 0};
+      if (!x[i].defined()) continue;
+      y[i] = at::empty(x[i].sizes(), x[i].options());
+      two[i] = {x[i].const_data_ptr(), y[i].mutable_data_ptr(), x[i].size(2), x[i].stride(0), x[i].stride(1), x[i].stride(2)};
+    }
+    check(lib.l8_rotary(two, B, S, D, rot, in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), P,
+                        pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kInt, pos_b, pos_s, stream_of(device)), "l8_rotary");
+  }
+  return tuple_of({y[0], y[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// One MXFP4 copy: rows of codes and of scales, as lingua_amd.ops lays them out.
+struct Mx {
+  Tensor q, s;
+  Mx() {}
+  Mx(int64_t rows, int64_t cols, const at::TensorOptions &o, bool on_lines) {
+    const int64_t blocks = (cols + 31) / 32, bytes = blocks * 16, padded = (bytes + 127) / 128 * 128;
+    q = at::empty_strided({rows, bytes}, {on_lines && (padded - bytes) * 8 <= bytes ? padded : bytes, 1}, o.dtype(at::kFloat4_e2m1fn_x2));
+    s = at::empty_strided({rows, blocks}, {(blocks + 15) / 16 * 16, 1}, o.dtype(at::kFloat8_e8m0fnu));
+  }
+  void *qp() const { return q.defined() ? q.mutable_data_ptr() : nullptr; }
+  void *sp() const { return s.defined() ? s.mutable_data_ptr() : nullptr; }
+  int64_t ldq() const { return q.defined() ? q.stride(0) : 0; }
+  int64_t lds() const { return s.defined() ? s.stride(0) : 0; }
+};
+// One that is handed in: 16 bytes and a scale per block, each row dense.
+struct MxRows {
+  const void *q = nullptr, *s = nullptr;
+  int64_t rows = 0, blocks = 0, ldq = 0, lds = 0;
+};
+bool as_mx(const Tensor &q, const Tensor &s, int device, MxRows &m) {
+  if (!q.defined() || !s.defined() || (q.scalar_type() != at::kFloat4_e2m1fn_x2 && q.scalar_type() != at::kByte) ||
+      (s.scalar_type() != at::kFloat8_e8m0fnu && s.scalar_type() != at::kByte) || q.layout() != at::kStrided || s.layout() != at::kStrided || !q.is_cuda() ||
+      !s.is_cuda() || q.get_device() != device || s.get_device() != device || q.dim() != 2 || s.dim() != 2)
+    return false;
+  m.rows = q.size(0), m.blocks = s.size(1);
+  if (m.rows < 1 || m.blocks < 1 || s.size(0) != m.rows || q.size(1) != 16 * m.blocks || q.stride(1) != 1 || s.stride(1) != 1) return false;
+  m.ldq = m.rows > 1 ? q.stride(0) : 16 * m.blocks;
+  m.lds = m.rows > 1 ? s.stride(0) : (m.blocks + 15) / 16 * 16;
+  m.q = q.const_data_ptr(), m.s = s.const_data_ptr();
+  return m.ldq >= 16 * m.blocks && m.ldq % 16 == 0 && m.lds >= m.blocks && ((uintptr_t)m.q % 16) == 0;
+}
+bool on_16_bytes(const Rows &m) { return ((uintptr_t)m.p % 16) == 0 && m.ld % 8 == 0 && m.cols % 8 == 0; }
+void cast_mx(const Rows &x, const Mx &rows, const Mx &cols, void *stream) {
+  check(lib.l8_cast_mxfp4(x.p, x.rows, x.cols, x.ld, rows.qp(), rows.ldq(), rows.sp(), rows.lds(), cols.qp(), cols.ldq(), cols.sp(), cols.lds(), stream), "l8_cast_mxfp4");
+}
+void gemm_mx(const MxRows &a, const MxRows &b, const Tensor &bias, const Tensor &out, void *stream) {
+  const int64_t K = a.blocks * 32, bytes = lib.l8_gemm_mxfp4_workspace(a.rows, b.rows, K);
+  const Space ws(out, bytes);
+  check(lib.l8_gemm_mxfp4_nt(a.q, a.s, b.q, b.s, a.rows, b.rows, K, a.ldq, a.lds, b.ldq, b.lds, bias.defined() ? bias.const_data_ptr() : nullptr, out.mutable_data_ptr(),
+                             b.rows, ws.p(), bytes, stream), "l8_gemm_mxfp4_nt");
+}
+MxRows rows_of(const Mx &m) {
+  MxRows r;
+  as_mx(m.q, m.s, m.q.get_device(), r);
+  return r;
+}
+
+// cast_mxfp4(x, rowwise, transposed, on_lines) -> (q, s, qt, st) or None
+PyObject *cast_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) throw std::runtime_error("cast_mxfp4: 4 arguments");
+  if (!tensors(args, 1) || args[0] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]);
+  const bool rowwise = truth(args[1]), transposed = truth(args[2]), on_lines = truth(args[3]);
+  if (!x.is_cuda() || x.dim() != 2 || (!rowwise && !transposed)) Py_RETURN_NONE;
+  const int device = x.get_device();
+  Rows rx;
+  if (!as_rows(x, device, rx) || c10::hip::current_device() != device) Py_RETURN_NONE;
+  Mx rows, cols;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (rowwise) rows = Mx(rx.rows, rx.cols, x.options(), on_lines);
+    if (transposed) cols = Mx(rx.cols, rx.rows, x.options(), on_lines);
+    cast_mx(rx, rows, cols, stream_of(device));
+  }
+  return tuple_of({rows.q, rows.s, cols.q, cols.s});
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_to_bf16(q, s, cols) -> y or None
+PyObject *mxfp4_to_bf16(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3) throw std::runtime_error("mxfp4_to_bf16: 3 arguments");
+  if (!tensors(args, 2) || args[0] == Py_None || args[1] == Py_None) Py_RETURN_NONE;
+  const Tensor &q = THPVariable_Unpack(args[0]), &s = THPVariable_Unpack(args[1]);
+  const int64_t cols = PyLong_AsLongLong(args[2]);
+  if (cols == -1 && PyErr_Occurred()) throw python_error();
+  if (!q.is_cuda()) Py_RETURN_NONE;
+  const int device = q.get_device();
+  MxRows m;
+  if (!as_mx(q, s, device, m) || cols < 1 || cols > 32 * m.blocks || c10::hip::current_device() != device) Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    y = at::empty({m.rows, cols}, q.options().dtype(at::kBFloat16));
+    check(lib.l8_mxfp4_to_bf16(m.q, m.ldq, m.s, m.lds, m.rows, cols, y.mutable_data_ptr(), cols, stream_of(device)), "l8_mxfp4_to_bf16");
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_linear(x, qw, sw, bias) -> y or None: the product with a weight kept in MXFP4
+PyObject *mxfp4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) throw std::runtime_error("mxfp4_linear: 4 arguments");
+  if (!tensors(args, 4) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]), &qw = THPVariable_Unpack(args[1]), &sw = THPVariable_Unpack(args[2]);
+  const Tensor bias = arg(args[3]);
+  if (!x.is_cuda() || x.dim() != 2) Py_RETURN_NONE;
+  const int device = x.get_device();
+  Rows rx;
+  MxRows w;
+  if (!as_rows(x, device, rx) || !on_16_bytes(rx) || !as_mx(qw, sw, device, w) || (rx.cols + 31) / 32 != w.blocks || c10::hip::current_device() != device ||
+      (rx.rows > 64 && (w.lds % 16 || ((uintptr_t)w.s % 16))) || (bias.defined() && !dense(bias, at::kBFloat16, w.rows, device)))
+    Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    y = at::empty({rx.rows, w.rows}, x.options());
+    const int64_t bytes = lib.l8_mxfp4_linear_workspace(rx.rows, w.rows, rx.cols);
+    const Space ws(x, bytes);
+    check(lib.l8_mxfp4_linear(rx.p, rx.rows, rx.cols, rx.ld, w.q, w.ldq, w.s, w.lds, w.rows, bias.defined() ? bias.const_data_ptr() : nullptr, y.mutable_data_ptr(), w.rows,
+                              ws.p(), bytes, stream_of(device)), "l8_mxfp4_linear");
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_fwd(a, w, bias, need_a, need_w) -> (y, qat, sat, qwt, swt) or None: the transposed copies that the gradients multiply with
+PyObject *mxfp4_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) throw std::runtime_error("mxfp4_fwd: 5 arguments");
+  if (!tensors(args, 3) || args[0] == Py_None || args[1] == Py_None) Py_RETURN_NONE;
+  const Tensor &a = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+  const Tensor bias = arg(args[2]);
+  const bool need_a = truth(args[3]), need_w = truth(args[4]);
+  if (!a.is_cuda() || a.dim() != 2 || w.dim() != 2) Py_RETURN_NONE;
+  const int device = a.get_device();
+  Rows ra, rw;
+  if (!as_rows(a, device, ra) || !as_rows(w, device, rw) || ra.cols != rw.cols || c10::hip::current_device() != device ||
+      (bias.defined() && !dense(bias, at::kBFloat16, rw.rows, device)))
+    Py_RETURN_NONE;
+  Tensor y;
+  Mx at, wt;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const auto o = a.options();
+    void *stream = stream_of(device);
+    const Mx qa(ra.rows, ra.cols, o, true), qw(rw.rows, rw.cols, o, true);
+    if (need_w) at = Mx(ra.cols, ra.rows, o, true);
+    if (need_a) wt = Mx(rw.cols, rw.rows, o, true);
+    cast_mx(ra, qa, at, stream);
+    cast_mx(rw, qw, wt, stream);
+    y = at::empty({ra.rows, rw.rows}, o);
+    gemm_mx(rows_of(qa), rows_of(qw), bias, y, stream);
+  }
+  return tuple_of({y, at.q, at.s, wt.q, wt.s});
+  END_HANDLE_TH_ERRORS
+}
+
+// mxfp4_bwd(gy, qat, sat, qwt, swt, need_bias) -> (ga, gw, gbias) or None; a copy that is None: its gradient is not wanted
+PyObject *mxfp4_bwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) throw std::runtime_error("mxfp4_bwd: 6 arguments");
+  if (!tensors(args, 5) || args[0] == Py_None) Py_RETURN_NONE;
+  const Tensor &gy = THPVariable_Unpack(args[0]);
+  const Tensor qat = arg(args[1]), sat = arg(args[2]), qwt = arg(args[3]), swt = arg(args[4]);
+  const bool need_bias = truth(args[5]);
+  if (!gy.is_cuda() || gy.dim() != 2) Py_RETURN_NONE;
+  const int device = gy.get_device();
+  Rows rg;
+  MxRows a, w;
+  if (!as_rows(gy, device, rg) || !on_16_bytes(rg) || c10::hip::current_device() != device || (qat.defined() && (!as_mx(qat, sat, device, a) || a.blocks != (rg.rows + 31) / 32)) ||
+      (qwt.defined() && (!as_mx(qwt, swt, device, w) || w.blocks != (rg.cols + 31) / 32)))
+    Py_RETURN_NONE;
+  Tensor ga, gw, gbias;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const auto o = gy.options();
+    void *stream = stream_of(device);
+    Mx rows, cols;
+    if (w.q) rows = Mx(rg.rows, rg.cols, o, true);
+    if (a.q) cols = Mx(rg.cols, rg.rows, o, true);
+    if (w.q || a.q) cast_mx(rg, rows, cols, stream);
+    if (w.q) {
+      ga = at::empty({rg.rows, w.rows}, o);
+      gemm_mx(rows_of(rows), w, Tensor(), ga, stream);
+    }
+    if (a.q) {
+      gw = at::empty({rg.cols, a.rows}, o);
+      gemm_mx(rows_of(cols), a, Tensor(), gw, stream);
+    }
+    if (need_bias) {
+      gbias = at::empty({rg.cols}, o);
+      const int64_t bytes = lib.l8_col_sum_workspace(rg.rows, rg.cols);
+      const Space ws(gy, bytes);
+      check(lib.l8_col_sum(rg.p, rg.rows, rg.cols, rg.ld, gbias.mutable_data_ptr(), ws.p(), bytes, stream), "l8_col_sum");
+    }
+  }
+  return tuple_of({ga, gw, gbias});
+  END_HANDLE_TH_ERRORS
+}
+
 // key(tensor) -> bytes: equal for two tensors of the same memory, shape, strides, type, device and version, seen from the
 // same current stream.
 PyObject *key(PyObject *, PyObject *o) {
@@ -737,6 +1047,14 @@ PyMethodDef methods[] = {
     {"shared_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(shared_bwd)), METH_FASTCALL, nullptr},
     {"swiglu_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(swiglu_fwd)), METH_FASTCALL, nullptr},
     {"swiglu_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(swiglu_bwd)), METH_FASTCALL, nullptr},
+    {"add_rmsnorm_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm_fwd)), METH_FASTCALL, nullptr},
+    {"add_rmsnorm_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm_bwd)), METH_FASTCALL, nullptr},
+    {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
+    {"cast_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cast_mxfp4)), METH_FASTCALL, nullptr},
+    {"mxfp4_to_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_to_bf16)), METH_FASTCALL, nullptr},
+    {"mxfp4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_linear)), METH_FASTCALL, nullptr},
+    {"mxfp4_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_fwd)), METH_FASTCALL, nullptr},
+    {"mxfp4_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_bwd)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

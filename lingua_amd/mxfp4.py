@@ -21,8 +21,8 @@ from typing import Optional
 
 import torch
 
+from . import _lib, ops
 from . import float8 as f8
-from . import ops
 
 
 def _check_operands(a, w):
@@ -42,9 +42,13 @@ class Mxfp4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, w, bias):
         need_a, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        if ops.kernel_timer is None:
+            res = _lib.native_for(a.get_device()).mxfp4_fwd(a, w, bias, need_a, need_w)
+            if res is not None:
+                ctx.save_for_backward(*res[1:])
+                return res[0]
         (qa, sa), at = ops.cast_mxfp4(a, transposed=need_w, on_lines=True)
         (qw, sw), wt = ops.cast_mxfp4(w, transposed=need_a, on_lines=True)
-        ctx.rows = a.shape[0]
         ctx.save_for_backward(*(at or (None, None)), *(wt or (None, None)))
         return ops.gemm_mxfp4_nt(qa, qw, sa, sw, bias)
 
@@ -55,6 +59,10 @@ class Mxfp4LinearFn(torch.autograd.Function):
             raise RuntimeError(f"mxfp4_linear backward: bf16 grad_out required, got {gy.dtype}")
         qat, sat, qwt, swt = ctx.saved_tensors
         need_a, need_w, need_bias = ctx.needs_input_grad
+        if ops.kernel_timer is None:
+            res = _lib.native_for(gy.get_device()).mxfp4_bwd(gy, qat, sat, qwt, swt, need_bias)
+            if res is not None:
+                return res
         ga = gw = gbias = None
         if need_a or need_w:
             rows, cols = ops.cast_mxfp4(gy, rowwise=need_a, transposed=need_w, on_lines=True)

@@ -66,8 +66,13 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
             raise RuntimeError(f"add_rmsnorm: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
         want_col = bool(training and f8.config.fp8_wgrad)
         x2d, r2d = x.flatten(end_dim=-2), residual.flatten(end_dim=-2)
-        col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
-        h2d, y2d, q, s, rstd = ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True)
+        res = None
+        if f8._native_call(x2d, 0):
+            res = _lib.native_for(x2d.get_device()).add_rmsnorm_fwd(x2d, r2d, weight, eps, True, want_col, True, True)
+        if res is None:
+            col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
+            res = (*ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True), col)
+        h2d, y2d, q, s, rstd, col = res
         if f8.config.share_input_casts:
             f8._fwd_cast.put(y2d, (q, s, col), "rmsnorm")
         ctx.set_materialize_grads(False)
@@ -89,7 +94,10 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
             if gh is None:
                 gx2d, gw = ops.rmsnorm_bwd(gy2d, h2d, weight, rstd, gw_dtype=weight.dtype)
             else:
-                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh.flatten(end_dim=-2), h2d, weight, rstd, gw_dtype=weight.dtype)
+                gh2d, res = gh.flatten(end_dim=-2), None
+                if f8._native_call(gy2d, 0):
+                    res = _lib.native_for(gy2d.get_device()).add_rmsnorm_bwd(gy2d, gh2d, h2d, weight, rstd)
+                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh2d, h2d, weight, rstd, gw_dtype=weight.dtype) if res is None else res
             gx = gx2d.reshape(ctx.x_shape)
         need = ctx.needs_input_grad
         return gx if need[0] else None, gx if need[1] else None, gw if need[2] else None, None, None

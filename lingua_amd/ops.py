@@ -770,6 +770,10 @@ def add_rmsnorm_cast_rowwise(x: torch.Tensor, residual: torch.Tensor, weight: to
     """h = bf16(x + residual) and ``rmsnorm_cast_rowwise`` of it in one pass.
     Returns (h [R,C] bf16, y [R,C] bf16, q [R,C] fp8 | None, scale [R,1] fp32 | None, rstd [R,1] fp32 | None)."""
     what = "add_rmsnorm_cast_rowwise"
+    if kernel_timer is None and x.is_cuda and col_amax is None:   # the same in one call, for operands that need no copies
+        res = _lib.native_for(x.get_device()).add_rmsnorm_fwd(x, residual, weight, eps, want_q, False, want_rstd, on_lines)
+        if res is not None:
+            return res[:5]
     x = _rows_2d(x, torch.bfloat16, what)
     residual = _rows_2d(residual, torch.bfloat16, what)
     if x.shape != residual.shape or x.device != residual.device:
@@ -834,6 +838,10 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
     cos, sin (fp32 [P, rot / 2]); positions int32 or int64, broadcastable to [B,S] (None: 0 .. S - 1).  ``inverse``: the transposed
     rotation.  Returns dense tensors of the same shapes.  A token at a position outside [0, P) becomes NaN."""
     what = "rotary"
+    if kernel_timer is None and cos.is_cuda:   # the same in one call, for operands that need no copies
+        res = _lib.native_for(cos.get_device()).rotary(xq, xk, cos, sin, positions, in_halves, inverse)
+        if res is not None:
+            return res
     xs = [t for t in (xq, xk) if t is not None]
     if not xs:
         raise RuntimeError(f"{what}: xq or xk is needed")
@@ -886,6 +894,7 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
 # ---- MXFP4: e2m1 codes, two a byte, in blocks of 32 along a row, with an e8m0 scale each ----
 
 MX_BLOCK = 32
+_MX_FEW_TOKENS = 64    # up to here a product reads rows of scales wherever they start
 
 
 def _empty_mxfp4(rows: int, cols: int, device, on_lines: bool):
@@ -926,6 +935,10 @@ def cast_mxfp4(x: torch.Tensor, rowwise: bool = True, transposed: bool = False, 
     """x [R,C] bf16 in MXFP4, blocks of 32 along its rows and / or along its columns (the copy of x.t()), from one read.
     Returns ((codes [R, 16 * ceil(C / 32)] float4_e2m1fn_x2, scales [R, ceil(C / 32)] float8_e8m0fnu) | None, the same of x.t() | None).
     Codes behind the last column are zeros.  ``on_lines``: codes have their rows on 128-byte lines where that adds little."""
+    if kernel_timer is None and x.is_cuda:   # the same in one call, for operands that need no copies
+        res = _lib.native_for(x.get_device()).cast_mxfp4(x, rowwise, transposed, on_lines)
+        if res is not None:
+            return res[:2] if rowwise else None, res[2:] if transposed else None
     x = _rows_2d(x, torch.bfloat16, "cast_mxfp4")
     st = _prep(x, "cast_mxfp4")
     if not rowwise and not transposed:
@@ -944,6 +957,10 @@ def cast_mxfp4(x: torch.Tensor, rowwise: bool = True, transposed: bool = False, 
 
 def mxfp4_to_bf16(q: torch.Tensor, s: torch.Tensor, cols: int) -> torch.Tensor:
     """bf16 [R, cols] values of MXFP4 codes and scales as ``cast_mxfp4`` makes them (or the same as uint8)."""
+    if kernel_timer is None and q.is_cuda:
+        y = _lib.native_for(q.get_device()).mxfp4_to_bf16(q, s, cols)
+        if y is not None:
+            return y
     q, s = _mx_operand(q, s, "mxfp4_to_bf16")
     st = _prep(q, "mxfp4_to_bf16")
     if not 0 <= cols <= MX_BLOCK * s.shape[1]:
@@ -996,9 +1013,31 @@ def gemm_mxfp4_nt(qa: torch.Tensor, qb: torch.Tensor, sa: torch.Tensor, sb: torc
 
 def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16 [M,N]: x [M,K] bf16 quantised along its rows times a weight kept in MXFP4 (codes [N, 16 * ceil(K / 32)] and scales), plus
-    bias."""
-    x = _rows_2d(x, torch.bfloat16, "mxfp4_linear_fwd")
-    if sw.dim() != 2 or (x.shape[1] + MX_BLOCK - 1) // MX_BLOCK != sw.shape[1]:
-        raise RuntimeError(f"mxfp4_linear_fwd: x {tuple(x.shape)} and a weight of scales {tuple(sw.shape)} do not fit")
-    (qx, sx), _ = cast_mxfp4(x, on_lines=True)
-    return gemm_mxfp4_nt(qx, qw, sx, sw, bias)
+    bias; one launch up to 16 tokens."""
+    what = "mxfp4_linear_fwd"
+    if kernel_timer is None and x.is_cuda:   # the same in one call, for operands that need no copies
+        y = _lib.native_for(x.get_device()).mxfp4_linear(x, qw, sw, bias)
+        if y is not None:
+            return y
+    x = _rows_2d(x, torch.bfloat16, what)
+    qw, sw = _mx_operand(qw, sw, what)
+    st = _prep(x, what)
+    M, K = x.shape
+    N = qw.shape[0]
+    if (K + MX_BLOCK - 1) // MX_BLOCK != sw.shape[1] or qw.device != x.device:
+        raise RuntimeError(f"{what}: x {tuple(x.shape)} on {x.device} and a weight of scales {tuple(sw.shape)} on {qw.device} do not fit")
+    bias = _mx_bias(bias, N, x.device, what)
+    if not rows_on_16_bytes(x):
+        x = x.clone(memory_format=torch.contiguous_format)
+    qw = _on_16_bytes(qw)
+    if M > _MX_FEW_TOKENS:
+        sw = _on_16_bytes(sw)
+    y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
+    with _timed("mxfp4_linear_fwd", 2 * M * N * K, x.device):
+        ws_bytes = _lib.load().l8_mxfp4_linear_workspace(M, N, K)   # (it goes by the device's compute units)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
+        code = _lib.load().l8_mxfp4_linear(x.data_ptr(), M, K, _ld(x), qw.data_ptr(), _ld16(qw), sw.data_ptr(), _ld(sw) if M <= _MX_FEW_TOKENS else _ld16(sw), N,
+                                           bias.data_ptr() if bias is not None else None, y.data_ptr(), max(N, 1), ws.data_ptr() if ws is not None else None,
+                                           ws_bytes, st)
+    _lib.check(code, "l8_mxfp4_linear")
+    return y
