@@ -7,7 +7,8 @@
 //
 // Structure
 //   * a stage is 128 bytes (256 codes, 8 blocks) of every row of the tile's operands, two matrix instructions deep; lane group g of
-//     the four takes blocks 2 g and 2 g + 1 of a stage, so that its two scale bytes lie side by side;
+//     the four takes blocks 2 g and 2 g + 1 of a stage, so that its two scale bytes lie side by side.  One half of a stage is multiplied
+//     while the next half's fragments are read;
 //   * codes go from memory to LDS without passing registers (buffer loads to LDS, whole 128-byte lines), into a ring of NS stages;
 //     scales of two stages (16 bytes a row) travel the same way into a ring of their own;
 //   * LDS rows are 128 bytes in 16-byte chunks, chunk c of row r at position c ^ f(r), f(r) = (r & 7) ^ ((r >> 3) & 1): the
@@ -42,6 +43,12 @@ struct MxGemmArgs {
 #define MX_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (0x7 << 4) | (0xF << 8) | ((((n) >> 4) & 0x3) << 14))
 #define MX_WAIT_LGKM0() __builtin_amdgcn_s_waitcnt(0xF | (0x7 << 4) | (0x0 << 8) | (0x3 << 14))
 
+// f(0), f(1), .. as straight code, each with its number as a constant
+template <typename F, int... I>
+L8_DEV void in_turn(std::integer_sequence<int, I...>, F &&f) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+
 template <int WM, int WN, int TM, int TN, int NS>
 __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -49,7 +56,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   constexpr int NLA = BM / 8 / NW, NLB = BN / 8 / NW;           // wave loads (8 rows) of a stage
   constexpr int STAGE = (BM + BN) * 128, SROWS = BM + BN, SLOADS = SROWS / 64, NSW = NS / 2 + 1;
   static_assert(NS % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && SROWS % 64 == 0 && BM % 64 == 0, "");
-  static_assert((NS - 1) * (NLA + NLB) <= 63, "vmcnt is a 6-bit counter");
+  static_assert((NS - 2) * (NLA + NLB) <= 63 && (NS - 1) * (NLA + NLB) + NS <= 63, "vmcnt is a 6-bit counter");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // NS stages, NSW windows of scales
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -80,22 +87,18 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   const int a_row = lrow * (int)p.lda, b_row = lrow * TN * (int)p.ldb;
   // row of B (in the tile) that LDS row r of its panel holds
   auto b_of = [](int r) { return r / (TN * 16) * (TN * 16) + TN * (r % 16) + r % (TN * 16) / 16; };
-  auto load_stage = [&](int j, int slot) {
+  // i-th wave load of stage j's panels into ring slot `slot`
+  auto load_one = [&](int j, int slot, int i) __attribute__((always_inline)) {
     const int k0 = j * 128;
-    const uint32_t off[2] = {(k0 + chunk[0] < kbytes) ? 0u : kBeyond, (k0 + chunk[1] < kbytes) ? 0u : kBeyond};
     const uint32_t dst = lds0 + slot * STAGE;
-#pragma unroll
-    for (int i = 0; i < NLA; ++i) {
-      const int g = wave * NLA + i;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, reinterpret_cast<lds_void_ptr>(dst + g * 1024), 16, (uint32_t)(a_row + chunk[g & 1]) | off[g & 1],
+    const int g = i < NLA ? wave * NLA + i : wave * NLB + i - NLA;
+    const uint32_t off = (k0 + chunk[g & 1] < kbytes) ? 0u : kBeyond;
+    if (i < NLA)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsA, reinterpret_cast<lds_void_ptr>(dst + g * 1024), 16, (uint32_t)(a_row + chunk[g & 1]) | off,
                                                k0 + g * 8 * (int)p.lda, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < NLB; ++i) {
-      const int g = wave * NLB + i;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, reinterpret_cast<lds_void_ptr>(dst + BM * 128 + g * 1024), 16, (uint32_t)(b_row + chunk[g & 1]) | off[g & 1],
+    else
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsB, reinterpret_cast<lds_void_ptr>(dst + BM * 128 + g * 1024), 16, (uint32_t)(b_row + chunk[g & 1]) | off,
                                                k0 + b_of(g * 8) * (int)p.ldb, 0, 0);
-    }
   };
   auto load_scales = [&](int w) {
     const uint32_t dst = lds0 + NS * STAGE + (w % NSW) * (SROWS * 16);
@@ -119,7 +122,8 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
 #pragma unroll
   for (int j = 0; j < NS; ++j) {
     if (j % 2 == 0) load_scales(j / 2);
-    load_stage(j, j);
+#pragma unroll
+    for (int i = 0; i < NLA + NLB; ++i) load_one(j, j, i);
   }
   const int frow = lane & 15, fg = lane >> 4;
   const int fr = (frow & 7) ^ (frow >> 3);
@@ -127,47 +131,90 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   typedef const __attribute__((address_space(3))) v4i *lds_v4i;
   typedef const __attribute__((address_space(3))) uint16_t *lds_u16;
 
-  for (int j = 0; j < stages; ++j) {
-    const int slot = j % NS;
-    MX_WAIT_VM((NS - 1) * (NLA + NLB));
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    uint32_t base = lds0 + slot * STAGE, sbase = lds0 + NS * STAGE + ((j >> 1) % NSW) * (SROWS * 16) + frow * 16 + (j & 1) * 8 + fg * 2;
-    asm volatile("" : "+v"(base), "+v"(sbase));
+  // Fragments of a stage's two halves of 128 codes (h: blocks 2 g + h), and scales of two stages, a byte for each half.
+  v4i fa[2][TM], fb[2][TN];
+  uint32_t sa[2][TM], sb[2][TN];
+  uint32_t at, sat, smask;   // of the stage that is read next
+  auto open = [&](int j) __attribute__((always_inline)) {
+    at = lds0 + (j % NS) * STAGE;
+    sat = lds0 + NS * STAGE + ((j >> 1) % NSW) * (SROWS * 16) + frow * 16 + (j & 1) * 8 + fg * 2;
+    asm volatile("" : "+v"(at), "+v"(sat));
     const int left = p.blocks - (j * 8 + fg * 2);
-    const uint32_t smask = left >= 2 ? 0xffffu : (left == 1 ? 0xffu : 0u);
-    v4i a[TM][2], b[TN][2];
-    uint32_t as[TM], bs[TN];
+    smask = left >= 2 ? 0xffffu : (left == 1 ? 0xffu : 0u);
+  };
+  auto read_frag = [&](int h, int r) __attribute__((always_inline)) {   // B0, A0, B1, .. in the order of their use
+    auto of_b = [&](int t) __attribute__((always_inline)) { fb[h][t] = *reinterpret_cast<lds_v4i>(at + BM * 128 + (wn * TN + t) * 2048 + foff[h]); };
+    auto of_a = [&](int t) __attribute__((always_inline)) { fa[h][t] = *reinterpret_cast<lds_v4i>(at + (wm * TM + t) * 2048 + foff[h]); };
+    if (r == 0) of_b(0);
+    else if (r == 1) of_a(0);
+    else if (r <= TN) of_b(r - 1);
+    else of_a(r - TN);
+  };
+  auto read_scale = [&](int to, int r) __attribute__((always_inline)) {
+    if (r < TN) sb[to][r] = *reinterpret_cast<lds_u16>(sat + (BM + (wn * TN + r) * 16) * 16);
+    else sa[to][r - TN] = *reinterpret_cast<lds_u16>(sat + (wm * TM + r - TN) * 256);
+  };
+  auto mask_scales = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < TN; ++t) {
+    for (int t = 0; t < TM; ++t) sa[to][t] &= smask;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) b[t][h] = *reinterpret_cast<lds_v4i>(base + BM * 128 + (wn * TN + t) * 2048 + foff[h]);
-      bs[t] = *reinterpret_cast<lds_u16>(sbase + (BM + (wn * TN + t) * 16) * 16) & smask;
-    }
+    for (int t = 0; t < TN; ++t) sb[to][t] &= smask;
+  };
+  constexpr int N_MMA = TM * TN, N_RD = TM + TN;
+  auto mma_one = [&](auto half, int cur, int i) __attribute__((always_inline)) {
+    constexpr int h = decltype(half)::value;
+    const v4i x = fa[h][i / TN], y = fb[h][i % TN];
+    const v8i a = {x[0], x[1], x[2], x[3], 0, 0, 0, 0}, b = {y[0], y[1], y[2], y[3], 0, 0, 0, 0};
+    acc[i / TN][i % TN] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i / TN][i % TN], 4, 4, h, (int)sa[cur][i / TN], h, (int)sb[cur][i % TN]);
+  };
+  constexpr std::integral_constant<int, 0> lower{};
+  constexpr std::integral_constant<int, 1> upper{};
+  // One stage.  Its lower half is multiplied while its upper half is read; at the barrier every wave has read all of it and the next
+  // stage has landed; its upper half is multiplied while the next stage's lower half and scales are read and the stage NS further on
+  // is requested into the slot that has become free.
+  auto trip = [&](int j, auto parity) __attribute__((always_inline)) {
+    constexpr int cur = decltype(parity)::value;
+    in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
+      constexpr int i = decltype(number)::value;
+      mma_one(lower, cur, i);
 #pragma unroll
-    for (int t = 0; t < TM; ++t) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) a[t][h] = *reinterpret_cast<lds_v4i>(base + (wm * TM + t) * 2048 + foff[h]);
-      as[t] = *reinterpret_cast<lds_u16>(sbase + (wm * TM + t) * 256) & smask;
-    }
-    MX_WAIT_LGKM0();
+      for (int r = (N_RD * i) / N_MMA; r < (N_RD * (i + 1)) / N_MMA; ++r) read_frag(1, r);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    __builtin_amdgcn_s_waitcnt((((NS - 2) * (NLA + NLB)) & 0xF) | (0x7 << 4) | ((((NS - 2) * (NLA + NLB)) >> 4) << 14));
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if ((j & 1) == 0) load_scales((j + NS) / 2);
-    load_stage(j + NS, slot);
+    open(j + 1);
+    if (cur == 0) load_scales((j + NS) / 2);
+    in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
+      constexpr int i = decltype(number)::value;
+      mma_one(upper, cur, i);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+      for (int r = (2 * N_RD * i) / N_MMA; r < (2 * N_RD * (i + 1)) / N_MMA; ++r) {
+        if (r < N_RD) read_frag(0, r);
+        else read_scale(1 - cur, r - N_RD);
+      }
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int l = ((NLA + NLB) * i) / N_MMA; l < ((NLA + NLB) * (i + 1)) / N_MMA; ++l) load_one(j + NS, j % NS, l);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    mask_scales(1 - cur);
+  };
+  MX_WAIT_VM((NS - 1) * (NLA + NLB));
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  open(0);
 #pragma unroll
-        for (int t = 0; t < TN; ++t) {
-          const v8i af = {a[i][h][0], a[i][h][1], a[i][h][2], a[i][h][3], 0, 0, 0, 0};
-          const v8i bf = {b[t][h][0], b[t][h][1], b[t][h][2], b[t][h][3], 0, 0, 0, 0};
-          if (h == 0) acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(af, bf, acc[i][t], 4, 4, 0, (int)as[i], 0, (int)bs[t]);
-          else acc[i][t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(af, bf, acc[i][t], 4, 4, 1, (int)as[i], 1, (int)bs[t]);
-        }
+  for (int r = 0; r < N_RD; ++r) {
+    read_frag(0, r);
+    read_scale(0, r);
+  }
+  mask_scales(0);
+  for (int j = 0; j < stages; j += 2) {
+    trip(j, lower);
+    if (j + 1 < stages) trip(j + 1, upper);
   }
   // what was requested beyond the last stage (zeros) must have landed before the workgroup's LDS is released
   MX_WAIT_VM(0);
@@ -271,12 +318,6 @@ __global__ __launch_bounds__(256) void mxfp4_lay_scales_kernel(const MxScaleArgs
   }
   *(v4i *)(p.t[o] + ((int64_t)chunk * p.windows + w0 + win) * 1024 + lane * 16) = out;
 #endif
-}
-
-// f(0), f(1), .. as straight code, each with its number as a constant
-template <typename F, int... I>
-L8_DEV void in_turn(std::integer_sequence<int, I...>, F &&f) {
-  (f(std::integral_constant<int, I>{}), ...);
 }
 
 template <bool HAS_BIAS>
@@ -627,7 +668,7 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
                         (const uint16_t *)bias, (uint16_t *)C, ldc, (int)M, (int)N, (int)blocks, 0, 0, false};
   hipStream_t st = (hipStream_t)stream;
   L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");
-  const int64_t big = ((M + 255) / 256) * ((N + 255) / 256), mid = ((M + 127) / 128) * ((N + 127) / 128);
+  const int64_t mid = ((M + 127) / 128) * ((N + 127) / 128);
   if (takes_stream(M, N, blocks)) {
     const int64_t need = l8_gemm_mxfp4_workspace(M, N, K);
     L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "l8_gemm_mxfp4_nt: needs a 16-byte aligned workspace of %lld bytes",
@@ -636,7 +677,9 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
     if (N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && (M + 255) / 256 + (N + 255) / 256 < 16384)
       return bias ? launch_gemm_mxfp4_stream<true>(a, (uint8_t *)workspace, st) : launch_gemm_mxfp4_stream<false>(a, (uint8_t *)workspace, st);
   }
-  if (big >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 8, 8, 2>(a, st);
-  if (mid >= num_cus() / 2) return launch_gemm_mxfp4<2, 2, 4, 4, 4>(a, st);
+  if (mid > num_cus()) return launch_gemm_mxfp4<2, 4, 4, 2, 2>(a, st);
+  if (mid >= num_cus() / 2) return launch_gemm_mxfp4<2, 4, 4, 2, 4>(a, st);
+  const int64_t small = ((M + 63) / 64) * ((N + 63) / 64);
+  if (small > num_cus()) return launch_gemm_mxfp4<2, 2, 2, 2, 2>(a, st);
   return launch_gemm_mxfp4<2, 2, 2, 2, 8>(a, st);
 }

@@ -10,9 +10,9 @@
 //     of 16 rows cover all banks once;
 //   * lane group g of the four takes blocks 4 g .. 4 g + 3 of a window, one per instruction: its four scale bytes are one dword, picked
 //     apart by the instruction's op_sel;
-//   * up to 16 tokens come in bf16 and are quantised on the way: 64 lanes hold a row's window, four lanes a block, and the codes and
-//     scales are written to LDS in the layout that they are read in.  More tokens are cast by a launch of their own: every
-//     workgroup would do it over again;
+//   * a few tokens come in bf16 and are quantised on the way: 64 lanes hold a row's window, four lanes a block, and the codes and
+//     scales are written to LDS in the layout that they are read in.  Every workgroup does it over again, so where that is much
+//     (quantised_inside below) a launch of their own casts them;
 //   * the eight partial tiles meet in LDS and are added in the order of the waves.
 #include "l8_common.h"
 #include "mxfp4.h"
@@ -29,7 +29,7 @@ template <int MT, int NT, int U, bool QX>
 __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFewArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(!QX || MT == 1, "x is quantised for one tile of tokens");
-  constexpr int kBuf = (NT + MT) * kFewTile + (QX ? 256 : 0), kRed = MT * NT * 1024;
+  constexpr int kBuf = kFewTile + (QX ? 256 : 0), kRed = MT * NT * 1024;   // (every tile of a wave goes through one buffer)
   __shared__ __attribute__((aligned(16))) uint8_t lds[kFewWaves * (kBuf > kRed ? kBuf : kRed)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -37,8 +37,8 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
   const int kbytes = p.blocks * 16, windows = (p.blocks + 15) >> 4;
   const int share = (windows + kFewWaves - 1) / kFewWaves;
   const int w_first = wave * share, w_last = w_first + share < windows ? w_first + share : windows;
-  uint8_t *const wbuf = lds + wave * kBuf, *const xbuf = wbuf + NT * kFewTile;
-  uint32_t *const xsc = (uint32_t *)(xbuf + MT * kFewTile);   // QX: scales of 16 tokens, a dword per lane group
+  uint8_t *const buf = lds + wave * kBuf;
+  uint32_t *const xsc = (uint32_t *)(buf + kFewTile);   // QX: scales of 16 tokens, a dword per lane group
 
   auto range = [](int64_t n) { return n < 0x7fffffff ? (uint32_t)n : 0x7fffffffu; };
   const __amdgpu_buffer_rsrc_t rsW = make_rsrc(p.qw + (int64_t)n0 * p.ldqw, range((int64_t)(p.N - n0 - 1) * p.ldqw + kbytes));
@@ -70,7 +70,7 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
     }
     return v;
   };
-  auto turn = [&](uint8_t *buf, const v4i (&v)[4], v4i (&f)[4]) {
+  auto turn = [&](const v4i (&v)[4], v4i (&f)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) *(v4i *)(buf + put(j * 4 + lrow, lchunk)) = v[j];
     __builtin_amdgcn_wave_barrier();
@@ -115,12 +115,12 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
           const uint32_t byte = mx_byte(quad_max(amax8(v)));
           const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], mx_scale(byte));
           const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
-          *(uint32_t *)(xbuf + put(m, lane >> 2) + (lane & 3) * 4) = codes;
+          *(uint32_t *)(buf + put(m, lane >> 2) + (lane & 3) * 4) = codes;
           if (lchunk == 0) xsc[m * 4 + lrow] = four;
         }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int s = 0; s < 4; ++s) xf[0][s] = *(const v4i *)(xbuf + put(fr, fg * 4 + s));
+        for (int s = 0; s < 4; ++s) xf[0][s] = *(const v4i *)(buf + put(fr, fg * 4 + s));
         xs[0] = xsc[fr * 4 + fg];
         __builtin_amdgcn_wave_barrier();
       } else {
@@ -129,13 +129,13 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
           v4i v[4];
           load_codes(rsX, p.ldx, i * 16, w + u, v, false);
           xs[i] = load_scale(p.sx, p.ldsx, i * 16 + fr, p.M, w + u);
-          turn(xbuf + i * kFewTile, v, xf[i]);
+          turn(v, xf[i]);
         }
       }
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         v4i wf[4];
-        turn(wbuf + t * kFewTile, wv[u][t], wf);
+        turn(wv[u][t], wf);
 #pragma unroll
         for (int i = 0; i < MT; ++i) acc[i][t] = mma(wf, ws[u][t], xf[i], xs[i], acc[i][t]);
       }
@@ -195,8 +195,15 @@ int mxfp4_few_packed(const MxFewArgs &a, hipStream_t st) {
 
 using namespace l8;
 
-// Tokens that the kernels above take, and that are quantised inside them.
-static constexpr int64_t kFewTokens = 64, kFewQuantised = 16;
+static constexpr int64_t kFewTokens = 64;   // that the kernels above take
+
+// Are the tokens quantised inside the product?  What a wave spends on it -- tokens times its windows, times the workgroups that a unit
+// runs one after the other -- against a launch.  us, inside / cast before: 8 tokens, [4096,4096] 7.1 / 8.1, [11008,4096] 14.2 /
+// 13.0, [4096,11008] 14.3 / 11.5, [2048,2048] 5.7 / 6.2; 4 tokens, [11008,4096] 12.2 / 13.0, [4096,11008] 11.1 / 11.5.
+static bool quantised_inside(int64_t M, int64_t N, int64_t K) {
+  const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves, rounds = ((N + 15) / 16 + num_cus() - 1) / num_cus();
+  return M <= 16 && (M == 1 || M * share * rounds <= 12);
+}
 
 // Codes and scales of the activation in the workspace, then the product's own.
 struct MxLinearPlan {
@@ -210,7 +217,7 @@ static MxLinearPlan plan_of(int64_t M, int64_t N, int64_t K) {
   p.q = 0;
   p.s = p.q + M * p.ldq;
   p.product = p.s + (M * p.lds + 15) / 16 * 16;
-  p.total = M <= kFewQuantised ? 0 : p.product + (M <= kFewTokens ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
+  p.total = quantised_inside(M, N, K) ? 0 : p.product + (M <= kFewTokens ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
   return p;
 }
 
@@ -235,10 +242,11 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
              "l8_mxfp4_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)plan.total);
   hipStream_t st = (hipStream_t)stream;
   MxFewArgs a = {x, nullptr, (const uint8_t *)qw, (const uint8_t *)sw, ldx, 0, ldqw, ldsw, (const uint16_t *)bias, (uint16_t *)y, ldy, (int)M, (int)N, (int)K, (int)blocks};
-  // (rows of x are addressed with 32 bits)
-  if (M <= kFewQuantised && ldx <= (1 << 25)) return mxfp4_few_bf16(a, st);
+  if (plan.total == 0) {
+    L8_REQUIRE(ldx <= (1 << 25), "l8_mxfp4_linear: rows of x further apart than 2^25 elements");   // (32-bit offsets)
+    return mxfp4_few_bf16(a, st);
+  }
   uint8_t *const ws = (uint8_t *)workspace;
-  L8_REQUIRE(M > kFewQuantised, "l8_mxfp4_linear: rows of x further apart than 2^25 elements");
   const int rc = l8_cast_mxfp4(x, M, K, ldx, ws + plan.q, plan.ldq, ws + plan.s, plan.lds, nullptr, 0, nullptr, 0, stream);
   if (rc != L8_OK) return rc;
   if (M <= kFewTokens) {

@@ -1013,7 +1013,7 @@ def gemm_mxfp4_nt(qa: torch.Tensor, qb: torch.Tensor, sa: torch.Tensor, sb: torc
 
 def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """bf16 [M,N]: x [M,K] bf16 quantised along its rows times a weight kept in MXFP4 (codes [N, 16 * ceil(K / 32)] and scales), plus
-    bias; one launch up to 16 tokens."""
+    bias; one launch for the fewest tokens."""
     what = "mxfp4_linear_fwd"
     if kernel_timer is None and x.is_cuda:   # the same in one call, for operands that need no copies
         y = _lib.native_for(x.get_device()).mxfp4_linear(x, qw, sw, bias)
