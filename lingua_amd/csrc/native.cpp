@@ -13,6 +13,8 @@
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -728,87 +730,6 @@ PyObject *add_rmsnorm_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// add_rmsnorm_bwd(gy, gh, h, weight, rstd) -> (gx, gw of the weight's type) or None
-PyObject *add_rmsnorm_bwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (n != 5) throw std::runtime_error("add_rmsnorm_bwd: 5 arguments");
-  if (!tensors(args, 5)) Py_RETURN_NONE;
-  for (int i = 0; i < 5; ++i)
-    if (args[i] == Py_None) Py_RETURN_NONE;
-  const Tensor &gy = THPVariable_Unpack(args[0]), &gh = THPVariable_Unpack(args[1]), &h = THPVariable_Unpack(args[2]), &w = THPVariable_Unpack(args[3]),
-               &rstd = THPVariable_Unpack(args[4]);
-  if (!h.is_cuda()) Py_RETURN_NONE;
-  const int device = h.get_device();
-  Rows rg, ru, rh;
-  if (!as_rows(gy, device, rg) || !as_rows(gh, device, ru) || !as_rows(h, device, rh) || rg.rows != rh.rows || rg.cols != rh.cols || ru.rows != rh.rows ||
-      ru.cols != rh.cols || c10::hip::current_device() != device)
-    Py_RETURN_NONE;
-  const int64_t R = rh.rows, C = rh.cols;
-  const bool f32 = w.scalar_type() == at::kFloat;
-  if (!dense(w, f32 ? at::kFloat : at::kBFloat16, C, device) || !dense(rstd, at::kFloat, R, device)) Py_RETURN_NONE;
-  Tensor gx, gw;
-  {
-    pybind11::gil_scoped_release no_gil;
-    const auto o = h.options();
-    gx = at::empty({R, C}, o), gw = at::empty({C}, w.options());
-    const int64_t ws_bytes = lib.l8_rmsnorm_bwd_workspace(R, C);
-    const Space ws(h, ws_bytes);
-    check(lib.l8_add_rmsnorm_bwd(rg.p, ru.p, rh.p, w.const_data_ptr(), f32, rstd.const_data_ptr<float>(), R, C, rg.ld, ru.ld, rh.ld, gx.mutable_data_ptr(), C,
-                                 gw.mutable_data_ptr(), f32, ws.p(), ws_bytes, stream_of(device)), "l8_add_rmsnorm_bwd");
-  }
-  return tuple_of({gx, gw});
-  END_HANDLE_TH_ERRORS
-}
-
-// rotary(xq, xk, cos, sin, positions, in_halves, inverse) -> (yq, yk) or None; either of xq and xk may be None
-PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  if (n != 7) throw std::runtime_error("rotary: 7 arguments");
-  if (!tensors(args, 5) || (args[0] == Py_None && args[1] == Py_None) || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
-  const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
-  const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]), &one = x[0].defined() ? x[0] : x[1];
-  const bool in_halves = truth(args[5]), inverse = truth(args[6]);
-  if (!one.is_cuda() || one.dim() != 4) Py_RETURN_NONE;
-  const int device = one.get_device();
-  const int64_t B = one.size(0), S = one.size(1), D = one.size(3);
-  if (c10::hip::current_device() != device) Py_RETURN_NONE;
-  for (const Tensor &t : x)
-    if (t.defined() && (t.scalar_type() != at::kBFloat16 || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || t.dim() != 4 || t.numel() < 1 ||
-                        t.size(0) != B || t.size(1) != S || t.size(3) != D || t.stride(3) != 1))
-      Py_RETURN_NONE;
-  for (const Tensor *t : {&cos, &sin})
-    if (t->scalar_type() != at::kFloat || t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device || t->dim() != 2 || t->sizes() != cos.sizes() ||
-        t->strides() != cos.strides())
-      Py_RETURN_NONE;
-  const int64_t P = cos.size(0), rot = 2 * cos.size(1);
-  if (rot < 2 || rot > D || (!pos.defined() && S > P)) Py_RETURN_NONE;
-  int64_t pos_b = 0, pos_s = 0;
-  if (pos.defined()) {   // [S], [1,S], [B,1] or [B,S]
-    if ((pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || pos.layout() != at::kStrided || !pos.is_cuda() || pos.get_device() != device ||
-        pos.dim() < 1 || pos.dim() > 2)
-      Py_RETURN_NONE;
-    const int64_t ps = pos.size(-1), pb = pos.dim() == 2 ? pos.size(0) : 1;
-    if ((ps != S && ps != 1) || (pb != B && pb != 1)) Py_RETURN_NONE;
-    pos_s = ps == 1 ? 0 : pos.stride(-1);
-    pos_b = pb == 1 ? 0 : pos.stride(0);
-  }
-  Tensor y[2];
-  {
-    pybind11::gil_scoped_release no_gil;
-    l8_rotary_operand two[2];
-    for (int i = 0; i < 2; ++i) {
-      two[i] = {nullptr, nullptr, 0, 0, 0, 0};
-      if (!x[i].defined()) continue;
-      y[i] = at::empty(x[i].sizes(), x[i].options());
-      two[i] = {x[i].const_data_ptr(), y[i].mutable_data_ptr(), x[i].size(2), x[i].stride(0), x[i].stride(1), x[i].stride(2)};
-    }
-    check(lib.l8_rotary(two, B, S, D, rot, in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), P,
-                        pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kInt, pos_b, pos_s, stream_of(device)), "l8_rotary");
-  }
-  return tuple_of({y[0], y[1]});
-  END_HANDLE_TH_ERRORS
-}
-
 // One MXFP4 copy: rows of codes and of scales, as lingua_amd.ops lays them out.
 struct Mx {
   Tensor q, s;
@@ -900,10 +821,10 @@ PyObject *mxfp4_to_bf16(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// mxfp4_linear(x, qw, sw, bias) -> y or None: the product with a weight kept in MXFP4
-PyObject *mxfp4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+// mxfp4_packed(x, qw, sw, bias) -> y or None: the product with a weight kept in MXFP4
+PyObject *mxfp4_packed(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 4) throw std::runtime_error("mxfp4_linear: 4 arguments");
+  if (n != 4) throw std::runtime_error("mxfp4_packed: 4 arguments");
   if (!tensors(args, 4) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None) Py_RETURN_NONE;
   const Tensor &x = THPVariable_Unpack(args[0]), &qw = THPVariable_Unpack(args[1]), &sw = THPVariable_Unpack(args[2]);
   const Tensor bias = arg(args[3]);
@@ -927,78 +848,295 @@ PyObject *mxfp4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// mxfp4_fwd(a, w, bias, need_a, need_w) -> (y, qat, sat, qwt, swt) or None: the transposed copies that the gradients multiply with
-PyObject *mxfp4_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+// ---- differentiable forms ----
+// The Python forms' backward passes take the interpreter from the thread that waits for them, at 20 to 30 us a node whatever the
+// kernels take; as nodes of their own these need it neither way.  us, forward + backward of small operands, Python / here: residual
+// norm 112 / 83, rotary 81 / 60, MXFP4 linear 111 / 93.  The Python forms run where operands need copies, under transforms and modes.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// Gradients as a pass that is itself differentiated hands them on: an error if anybody asks for more.
+variable_list once(variable_list grads, const char *what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  return torch::autograd::DelayedError(std::string(what) + " is not differentiable twice", (int)grads.size())(std::move(grads));
+}
+// A gradient as the kernels take it: bf16, of `sizes`, dense rows.
+Tensor gradient(const Tensor &g, const char *what) {
+  TORCH_CHECK(g.scalar_type() == at::kBFloat16, what, " backward: bf16 gradients required, got ", g.scalar_type());
+  Rows r;
+  return as_rows(g, g.get_device(), r) && on_16_bytes(r) ? g : g.clone(at::MemoryFormat::Contiguous);
+}
+Rows rows_of(const Tensor &t) {
+  Rows r;
+  TORCH_CHECK(as_rows(t, t.get_device(), r), "gradient rows");
+  return r;
+}
+
+struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
+  static constexpr const char *kName = "add_rmsnorm";
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const Tensor &res, const Tensor &w, double eps, bool want_col) {
+    const Rows rx = rows_of(x), rr = rows_of(res);
+    const int64_t R = rx.rows, C = rx.cols;
+    const int device = x.get_device();
+    const auto o = x.options();
+    const Tensor h = at::empty(x.sizes(), o), y = at::empty(x.sizes(), o), q = empty_fp8(R, C, o), s = at::empty({R, 1}, o.dtype(at::kFloat)),
+                 rstd = at::empty({R, 1}, o.dtype(at::kFloat)), col = want_col ? at::empty({C}, o.dtype(at::kFloat)) : Tensor();
+    const int64_t ws_bytes = want_col ? lib.l8_rmsnorm_workspace(R, C) : 0;
+    const Space ws(x, ws_bytes);
+    check(lib.l8_add_rmsnorm_cast_rowwise(rx.p, rr.p, w.const_data_ptr(), w.scalar_type() == at::kFloat, R, C, rx.ld, rr.ld, (float)eps, h.mutable_data_ptr(), C,
+                                          y.mutable_data_ptr(), C, q.mutable_data_ptr(), q.stride(0), s.mutable_data_ptr<float>(), rstd.mutable_data_ptr<float>(),
+                                          want_col ? col.mutable_data_ptr<float>() : nullptr, ws.p(), ws_bytes, stream_of(device)), "l8_add_rmsnorm_cast_rowwise");
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({h, w, rstd});
+    variable_list out = {h, y, q, s};
+    if (want_col) out.push_back(col);
+    ctx->mark_non_differentiable({out.begin() + 2, out.end()});
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
+    Tensor gx, gw;
+    if (grads[1].defined()) {
+      const Tensor gy = gradient(grads[1], kName), gh = grads[0].defined() ? gradient(grads[0], kName) : Tensor();
+      const Rows rg = rows_of(gy), rh = rows_of(h);
+      const Rows ru = gh.defined() ? rows_of(gh) : Rows();
+      const bool f32 = w.scalar_type() == at::kFloat;
+      const int device = h.get_device();
+      const c10::DeviceGuard guard(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+      gx = at::empty(h.sizes(), h.options()), gw = at::empty({rh.cols}, w.options());
+      const int64_t ws_bytes = lib.l8_rmsnorm_bwd_workspace(rh.rows, rh.cols);
+      const Space ws(h, ws_bytes);
+      if (gh.defined())
+        check(lib.l8_add_rmsnorm_bwd(rg.p, ru.p, rh.p, w.const_data_ptr(), f32, rstd.const_data_ptr<float>(), rh.rows, rh.cols, rg.ld, ru.ld, rh.ld, gx.mutable_data_ptr(),
+                                     rh.cols, gw.mutable_data_ptr(), f32, ws.p(), ws_bytes, stream_of(device)), "l8_add_rmsnorm_bwd");
+      else
+        check(lib.l8_rmsnorm_bwd_as(rg.p, rh.p, w.const_data_ptr(), f32, rstd.const_data_ptr<float>(), rh.rows, rh.cols, rg.ld, rh.ld, gx.mutable_data_ptr(), rh.cols,
+                                    gw.mutable_data_ptr(), f32, ws.p(), ws_bytes, stream_of(device)), "l8_rmsnorm_bwd");
+    } else if (grads[0].defined()) {   // only the sum was used
+      TORCH_CHECK(grads[0].scalar_type() == at::kBFloat16, kName, " backward: bf16 gradients required, got ", grads[0].scalar_type());
+      gx = grads[0];
+    }
+    return once({gx, gx, gw, Tensor(), Tensor()}, kName);
+  }
+};
+
+// add_rmsnorm(x, residual, weight, eps, want_col) -> (h, y, q, scale, col amax) or None
+PyObject *add_rmsnorm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 5) throw std::runtime_error("mxfp4_fwd: 5 arguments");
-  if (!tensors(args, 3) || args[0] == Py_None || args[1] == Py_None) Py_RETURN_NONE;
-  const Tensor &a = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
-  const Tensor bias = arg(args[2]);
-  const bool need_a = truth(args[3]), need_w = truth(args[4]);
-  if (!a.is_cuda() || a.dim() != 2 || w.dim() != 2) Py_RETURN_NONE;
-  const int device = a.get_device();
-  Rows ra, rw;
-  if (!as_rows(a, device, ra) || !as_rows(w, device, rw) || ra.cols != rw.cols || c10::hip::current_device() != device ||
-      (bias.defined() && !dense(bias, at::kBFloat16, rw.rows, device)))
+  if (n != 5) throw std::runtime_error("add_rmsnorm: 5 arguments");
+  if (!tensors(args, 3) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]), &res = THPVariable_Unpack(args[1]), &w = THPVariable_Unpack(args[2]);
+  const double eps = PyFloat_AsDouble(args[3]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  const bool want_col = truth(args[4]);
+  if (!x.is_cuda()) Py_RETURN_NONE;
+  const int device = x.get_device();
+  Rows rx, rr;
+  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || x.sizes() != res.sizes() || c10::hip::current_device() != device ||
+      !dense(w, w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16, rx.cols, device))
     Py_RETURN_NONE;
-  Tensor y;
-  Mx at, wt;
+  variable_list out;
   {
     pybind11::gil_scoped_release no_gil;
-    const auto o = a.options();
-    void *stream = stream_of(device);
-    const Mx qa(ra.rows, ra.cols, o, true), qw(rw.rows, rw.cols, o, true);
-    if (need_w) at = Mx(ra.cols, ra.rows, o, true);
-    if (need_a) wt = Mx(rw.cols, rw.rows, o, true);
-    cast_mx(ra, qa, at, stream);
-    cast_mx(rw, qw, wt, stream);
-    y = at::empty({ra.rows, rw.rows}, o);
-    gemm_mx(rows_of(qa), rows_of(qw), bias, y, stream);
+    out = AddRMSNorm::apply(x, res, w, eps, want_col);
   }
-  return tuple_of({y, at.q, at.s, wt.q, wt.s});
+  return tuple_of({out[0], out[1], out[2], out[3], want_col ? out[4] : Tensor()});
   END_HANDLE_TH_ERRORS
 }
 
-// mxfp4_bwd(gy, qat, sat, qwt, swt, need_bias) -> (ga, gw, gbias) or None; a copy that is None: its gradient is not wanted
-PyObject *mxfp4_bwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+// Both forms of a rotation: y of x, either of them possibly undefined.
+void rotate(const Tensor (&x)[2], Tensor (&y)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves, bool inverse) {
+  const Tensor &one = x[0].defined() ? x[0] : x[1];
+  const int64_t B = one.size(0), S = one.size(1), D = one.size(3);
+  int64_t pos_b = 0, pos_s = 0;
+  if (pos.defined()) {
+    pos_s = pos.size(-1) == 1 ? 0 : pos.stride(-1);
+    pos_b = pos.dim() == 1 || pos.size(0) == 1 ? 0 : pos.stride(0);
+  }
+  l8_rotary_operand two[2];
+  for (int i = 0; i < 2; ++i) {
+    two[i] = {nullptr, nullptr, 0, 0, 0, 0};
+    if (!x[i].defined()) continue;
+    y[i] = at::empty(x[i].sizes(), x[i].options());
+    two[i] = {x[i].const_data_ptr(), y[i].mutable_data_ptr(), x[i].size(2), x[i].stride(0), x[i].stride(1), x[i].stride(2)};
+  }
+  check(lib.l8_rotary(two, B, S, D, 2 * cos.size(1), in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), cos.size(0),
+                      pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kInt, pos_b, pos_s, stream_of(one.get_device())), "l8_rotary");
+}
+// May the extension take these operands?
+bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos) {
+  const Tensor &one = x[0].defined() ? x[0] : x[1];
+  if (!one.is_cuda() || one.dim() != 4) return false;
+  const int device = one.get_device();
+  const int64_t B = one.size(0), S = one.size(1), D = one.size(3);
+  if (c10::hip::current_device() != device) return false;
+  for (const Tensor &t : x)
+    if (t.defined() && (t.scalar_type() != at::kBFloat16 || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || t.dim() != 4 || t.numel() < 1 ||
+                        t.size(0) != B || t.size(1) != S || t.size(3) != D || t.stride(3) != 1))
+      return false;
+  for (const Tensor *t : {&cos, &sin})
+    if (t->scalar_type() != at::kFloat || t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device || t->dim() != 2 || t->sizes() != cos.sizes() ||
+        t->strides() != cos.strides())
+      return false;
+  const int64_t P = cos.size(0), rot = 2 * cos.size(1);
+  if (rot < 2 || rot > D || (!pos.defined() && S > P)) return false;
+  if (pos.defined()) {   // [S], [1], [1,S], [B,1] or [B,S]
+    if ((pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || pos.layout() != at::kStrided || !pos.is_cuda() || pos.get_device() != device ||
+        pos.dim() < 1 || pos.dim() > 2)
+      return false;
+    const int64_t ps = pos.size(-1), pb = pos.dim() == 2 ? pos.size(0) : 1;
+    if ((ps != S && ps != 1) || (pb != B && pb != 1)) return false;
+  }
+  return true;
+}
+
+struct Rotary : torch::autograd::Function<Rotary> {
+  static variable_list forward(AutogradContext *ctx, const Tensor &xq, const Tensor &xk, const Tensor &cos, const Tensor &sin, const std::optional<Tensor> &at, bool in_halves) {
+    const Tensor x[2] = {xq, xk}, pos = at.value_or(Tensor());
+    Tensor y[2];
+    rotate(x, y, cos, sin, pos, in_halves, false);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({cos, sin, pos});
+    ctx->saved_data["half"] = in_halves;
+    return {y[0], y[1]};
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    Tensor g[2], x[2];
+    for (int i = 0; i < 2; ++i) {
+      if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
+      TORCH_CHECK(grads[i].scalar_type() == at::kBFloat16, "rotary backward: bf16 gradients required, got ", grads[i].scalar_type());
+      x[i] = grads[i].stride(3) == 1 ? grads[i] : grads[i].contiguous();
+    }
+    if (x[0].defined() || x[1].defined()) {
+      const c10::DeviceGuard guard((x[0].defined() ? x[0] : x[1]).device());
+      const Tensor in[2] = {x[0], x[1]};
+      rotate(in, g, saved[0], saved[1], saved[2], ctx->saved_data["half"].toBool(), true);
+    }
+    return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()}, "rotary");
+  }
+};
+
+// rotary(xq, xk, cos, sin, positions, in_halves, inverse) -> (yq, yk) or None; either of xq and xk may be None
+PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 6) throw std::runtime_error("mxfp4_bwd: 6 arguments");
-  if (!tensors(args, 5) || args[0] == Py_None) Py_RETURN_NONE;
-  const Tensor &gy = THPVariable_Unpack(args[0]);
-  const Tensor qat = arg(args[1]), sat = arg(args[2]), qwt = arg(args[3]), swt = arg(args[4]);
-  const bool need_bias = truth(args[5]);
-  if (!gy.is_cuda() || gy.dim() != 2) Py_RETURN_NONE;
-  const int device = gy.get_device();
-  Rows rg;
-  MxRows a, w;
-  if (!as_rows(gy, device, rg) || !on_16_bytes(rg) || c10::hip::current_device() != device || (qat.defined() && (!as_mx(qat, sat, device, a) || a.blocks != (rg.rows + 31) / 32)) ||
-      (qwt.defined() && (!as_mx(qwt, swt, device, w) || w.blocks != (rg.cols + 31) / 32)))
-    Py_RETURN_NONE;
-  Tensor ga, gw, gbias;
+  if (n != 7) throw std::runtime_error("rotary: 7 arguments");
+  if (!tensors(args, 5) || (args[0] == Py_None && args[1] == Py_None) || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
+  const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
+  const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
+  const bool in_halves = truth(args[5]), inverse = truth(args[6]);
+  if (!rotates(x, cos, sin, pos)) Py_RETURN_NONE;
+  Tensor y[2];
   {
     pybind11::gil_scoped_release no_gil;
+    rotate(x, y, cos, sin, pos, in_halves, inverse);
+  }
+  return tuple_of({y[0], y[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// rotary_pair(xq, xk, cos, sin, positions, in_halves) -> (yq, yk), differentiable, or None
+PyObject *rotary_pair(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 6) throw std::runtime_error("rotary_pair: 6 arguments");
+  if (!tensors(args, 5) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
+  const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
+  const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
+  const bool in_halves = truth(args[5]);
+  if (!rotates(x, cos, sin, pos)) Py_RETURN_NONE;
+  variable_list y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    y = Rotary::apply(x[0], x[1], cos, sin, pos.defined() ? std::optional<Tensor>(pos) : std::nullopt, in_halves);
+  }
+  return tuple_of({y[0], y[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// MXFP4 linear: what its two passes compute.
+Tensor mx_forward(const Tensor &a, const Tensor &w, const Tensor &bias, bool need_a, bool need_w, Mx &at, Mx &wt) {
+  const Rows ra = rows_of(a), rw = rows_of(w);
+  const auto o = a.options();
+  void *stream = stream_of(a.get_device());
+  const Mx qa(ra.rows, ra.cols, o, true), qw(rw.rows, rw.cols, o, true);
+  if (need_w) at = Mx(ra.cols, ra.rows, o, true);
+  if (need_a) wt = Mx(rw.cols, rw.rows, o, true);
+  cast_mx(ra, qa, at, stream);
+  cast_mx(rw, qw, wt, stream);
+  auto sizes = a.sizes().vec();
+  sizes.back() = rw.rows;
+  const Tensor y = at::empty(sizes, o);
+  gemm_mx(rows_of(qa), rows_of(qw), bias, y, stream);
+  return y;
+}
+bool mx_linear_takes(const Tensor &a, const Tensor &w, const Tensor &bias) {
+  if (!a.is_cuda() || w.dim() != 2) return false;
+  const int device = a.get_device();
+  Rows ra, rw;
+  return as_rows(a, device, ra) && as_rows(w, device, rw) && on_16_bytes(ra) && on_16_bytes(rw) && ra.cols == rw.cols && ra.cols % 16 == 0 && rw.rows % 16 == 0 &&
+         c10::hip::current_device() == device && (!bias.defined() || dense(bias, at::kBFloat16, rw.rows, device));
+}
+
+struct Mxfp4Linear : torch::autograd::Function<Mxfp4Linear> {
+  static Tensor forward(AutogradContext *ctx, const Tensor &a, const Tensor &w, const std::optional<Tensor> &bias, bool need_a, bool need_w) {
+    Mx at, wt;
+    const Tensor y = mx_forward(a, w, bias.value_or(Tensor()), need_a, need_w, at, wt);
+    ctx->save_for_backward({at.q, at.s, wt.q, wt.s});
+    ctx->saved_data["like"] = a.sizes().vec();
+    ctx->saved_data["bias"] = bias.has_value();
+    return y;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor gy = gradient(grads[0], "mxfp4_linear");
+    const int device = gy.get_device();
+    const c10::DeviceGuard guard(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+    const Rows rg = rows_of(gy);
     const auto o = gy.options();
     void *stream = stream_of(device);
+    // (asked for when the graph was made, and again now: a part of the graph may be left out)
+    const bool need_a = saved[2].defined() && ctx->needs_input_grad(0), need_w = saved[0].defined() && ctx->needs_input_grad(1);
     Mx rows, cols;
-    if (w.q) rows = Mx(rg.rows, rg.cols, o, true);
-    if (a.q) cols = Mx(rg.cols, rg.rows, o, true);
-    if (w.q || a.q) cast_mx(rg, rows, cols, stream);
-    if (w.q) {
-      ga = at::empty({rg.rows, w.rows}, o);
+    MxRows a, w;
+    TORCH_CHECK((!need_w || as_mx(saved[0], saved[1], device, a)) && (!need_a || as_mx(saved[2], saved[3], device, w)), "mxfp4_linear backward: saved copies");
+    if (need_a) rows = Mx(rg.rows, rg.cols, o, true);
+    if (need_w) cols = Mx(rg.cols, rg.rows, o, true);
+    if (need_a || need_w) cast_mx(rg, rows, cols, stream);
+    Tensor ga, gw, gbias;
+    if (need_a) {
+      ga = at::empty(ctx->saved_data["like"].toIntVector(), o);
       gemm_mx(rows_of(rows), w, Tensor(), ga, stream);
     }
-    if (a.q) {
+    if (need_w) {
       gw = at::empty({rg.cols, a.rows}, o);
       gemm_mx(rows_of(cols), a, Tensor(), gw, stream);
     }
-    if (need_bias) {
+    if (ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2)) {
       gbias = at::empty({rg.cols}, o);
       const int64_t bytes = lib.l8_col_sum_workspace(rg.rows, rg.cols);
       const Space ws(gy, bytes);
       check(lib.l8_col_sum(rg.p, rg.rows, rg.cols, rg.ld, gbias.mutable_data_ptr(), ws.p(), bytes, stream), "l8_col_sum");
     }
+    return once({ga, gw, gbias, Tensor(), Tensor()}, "mxfp4_linear");
   }
-  return tuple_of({ga, gw, gbias});
+};
+
+// mxfp4_linear(a, w, bias) -> y, differentiable, or None
+PyObject *mxfp4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 3) throw std::runtime_error("mxfp4_linear: 3 arguments");
+  if (!tensors(args, 3) || args[0] == Py_None || args[1] == Py_None) Py_RETURN_NONE;
+  const Tensor &a = THPVariable_Unpack(args[0]), &w = THPVariable_Unpack(args[1]);
+  const Tensor bias = arg(args[2]);
+  if (!mx_linear_takes(a, w, bias)) Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool grad = at::GradMode::is_enabled();
+    y = Mxfp4Linear::apply(a, w, bias.defined() ? std::optional<Tensor>(bias) : std::nullopt, grad && a.requires_grad(), grad && w.requires_grad());
+  }
+  return wrap(y);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1048,13 +1186,13 @@ PyMethodDef methods[] = {
     {"swiglu_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(swiglu_fwd)), METH_FASTCALL, nullptr},
     {"swiglu_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(swiglu_bwd)), METH_FASTCALL, nullptr},
     {"add_rmsnorm_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm_fwd)), METH_FASTCALL, nullptr},
-    {"add_rmsnorm_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm_bwd)), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary)), METH_FASTCALL, nullptr},
     {"cast_mxfp4", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cast_mxfp4)), METH_FASTCALL, nullptr},
     {"mxfp4_to_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_to_bf16)), METH_FASTCALL, nullptr},
+    {"add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm)), METH_FASTCALL, nullptr},
+    {"rotary_pair", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_pair)), METH_FASTCALL, nullptr},
+    {"mxfp4_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_packed)), METH_FASTCALL, nullptr},
     {"mxfp4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_linear)), METH_FASTCALL, nullptr},
-    {"mxfp4_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_fwd)), METH_FASTCALL, nullptr},
-    {"mxfp4_bwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_bwd)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -42,11 +42,6 @@ class Mxfp4LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, w, bias):
         need_a, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        if ops.kernel_timer is None:
-            res = _lib.native_for(a.get_device()).mxfp4_fwd(a, w, bias, need_a, need_w)
-            if res is not None:
-                ctx.save_for_backward(*res[1:])
-                return res[0]
         (qa, sa), at = ops.cast_mxfp4(a, transposed=need_w, on_lines=True)
         (qw, sw), wt = ops.cast_mxfp4(w, transposed=need_a, on_lines=True)
         ctx.save_for_backward(*(at or (None, None)), *(wt or (None, None)))
@@ -59,10 +54,6 @@ class Mxfp4LinearFn(torch.autograd.Function):
             raise RuntimeError(f"mxfp4_linear backward: bf16 grad_out required, got {gy.dtype}")
         qat, sat, qwt, swt = ctx.saved_tensors
         need_a, need_w, need_bias = ctx.needs_input_grad
-        if ops.kernel_timer is None:
-            res = _lib.native_for(gy.get_device()).mxfp4_bwd(gy, qat, sat, qwt, swt, need_bias)
-            if res is not None:
-                return res
         ga = gw = gbias = None
         if need_a or need_w:
             rows, cols = ops.cast_mxfp4(gy, rowwise=need_a, transposed=need_w, on_lines=True)
@@ -77,6 +68,10 @@ class Mxfp4LinearFn(torch.autograd.Function):
 
 def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x @ weight.T + bias`` in MXFP4, x [..., K] and weight [N, K] bf16, K and N multiples of 16; differentiable."""
+    if f8._native_call(x, 0) and f8._plain_call():
+        y = _lib.native_for(x.get_device()).mxfp4_linear(x, weight, bias)
+        if y is not None:
+            return y
     _check_operands(x, weight)
     if x.dim() == 2:
         return Mxfp4LinearFn.apply(x, weight, bias)

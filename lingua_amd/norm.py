@@ -66,13 +66,8 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
             raise RuntimeError(f"add_rmsnorm: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
         want_col = bool(training and f8.config.fp8_wgrad)
         x2d, r2d = x.flatten(end_dim=-2), residual.flatten(end_dim=-2)
-        res = None
-        if f8._native_call(x2d, 0):
-            res = _lib.native_for(x2d.get_device()).add_rmsnorm_fwd(x2d, r2d, weight, eps, True, want_col, True, True)
-        if res is None:
-            col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
-            res = (*ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True), col)
-        h2d, y2d, q, s, rstd, col = res
+        col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
+        h2d, y2d, q, s, rstd = ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True)
         if f8.config.share_input_casts:
             f8._fwd_cast.put(y2d, (q, s, col), "rmsnorm")
         ctx.set_materialize_grads(False)
@@ -81,6 +76,7 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
         return h2d.unflatten(0, x.shape[:-1]), y2d.unflatten(0, x.shape[:-1])
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, gh, gy):
         h2d, weight, rstd = ctx.saved_tensors
         for g in (gh, gy):
@@ -94,10 +90,7 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
             if gh is None:
                 gx2d, gw = ops.rmsnorm_bwd(gy2d, h2d, weight, rstd, gw_dtype=weight.dtype)
             else:
-                gh2d, res = gh.flatten(end_dim=-2), None
-                if f8._native_call(gy2d, 0):
-                    res = _lib.native_for(gy2d.get_device()).add_rmsnorm_bwd(gy2d, gh2d, h2d, weight, rstd)
-                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh2d, h2d, weight, rstd, gw_dtype=weight.dtype) if res is None else res
+                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh.flatten(end_dim=-2), h2d, weight, rstd, gw_dtype=weight.dtype)
             gx = gx2d.reshape(ctx.x_shape)
         need = ctx.needs_input_grad
         return gx if need[0] else None, gx if need[1] else None, gw if need[2] else None, None, None
@@ -108,7 +101,15 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, e
     linears that are called on ``y`` find it quantised, as behind an ``Fp8RMSNorm``."""
     if x.dim() < 2:
         raise RuntimeError(f"add_rmsnorm: expected [..., C] with at least one leading dimension, got {tuple(x.shape)}")
-    return Fp8AddRMSNormFn.apply(x, residual, weight, eps, torch.is_grad_enabled())
+    training = torch.is_grad_enabled()
+    if f8._native_call(x, 0) and f8._plain_call():
+        res = _lib.native_for(x.get_device()).add_rmsnorm(x, residual, weight, eps, bool(training and f8.config.fp8_wgrad))
+        if res is not None:
+            h, y, q, s, col = res
+            if f8.config.share_input_casts:   # (the memo keeps its tensor: not the graph behind it)
+                f8._fwd_cast.put(y.detach().flatten(end_dim=-2), (q, s, col), "rmsnorm")
+            return h, y
+    return Fp8AddRMSNormFn.apply(x, residual, weight, eps, training)
 
 
 class Fp8RMSNorm(torch.nn.Module):

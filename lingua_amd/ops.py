@@ -1016,7 +1016,7 @@ def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: 
     bias; one launch for the fewest tokens."""
     what = "mxfp4_linear_fwd"
     if kernel_timer is None and x.is_cuda:   # the same in one call, for operands that need no copies
-        y = _lib.native_for(x.get_device()).mxfp4_linear(x, qw, sw, bias)
+        y = _lib.native_for(x.get_device()).mxfp4_packed(x, qw, sw, bias)
         if y is not None:
             return y
     x = _rows_2d(x, torch.bfloat16, what)

@@ -10,7 +10,8 @@ from typing import Optional
 
 import torch
 
-from . import ops
+from . import _lib, ops
+from . import float8 as f8
 
 LAYOUTS = ("interleaved", "half")
 
@@ -49,6 +50,10 @@ def rotary(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Ten
     """
     if layout not in LAYOUTS:
         raise RuntimeError(f"rotary: unknown layout {layout!r}, one of {LAYOUTS}")
+    if f8._native_call(xq, 0) and f8._plain_call():
+        res = _lib.native_for(xq.get_device()).rotary_pair(xq, xk, cos, sin, positions, layout == "half")
+        if res is not None:
+            return res
     return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half")
 
 

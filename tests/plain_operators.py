@@ -1,5 +1,6 @@
 """The residual norm, the rotary positions and MXFP4 in 64 bits, from their definitions, in plain PyTorch: what the kernels are held
-against.  Runs on any device and uses nothing of the package."""
+against.  Runs on any device and uses nothing of the package.  Beside it a fixture that the tests of these operators share."""
+import pytest
 import torch
 
 E2M1 = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
@@ -88,3 +89,12 @@ def within(got, want, size):
     got, want = got.double().cpu(), want.cpu()
     bound = want.abs() * HALF_STEP + size.cpu() * (1 + HALF_STEP) + 2.0 ** -134
     return bool(((got - want).abs() <= bound).all())
+
+
+@pytest.fixture(params=["extension", "python"])
+def host(request, monkeypatch):
+    """Both host paths of an operator: a kernel timer wants to see single launches, which the host extension does not show."""
+    if request.param == "python":
+        from lingua_amd import ops
+        monkeypatch.setattr(ops, "kernel_timer", [])
+    return request.param

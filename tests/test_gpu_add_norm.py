@@ -8,6 +8,7 @@ import torch
 
 import plain_operators as plain
 from conftest import seeded_bf16
+from plain_operators import host  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -48,7 +49,7 @@ def test_forward(shape, w_dtype, with_col):
 
 @pytest.mark.parametrize("shape", SHAPES)
 @pytest.mark.parametrize("w_dtype", [torch.bfloat16, torch.float32])
-def test_backward(shape, w_dtype):
+def test_backward(shape, w_dtype, host):
     """gx: the terms' magnitudes times the roundings of r (128), of the row's mean (128) and a few products.  gw: 512 workgroups add up
     their rows one by one, then eight sums of 64 and those eight."""
     from lingua_amd import norm
@@ -90,7 +91,7 @@ def test_gradients_of_the_formula_against_differences():
 
 
 @pytest.mark.parametrize("used", ["both", "sum", "norm"])
-def test_either_output_alone(used):
+def test_either_output_alone(used, host):
     from lingua_amd import norm, ops
     x, res, w = (t.cuda() for t in inputs((70, 520), torch.float32))
     leaves = [t.clone().requires_grad_() for t in (x, res, w)]

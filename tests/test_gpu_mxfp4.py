@@ -7,6 +7,7 @@ import torch
 
 import plain_operators as plain
 from conftest import seeded_bf16
+from plain_operators import host  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -201,7 +202,7 @@ def test_linear_with_a_packed_weight_and_rows_that_are_not_finite():
 
 @pytest.mark.parametrize("M,K,N", [(1, 16, 32), (9, 48, 64), (33, 272, 144), (130, 512, 528), (515, 1040, 784)])
 @pytest.mark.parametrize("with_bias", [False, True])
-def test_linear_gradients(M, K, N, with_bias):
+def test_linear_gradients(M, K, N, with_bias, host):
     from lingua_amd import mxfp4
     x, w, gy = seeded_bf16((M, K), seed=M), seeded_bf16((N, K), std=0.02, seed=K), seeded_bf16((M, N), std=1e-3, seed=N)
     bias = seeded_bf16((N,), seed=4) if with_bias else None
@@ -221,9 +222,15 @@ def test_linear_gradients(M, K, N, with_bias):
 
 def test_gradients_that_nobody_asks_for_are_not_made():
     from lingua_amd import mxfp4
+    big, w = torch.zeros(2048, 1024, dtype=torch.bfloat16, device="cuda"), torch.zeros(1024, 1024, dtype=torch.bfloat16, device="cuda")
+    for x_learns, w_learns, held in ((True, False, w.numel()), (False, True, big.numel()), (True, True, big.numel() + w.numel()), (False, False, 0)):
+        xl, wl = big.clone().requires_grad_(x_learns), w.clone().requires_grad_(w_learns)
+        before = torch.cuda.memory_allocated()
+        y = mxfp4.mxfp4_linear(xl, wl)
+        assert torch.cuda.memory_allocated() - before <= 2 * y.numel() + held * 17 // 32 + 8192
+        del y
     x, w = seeded_bf16((40, 64), seed=1).cuda(), seeded_bf16((48, 64), seed=2).cuda()
     y = mxfp4.mxfp4_linear(x.clone().requires_grad_(), w)
-    assert len([t for t in y.grad_fn.saved_tensors if t is not None]) == 2
     y.sum().backward()                                   # a gradient of stride 0
     wl = w.clone().requires_grad_()
     y = mxfp4.mxfp4_linear(x, wl)

@@ -5,6 +5,7 @@ import torch
 
 import plain_operators as plain
 from conftest import seeded_bf16
+from plain_operators import host  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -38,7 +39,7 @@ def test_rotation(D, rot, layout, B, S, H, K):
 
 @pytest.mark.parametrize("layout", ["interleaved", "half"])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-def test_positions_strides_and_gradients(layout, dtype):
+def test_positions_strides_and_gradients(layout, dtype, host):
     """q and k are column slices of one product, gradients come with heads in front of tokens; positions far and in any order."""
     from lingua_amd import rope
     B, S, H, K, D, rot = 3, 17, 6, 2, 64, 48
