@@ -158,6 +158,22 @@ class _ResidualNormForward:
         h, y = self.ffn_norm.add(x, self.attention(self.attention_norm(x), *args, **kwargs))
         return h + self.feed_forward(y)
 
+    def __reduce_ex__(self, protocol):   # pickled by the class that it was fused from
+        return _fused_like, (type(self).__mro__[2],), self.__dict__
+
+
+_fused_classes = {}
+
+
+def _fused_class(cls):
+    if cls not in _fused_classes:
+        _fused_classes[cls] = type(cls.__name__, (_ResidualNormForward, cls), {"__module__": cls.__module__})
+    return _fused_classes[cls]
+
+
+def _fused_like(cls):
+    return cls.__new__(_fused_class(cls))
+
 
 def fuse_residual_norm(root_module: torch.nn.Module, filter: str = r"layers\.[0-9]+$") -> torch.nn.Module:
     """In every module whose dotted name matches ``filter`` and whose children are exactly ``attention``, ``feed_forward``,
@@ -173,6 +189,5 @@ def fuse_residual_norm(root_module: torch.nn.Module, filter: str = r"layers\.[0-
                 list(module.parameters(recurse=False))):
             raise RuntimeError(f"fuse_residual_norm: {name!r} ({type(module).__name__}) is not a block of attention, feed_forward, "
                                "attention_norm and an Fp8RMSNorm ffn_norm (run fuse_rmsnorm first)")
-        cls = type(module)
-        module.__class__ = type(cls.__name__, (_ResidualNormForward, cls), {"__module__": cls.__module__})
+        module.__class__ = _fused_class(type(module))
     return root_module

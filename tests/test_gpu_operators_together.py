@@ -1,0 +1,155 @@
+"""A run of the residual norm, the rotary positions and MXFP4 linears, as a model uses them: in training inside the stand-in model of the
+benchmark, and in generation as one captured step."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+import plain_operators as plain
+from bench_workloads import Attention, Llama
+from conftest import seeded_bf16
+
+pytestmark = pytest.mark.gpu
+
+
+class RotaryAttention(Attention):
+    """The stand-in attention with its rotary positions by the kernel."""
+
+    def forward(self, x, cos, sin):
+        from lingua_amd import rope
+        B, S, _ = x.shape
+        q, k, v = (lin(x).view(B, S, self.n_heads, self.head_dim) for lin in (self.wq, self.wk, self.wv))
+        q, k = rope.rotary(q, k, cos, sin)
+        o = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2), is_causal=True)
+        return self.wo(o.transpose(1, 2).reshape(B, S, -1))
+
+
+def model_of(new):
+    """fp8 attention, MXFP4 MLP; `new`: with the residual norm and the rotary kernel in place of the eager chains."""
+    from lingua_amd import convert_linears_to_fp8, mxfp4, norm
+    from lingua_amd.qkv import fuse_qkv
+    model = Llama(n_layers=2, dim=256, n_heads=4, ffn_dim=720, vocab=64).to("cuda", torch.bfloat16)
+    model.init_weights(seed=1)
+    convert_linears_to_fp8(model, "rowwise", r"layers\.[0-9]+\.attention\.")
+    mxfp4.convert_linears_to_mxfp4(model, r"layers\.[0-9]+\.feed_forward\.")
+    norm.fuse_rmsnorm(model)
+    fuse_qkv(model)
+    if new:
+        norm.fuse_residual_norm(model)
+        for layer in model.layers:
+            layer.attention.__class__ = RotaryAttention
+    return model
+
+
+def sum_error(a, b, K):
+    return (a.abs() @ b.abs().t()) * (K * plain.FP32)
+
+
+def test_training_step():
+    """Logits are those of the model without the two fusions, bit for bit; every MXFP4 linear's output and gradients are what the format
+    makes of its own input, weight and output gradient; a second step gives the same bits."""
+    from lingua_amd import mxfp4
+    tokens = torch.randint(0, 64, (3, 37), generator=torch.Generator().manual_seed(2)).cuda()
+    with torch.no_grad():
+        plain_logits = model_of(False)(tokens)
+    model = model_of(True)
+    seen = []
+
+    def keep(module, args, out):
+        entry = {"module": module, "x": args[0].detach().flatten(end_dim=-2), "y": out.detach().flatten(end_dim=-2)}
+        args[0].register_hook(lambda g: entry.update(gx_sum=g.detach()))
+        out.register_hook(lambda g: entry.update(gy=g.detach().flatten(end_dim=-2)))
+        seen.append(entry)
+
+    handles = [m.register_forward_hook(keep) for m in model.modules() if type(m) is mxfp4.Mxfp4Linear]
+    logits = model(tokens)
+    assert torch.equal(logits, plain_logits)
+    F.cross_entropy(logits.flatten(0, 1).float(), tokens.flatten()).backward()
+    for h in handles:
+        h.remove()
+    assert len(seen) == 6
+    q = plain.mx_rounded
+    for e in seen:
+        x, w, gy = e["x"].cpu(), e["module"].weight.detach().cpu(), e["gy"].cpu()
+        want = q(x) @ q(w).t()
+        assert plain.within(e["y"], want, sum_error(q(x), q(w), x.shape[1]))
+        gt, xt = q(gy.t().contiguous()), q(x.t().contiguous())
+        assert plain.within(e["module"].weight.grad, gt @ xt.t(), sum_error(gt, xt, x.shape[0]))
+        if e["module"] in [layer.feed_forward.w2 for layer in model.layers]:   # (w1 and w3 share an input: autograd adds two gradients)
+            gn, wn = q(gy), q(w.t().contiguous())
+            assert plain.within(e["gx_sum"].flatten(end_dim=-2), gn @ wn.t(), sum_error(gn, wn, gy.shape[1]))
+    grads = [p.grad.clone() for p in model.parameters()]
+    assert all(bool(torch.isfinite(g).all()) for g in grads)
+    model.zero_grad()
+    F.cross_entropy(model(tokens).flatten(0, 1).float(), tokens.flatten()).backward()
+    for (name, p), g in zip(model.named_parameters(), grads):
+        assert name == "tok_embeddings.weight" or torch.equal(p.grad, g), name     # (an embedding's gradient is added up by atomics)
+
+
+def test_generation_step_in_a_graph():
+    """Residual norm, packed projections, rotary positions, packed output: one captured step for several sequences, replayed with new
+    tokens and positions and with eager work in between, equals the eager step."""
+    from lingua_amd import mxfp4, norm, rope
+    B, dim, H, D = 5, 256, 4, 64
+    wq, wo = (mxfp4.pack(seeded_bf16((n, k), std=0.05, seed=n).cuda()) for n, k in ((2 * H * D, dim), (dim, H * D)))
+    gain = seeded_bf16((dim,), seed=7).cuda()
+    cos, sin = (t.cuda() for t in rope.rotary_tables(D, 10000, scaling="linear", factor=4))
+    x, res, pos = seeded_bf16((B, dim), seed=8).cuda(), seeded_bf16((B, dim), seed=9).cuda(), torch.arange(B, device="cuda")[:, None]
+
+    def step():
+        h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+        qk = mxfp4.linear_packed(y, *wq).view(B, 1, 2 * H, D)
+        q, k = rope.rotary(qk[:, :, :H], qk[:, :, H:], cos, sin, positions=pos, layout="half")
+        return h, k, mxfp4.linear_packed(q.reshape(B, H * D), *wo)
+
+    with torch.no_grad():
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for i in range(3):
+            x.copy_(seeded_bf16((B, dim), seed=20 + i))
+            pos.add_(997)
+            want = step()
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_backward_in_a_graph():
+    """A training step of the three operators captured whole, leaves of its own: replays equal the eager step."""
+    from lingua_amd import mxfp4, norm, rope
+    B, S, H, D = 2, 24, 4, 32
+    make = lambda: [seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((B * S, H * D), (B * S, H * D), (H * D,), (H * D, H * D)))]  # noqa: E731
+    cos, sin = (t.cuda() for t in rope.rotary_tables(D, S))
+    gy = seeded_bf16((B, S, H, D), std=0.01, seed=9).cuda()
+
+    def step(x, res, gain, w):
+        h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+        q = mxfp4.mxfp4_linear(y, w).view(B, S, H, D)
+        q, _ = rope.rotary(q, h.view(B, S, H, D), cos, sin)
+        return torch.autograd.grad(q, (x, res, gain, w), gy)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    captured = make()
+    with torch.cuda.stream(stream):
+        for _ in range(2):
+            step(*captured)
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(*captured)
+    for i in range(3):
+        with torch.no_grad():
+            captured[0].copy_(seeded_bf16((B * S, H * D), seed=30 + i))
+        eager = make()
+        with torch.no_grad():
+            eager[0].copy_(captured[0])
+        want = step(*eager)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
