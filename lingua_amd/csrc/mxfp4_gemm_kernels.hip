@@ -223,28 +223,35 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   float bv[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) bv[t] = p.bias && col + t < p.N ? bf16_bits_to_f32(p.bias[col + t]) : 0.0f;
+  if (p.wide) {   // through a buffer: rows beyond M lie outside it
+    const __amdgpu_buffer_rsrc_t rsC = make_rsrc(p.C + (int64_t)m0 * p.ldc + n0, range(((int64_t)(p.M - m0 - 1) * p.ldc + (p.N - n0)) * 2));
+    const int ldc2 = (int)p.ldc * 2;
+    const uint32_t voff = col < p.N ? (uint32_t)((wm * TM * 16 + fg * 4) * ldc2 + (col - n0) * 2) : kBeyond;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t out[TN / 2];
+#pragma unroll
+        for (int t = 0; t < TN / 2; ++t)
+          out[t] = bf16_rne_bits(acc[i][2 * t][e] + bv[2 * t]) | (bf16_rne_bits(acc[i][2 * t + 1][e] + bv[2 * t + 1]) << 16);
+        const int soff = (i * 16 + e) * ldc2;
+        if constexpr (TN == 8) __builtin_amdgcn_raw_buffer_store_b128(v4i{(int)out[0], (int)out[1], (int)out[2], (int)out[3]}, rsC, (int)(voff + soff), 0, 0);
+        else if constexpr (TN == 4) __builtin_amdgcn_raw_buffer_store_b64(v2i{(int)out[0], (int)out[1]}, rsC, (int)(voff + soff), 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32((int)out[0], rsC, (int)(voff + soff), 0, 0);
+      }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int row = m0 + (wm * TM + i) * 16 + fg * 4 + e;
-      uint32_t out[TN / 2];
-#pragma unroll
-      for (int t = 0; t < TN / 2; ++t)
-        out[t] = bf16_rne_bits(acc[i][2 * t][e] + bv[2 * t]) | (bf16_rne_bits(acc[i][2 * t + 1][e] + bv[2 * t + 1]) << 16);
       if (row >= p.M) continue;
       uint16_t *dst = p.C + (int64_t)row * p.ldc + col;
-      if (p.wide) {
-        if (col < p.N) {
-          if constexpr (TN == 8) *(v4i *)dst = v4i{(int)out[0], (int)out[1], (int)out[2], (int)out[3]};
-          else if constexpr (TN == 4) *(v2i *)dst = v2i{(int)out[0], (int)out[1]};
-          else *(uint32_t *)dst = out[0];
-        }
-      } else {
 #pragma unroll
-        for (int t = 0; t < TN; ++t)
-          if (col + t < p.N) dst[t] = (uint16_t)(t & 1 ? out[t / 2] >> 16 : out[t / 2] & 0xffffu);
-      }
+      for (int t = 0; t < TN; ++t)
+        if (col + t < p.N) dst[t] = (uint16_t)bf16_rne_bits(acc[i][t][e] + bv[t]);
     }
 #endif
 }
@@ -596,7 +603,7 @@ static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
   constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
   constexpr int lds = NS * (BM + BN) * 128 + (NS / 2 + 1) * (BM + BN) * 16;
   a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN;
-  a.wide = a.N % TN == 0 && a.ldc % TN == 0 && ((uintptr_t)a.C % (TN * 2)) == 0;
+  a.wide = a.N % TN == 0 && a.ldc % TN == 0 && ((uintptr_t)a.C % (TN * 2)) == 0 && a.ldc < (1 << 22);
   static bool ready[kMaxDev];   // benign race: every thread sets the same attribute
   const int slot = device_slot();
   if (slot < 0 || !ready[slot]) {
@@ -677,8 +684,8 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
     if (N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && (M + 255) / 256 + (N + 255) / 256 < 16384)
       return bias ? launch_gemm_mxfp4_stream<true>(a, (uint8_t *)workspace, st) : launch_gemm_mxfp4_stream<false>(a, (uint8_t *)workspace, st);
   }
-  if (mid > num_cus()) return launch_gemm_mxfp4<2, 4, 4, 2, 2>(a, st);
-  if (mid >= num_cus() / 2) return launch_gemm_mxfp4<2, 4, 4, 2, 4>(a, st);
+  if (mid > num_cus()) return launch_gemm_mxfp4<4, 2, 2, 4, 2>(a, st);
+  if (mid >= num_cus() / 2) return launch_gemm_mxfp4<4, 2, 2, 4, 4>(a, st);
   const int64_t small = ((M + 63) / 64) * ((N + 63) / 64);
   if (small > num_cus()) return launch_gemm_mxfp4<2, 2, 2, 2, 2>(a, st);
   return launch_gemm_mxfp4<2, 2, 2, 2, 8>(a, st);

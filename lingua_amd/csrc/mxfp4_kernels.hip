@@ -12,8 +12,8 @@
 //   * rows: a lane takes 8 columns (16 bytes), four neighbours share a block: its amax takes two DPP steps, the four lanes' codes
 //     leave as 16 bytes side by side;
 //   * columns: a workgroup passes a tile of 256 rows x 128 columns through LDS, so that rows are read in 256-byte pieces and the
-//     transposed copy is written in whole 128-byte lines: 8 lanes side by side take the 8 blocks of one pair of columns.  The
-//     block index shifts a lane's LDS address by 8 banks, so the 64 lanes of a read touch every bank once.  Where such tiles would
+//     transposed copy is written in whole 128-byte lines: 8 lanes side by side take the 8 blocks of one column.  The block index
+//     shifts a lane's LDS address by 8 banks, so the lanes of a read touch no bank twice.  Where such tiles would
 //     leave units without work, tiles of 64 rows: [1021,2048] 7.4 -> 4.4 us.
 #include "mxfp4.h"
 
@@ -66,13 +66,14 @@ __global__ __launch_bounds__(256) void mxfp4_rows_kernel(const MxCastArgs p) {
 #endif
 }
 
-// Columns, and rows from the same read where ROWS; BANDS blocks of 32 rows to a tile; COLS columns of it to a thread.
-template <bool ROWS, int BANDS, int COLS>
-__global__ __launch_bounds__(BANDS * 128 / COLS) void mxfp4_tile_kernel(const MxCastArgs p) {
+// Columns, and rows from the same read where ROWS; BANDS blocks of 32 rows to a tile, one block of a column to a
+// thread.
+template <bool ROWS, int BANDS>
+__global__ __launch_bounds__(BANDS * 128) void mxfp4_tile_kernel(const MxCastArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   // LDS image of a tile: bands of rows of 64 dwords, each band padded so that the bands' first dwords share the banks evenly
   constexpr int kBandDwords = kMxBlock * (kMxTileC / 2) + 64 / BANDS;
-  constexpr int kLanes = kMxTileC / 8, kStep = BANDS * 128 / COLS / kLanes, kLoads = BANDS * kMxBlock / kStep;   // 16 lanes a row, kStep rows a load
+  constexpr int kLanes = kMxTileC / 8, kStep = BANDS * 128 / kLanes, kLoads = BANDS * kMxBlock / kStep;   // 16 lanes a row, kStep rows a load
   __shared__ __attribute__((aligned(16))) uint32_t tile[BANDS * kBandDwords];
   const int64_t r0 = (int64_t)blockIdx.y * (BANDS * kMxBlock), c0 = (int64_t)blockIdx.x * kMxTileC;
   const int lr = threadIdx.x / kLanes, lc = (threadIdx.x % kLanes) * 8;
@@ -94,36 +95,32 @@ __global__ __launch_bounds__(BANDS * 128 / COLS) void mxfp4_tile_kernel(const Mx
   }
   __syncthreads();
   const int64_t bands = (p.R + kMxBlock - 1) / kMxBlock;
-  const int band = threadIdx.x % BANDS, pair = threadIdx.x / BANDS * COLS / 2;   // this thread's block of 32 rows, its columns
-  const int64_t gb = r0 / kMxBlock + band, col = c0 + pair * 2;
+  const int band = threadIdx.x % BANDS, half = threadIdx.x / BANDS & 1, pair = threadIdx.x / (2 * BANDS);   // this thread's block of 32 rows, its column
+  const int64_t gb = r0 / kMxBlock + band, col = c0 + pair * 2 + half;
   uint32_t w[kMxBlock], m = 0;
 #pragma unroll
   for (int i = 0; i < kMxBlock; ++i) {
     w[i] = tile[band * kBandDwords + i * (kMxTileC / 2) + pair];
     m = pk_absmax_u16(m, w[i]);
   }
+  const uint32_t byte = mx_byte(half ? m >> 16 : m & 0xffffu);
+  const float scale = mx_scale(byte);
+  const uint32_t pick = half ? 0x07060302u : 0x05040100u;   // this column of two neighbouring rows
+  v4i codes;
 #pragma unroll
-  for (int n = 0; n < COLS; ++n) {
-    const int half = COLS == 2 ? n : (threadIdx.x / BANDS) & 1;
-    const uint32_t byte = mx_byte(half ? m >> 16 : m & 0xffffu);
-    const float scale = mx_scale(byte);
-    v4i codes;
+  for (int k = 0; k < 4; ++k) {
+    uint32_t pr[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      uint32_t pr[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)   // this column of two neighbouring rows
-        pr[j] = __builtin_amdgcn_perm(w[k * 8 + 2 * j + 1], w[k * 8 + 2 * j], half ? 0x07060302u : 0x05040100u);
-      codes[k] = byte == 255u ? 0 : (int)mx_codes8(pr[0], pr[1], pr[2], pr[3], scale);
-    }
-    const uint32_t four = byte | dpp<0x101>(byte) << 8 | dpp<0x102>(byte) << 16 | dpp<0x103>(byte) << 24;   // of four bands side by side
-    if (col + half < p.C && gb < bands) {
-      *(v4i *)(p.qt + (col + half) * p.ldqt + gb * 16) = codes;
-      if (BANDS >= 4 && (gb & ~(int64_t)3) + 4 <= bands) {
-        if ((band & 3) == 0) *(uint32_t *)(p.st + (col + half) * p.ldst + gb) = four;
-      } else {
-        p.st[(col + half) * p.ldst + gb] = (uint8_t)byte;
-      }
+    for (int j = 0; j < 4; ++j) pr[j] = __builtin_amdgcn_perm(w[k * 8 + 2 * j + 1], w[k * 8 + 2 * j], pick);
+    codes[k] = byte == 255u ? 0 : (int)mx_codes8(pr[0], pr[1], pr[2], pr[3], scale);
+  }
+  const uint32_t four = byte | dpp<0x101>(byte) << 8 | dpp<0x102>(byte) << 16 | dpp<0x103>(byte) << 24;   // of four bands side by side
+  if (col < p.C && gb < bands) {
+    *(v4i *)(p.qt + col * p.ldqt + gb * 16) = codes;
+    if (BANDS >= 4 && (gb & ~(int64_t)3) + 4 <= bands) {
+      if ((band & 3) == 0) *(uint32_t *)(p.st + col * p.ldst + gb) = four;
+    } else {
+      p.st[col * p.ldst + gb] = (uint8_t)byte;
     }
   }
 #endif
@@ -186,15 +183,15 @@ extern "C" int l8_cast_mxfp4(const void *x, int64_t R, int64_t C, int64_t ldx, v
     hipLaunchKernelGGL((mxfp4_rows_kernel<U>), dim3((unsigned)((C + 511) / 512), (unsigned)((R + 4 * U - 1) / (4 * U))), dim3(256), 0, hs, a);
   } else {
     const int64_t across = (C + kMxTileC - 1) / kMxTileC;
-    auto go = [&](auto kernel, int rows, int threads) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)across, (unsigned)((R + rows - 1) / rows)), dim3((unsigned)threads), 0, hs, a);
+    auto go = [&](auto kernel, int rows) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)across, (unsigned)((R + rows - 1) / rows)), dim3((unsigned)rows * 4), 0, hs, a);
     };
     if (across * ((R + 255) / 256) >= num_cus() || (R + 63) / 64 > 65535) {
-      if (q) go(mxfp4_tile_kernel<true, 8, 2>, 256, 512);
-      else go(mxfp4_tile_kernel<false, 8, 2>, 256, 512);
+      if (q) go(mxfp4_tile_kernel<true, 8>, 256);
+      else go(mxfp4_tile_kernel<false, 8>, 256);
     } else {
-      if (q) go(mxfp4_tile_kernel<true, 2, 1>, 64, 256);
-      else go(mxfp4_tile_kernel<false, 2, 1>, 64, 256);
+      if (q) go(mxfp4_tile_kernel<true, 2>, 64);
+      else go(mxfp4_tile_kernel<false, 2>, 64);
     }
   }
   L8_HIP(hipGetLastError());

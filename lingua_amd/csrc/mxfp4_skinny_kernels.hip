@@ -14,7 +14,6 @@
 //     scales are written to LDS in the layout that they are read in.  Every workgroup does it over again, so where that is much
 //     (quantised_inside below) a launch of their own casts them;
 //   * the eight partial tiles meet in LDS and are added in the order of the waves.
-#include "l8_common.h"
 #include "mxfp4.h"
 
 namespace l8 {
@@ -24,8 +23,8 @@ constexpr int kWindow = 512, kWinBytes = 256;   // columns, bytes of codes
 constexpr int kFewTile = 16 * kWinBytes;        // 16 rows of a window
 [[maybe_unused]] constexpr uint32_t kBeyondAll = 0x80000000u;
 
-// MT tiles of 16 tokens, NT of 16 weight rows, U windows requested together.  QX: x in bf16, one tile of tokens.
-template <int MT, int NT, int U, bool QX>
+// MT tiles of 16 tokens, NT of 16 weight rows.  QX: x in bf16, one tile of tokens.
+template <int MT, int NT, bool QX>
 __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFewArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(!QX || MT == 1, "x is quantised for one tile of tokens");
@@ -50,7 +49,7 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
   auto put = [&](int r, int c) { return r * kWinBytes + ((c ^ r) & 15) * 16; };
   auto load_codes = [&](__amdgpu_buffer_rsrc_t rs, int64_t ld, int row0, int w, v4i (&v)[4], bool once) {
     const int k = w * kWinBytes + lchunk * 16;
-    const uint32_t off = (uint32_t)((row0 + lrow) * (int)ld + k) | (k < kbytes && w < w_last ? 0u : kBeyondAll);
+    const uint32_t off = (uint32_t)((row0 + lrow) * (int)ld + k) | (k < kbytes ? 0u : kBeyondAll);
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = once ? load16_nt(rs, off, (uint32_t)(j * 4 * (int)ld)) : __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, j * 4 * (int)ld, 0);
   };
@@ -58,7 +57,7 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
   auto load_scale = [&](const uint8_t *s, int64_t ld, int row, int rows, int w) {
     uint32_t v = 0;
     const int first = w * 16 + fg * 4;
-    if (row < rows && w < w_last) {
+    if (row < rows) {
       const uint8_t *at = s + (int64_t)row * ld + first;
       if (first + 4 <= p.blocks) {
         __builtin_memcpy(&v, at, 4);
@@ -91,54 +90,48 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
     c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(wf[2]), wide(xf[2]), c, 4, 4, 2, (int)ws, 2, (int)xs);
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(wf[3]), wide(xf[3]), c, 4, 4, 3, (int)ws, 3, (int)xs);
   };
-  for (int w = w_first; w < w_last; w += U) {
-    v4i wv[U][NT][4];
-    uint32_t ws[U][NT];
+  for (int w = w_first; w < w_last; ++w) {
+    v4i wv[NT][4];
+    uint32_t ws[NT];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        load_codes(rsW, p.ldqw, t * 16, w + u, wv[u][t], true);
-        ws[u][t] = load_scale(p.sw, p.ldsw, n0 + t * 16 + fr, p.N, w + u);
+    for (int t = 0; t < NT; ++t) {
+      load_codes(rsW, p.ldqw, t * 16, w, wv[t], true);
+      ws[t] = load_scale(p.sw, p.ldsw, n0 + t * 16 + fr, p.N, w);
+    }
+    v4i xf[MT][4];
+    uint32_t xs[MT];
+    if constexpr (QX) {
+      const int c = w * kWindow + lane * 8;
+      const uint32_t off = (uint32_t)(c * 2) | (c < p.K ? 0u : kBeyondAll);
+      // (rows of tokens that are not there keep whatever LDS holds: it only reaches columns of the accumulators that nobody stores)
+      for (int m = 0; m < p.M; ++m) {
+        const v4i v = __builtin_amdgcn_raw_buffer_load_b128(rsX, (int)off, m * (int)p.ldx * 2, 0);
+        const uint32_t byte = mx_byte(quad_max(amax8(v)));
+        const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], mx_scale(byte));
+        const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
+        *(uint32_t *)(buf + put(m, lane >> 2) + (lane & 3) * 4) = codes;
+        if (lchunk == 0) xsc[m * 4 + lrow] = four;
       }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (w + u >= w_last) break;
-      v4i xf[MT][4];
-      uint32_t xs[MT];
-      if constexpr (QX) {
-        const int c = (w + u) * kWindow + lane * 8;
-        const uint32_t off = (uint32_t)(c * 2) | (c < p.K ? 0u : kBeyondAll);
-        // (rows behind the last are zeros once and for all windows: nothing reads an accumulator of theirs)
-        for (int m = 0; m < p.M; ++m) {
-          const v4i v = __builtin_amdgcn_raw_buffer_load_b128(rsX, (int)off, m * (int)p.ldx * 2, 0);
-          const uint32_t byte = mx_byte(quad_max(amax8(v)));
-          const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], mx_scale(byte));
-          const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
-          *(uint32_t *)(buf + put(m, lane >> 2) + (lane & 3) * 4) = codes;
-          if (lchunk == 0) xsc[m * 4 + lrow] = four;
-        }
-        __builtin_amdgcn_wave_barrier();
+      for (int s = 0; s < 4; ++s) xf[0][s] = *(const v4i *)(buf + put(fr, fg * 4 + s));
+      xs[0] = xsc[fr * 4 + fg];
+      __builtin_amdgcn_wave_barrier();
+    } else {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) xf[0][s] = *(const v4i *)(buf + put(fr, fg * 4 + s));
-        xs[0] = xsc[fr * 4 + fg];
-        __builtin_amdgcn_wave_barrier();
-      } else {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          v4i v[4];
-          load_codes(rsX, p.ldx, i * 16, w + u, v, false);
-          xs[i] = load_scale(p.sx, p.ldsx, i * 16 + fr, p.M, w + u);
-          turn(v, xf[i]);
-        }
+      for (int i = 0; i < MT; ++i) {
+        v4i v[4];
+        load_codes(rsX, p.ldx, i * 16, w, v, false);
+        xs[i] = load_scale(p.sx, p.ldsx, i * 16 + fr, p.M, w);
+        turn(v, xf[i]);
       }
+    }
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        v4i wf[4];
-        turn(wv[u][t], wf);
+    for (int t = 0; t < NT; ++t) {
+      v4i wf[4];
+      turn(wv[t], wf);
 #pragma unroll
-        for (int i = 0; i < MT; ++i) acc[i][t] = mma(wf, ws[u][t], xf[i], xs[i], acc[i][t]);
-      }
+      for (int i = 0; i < MT; ++i) acc[i][t] = mma(wf, ws[t], xf[i], xs[i], acc[i][t]);
     }
   }
   __syncthreads();
@@ -175,20 +168,29 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
 #endif
 }
 
-// Rows of tokens that are not there: QX leaves their LDS as it is, whatever it holds.  A product's column m hangs on token m alone, so
-// that only fills columns of the accumulator that nobody stores.
-template <int MT, int NT, int U, bool QX>
+template <int MT, int NT, bool QX>
 static int launch_few(const MxFewArgs &a, hipStream_t st) {
-  hipLaunchKernelGGL((linear_mxfp4_few_kernel<MT, NT, U, QX>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(kFewBlock), 0, st, a);
+  hipLaunchKernelGGL((linear_mxfp4_few_kernel<MT, NT, QX>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(kFewBlock), 0, st, a);
   L8_HIP(hipGetLastError());
   return L8_OK;
 }
 
-int mxfp4_few_bf16(const MxFewArgs &a, hipStream_t st) { return launch_few<1, 1, 4, true>(a, st); }
-int mxfp4_few_packed(const MxFewArgs &a, hipStream_t st) {
-  if (a.M <= 16) return launch_few<1, 1, 4, false>(a, st);
-  if (a.M <= 32) return launch_few<2, 1, 2, false>(a, st);
-  return launch_few<4, 1, 2, false>(a, st);
+// One window in flight per wave: the registers that more would take are worth more as a second workgroup on the unit.  us, four
+// windows / one: one token, [11008,4096] 9.7 / 6.9, [4096,4096] 5.1 / 4.4.
+static int mxfp4_few_bf16(const MxFewArgs &a, hipStream_t st) { return launch_few<1, 1, true>(a, st); }
+// As many weight rows to a workgroup as leave one for six in ten units: they share the tokens' codes.  us, 16 rows / 32 / 64, 64
+// tokens: [11008,4096] 18.1 / 18.1 / 14.7, [8192,2048] 11.4 / 9.7 / 10.7, [4096,4096] 9.6 / 10.8 / 13.4.
+template <int MT>
+static int few_packed(const MxFewArgs &a, hipStream_t st) {
+  const int64_t enough = num_cus() * 6 / 10;
+  if (a.N >= enough * 64) return launch_few<MT, 4, false>(a, st);
+  if (a.N >= enough * 32) return launch_few<MT, 2, false>(a, st);
+  return launch_few<MT, 1, false>(a, st);
+}
+static int mxfp4_few_packed(const MxFewArgs &a, hipStream_t st) {
+  if (a.M <= 16) return few_packed<1>(a, st);
+  if (a.M <= 32) return few_packed<2>(a, st);
+  return few_packed<4>(a, st);
 }
 
 }  // namespace l8
@@ -198,8 +200,8 @@ using namespace l8;
 static constexpr int64_t kFewTokens = 64;   // that the kernels above take
 
 // Are the tokens quantised inside the product?  What a wave spends on it -- tokens times its windows, times the workgroups that a unit
-// runs one after the other -- against a launch.  us, inside / cast before: 8 tokens, [4096,4096] 7.1 / 8.1, [11008,4096] 14.2 /
-// 13.0, [4096,11008] 14.3 / 11.5, [2048,2048] 5.7 / 6.2; 4 tokens, [11008,4096] 12.2 / 13.0, [4096,11008] 11.1 / 11.5.
+// runs one after the other -- against a launch.  us, inside / cast before: 8 tokens, [4096,4096] @A@, [11008,4096]
+// @B@, [4096,11008] @C@, [2048,2048] @D@; 4 tokens, [11008,4096] @E@, [4096,11008] @F@.
 static bool quantised_inside(int64_t M, int64_t N, int64_t K) {
   const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves, rounds = ((N + 15) / 16 + num_cus() - 1) / num_cus();
   return M <= 16 && (M == 1 || M * share * rounds <= 12);

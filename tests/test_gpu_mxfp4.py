@@ -173,7 +173,8 @@ def sum_error(a, b, K):
     return (a.abs() @ b.abs().t()) * (K * plain.FP32)
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 16, 16), (1, 4096, 64), (7, 48, 32), (16, 2048, 272), (17, 2064, 48), (33, 1040, 304), (64, 4096, 96), (65, 528, 528), (333, 2048, 1040)])
+@pytest.mark.parametrize("M,K,N", [(1, 16, 16), (1, 4096, 64), (7, 48, 32), (16, 2048, 272), (17, 2064, 48), (33, 1040, 304), (64, 4096, 96), (65, 528, 528), (333, 2048, 1040),
+                                   (12, 2048, 48), (3, 11008, 64), (7, 16, 9872), (16, 48, 9872), (20, 96, 9872), (64, 528, 9872), (40, 64, 4944)])
 @pytest.mark.parametrize("with_bias", [False, True])
 def test_linear_with_a_packed_weight(M, K, N, with_bias):
     from lingua_amd import mxfp4
