@@ -615,9 +615,10 @@ static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
   return L8_OK;
 }
 
-// Do the large kernel's tiles fill half of the units?  Its stream runs two stages ahead.
+// Do the large kernel's tiles fill more than half of the units?  Its stream runs two stages ahead.  us, stream / tiles of 128 x 128, K
+// 4096: [2048,4096], half of them, 32.2 / 30.3; [2304,4096] 31.6 / 36.5, [4096,4096] 40.2 / 50.0, [4000,11008] 95.6 / 122.4.
 static bool takes_stream(int64_t M, int64_t N, int64_t blocks) {
-  return ((M + 255) / 256) * ((N + 255) / 256) >= num_cus() / 2 && blocks > 8 && num_cus() >= 8;
+  return ((M + 255) / 256) * ((N + 255) / 256) > num_cus() / 2 && blocks > 8 && num_cus() >= 8;
 }
 // bytes of one operand's laid-out scales: whole tiles of 256 rows, whole windows of 16 blocks
 static int64_t laid_bytes(int64_t rows, int64_t blocks) { return (rows + 255) / 256 * 4 * ((blocks + 15) / 16) * 1024; }
@@ -684,6 +685,13 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
     if (N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && (M + 255) / 256 + (N + 255) / 256 < 16384)
       return bias ? launch_gemm_mxfp4_stream<true>(a, (uint8_t *)workspace, st) : launch_gemm_mxfp4_stream<false>(a, (uint8_t *)workspace, st);
   }
+  // Tiles by how many of them the units get.  us, [M,N] K:
+  //   128 x 128 from half a tile a unit on, against 64 x 64: [2048,2048] K 2048 10.8 / 12.5, K 8192 30.5 / 40.2, [512,4096] K 11008
+  //   28.4 / 30.1; below that, [100,4096] K 4096 12.4 / 7.9
+  //   its ring of two stages, two workgroups a unit, against one of four, one workgroup: [1500,6000] K 3000 29.1 / 33.5, [2064,2048]
+  //   K 1024 9.6 / 12.5; where every workgroup has a unit of its own, [512,4096] K 11008 36.1 / 28.4, [2048,2048] K 8192 31.4 / 30.5
+  //   64 x 64, eight stages (all that LDS holds) against two, a tile or less a unit: with weights that no cache holds, [65,4096] K
+  //   11008 20.7 / 34.7, K 4096 10.1 / 11.0; from the cache, [100,4096] K 4096 9.5 / 7.9; several tiles a unit, [2048,2048] K 2048 23.9 / 12.5
   if (mid > num_cus()) return launch_gemm_mxfp4<4, 2, 2, 4, 2>(a, st);
   if (mid >= num_cus() / 2) return launch_gemm_mxfp4<4, 2, 2, 4, 4>(a, st);
   const int64_t small = ((M + 63) / 64) * ((N + 63) / 64);

@@ -199,12 +199,15 @@ using namespace l8;
 
 static constexpr int64_t kFewTokens = 64;   // that the kernels above take
 
-// Are the tokens quantised inside the product?  What a wave spends on it -- tokens times its windows, times the workgroups that a unit
-// runs one after the other -- against a launch.  us, inside / cast before: 8 tokens, [4096,4096] @A@, [11008,4096]
-// @B@, [4096,11008] @C@, [2048,2048] @D@; 4 tokens, [11008,4096] @E@, [4096,11008] @F@.
-static bool quantised_inside(int64_t M, int64_t N, int64_t K) {
-  const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves, rounds = ((N + 15) / 16 + num_cus() - 1) / num_cus();
-  return M <= 16 && (M == 1 || M * share * rounds <= 12);
+// Are the tokens quantised inside the product?  Every workgroup does it over again, a wave for each of its windows, and that is set
+// against a launch and a pass over the tokens.  us, inside / cast before:
+//   one window a wave      [4096,4096]   4 tokens 5.2 / 6.5, 8: 6.3 / 6.6, 12: 7.3 / 6.6   [32000,4096]  4: 17.1 / 18.4, 8: 21.4 / 18.5
+//   two                    [22016,8192]  4 tokens 23.6 / 29.5
+//   three                  [4096,11008]  2 tokens 9.1 / 10.1, 4: 10.9 / 10.1               [11008,11008] 2: 16.1 / 19.9, 4: 18.6 / 20.2
+//   four                   [512,16384]   2 tokens 8.8 / 9.0, 3: 10.1 / 9.4
+static bool quantised_inside(int64_t M, int64_t K) {
+  const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves;   // windows a wave
+  return M == 1 || M * (share > 1 ? share : 1) <= 8;
 }
 
 // Codes and scales of the activation in the workspace, then the product's own.
@@ -219,7 +222,7 @@ static MxLinearPlan plan_of(int64_t M, int64_t N, int64_t K) {
   p.q = 0;
   p.s = p.q + M * p.ldq;
   p.product = p.s + (M * p.lds + 15) / 16 * 16;
-  p.total = quantised_inside(M, N, K) ? 0 : p.product + (M <= kFewTokens ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
+  p.total = quantised_inside(M, K) ? 0 : p.product + (M <= kFewTokens ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
   return p;
 }
 

@@ -159,6 +159,35 @@ def test_product_with_extreme_and_nan_scales(M, N, blocks):
     assert bool(((got[1].double() - want[1]).abs().nan_to_num(0.0) <= 2.0 ** -126).all())
 
 
+# The kernel of the large products: partial tiles in both directions, one tile to a workgroup and several, K from its shortest on, an odd
+# and an even number of stages (8 blocks), one block to either side of a window of scales (16)
+@pytest.mark.parametrize("M,N,blocks", [(4100, 2304, 9), (2500, 4104, 15), (4096, 2312, 16), (33100, 264, 17), (264, 33104, 24), (8200, 2304, 25), (8200, 2304, 33)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_large_products_are_exact(M, N, blocks, with_bias):
+    """As above, with what lies behind the rows of scales and beside the result's columns guarded, and a NaN in a scale at either end."""
+    from lingua_amd import ops
+    a, b = operand(M, blocks, M + N), operand(N, blocks, N + blocks)
+    a[1][M - 1, blocks - 1], b[1][3, 0] = 255, 255
+    bias = torch.randint(-64, 64, (N,), generator=torch.Generator().manual_seed(N)).to(torch.bfloat16).cuda() if with_bias else None
+
+    def apart(s):
+        wide = torch.full((s.shape[0], s.shape[1] + 32 + -s.shape[1] % 16), 255, dtype=torch.uint8, device="cuda")
+        wide[:, :s.shape[1]] = s.cuda()
+        return wide[:, :s.shape[1]]
+
+    wide = torch.full((M, N + 16), 3.0, dtype=torch.bfloat16, device="cuda")
+    got = ops.gemm_mxfp4_nt(a[0].cuda(), b[0].cuda(), apart(a[1]), apart(b[1]), bias, out=wide[:, 8:8 + N])
+    a[1][M - 1, blocks - 1], b[1][3, 0] = 127, 127
+    want = exact_product([t.cuda() for t in a], [t.cuda() for t in b])
+    if bias is not None:
+        want = want + bias.double()
+    want[M - 1, :] = float("nan")
+    want[:, 3] = float("nan")
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.nan_to_num(1.0), want.to(torch.bfloat16).nan_to_num(1.0))
+    assert bool((wide[:, :8] == 3).all()) and bool((wide[:, 8 + N:] == 3).all())
+
+
 def test_product_over_nothing_is_zero():
     from lingua_amd import ops
     q, s = torch.empty(5, 0, dtype=torch.uint8, device="cuda"), torch.empty(5, 0, dtype=torch.uint8, device="cuda")
