@@ -10,12 +10,14 @@
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPFunctions.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "../../include/lingua_fp8.h"
@@ -860,6 +862,30 @@ variable_list once(variable_list grads, const char *what) {
   if (!at::GradMode::is_enabled()) return grads;
   return torch::autograd::DelayedError(std::string(what) + " is not differentiable twice", (int)grads.size())(std::move(grads));
 }
+// A leaf's gradient is accumulated on the stream that its node was made on, and the node lives as long as a graph that holds it.  One
+// made on the default stream cannot take part in a capture: the captured backward pass would end the process.
+void refuse_captured(std::initializer_list<const Tensor *> inputs, const char *what) {
+  bool capturing = false, asked = false;
+  for (const Tensor *t : inputs) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (!node) continue;
+    const auto stream = node->stream();
+    if (!stream || stream->id() != 0) continue;
+    if (!asked) capturing = c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None, asked = true;
+    TORCH_CHECK(!capturing, what, ": captured while a graph of the same leaf, made on the default stream, is alive: release it first, or make it on another stream");
+  }
+}
+PyObject *refuse_captured_py(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 4) throw std::runtime_error("refuse_captured: 4 arguments");
+  Tensor t[3];
+  for (int i = 0; i < 3; ++i)
+    if (THPVariable_Check(args[i])) t[i] = THPVariable_Unpack(args[i]);
+  if (at::GradMode::is_enabled()) refuse_captured({&t[0], &t[1], &t[2]}, PyUnicode_AsUTF8(args[3]));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
 // A gradient as the kernels take it: bf16, of `sizes`, dense rows.
 Tensor gradient(const Tensor &g, const char *what) {
   TORCH_CHECK(g.scalar_type() == at::kBFloat16, what, " backward: bf16 gradients required, got ", g.scalar_type());
@@ -939,6 +965,7 @@ PyObject *add_rmsnorm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   variable_list out;
   {
     pybind11::gil_scoped_release no_gil;
+    if (at::GradMode::is_enabled()) refuse_captured({&x, &res, &w}, AddRMSNorm::kName);
     out = AddRMSNorm::apply(x, res, w, eps, want_col);
   }
   return tuple_of({out[0], out[1], out[2], out[3], want_col ? out[4] : Tensor()});
@@ -1048,6 +1075,7 @@ PyObject *rotary_pair(PyObject *, PyObject *const *args, Py_ssize_t n) {
   variable_list y;
   {
     pybind11::gil_scoped_release no_gil;
+    if (at::GradMode::is_enabled()) refuse_captured({&x[0], &x[1]}, "rotary");
     y = Rotary::apply(x[0], x[1], cos, sin, pos.defined() ? std::optional<Tensor>(pos) : std::nullopt, in_halves);
   }
   return tuple_of({y[0], y[1]});
@@ -1134,6 +1162,7 @@ PyObject *mxfp4_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
   {
     pybind11::gil_scoped_release no_gil;
     const bool grad = at::GradMode::is_enabled();
+    if (grad) refuse_captured({&a, &w, &bias}, "mxfp4_linear");
     y = Mxfp4Linear::apply(a, w, bias.defined() ? std::optional<Tensor>(bias) : std::nullopt, grad && a.requires_grad(), grad && w.requires_grad());
   }
   return wrap(y);
@@ -1191,6 +1220,7 @@ PyMethodDef methods[] = {
     {"mxfp4_to_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_to_bf16)), METH_FASTCALL, nullptr},
     {"add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm)), METH_FASTCALL, nullptr},
     {"rotary_pair", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_pair)), METH_FASTCALL, nullptr},
+    {"refuse_captured", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(refuse_captured_py)), METH_FASTCALL, nullptr},
     {"mxfp4_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_packed)), METH_FASTCALL, nullptr},
     {"mxfp4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_linear)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -599,6 +599,12 @@ def _plain_call():
             torch._C._get_tracing_state() is None and not torch.compiler.is_compiling())
 
 
+def _refuse_captured(a, b, c, what):
+    """An error where a captured backward pass of these leaves would end the process (csrc/native.cpp)."""
+    if a.is_cuda and not torch.compiler.is_compiling():
+        _lib.native_for(a.get_device()).refuse_captured(a, b, c, what)
+
+
 class Fp8Linear(torch.nn.Linear):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         weight, bias = self.weight, self.bias

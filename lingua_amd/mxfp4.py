@@ -73,6 +73,7 @@ def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Ten
         if y is not None:
             return y
     _check_operands(x, weight)
+    f8._refuse_captured(x, weight, bias, "mxfp4_linear")
     if x.dim() == 2:
         return Mxfp4LinearFn.apply(x, weight, bias)
     return Mxfp4LinearFn.apply(x.flatten(end_dim=-2), weight, bias).unflatten(0, x.shape[:-1])

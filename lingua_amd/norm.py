@@ -109,6 +109,7 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, e
             if f8.config.share_input_casts:   # (the memo keeps its tensor: not the graph behind it)
                 f8._fwd_cast.put(y.detach().flatten(end_dim=-2), (q, s, col), "rmsnorm")
             return h, y
+    f8._refuse_captured(x, residual, weight, "add_rmsnorm")
     return Fp8AddRMSNormFn.apply(x, residual, weight, eps, training)
 
 

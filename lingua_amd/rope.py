@@ -54,6 +54,7 @@ def rotary(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Ten
         res = _lib.native_for(xq.get_device()).rotary_pair(xq, xk, cos, sin, positions, layout == "half")
         if res is not None:
             return res
+    f8._refuse_captured(xq, xk, None, "rotary")
     return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half")
 
 

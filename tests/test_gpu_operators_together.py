@@ -153,3 +153,61 @@ def test_backward_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def calls(x, w, gain, cos, sin):
+    """Each operator's differentiable call on the leaves x [8,64], w [64,64] and gain [64]."""
+    from lingua_amd import mxfp4, norm, rope
+    return {"add_rmsnorm": lambda: norm.add_rmsnorm(x, x.detach(), gain, 1e-5)[1],
+            "rotary": lambda: rope.rotary(x.view(1, 8, 2, 32), x.view(1, 8, 2, 32).detach(), cos, sin)[0],
+            "mxfp4_linear": lambda: mxfp4.mxfp4_linear(x, w)}
+
+
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("name", ["add_rmsnorm", "mxfp4_linear"])
+def test_capture_is_refused_while_a_graph_of_the_leaves_lives(name, native, monkeypatch):
+    from lingua_amd import float8, rope
+    if not native:
+        monkeypatch.setattr(float8, "_plain_call", lambda: False)
+    x, w, gain = (seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (64, 64), (64,))))
+    call = calls(x, w, gain, *(t.cuda() for t in rope.rotary_tables(32, 8)))[name]
+    want = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="same leaf"):
+            call()
+        with torch.no_grad():
+            out = call()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want.detach())
+
+
+def test_operands_do_not_share_a_gradient():
+    """Both operands of the residual sum have the same gradient, each in memory of its own."""
+    from lingua_amd import norm
+    x, res, gain = (seeded_bf16(s, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (8, 64), (64,))))
+    for _ in range(2):
+        h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+        (h.sum() + y.sum()).backward()
+        assert x.grad.data_ptr() != res.grad.data_ptr() and torch.equal(x.grad, res.grad)
+
+
+@pytest.mark.parametrize("name", ["add_rmsnorm", "rotary", "mxfp4_linear"])
+def test_compiled_calls_equal_eager_ones(name):
+    """A compiler's tracer does not see into the calls: they stay whole, and so do their gradients."""
+    from lingua_amd import rope
+    leaves = [seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (64, 64), (64,)))]
+    tables = [t.cuda() for t in rope.rotary_tables(32, 8)]
+
+    def run(x, w, gain):
+        return calls(x, w, gain, *tables)[name]() * 2.0
+
+    torch._dynamo.reset()
+    want, got = run(*leaves), torch.compile(run, backend="eager")(*leaves)
+    torch._dynamo.reset()
+    gy = seeded_bf16(tuple(want.shape), std=0.01, seed=5).cuda()
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, leaves, gy, allow_unused=True), torch.autograd.grad(want, leaves, gy, allow_unused=True)):
+        assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
