@@ -345,7 +345,8 @@ int l8_add_rmsnorm_bwd(const void *gy, const void *gh, const void *h, const void
  *   positions int64 or (positions_i32) int32, element (b,s) at b * pos_b + s * pos_s; NULL: s.  A token at a position outside
  *   [0, length) becomes NaN.
  *   inverse: the transposed rotation, which is the backward pass.
- * Requires D even, at most 512, rot even and at least 2, fewer than 2^24 tokens.  x and y may not overlap. */
+ * Requires D even, at most 512, rot even and at least 2, fewer than 2^24 tokens; without in_halves x on 4-byte lines and strides even.  x and
+ * y may not overlap. */
 typedef struct {
   const void *x;
   void *y;

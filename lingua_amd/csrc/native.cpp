@@ -991,8 +991,17 @@ void rotate(const Tensor (&x)[2], Tensor (&y)[2], const Tensor &cos, const Tenso
   check(lib.l8_rotary(two, B, S, D, 2 * cos.size(1), in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), cos.size(0),
                       pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kInt, pos_b, pos_s, stream_of(one.get_device())), "l8_rotary");
 }
+// Dense heads, and for the interleaved layout pairs on 4-byte lines?
+bool heads_fit(const Tensor &t, bool in_halves) {
+  if (t.stride(3) != 1) return false;
+  if (in_halves) return true;
+  int64_t odd = (int64_t)((uintptr_t)t.const_data_ptr() >> 1);
+  for (int i = 0; i < 3; ++i)
+    if (t.size(i) > 1) odd |= t.stride(i);
+  return (odd & 1) == 0;
+}
 // May the extension take these operands?
-bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos) {
+bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves) {
   const Tensor &one = x[0].defined() ? x[0] : x[1];
   if (!one.is_cuda() || one.dim() != 4) return false;
   const int device = one.get_device();
@@ -1000,7 +1009,7 @@ bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const T
   if (c10::hip::current_device() != device) return false;
   for (const Tensor &t : x)
     if (t.defined() && (t.scalar_type() != at::kBFloat16 || t.layout() != at::kStrided || !t.is_cuda() || t.get_device() != device || t.dim() != 4 || t.numel() < 1 ||
-                        t.size(0) != B || t.size(1) != S || t.size(3) != D || t.stride(3) != 1))
+                        t.size(0) != B || t.size(1) != S || t.size(3) != D || !heads_fit(t, in_halves)))
       return false;
   for (const Tensor *t : {&cos, &sin})
     if (t->scalar_type() != at::kFloat || t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device || t->dim() != 2 || t->sizes() != cos.sizes() ||
@@ -1034,7 +1043,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     for (int i = 0; i < 2; ++i) {
       if (!grads[i].defined() || !ctx->needs_input_grad(i)) continue;
       TORCH_CHECK(grads[i].scalar_type() == at::kBFloat16, "rotary backward: bf16 gradients required, got ", grads[i].scalar_type());
-      x[i] = grads[i].stride(3) == 1 ? grads[i] : grads[i].contiguous();
+      x[i] = heads_fit(grads[i], ctx->saved_data["half"].toBool()) ? grads[i] : grads[i].clone(at::MemoryFormat::Contiguous);
     }
     if (x[0].defined() || x[1].defined()) {
       const c10::DeviceGuard guard((x[0].defined() ? x[0] : x[1]).device());
@@ -1053,7 +1062,7 @@ PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
   const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
   const bool in_halves = truth(args[5]), inverse = truth(args[6]);
-  if (!rotates(x, cos, sin, pos)) Py_RETURN_NONE;
+  if (!rotates(x, cos, sin, pos, in_halves)) Py_RETURN_NONE;
   Tensor y[2];
   {
     pybind11::gil_scoped_release no_gil;
@@ -1071,7 +1080,7 @@ PyObject *rotary_pair(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
   const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
   const bool in_halves = truth(args[5]);
-  if (!rotates(x, cos, sin, pos)) Py_RETURN_NONE;
+  if (!rotates(x, cos, sin, pos, in_halves)) Py_RETURN_NONE;
   variable_list y;
   {
     pybind11::gil_scoped_release no_gil;

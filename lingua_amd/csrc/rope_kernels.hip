@@ -128,10 +128,16 @@ __global__ __launch_bounds__(kRotBlock) void rotary_kernel(const RotaryArgs p) {
 
 using namespace l8;
 
-extern "C" int l8_rotary(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, int64_t rot, int in_halves, int inverse,
+extern "C" int l8_rotary(const l8_rotary_operand *given, int64_t B, int64_t S, int64_t D, int64_t rot, int in_halves, int inverse,
                          const float *cos, const float *sin, int64_t table_row, int64_t table_col, int64_t length,
                          const void *positions, int positions_i32, int64_t pos_b, int64_t pos_s, void *stream) {
-  L8_REQUIRE(two && B >= 0 && S >= 0 && D >= 0 && two[0].heads >= 0 && two[1].heads >= 0, "l8_rotary: null pointer or negative shape");
+  L8_REQUIRE(given && B >= 0 && S >= 0 && D >= 0 && given[0].heads >= 0 && given[1].heads >= 0, "l8_rotary: null pointer or negative shape");
+  l8_rotary_operand two[2] = {given[0], given[1]};
+  for (auto &t : two) {   // the stride of a single one is never used
+    if (B <= 1) t.ldb = 0;
+    if (S <= 1) t.lds = 0;
+    if (t.heads <= 1) t.ldh = 0;
+  }
   if (B == 0 || S == 0 || D == 0 || (two[0].heads == 0 && two[1].heads == 0)) return L8_OK;
   L8_REQUIRE(D <= 2 * kRotBlock && D % 2 == 0, "l8_rotary: heads of an even number of columns up to %d, got %lld", 2 * kRotBlock, (long long)D);
   L8_REQUIRE(rot >= 2 && rot % 2 == 0 && rot <= D, "l8_rotary: an even number of columns up to the head's %lld turns, got %lld", (long long)D, (long long)rot);

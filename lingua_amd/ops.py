@@ -878,8 +878,9 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
             outs.append(None)
             items += [0] * 6
             continue
-        if t.numel() and (t.stride(3) != 1 or t.data_ptr() % 2):
-            t = t.contiguous()
+        # (the interleaved layout reads pairs from 4-byte lines)
+        if t.numel() and (t.stride(3) != 1 or (not in_halves and (t.data_ptr() % 4 or any(n > 1 and step % 2 for n, step in zip(t.shape[:3], t.stride()))))):
+            t = t.clone(memory_format=torch.contiguous_format)
         y = torch.empty(t.shape, dtype=torch.bfloat16, device=dev)
         keep.append(t)
         outs.append(y)

@@ -67,6 +67,21 @@ def test_positions_strides_and_gradients(layout, dtype, host):
     check(oq.detach(), q.detach().cpu(), cos[pos[1].long()][None, :, None], sin[pos[1].long()][None, :, None], half)
 
 
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("B,S,H", [(2, 5, 3), (1, 7, 1), (4, 1, 2)])
+def test_heads_at_odd_elements(layout, B, S, H, host):
+    """Operands and gradients that start at an odd element and whose rows are an odd number of elements apart."""
+    from lingua_amd import rope
+    D, rot = 32, 16
+    cos, sin = rope.rotary_tables(rot, S)
+    odd = [seeded_bf16((B * S, H * D + 5), seed=i).cuda()[:, 3:3 + H * D].unflatten(1, (H, D)).unflatten(0, (B, S)) for i in range(3)]
+    q, k = odd[0].detach().requires_grad_(), odd[1].detach()
+    oq, ok = rope.rotary(q, k, cos.cuda(), sin.cuda(), layout=layout)
+    (dq,) = torch.autograd.grad(oq, q, odd[2])
+    for got, x, s in ((oq.detach(), odd[0], sin), (ok, odd[1], sin), (dq, odd[2], -sin)):
+        check(got, x.cpu(), cos[None, :, None], s[None, :, None], layout == "half")
+
+
 def test_it_is_the_eager_chain_bit_for_bit():
     """The chain that the benchmark's model runs between its projections and its attention."""
     from bench_workloads import apply_rope, rope_tables
