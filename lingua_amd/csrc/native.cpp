@@ -71,6 +71,8 @@ bool as_rows(const Tensor &t, int device, Rows &m) {
   return true;
 }
 
+// Rows on 16-byte lines?
+bool on_16_bytes(const Rows &m) { return ((uintptr_t)m.p % 16) == 0 && m.ld % 8 == 0 && m.cols % 8 == 0; }
 // A dense tensor of `n` elements of one type (quantised copies, scales, amaxes, bias).
 bool dense(const Tensor &t, at::ScalarType type, int64_t n, int device) {
   return t.defined() && t.scalar_type() == type && t.layout() == at::kStrided && t.is_cuda() && t.get_device() == device && t.numel() == n && t.is_contiguous();
@@ -709,7 +711,9 @@ PyObject *add_rmsnorm_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!x.is_cuda() || x.dim() != 2 || res.dim() != 2 || (want_col && !want_q)) Py_RETURN_NONE;
   const int device = x.get_device();
   Rows rx, rr;
-  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || rr.rows != rx.rows || rr.cols != rx.cols || c10::hip::current_device() != device) Py_RETURN_NONE;
+  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || rr.rows != rx.rows || rr.cols != rx.cols || !on_16_bytes(rx) || !on_16_bytes(rr) ||
+      c10::hip::current_device() != device)
+    Py_RETURN_NONE;
   const int64_t R = rx.rows, C = rx.cols;
   const bool f32 = w.scalar_type() == at::kFloat;
   if (!dense(w, f32 ? at::kFloat : at::kBFloat16, C, device)) Py_RETURN_NONE;
@@ -763,7 +767,6 @@ bool as_mx(const Tensor &q, const Tensor &s, int device, MxRows &m) {
   m.q = q.const_data_ptr(), m.s = s.const_data_ptr();
   return m.ldq >= 16 * m.blocks && m.ldq % 16 == 0 && m.lds >= m.blocks && ((uintptr_t)m.q % 16) == 0;
 }
-bool on_16_bytes(const Rows &m) { return ((uintptr_t)m.p % 16) == 0 && m.ld % 8 == 0 && m.cols % 8 == 0; }
 void cast_mx(const Rows &x, const Mx &rows, const Mx &cols, void *stream) {
   check(lib.l8_cast_mxfp4(x.p, x.rows, x.cols, x.ld, rows.qp(), rows.ldq(), rows.sp(), rows.lds(), cols.qp(), cols.ldq(), cols.sp(), cols.lds(), stream), "l8_cast_mxfp4");
 }
@@ -789,7 +792,7 @@ PyObject *cast_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!x.is_cuda() || x.dim() != 2 || (!rowwise && !transposed)) Py_RETURN_NONE;
   const int device = x.get_device();
   Rows rx;
-  if (!as_rows(x, device, rx) || c10::hip::current_device() != device) Py_RETURN_NONE;
+  if (!as_rows(x, device, rx) || !on_16_bytes(rx) || c10::hip::current_device() != device) Py_RETURN_NONE;
   Mx rows, cols;
   {
     pybind11::gil_scoped_release no_gil;
@@ -959,7 +962,7 @@ PyObject *add_rmsnorm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   if (!x.is_cuda()) Py_RETURN_NONE;
   const int device = x.get_device();
   Rows rx, rr;
-  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || x.sizes() != res.sizes() || c10::hip::current_device() != device ||
+  if (!as_rows(x, device, rx) || !as_rows(res, device, rr) || x.sizes() != res.sizes() || !on_16_bytes(rx) || !on_16_bytes(rr) || c10::hip::current_device() != device ||
       !dense(w, w.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16, rx.cols, device))
     Py_RETURN_NONE;
   variable_list out;

@@ -88,6 +88,12 @@ def _rows_2d(t: torch.Tensor, dtype, what: str) -> torch.Tensor:
     return t
 
 
+def _rows_on_lines(t: torch.Tensor, dtype, what: str):
+    """The same, and a copy where a row does not start on a 16-byte line."""
+    t = _rows_2d(t, dtype, what)
+    return t if not t.numel() or t.shape[1] % 8 or rows_on_16_bytes(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def _rows_apart(t: torch.Tensor) -> bool:
     """Is each row dense, whatever lies between two of them?"""
     return t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])
@@ -774,8 +780,8 @@ def add_rmsnorm_cast_rowwise(x: torch.Tensor, residual: torch.Tensor, weight: to
         res = _lib.native_for(x.get_device()).add_rmsnorm_fwd(x, residual, weight, eps, want_q, False, want_rstd, on_lines)
         if res is not None:
             return res[:5]
-    x = _rows_2d(x, torch.bfloat16, what)
-    residual = _rows_2d(residual, torch.bfloat16, what)
+    x = _rows_on_lines(x, torch.bfloat16, what)
+    residual = _rows_on_lines(residual, torch.bfloat16, what)
     if x.shape != residual.shape or x.device != residual.device:
         raise RuntimeError(f"{what}: x and residual must have the same shape and device, got {tuple(x.shape)} and {tuple(residual.shape)}")
     st = _prep(x, what)
@@ -807,7 +813,7 @@ def add_rmsnorm_bwd(gy: torch.Tensor, gh: torch.Tensor, h: torch.Tensor, weight:
     """Backward of the norm of a sum: returns (gx [R,C] bf16, the gradient of either operand, gw [C] of ``gw_dtype``) from the
     gradients gy of the norm and gh of the sum, the sum h (bf16 [R,C]), weight [C], rstd [R,1] fp32."""
     what = "add_rmsnorm_bwd"
-    gy, gh, h = (_rows_2d(t, torch.bfloat16, f"{what}({n})") for t, n in ((gy, "gy"), (gh, "gh"), (h, "h")))
+    gy, gh, h = (_rows_on_lines(t, torch.bfloat16, f"{what}({n})") for t, n in ((gy, "gy"), (gh, "gh"), (h, "h")))
     if gy.shape != h.shape or gh.shape != h.shape or gy.device != h.device or gh.device != h.device:
         raise RuntimeError(f"{what}: gy, gh and h must have the same shape and device")
     st = _prep(h, what)
@@ -940,7 +946,7 @@ def cast_mxfp4(x: torch.Tensor, rowwise: bool = True, transposed: bool = False, 
         res = _lib.native_for(x.get_device()).cast_mxfp4(x, rowwise, transposed, on_lines)
         if res is not None:
             return res[:2] if rowwise else None, res[2:] if transposed else None
-    x = _rows_2d(x, torch.bfloat16, "cast_mxfp4")
+    x = _rows_on_lines(x, torch.bfloat16, "cast_mxfp4")
     st = _prep(x, "cast_mxfp4")
     if not rowwise and not transposed:
         raise RuntimeError("cast_mxfp4: rowwise or transposed, or both")
@@ -1020,7 +1026,7 @@ def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: 
         y = _lib.native_for(x.get_device()).mxfp4_packed(x, qw, sw, bias)
         if y is not None:
             return y
-    x = _rows_2d(x, torch.bfloat16, what)
+    x = _rows_on_lines(x, torch.bfloat16, what)
     qw, sw = _mx_operand(qw, sw, what)
     st = _prep(x, what)
     M, K = x.shape
@@ -1028,8 +1034,6 @@ def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: 
     if (K + MX_BLOCK - 1) // MX_BLOCK != sw.shape[1] or qw.device != x.device:
         raise RuntimeError(f"{what}: x {tuple(x.shape)} on {x.device} and a weight of scales {tuple(sw.shape)} on {qw.device} do not fit")
     bias = _mx_bias(bias, N, x.device, what)
-    if not rows_on_16_bytes(x):
-        x = x.clone(memory_format=torch.contiguous_format)
     qw = _on_16_bytes(qw)
     if M > _MX_FEW_TOKENS:
         sw = _on_16_bytes(sw)

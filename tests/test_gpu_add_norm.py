@@ -198,6 +198,22 @@ def test_captured_norm_replays():
         assert all(torch.equal(bits(a), bits(b)) for a, b in zip(out, want))
 
 
+def test_rows_off_their_lines(host):
+    """Operands and gradients that start at odd elements, an odd number of elements apart: copied, with the results of dense ones."""
+    from lingua_amd import norm
+    R, C = 5, 72
+    odd = [seeded_bf16((R, C + 3), seed=i).cuda()[:, 1:1 + C] for i in range(4)]
+    w = seeded_bf16((C,), seed=9).cuda()
+
+    def run(x, res, gh, gy):
+        x, res = x.detach().requires_grad_(), res.detach().requires_grad_()
+        h, y = norm.add_rmsnorm(x, res, w, EPS)
+        return (h, y) + torch.autograd.grad((h, y), (x, res), (gh, gy))
+
+    for got, want in zip(run(*odd), run(*(t.contiguous() for t in odd))):
+        assert torch.equal(got, want)
+
+
 def test_refusals():
     from lingua_amd import norm, ops
     x, res, w = (t.cuda() for t in inputs((4, 64), torch.bfloat16))

@@ -342,6 +342,22 @@ def test_two_streams_at_once():
     assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
 
 
+def test_rows_off_their_lines(host):
+    """Operands and gradients that start at odd elements, an odd number of elements apart: copied, with the results of dense ones."""
+    from lingua_amd import mxfp4, ops
+    M, K, N = 5, 64, 48
+    x, w, gy = (seeded_bf16((r, c + 3), seed=r + c).cuda()[:, 1:1 + c] for r, c in ((M, K), (N, K), (M, N)))
+
+    def run(x, w, gy):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = mxfp4.mxfp4_linear(x, w)
+        packed = mxfp4.pack(w)
+        return (y, *torch.autograd.grad(y, (x, w), gy), mxfp4.linear_packed(x, *packed), ops.mxfp4_to_bf16(*packed, K))
+
+    for got, want in zip(run(x, w, gy), run(*(t.contiguous() for t in (x, w, gy)))):
+        assert torch.equal(got, want)
+
+
 def test_refusals():
     from lingua_amd import mxfp4, ops
     x = seeded_bf16((4, 64), seed=1).cuda()
