@@ -6,18 +6,20 @@
 // and a byte of scale for it, so the scaling costs no instruction of its own.
 //
 // Structure
-//   * a stage is 128 bytes (256 codes, 8 blocks) of every row of the tile's operands, two matrix instructions deep; lane group g of
-//     the four takes blocks 2 g and 2 g + 1 of a stage, so that its two scale bytes lie side by side.  One half of a stage is multiplied
-//     while the next half's fragments are read;
+//   * a stage is 128 bytes (256 codes, 8 blocks) of every row of the tile's operands, four matrix instructions (32 x 32 x 64) deep; the
+//     lower half of a wave takes blocks 0 .. 3 of a stage, the upper 4 .. 7, so that a lane's four scale bytes are one dword, picked
+//     apart by the instruction's op_sel.  Half of a stage is multiplied while the next half's fragments are read;
 //   * codes go from memory to LDS without passing registers (buffer loads to LDS, whole 128-byte lines), into a ring of NS stages;
 //     scales of two stages (16 bytes a row) travel the same way into a ring of their own;
 //   * LDS rows are 128 bytes in 16-byte chunks, chunk c of row r at position c ^ f(r), f(r) = (r & 7) ^ ((r >> 3) & 1): the
 //     fragment reads of 16 rows cover all banks once.  The permutation is applied on the global side of the loads;
-//   * LDS row tn * 16 + j of a wave's share of B holds row TN * j + tn of that share, so that lane j ends up with TN consecutive
+//   * LDS row tn * 32 + j of a wave's share of B holds row TN * j + tn of that share, so that lane j ends up with TN neighbouring
 //     columns of C and stores them straight from the accumulators;
 //   * rows beyond M / N and chunks beyond K lie outside the buffers' ranges: zeros.  Scale bytes beyond K are cleared when they are
 //     read (what lies behind a row's end may be a NaN);
 //   * workgroups are dealt to the 8 XCDs in contiguous ranges of a grouped tile order, so that an XCD's share panels in its L2.
+// Bound by what a stage costs beside its matrix instructions (512 of some 1200 cycles for a 128 x 128 tile): scales, 16 bytes from every
+// row, fragment reads, the loads' way through the L2, the barrier.
 #include <type_traits>
 #include <utility>
 
@@ -52,10 +54,10 @@ L8_DEV void in_turn(std::integer_sequence<int, I...>, F &&f) {
 template <int WM, int WN, int TM, int TN, int NS>
 __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArgs p) {
 #if defined(__HIP_DEVICE_COMPILE__)
-  constexpr int BM = WM * TM * 16, BN = WN * TN * 16, NW = WM * WN, GROUP = 8;
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32, NW = WM * WN, GROUP = 8;
   constexpr int NLA = BM / 8 / NW, NLB = BN / 8 / NW;           // wave loads (8 rows) of a stage
   constexpr int STAGE = (BM + BN) * 128, SROWS = BM + BN, SLOADS = SROWS / 64, NSW = NS / 2 + 1;
-  static_assert(NS % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && SROWS % 64 == 0 && BM % 64 == 0, "");
+  static_assert((TN == 1 || TN == 2) && NS % 2 == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && SROWS % 64 == 0 && BM % 64 == 0, "");
   static_assert((NS - 2) * (NLA + NLB) <= 63 && (NS - 1) * (NLA + NLB) + NS <= 63, "vmcnt is a 6-bit counter");
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];   // NS stages, NSW windows of scales
   const int lane = threadIdx.x & 63;
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   const int chunk[2] = {(lpos ^ lrow) * 16, (lpos ^ lrow ^ 1) * 16};   // of even and odd groups of 8 rows
   const int a_row = lrow * (int)p.lda, b_row = lrow * TN * (int)p.ldb;
   // row of B (in the tile) that LDS row r of its panel holds
-  auto b_of = [](int r) { return r / (TN * 16) * (TN * 16) + TN * (r % 16) + r % (TN * 16) / 16; };
+  auto b_of = [](int r) { return r / (TN * 32) * (TN * 32) + TN * (r % 32) + r % (TN * 32) / 32; };
   // i-th wave load of stage j's panels into ring slot `slot`
   auto load_one = [&](int j, int slot, int i) __attribute__((always_inline)) {
     const int k0 = j * 128;
@@ -112,11 +114,13 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
     }
   };
 
-  v4f acc[TM][TN];
+  v16f acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
   const int stages = (p.blocks + 7) / 8;
 #pragma unroll
@@ -125,34 +129,37 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
 #pragma unroll
     for (int i = 0; i < NLA + NLB; ++i) load_one(j, j, i);
   }
-  const int frow = lane & 15, fg = lane >> 4;
-  const int fr = (frow & 7) ^ (frow >> 3);
-  const uint32_t foff[2] = {(uint32_t)(frow * 128 + (((fg * 2) ^ fr) * 16)), (uint32_t)(frow * 128 + (((fg * 2 + 1) ^ fr) * 16))};
+  const int frow = lane & 31, fg = lane >> 5;
+  const int fr = (frow & 7) ^ (frow >> 3 & 1);
+  uint32_t foff[4];   // block 4 g + s of a stage
+#pragma unroll
+  for (int s = 0; s < 4; ++s) foff[s] = (uint32_t)(frow * 128 + (((fg * 4 + s) ^ fr) * 16));
   typedef const __attribute__((address_space(3))) v4i *lds_v4i;
-  typedef const __attribute__((address_space(3))) uint16_t *lds_u16;
+  typedef const __attribute__((address_space(3))) uint32_t *lds_u32;
 
-  // Fragments of a stage's two halves of 128 codes (h: blocks 2 g + h), and scales of two stages, a byte for each half.
-  v4i fa[2][TM], fb[2][TN];
+  // Fragments of a stage's four steps of 64 codes (s: blocks 4 g + s), and scales of two stages, a byte for each step.
+  v4i fa[4][TM], fb[4][TN];
   uint32_t sa[2][TM], sb[2][TN];
   uint32_t at, sat, smask;   // of the stage that is read next
   auto open = [&](int j) __attribute__((always_inline)) {
     at = lds0 + (j % NS) * STAGE;
-    sat = lds0 + NS * STAGE + ((j >> 1) % NSW) * (SROWS * 16) + frow * 16 + (j & 1) * 8 + fg * 2;
+    sat = lds0 + NS * STAGE + ((j >> 1) % NSW) * (SROWS * 16) + frow * 16 + (j & 1) * 8 + fg * 4;
     asm volatile("" : "+v"(at), "+v"(sat));
-    const int left = p.blocks - (j * 8 + fg * 2);
-    smask = left >= 2 ? 0xffffu : (left == 1 ? 0xffu : 0u);
+    const int left = p.blocks - (j * 8 + fg * 4);
+    smask = left >= 4 ? 0xffffffffu : left <= 0 ? 0u : (1u << (8 * left)) - 1u;
   };
-  auto read_frag = [&](int h, int r) __attribute__((always_inline)) {   // B0, A0, B1, .. in the order of their use
-    auto of_b = [&](int t) __attribute__((always_inline)) { fb[h][t] = *reinterpret_cast<lds_v4i>(at + BM * 128 + (wn * TN + t) * 2048 + foff[h]); };
-    auto of_a = [&](int t) __attribute__((always_inline)) { fa[h][t] = *reinterpret_cast<lds_v4i>(at + (wm * TM + t) * 2048 + foff[h]); };
-    if (r == 0) of_b(0);
-    else if (r == 1) of_a(0);
-    else if (r <= TN) of_b(r - 1);
-    else of_a(r - TN);
+  auto read_frag = [&](int h, int r) __attribute__((always_inline)) {   // r-th read of half h: two steps of TM + TN
+    const int s = 2 * h + r / (TM + TN), q = r % (TM + TN);
+    auto of_b = [&](int t) __attribute__((always_inline)) { fb[s][t] = *reinterpret_cast<lds_v4i>(at + BM * 128 + (wn * TN + t) * 4096 + foff[s]); };
+    auto of_a = [&](int t) __attribute__((always_inline)) { fa[s][t] = *reinterpret_cast<lds_v4i>(at + (wm * TM + t) * 4096 + foff[s]); };
+    if (q == 0) of_b(0);
+    else if (q == 1) of_a(0);
+    else if (q <= TN) of_b(q - 1);
+    else of_a(q - TN);
   };
   auto read_scale = [&](int to, int r) __attribute__((always_inline)) {
-    if (r < TN) sb[to][r] = *reinterpret_cast<lds_u16>(sat + (BM + (wn * TN + r) * 16) * 16);
-    else sa[to][r - TN] = *reinterpret_cast<lds_u16>(sat + (wm * TM + r - TN) * 256);
+    if (r < TN) sb[to][r] = *reinterpret_cast<lds_u32>(sat + (BM + (wn * TN + r) * 32) * 16);
+    else sa[to][r - TN] = *reinterpret_cast<lds_u32>(sat + (wm * TM + r - TN) * 512);
   };
   auto mask_scales = [&](int to) __attribute__((always_inline)) {
 #pragma unroll
@@ -160,12 +167,12 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
 #pragma unroll
     for (int t = 0; t < TN; ++t) sb[to][t] &= smask;
   };
-  constexpr int N_MMA = TM * TN, N_RD = TM + TN;
-  auto mma_one = [&](auto half, int cur, int i) __attribute__((always_inline)) {
-    constexpr int h = decltype(half)::value;
-    const v4i x = fa[h][i / TN], y = fb[h][i % TN];
+  constexpr int N_MMA = 2 * TM * TN, N_RD = 2 * (TM + TN), N_SC = TM + TN;
+  auto mma_one = [&](auto half, int cur, auto number) __attribute__((always_inline)) {
+    constexpr int i = decltype(number)::value, s = 2 * decltype(half)::value + i / (TM * TN), tm = i % (TM * TN) / TN, tn = i % TN;
+    const v4i x = fa[s][tm], y = fb[s][tn];
     const v8i a = {x[0], x[1], x[2], x[3], 0, 0, 0, 0}, b = {y[0], y[1], y[2], y[3], 0, 0, 0, 0};
-    acc[i / TN][i % TN] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i / TN][i % TN], 4, 4, h, (int)sa[cur][i / TN], h, (int)sb[cur][i % TN]);
+    acc[tm][tn] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, acc[tm][tn], 4, 4, s, (int)sa[cur][tm], s, (int)sb[cur][tn]);
   };
   constexpr std::integral_constant<int, 0> lower{};
   constexpr std::integral_constant<int, 1> upper{};
@@ -176,7 +183,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
     constexpr int cur = decltype(parity)::value;
     in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
       constexpr int i = decltype(number)::value;
-      mma_one(lower, cur, i);
+      mma_one(lower, cur, number);
 #pragma unroll
       for (int r = (N_RD * i) / N_MMA; r < (N_RD * (i + 1)) / N_MMA; ++r) read_frag(1, r);
       __builtin_amdgcn_sched_barrier(0);
@@ -189,9 +196,9 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
     if (cur == 0) load_scales((j + NS) / 2);
     in_turn(std::make_integer_sequence<int, N_MMA>{}, [&](auto number) __attribute__((always_inline)) {
       constexpr int i = decltype(number)::value;
-      mma_one(upper, cur, i);
+      mma_one(upper, cur, number);
 #pragma unroll
-      for (int r = (2 * N_RD * i) / N_MMA; r < (2 * N_RD * (i + 1)) / N_MMA; ++r) {
+      for (int r = ((N_RD + N_SC) * i) / N_MMA; r < ((N_RD + N_SC) * (i + 1)) / N_MMA; ++r) {
         if (r < N_RD) read_frag(0, r);
         else read_scale(1 - cur, r - N_RD);
       }
@@ -207,46 +214,48 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
   asm volatile("" ::: "memory");
   open(0);
 #pragma unroll
-  for (int r = 0; r < N_RD; ++r) {
-    read_frag(0, r);
-    read_scale(0, r);
-  }
+  for (int r = 0; r < N_RD; ++r) read_frag(0, r);
+#pragma unroll
+  for (int r = 0; r < N_SC; ++r) read_scale(0, r);
   mask_scales(0);
-  for (int j = 0; j < stages; j += 2) {
+  // (a last stage that stands alone is a trip of its own: with a branch around the second of a pair the accumulators were copied in every trip)
+  int j = 0;
+#pragma unroll 1
+  for (; j + 2 <= stages; j += 2) {
     trip(j, lower);
-    if (j + 1 < stages) trip(j + 1, upper);
+    trip(j + 1, upper);
   }
+  if (j < stages) trip(j, lower);
   // what was requested beyond the last stage (zeros) must have landed before the workgroup's LDS is released
   MX_WAIT_VM(0);
 
-  const int col = n0 + wn * (TN * 16) + TN * frow;
+  const int col = n0 + wn * (TN * 32) + TN * frow;
   float bv[TN];
 #pragma unroll
   for (int t = 0; t < TN; ++t) bv[t] = p.bias && col + t < p.N ? bf16_bits_to_f32(p.bias[col + t]) : 0.0f;
   if (p.wide) {   // through a buffer: rows beyond M lie outside it
     const __amdgpu_buffer_rsrc_t rsC = make_rsrc(p.C + (int64_t)m0 * p.ldc + n0, range(((int64_t)(p.M - m0 - 1) * p.ldc + (p.N - n0)) * 2));
     const int ldc2 = (int)p.ldc * 2;
-    const uint32_t voff = col < p.N ? (uint32_t)((wm * TM * 16 + fg * 4) * ldc2 + (col - n0) * 2) : kBeyond;
+    const uint32_t voff = col < p.N ? (uint32_t)((wm * TM * 32 + fg * 4) * ldc2 + (col - n0) * 2) : kBeyond;
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t out[TN / 2];
-#pragma unroll
-        for (int t = 0; t < TN / 2; ++t)
-          out[t] = bf16_rne_bits(acc[i][2 * t][e] + bv[2 * t]) | (bf16_rne_bits(acc[i][2 * t + 1][e] + bv[2 * t + 1]) << 16);
-        const int soff = (i * 16 + e) * ldc2;
-        if constexpr (TN == 8) __builtin_amdgcn_raw_buffer_store_b128(v4i{(int)out[0], (int)out[1], (int)out[2], (int)out[3]}, rsC, (int)(voff + soff), 0, 0);
-        else if constexpr (TN == 4) __builtin_amdgcn_raw_buffer_store_b64(v2i{(int)out[0], (int)out[1]}, rsC, (int)(voff + soff), 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b32((int)out[0], rsC, (int)(voff + soff), 0, 0);
+      for (int e = 0; e < 16; ++e) {
+        const int soff = (i * 32 + e / 4 * 8 + e % 4) * ldc2;
+        if constexpr (TN == 1) {
+          __builtin_amdgcn_raw_buffer_store_b16((short)bf16_rne_bits(acc[i][0][e] + bv[0]), rsC, (int)voff, soff, 0);
+        } else {
+          const uint32_t two = bf16_rne_bits(acc[i][0][e] + bv[0]) | (bf16_rne_bits(acc[i][1][e] + bv[1]) << 16);
+          __builtin_amdgcn_raw_buffer_store_b32((int)two, rsC, (int)voff, soff, 0);
+        }
       }
     return;
   }
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int row = m0 + (wm * TM + i) * 16 + fg * 4 + e;
+    for (int e = 0; e < 16; ++e) {
+      const int row = m0 + (wm * TM + i) * 32 + fg * 4 + e / 4 * 8 + e % 4;
       if (row >= p.M) continue;
       uint16_t *dst = p.C + (int64_t)row * p.ldc + col;
 #pragma unroll
@@ -600,7 +609,7 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
 
 template <int WM, int WN, int TM, int TN, int NS>
 static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
-  constexpr int BM = WM * TM * 16, BN = WN * TN * 16;
+  constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int lds = NS * (BM + BN) * 128 + (NS / 2 + 1) * (BM + BN) * 16;
   a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN;
   a.wide = a.N % TN == 0 && a.ldc % TN == 0 && ((uintptr_t)a.C % (TN * 2)) == 0 && a.ldc < (1 << 22);
@@ -676,7 +685,6 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
                         (const uint16_t *)bias, (uint16_t *)C, ldc, (int)M, (int)N, (int)blocks, 0, 0, false};
   hipStream_t st = (hipStream_t)stream;
   L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");
-  const int64_t mid = ((M + 127) / 128) * ((N + 127) / 128);
   if (takes_stream(M, N, blocks)) {
     const int64_t need = l8_gemm_mxfp4_workspace(M, N, K);
     L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "l8_gemm_mxfp4_nt: needs a 16-byte aligned workspace of %lld bytes",
@@ -685,16 +693,17 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
     if (N % 8 == 0 && ldc % 8 == 0 && ((uintptr_t)C % 16) == 0 && ldc < (1 << 22) && ((uintptr_t)bias % 4) == 0 && (M + 255) / 256 + (N + 255) / 256 < 16384)
       return bias ? launch_gemm_mxfp4_stream<true>(a, (uint8_t *)workspace, st) : launch_gemm_mxfp4_stream<false>(a, (uint8_t *)workspace, st);
   }
-  // Tiles by how many of them the units get.  us, [M,N] K:
-  //   128 x 128 from half a tile a unit on, against 64 x 64: [2048,2048] K 2048 10.8 / 12.5, K 8192 30.5 / 40.2, [512,4096] K 11008
-  //   28.4 / 30.1; below that, [100,4096] K 4096 12.4 / 7.9
-  //   its ring of two stages, two workgroups a unit, against one of four, one workgroup: [1500,6000] K 3000 29.1 / 33.5, [2064,2048]
-  //   K 1024 9.6 / 12.5; where every workgroup has a unit of its own, [512,4096] K 11008 36.1 / 28.4, [2048,2048] K 8192 31.4 / 30.5
-  //   64 x 64, eight stages (all that LDS holds) against two, a tile or less a unit: with weights that no cache holds, [65,4096] K
-  //   11008 20.7 / 34.7, K 4096 10.1 / 11.0; from the cache, [100,4096] K 4096 9.5 / 7.9; several tiles a unit, [2048,2048] K 2048 23.9 / 12.5
-  if (mid > num_cus()) return launch_gemm_mxfp4<4, 2, 2, 4, 2>(a, st);
-  if (mid >= num_cus() / 2) return launch_gemm_mxfp4<4, 2, 2, 4, 4>(a, st);
-  const int64_t small = ((M + 63) / 64) * ((N + 63) / 64);
-  if (small > num_cus()) return launch_gemm_mxfp4<2, 2, 2, 2, 2>(a, st);
-  return launch_gemm_mxfp4<2, 2, 2, 2, 8>(a, st);
+  // Otherwise the smallest tile that gives no compute unit a second workgroup, with a ring of four stages; beyond, 128 x 128 ones with
+  // two stages, two workgroups a unit.  us, weights that no cache holds, [M,N] K: 64 x 64 / 128 x 64 / 64 x 128 / 128 x 128 / the last:
+  //   [65,4096] 4096 8.3 / 9.7 / 10.1 / 12.0 / 13.9, [333,2048] 8192 13.0 / 15.6 / 15.9 / 19.5 / 24.5, [300,4096] 4096 11.0 / 10.4 / 10.5 /
+  //   12.4 / 14.2, [128,11008] 4096 16.3 / 13.6 / 14.0 / 16.8 / 20.1, [256,11008] 4096 22.1 / 23.2 / 24.4 / 16.9 / 20.3, from the cache
+  //   [2064,2048] 1024 11.9 / 14.9 / 14.9 / 11.9 / 9.3
+  // Other rings: 64 x 64 with two stages 11.0 and with eight 8.9 on the first, 128 x 64 with six 11.1 on the third.
+  auto tiles = [&](int64_t bm, int64_t bn) { return ((M + bm - 1) / bm) * ((N + bn - 1) / bn); };
+  const int64_t cus = num_cus();
+  if (tiles(64, 64) <= cus) return launch_gemm_mxfp4<2, 2, 1, 1, 4>(a, st);
+  if (tiles(128, 64) <= cus) return launch_gemm_mxfp4<2, 2, 2, 1, 4>(a, st);
+  if (tiles(64, 128) <= cus) return launch_gemm_mxfp4<2, 2, 1, 2, 4>(a, st);
+  if (tiles(128, 128) <= cus) return launch_gemm_mxfp4<4, 2, 1, 2, 4>(a, st);
+  return launch_gemm_mxfp4<4, 2, 1, 2, 2>(a, st);
 }
