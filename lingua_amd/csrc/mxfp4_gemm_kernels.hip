@@ -2,8 +2,8 @@
 //
 //   C[m,n] = bf16( sum over blocks b of 2^(sa[m,b] + sb[n,b] - 254) * sum over 32 k of A[m,32 b + k] * B[n,32 b + k]  + bias[n] )
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands' scales: a lane holds 32 consecutive codes of one row -- exactly one block --
-// and a byte of scale for it, so the scaling costs no instruction of its own.
+// v_mfma_scale_f32_32x32x64_f8f6f4 and its 16x16x128 form take both operands' scales: a lane holds 32 consecutive codes of one row --
+// exactly one block -- and a byte of scale for it, so the scaling costs no instruction of its own.
 //
 // Structure
 //   * a stage is 128 bytes (256 codes, 8 blocks) of every row of the tile's operands, four matrix instructions (32 x 32 x 64) deep; the

@@ -159,6 +159,13 @@ def test_product_with_extreme_and_nan_scales(M, N, blocks):
     assert bool(((got[1].double() - want[1]).abs().nan_to_num(0.0) <= 2.0 ** -126).all())
 
 
+# Tiles of 128 x 64 and of 64 x 128 (few rows, many columns), partial in both directions, an even and an odd number of columns
+@pytest.mark.parametrize("M,N,blocks", [(290, 4104, 11), (257, 4163, 24), (130, 9000, 1), (190, 9990, 6), (129, 11001, 9), (192, 9984, 32)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_products_on_oblong_tiles_are_exact(M, N, blocks, with_bias):
+    test_products_are_exact(M, N, blocks, with_bias)
+
+
 # The kernel of the large products: partial tiles in both directions, one tile to a workgroup and several, K from its shortest on, an odd
 # and an even number of stages (8 blocks), one block to either side of a window of scales (16)
 @pytest.mark.parametrize("M,N,blocks", [(4100, 2304, 9), (2500, 4104, 15), (4096, 2312, 16), (33100, 264, 17), (264, 33104, 24), (8200, 2304, 25), (8200, 2304, 33)])
