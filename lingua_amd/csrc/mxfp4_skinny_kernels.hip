@@ -104,13 +104,22 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
       const int c = w * kWindow + lane * 8;
       const uint32_t off = (uint32_t)(c * 2) | (c < p.K ? 0u : kBeyondAll);
       // (rows of tokens that are not there keep whatever LDS holds: it only reaches columns of the accumulators that nobody stores)
-      for (int m = 0; m < p.M; ++m) {
-        const v4i v = __builtin_amdgcn_raw_buffer_load_b128(rsX, (int)off, m * (int)p.ldx * 2, 0);
-        const uint32_t byte = mx_byte(quad_max(amax8(v)));
-        const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[0], (uint32_t)v[1], (uint32_t)v[2], (uint32_t)v[3], mx_scale(byte));
-        const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
-        *(uint32_t *)(buf + put(m, lane >> 2) + (lane & 3) * 4) = codes;
-        if (lchunk == 0) xsc[m * 4 + lrow] = four;
+      // two rows requested together: 8 tokens, [4096,4096] 6.3 -> 5.8 us, [32000,4096] 21.5 -> 20.2; with four 5.6 and 21.3, their registers
+      // cost one token through [32000,4096] 13.2 -> 14.0
+      constexpr int AT_ONCE = 2;
+      for (int m0 = 0; m0 < p.M; m0 += AT_ONCE) {
+        v4i v[AT_ONCE];
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) v[u] = __builtin_amdgcn_raw_buffer_load_b128(rsX, (int)off, (m0 + u) * (int)p.ldx * 2, 0);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          if (m0 + u >= p.M) break;
+          const uint32_t byte = mx_byte(quad_max(amax8(v[u])));
+          const uint32_t codes = byte == 255u ? 0u : mx_codes8((uint32_t)v[u][0], (uint32_t)v[u][1], (uint32_t)v[u][2], (uint32_t)v[u][3], mx_scale(byte));
+          const uint32_t four = byte | dpp<0x104>(byte) << 8 | dpp<0x108>(byte) << 16 | dpp<0x10C>(byte) << 24;
+          *(uint32_t *)(buf + put(m0 + u, lane >> 2) + (lane & 3) * 4) = codes;
+          if (lchunk == 0) xsc[(m0 + u) * 4 + lrow] = four;
+        }
       }
       __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -201,13 +210,13 @@ static constexpr int64_t kFewTokens = 64;   // that the kernels above take
 
 // Are the tokens quantised inside the product?  Every workgroup does it over again, a wave for each of its windows, and that is set
 // against a launch and a pass over the tokens.  us, inside / cast before:
-//   one window a wave      [4096,4096]   4 tokens 5.2 / 6.5, 8: 6.3 / 6.6, 12: 7.3 / 6.6   [32000,4096]  4: 17.1 / 18.4, 8: 21.4 / 18.5
-//   two                    [22016,8192]  4 tokens 23.6 / 29.5
-//   three                  [4096,11008]  2 tokens 9.1 / 10.1, 4: 10.9 / 10.1               [11008,11008] 2: 16.1 / 19.9, 4: 18.6 / 20.2
-//   four                   [512,16384]   2 tokens 8.8 / 9.0, 3: 10.1 / 9.4
+//   one window a wave   [4096,4096]   4 tokens 5.0 / 6.5, 8: 6.1 / 7.0, 12: 6.9 / 7.0   [32000,4096]  4: 15.7 / 18.3, 8: 20.2 / 18.5, 12: 24.6 / 18.9
+//   two                 [4096,8192]   4 tokens 7.7 / 9.1, 6: 8.8 / 8.7, 8: 9.7 / 8.7    [22016,8192]  6: 25.3 / 29.4, 8: 28.8 / 29.6
+//   three               [4096,11008]  2 tokens 8.0 / 9.5, 4: 9.6 / 10.0, 5: 10.9 / 10.2 [11008,11008] 4: 17.7 / 19.9, 6: 20.0 / 20.0
+//   four                [512,16384]   2 tokens 7.6 / 9.1, 3: 9.7 / 9.1                  [8192,16384]  3: 16.5 / 19.4, 6: 20.5 / 19.7
 static bool quantised_inside(int64_t M, int64_t K) {
   const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves;   // windows a wave
-  return M == 1 || M * (share > 1 ? share : 1) <= 8;
+  return M == 1 || (M <= 8 && M * share <= 12);
 }
 
 // Codes and scales of the activation in the workspace, then the product's own.
