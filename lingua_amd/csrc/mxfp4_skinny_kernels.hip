@@ -127,13 +127,14 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
       xs[0] = xsc[fr * 4 + fg];
       __builtin_amdgcn_wave_barrier();
     } else {
+      v4i v[MT][4];   // all tiles requested, then turned: 64 tokens, [4096,4096] 9.6 -> 9.4 us, [8192,2048] 9.6 -> 9.2
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        v4i v[4];
-        load_codes(rsX, p.ldx, i * 16, w, v, false);
+        load_codes(rsX, p.ldx, i * 16, w, v[i], false);
         xs[i] = load_scale(p.sx, p.ldsx, i * 16 + fr, p.M, w);
-        turn(v, xf[i]);
       }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) turn(v[i], xf[i]);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
@@ -187,36 +188,37 @@ static int launch_few(const MxFewArgs &a, hipStream_t st) {
 // One window in flight per wave: the registers that more would take are worth more as a second workgroup on the unit.  us, four
 // windows / one: one token, [11008,4096] 9.7 / 6.9, [4096,4096] 5.1 / 4.4.
 static int mxfp4_few_bf16(const MxFewArgs &a, hipStream_t st) { return launch_few<1, 1, true>(a, st); }
-// As many weight rows to a workgroup as leave one for six in ten units: they share the tokens' codes.  us, 16 rows / 32 / 64, 64
-// tokens: [11008,4096] 18.1 / 18.1 / 14.7, [8192,2048] 11.4 / 9.7 / 10.7, [4096,4096] 9.6 / 10.8 / 13.4.
-template <int MT>
-static int few_packed(const MxFewArgs &a, hipStream_t st) {
-  const int64_t enough = num_cus() * 6 / 10;
-  if (a.N >= enough * 64) return launch_few<MT, 4, false>(a, st);
-  if (a.N >= enough * 32) return launch_few<MT, 2, false>(a, st);
-  return launch_few<MT, 1, false>(a, st);
-}
+// Two tiles of weight rows to a workgroup, which share the tokens' codes, where six in ten units still get one and the tokens are more
+// than one tile.  us, one tile / two: 32 tokens, [8192,2048] 8.3 / 7.9, [5504,4096] 9.8 / 9.2, [4096,4096] 8.0 / 8.9; 64 tokens,
+// [8192,2048] 11.3 / 9.4, [5504,4096] 13.4 / 10.9, [4096,4096] 9.5 / 10.4; 16 tokens, [11008,4096] 10.5 / 11.0, [8192,2048] 6.8 / 7.2.
+static int64_t enough_groups() { return num_cus() * 6 / 10; }
 static int mxfp4_few_packed(const MxFewArgs &a, hipStream_t st) {
-  if (a.M <= 16) return few_packed<1>(a, st);
-  if (a.M <= 32) return few_packed<2>(a, st);
-  return few_packed<4>(a, st);
+  if (a.M <= 16) return launch_few<1, 1, false>(a, st);
+  const bool two = a.N >= enough_groups() * 32;
+  if (a.M <= 32) return two ? launch_few<2, 2, false>(a, st) : launch_few<2, 1, false>(a, st);
+  return two ? launch_few<4, 2, false>(a, st) : launch_few<4, 1, false>(a, st);
 }
 
 }  // namespace l8
 
 using namespace l8;
 
-static constexpr int64_t kFewTokens = 64;   // that the kernels above take
+// Do the kernels above take the problem?  Beyond one tile of tokens a weight of a row of tiles for six in ten units is the product's.  us,
+// here / there: 32 tokens, [8192,8192] 15.5 / 16.9, [11008,4096] 11.4 / 11.1, [22016,8192] 33.4 / 29.6, [32000,4096] 21.6 / 19.5; 64 tokens,
+// [4096,11008] 16.3 / 18.7, [8192,8192] 18.4 / 17.9, [11008,4096] 13.5 / 11.3, [32000,4096] 25.8 / 20.3.
+static bool few_tokens(int64_t M, int64_t N) { return M <= 16 || (M <= 64 && N < enough_groups() * 64); }
 
 // Are the tokens quantised inside the product?  Every workgroup does it over again, a wave for each of its windows, and that is set
-// against a launch and a pass over the tokens.  us, inside / cast before:
-//   one window a wave   [4096,4096]   4 tokens 5.0 / 6.5, 8: 6.1 / 7.0, 12: 6.9 / 7.0   [32000,4096]  4: 15.7 / 18.3, 8: 20.2 / 18.5, 12: 24.6 / 18.9
-//   two                 [4096,8192]   4 tokens 7.7 / 9.1, 6: 8.8 / 8.7, 8: 9.7 / 8.7    [22016,8192]  6: 25.3 / 29.4, 8: 28.8 / 29.6
-//   three               [4096,11008]  2 tokens 8.0 / 9.5, 4: 9.6 / 10.0, 5: 10.9 / 10.2 [11008,11008] 4: 17.7 / 19.9, 6: 20.0 / 20.0
+// against a launch and a pass over the tokens; where a unit has several workgroups one after the other it counts as often.  us, inside /
+// cast before:
+//   one window a wave   [4096,4096]   4 tokens 5.0 / 6.5, 8: 6.1 / 7.0, 12: 6.9 / 7.0   [32000,4096]  4: 15.7 / 15.8, 6: 18.0 / 15.9
+//                                                                                       [11008,4096]  4: 7.8 / 8.9, 6: 9.0 / 9.0
+//   two                 [4096,8192]   4 tokens 7.7 / 9.1, 6: 8.8 / 8.7, 8: 9.7 / 8.7    [22016,8192]  3: 21.2 / 22.2, 5: 24.1 / 22.5
+//   three               [4096,11008]  2 tokens 8.0 / 9.5, 4: 9.6 / 10.0, 5: 10.9 / 10.2 [11008,11008] 3: 16.5 / 17.2, 4: 17.6 / 17.3
 //   four                [512,16384]   2 tokens 7.6 / 9.1, 3: 9.7 / 9.1                  [8192,16384]  3: 16.5 / 19.4, 6: 20.5 / 19.7
-static bool quantised_inside(int64_t M, int64_t K) {
+static bool quantised_inside(int64_t M, int64_t N, int64_t K) {
   const int64_t share = ((K + kWindow - 1) / kWindow + kFewWaves - 1) / kFewWaves;   // windows a wave
-  return M == 1 || (M <= 8 && M * share <= 12);
+  return M == 1 || (M <= (N < enough_groups() * 64 ? 8 : 4) && M * share <= 12);
 }
 
 // Codes and scales of the activation in the workspace, then the product's own.
@@ -231,9 +233,11 @@ static MxLinearPlan plan_of(int64_t M, int64_t N, int64_t K) {
   p.q = 0;
   p.s = p.q + M * p.ldq;
   p.product = p.s + (M * p.lds + 15) / 16 * 16;
-  p.total = quantised_inside(M, K) ? 0 : p.product + (M <= kFewTokens ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
+  p.total = quantised_inside(M, N, K) ? 0 : p.product + (few_tokens(M, N) ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
   return p;
 }
+
+extern "C" int l8_mxfp4_linear_few(int64_t M, int64_t N) { return few_tokens(M, N); }
 
 extern "C" int64_t l8_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
@@ -263,7 +267,7 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
   uint8_t *const ws = (uint8_t *)workspace;
   const int rc = l8_cast_mxfp4(x, M, K, ldx, ws + plan.q, plan.ldq, ws + plan.s, plan.lds, nullptr, 0, nullptr, 0, stream);
   if (rc != L8_OK) return rc;
-  if (M <= kFewTokens) {
+  if (few_tokens(M, N)) {
     a.x = ws + plan.q, a.ldx = plan.ldq, a.sx = ws + plan.s, a.ldsx = plan.lds;
     return mxfp4_few_packed(a, st);
   }
