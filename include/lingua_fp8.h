@@ -382,12 +382,11 @@ int64_t l8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
 
 /* y [M,N] bf16 (ldy) = x [M,K] . w [N,K]^T + bias with x bf16 (ldx, elements) quantised as l8_cast_mxfp4 does and w kept in MXFP4:
  * codes qw (ldqw bytes, a multiple of 16, 16-byte aligned) and scales sw (ldsw bytes, any).  Up to 64 tokens (16, where the weight is
- * wide) run on a kernel of their own, the first few of them in that one launch; more as l8_cast_mxfp4 and l8_gemm_mxfp4_nt (which
- * wants ldsw % 16 == 0 and sw 16-byte aligned); l8_mxfp4_linear_few tells which, 1 or 0.  K % 8 == 0, ldx % 8 == 0, x 16-byte aligned; workspace of l8_mxfp4_linear_workspace(M, N, K) bytes, 16-byte aligned. */
+ * wide) run on a kernel of their own, the first few of them in that one launch; more as l8_cast_mxfp4 and l8_gemm_mxfp4_nt, with the
+ * scales copied onto 16-byte lines where they do not lie on them.  K % 8 == 0, ldx % 8 == 0, x 16-byte aligned; workspace of l8_mxfp4_linear_workspace(M, N, K) bytes, 16-byte aligned. */
 int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx, const void *qw, int64_t ldqw, const void *sw, int64_t ldsw, int64_t N,
                     const void *bias, void *y, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream);
 int64_t l8_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K);
-int l8_mxfp4_linear_few(int64_t M, int64_t N);
 
 int l8_gemm_algo_count(void);
 /* human-readable description of tile configuration `algo` (1-based), or NULL */

@@ -70,7 +70,6 @@ SIGNATURES = {
     "l8_gemm_mxfp4_workspace": [_i64, _i64, _i64],
     "l8_mxfp4_linear": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _i64, _p, _p, _i64, _p, _i64, _p],
     "l8_mxfp4_linear_workspace": [_i64, _i64, _i64],
-    "l8_mxfp4_linear_few": [_i64, _i64],
     "l8_linear_fwd": [ctypes.c_char_p],
     "l8_linear_fwd_workspace": [ctypes.c_char_p],
     "l8_linear_fwd_rows": [ctypes.c_char_p, _i64, _i64],

@@ -178,6 +178,25 @@ __global__ __launch_bounds__(kFewBlock) void linear_mxfp4_few_kernel(const MxFew
 #endif
 }
 
+// Rows of scales onto 16-byte lines, where the product's tiles want them: 16 bytes a thread.
+__global__ __launch_bounds__(256) void mxfp4_scales_on_lines_kernel(const uint8_t *__restrict__ s, int64_t lds, int64_t rows, int blocks, uint8_t *__restrict__ t, int pieces) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / pieces;
+  if (row >= rows) return;
+  const int first = (int)(i - row * pieces) * 16;
+  const uint8_t *const at = s + row * lds + first;
+  uint32_t v[4] = {0, 0, 0, 0};
+  if (first + 16 <= blocks) {
+    __builtin_memcpy(v, at, 16);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (first + k < blocks) v[k >> 2] |= (uint32_t)at[k] << (8 * (k & 3));
+  }
+  *(v4i *)(t + i * 16) = v4i{(int)v[0], (int)v[1], (int)v[2], (int)v[3]};
+#endif
+}
+
 template <int MT, int NT, bool QX>
 static int launch_few(const MxFewArgs &a, hipStream_t st) {
   hipLaunchKernelGGL((linear_mxfp4_few_kernel<MT, NT, QX>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(kFewBlock), 0, st, a);
@@ -223,7 +242,7 @@ static bool quantised_inside(int64_t M, int64_t N, int64_t K) {
 
 // Codes and scales of the activation in the workspace, then the product's own.
 struct MxLinearPlan {
-  int64_t ldq, lds, q, s, product, total;
+  int64_t ldq, lds, q, s, product, scales, total;   // scales: of the weight, on lines
 };
 static MxLinearPlan plan_of(int64_t M, int64_t N, int64_t K) {
   const int64_t blocks = (K + 31) / 32;
@@ -233,11 +252,11 @@ static MxLinearPlan plan_of(int64_t M, int64_t N, int64_t K) {
   p.q = 0;
   p.s = p.q + M * p.ldq;
   p.product = p.s + (M * p.lds + 15) / 16 * 16;
-  p.total = quantised_inside(M, N, K) ? 0 : p.product + (few_tokens(M, N) ? 0 : l8_gemm_mxfp4_workspace(M, N, K));
+  const bool few = few_tokens(M, N);
+  p.scales = p.product + (few ? 0 : (l8_gemm_mxfp4_workspace(M, N, K) + 15) / 16 * 16);
+  p.total = quantised_inside(M, N, K) ? 0 : p.scales + (few ? 0 : N * p.lds);
   return p;
 }
-
-extern "C" int l8_mxfp4_linear_few(int64_t M, int64_t N) { return few_tokens(M, N); }
 
 extern "C" int64_t l8_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
@@ -251,8 +270,9 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
   const int64_t blocks = (K + 31) / 32;
   L8_REQUIRE(y && ldy >= N && ((uintptr_t)y % 2) == 0 && ((uintptr_t)bias % 2) == 0, "l8_mxfp4_linear: null or misaligned y, or ldy < N");
   L8_REQUIRE(K == 0 || (x && qw && sw), "l8_mxfp4_linear: null pointer");
-  L8_REQUIRE(K % 8 == 0 && ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0, "l8_mxfp4_linear: K=%lld and ldx must be multiples of 8, x 16-byte aligned", (long long)K);
+  L8_REQUIRE(K == 0 || (K % 8 == 0 && ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0), "l8_mxfp4_linear: K=%lld and ldx must be multiples of 8, x 16-byte aligned", (long long)K);
   L8_REQUIRE(M < (1 << 20) - 16 && N < (1 << 28) && K < (1 << 24), "l8_mxfp4_linear: M < 2^20 - 16, N < 2^28 and K < 2^24 are served");
+  if (K == 0) ldx = ldqw = ldsw = 0;
   L8_REQUIRE(ldqw % 16 == 0 && ldqw >= blocks * 16 && ldqw <= (1 << 23) - 16 && ((uintptr_t)qw % 16) == 0 && ldsw >= blocks,
              "l8_mxfp4_linear: rows of codes on 16-byte lines less than 2^23 bytes apart, and a scale per block, are wanted");
   const MxLinearPlan plan = plan_of(M, N, K);
@@ -260,7 +280,7 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
              "l8_mxfp4_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)plan.total);
   hipStream_t st = (hipStream_t)stream;
   MxFewArgs a = {x, nullptr, (const uint8_t *)qw, (const uint8_t *)sw, ldx, 0, ldqw, ldsw, (const uint16_t *)bias, (uint16_t *)y, ldy, (int)M, (int)N, (int)K, (int)blocks};
-  if (plan.total == 0) {
+  if (quantised_inside(M, N, K)) {
     L8_REQUIRE(ldx <= (1 << 25), "l8_mxfp4_linear: rows of x further apart than 2^25 elements");   // (32-bit offsets)
     return mxfp4_few_bf16(a, st);
   }
@@ -271,6 +291,13 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
     a.x = ws + plan.q, a.ldx = plan.ldq, a.sx = ws + plan.s, a.ldsx = plan.lds;
     return mxfp4_few_packed(a, st);
   }
+  if (ldsw % 16 || ldsw > (1 << 23) - 16 || ((uintptr_t)sw % 16)) {   // a launch of 3 us
+    const int64_t pieces = plan.lds / 16, grid = (N * pieces + 255) / 256;
+    L8_REQUIRE(grid < (1LL << 31), "l8_mxfp4_linear: more scales than a grid has threads");
+    hipLaunchKernelGGL(mxfp4_scales_on_lines_kernel, dim3((unsigned)grid), dim3(256), 0, st, (const uint8_t *)sw, ldsw, N, (int)blocks, ws + plan.scales, (int)pieces);
+    L8_HIP(hipGetLastError());
+    sw = ws + plan.scales, ldsw = plan.lds;
+  }
   return l8_gemm_mxfp4_nt(ws + plan.q, ws + plan.s, qw, sw, M, N, K, plan.ldq, plan.lds, ldqw, ldsw, bias, y, ldy, ws + plan.product,
-                          workspace_bytes - plan.product, stream);
+                          plan.scales - plan.product, stream);
 }

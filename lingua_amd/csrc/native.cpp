@@ -35,7 +35,7 @@ struct Library {
   X(l8_cast_rowwise_many) X(l8_cast_rowwise_cols_many) X(l8_gemm_nt_multi) X(l8_gemm_nt_sum) X(l8_rmsnorm_cast_rowwise)            \
   X(l8_rmsnorm_workspace) X(l8_rmsnorm_bwd_as) X(l8_rmsnorm_bwd_workspace) X(l8_swiglu_cast_rowwise) X(l8_swiglu_workspace)        \
   X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed) X(l8_add_rmsnorm_cast_rowwise) X(l8_add_rmsnorm_bwd) X(l8_rotary)     \
-  X(l8_cast_mxfp4) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace) X(l8_mxfp4_linear_few)
+  X(l8_cast_mxfp4) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
   L8_ENTRIES(L8_ENTRY)
 #undef L8_ENTRY
 } lib;
@@ -838,7 +838,7 @@ PyObject *mxfp4_packed(PyObject *, PyObject *const *args, Py_ssize_t n) {
   Rows rx;
   MxRows w;
   if (!as_rows(x, device, rx) || !on_16_bytes(rx) || !as_mx(qw, sw, device, w) || (rx.cols + 31) / 32 != w.blocks || c10::hip::current_device() != device ||
-      ((w.lds % 16 || ((uintptr_t)w.s % 16)) && !lib.l8_mxfp4_linear_few(rx.rows, w.rows)) || (bias.defined() && !dense(bias, at::kBFloat16, w.rows, device)))
+      (bias.defined() && !dense(bias, at::kBFloat16, w.rows, device)))
     Py_RETURN_NONE;
   Tensor y;
   {

@@ -1034,14 +1034,11 @@ def mxfp4_linear_fwd(x: torch.Tensor, qw: torch.Tensor, sw: torch.Tensor, bias: 
         raise RuntimeError(f"{what}: x {tuple(x.shape)} on {x.device} and a weight of scales {tuple(sw.shape)} on {qw.device} do not fit")
     bias = _mx_bias(bias, N, x.device, what)
     qw = _on_16_bytes(qw)
-    few = bool(_lib.load().l8_mxfp4_linear_few(M, N))   # (reads rows of scales wherever they start)
-    if not few:
-        sw = _on_16_bytes(sw)
     y = torch.empty((M, N), dtype=torch.bfloat16, device=x.device)
     with _timed("mxfp4_linear_fwd", 2 * M * N * K, x.device):
         ws_bytes = _lib.load().l8_mxfp4_linear_workspace(M, N, K)   # (it goes by the device's compute units)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device) if ws_bytes else None
-        code = _lib.load().l8_mxfp4_linear(x.data_ptr(), M, K, _ld(x), qw.data_ptr(), _ld16(qw), sw.data_ptr(), _ld(sw) if few else _ld16(sw), N,
+        code = _lib.load().l8_mxfp4_linear(x.data_ptr(), M, K, _ld(x), qw.data_ptr(), _ld16(qw), sw.data_ptr(), _ld(sw), N,
                                            bias.data_ptr() if bias is not None else None, y.data_ptr(), max(N, 1), ws.data_ptr() if ws is not None else None,
                                            ws_bytes, st)
     _lib.check(code, "l8_mxfp4_linear")

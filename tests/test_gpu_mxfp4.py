@@ -229,6 +229,28 @@ def test_linear_with_a_packed_weight(M, K, N, with_bias):
     assert three.shape == (1, M, N) and torch.equal(three[0], got)
 
 
+@pytest.mark.parametrize("M", [1, 3, 12, 20, 70, 300])
+def test_linear_over_nothing_is_its_bias(M):
+    from lingua_amd import mxfp4
+    q, s = torch.empty(24, 0, dtype=torch.uint8, device="cuda"), torch.empty(24, 0, dtype=torch.uint8, device="cuda")
+    x, bias = torch.empty(M, 0, dtype=torch.bfloat16, device="cuda"), torch.arange(24, device="cuda").to(torch.bfloat16)
+    assert torch.equal(mxfp4.linear_packed(x, q, s, bias), bias.expand(M, 24))
+    assert torch.equal(mxfp4.linear_packed(x, q, s), torch.zeros(M, 24, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("M,K,N", [(5, 2608, 40), (40, 1040, 64), (40, 528, 9888), (171, 3856, 368), (700, 1296, 2064), (4200, 528, 2304)])
+def test_scales_at_any_address(M, K, N, host):
+    """Rows of scales an odd number of bytes apart, from an odd address on, NaN bytes between them: the product of those on lines."""
+    from lingua_amd import mxfp4
+    x, w = seeded_bf16((M, K), seed=M).cuda(), seeded_bf16((N, K), std=0.02, seed=N).cuda()
+    codes, scales = mxfp4.pack(w)
+    blocks = scales.shape[1]
+    odd = torch.full((N, blocks + 5 + blocks % 2), 255, dtype=torch.uint8, device="cuda")
+    odd[:, 3:3 + blocks] = scales.view(torch.uint8)
+    assert odd.stride(0) % 2 == 1
+    assert torch.equal(mxfp4.linear_packed(x, codes, odd[:, 3:3 + blocks]), mxfp4.linear_packed(x, codes, scales))
+
+
 def test_linear_with_a_packed_weight_and_rows_that_are_not_finite():
     from lingua_amd import mxfp4
     x, w = seeded_bf16((5, 256), seed=1), seeded_bf16((64, 256), std=0.02, seed=2)
