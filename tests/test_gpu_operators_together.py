@@ -211,3 +211,39 @@ def test_compiled_calls_equal_eager_ones(name):
     assert torch.equal(got, want)
     for a, b in zip(torch.autograd.grad(got, leaves, gy, allow_unused=True), torch.autograd.grad(want, leaves, gy, allow_unused=True)):
         assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+
+
+def test_threads_at_once():
+    """Four threads, each on a stream of its own, through every operator forward and backward: the results of one after the other."""
+    import threading
+    from lingua_amd import mxfp4, norm, rope
+    cos, sin = (t.cuda() for t in rope.rotary_tables(32, 16))
+
+    def operands(i):
+        leaves = [seeded_bf16(s, std=0.1, seed=10 * i + j).cuda().requires_grad_() for j, s in enumerate(((16, 128), (16, 128), (128,), (128, 128)))]
+        return leaves, seeded_bf16((1, 16, 4, 32), std=0.01, seed=i).cuda(), mxfp4.pack(leaves[3])
+
+    def step(leaves, gy, packed):
+        x, res, gain, w = leaves
+        h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+        q, _ = rope.rotary(mxfp4.mxfp4_linear(y, w).view(1, 16, 4, 32), h.view(1, 16, 4, 32), cos, sin)
+        return (q.detach(), mxfp4.linear_packed(y, *packed)) + torch.autograd.grad(q, leaves, gy)
+
+    sets = [operands(i) for i in range(4)]
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got, streams = [None] * 4, [torch.cuda.Stream() for _ in range(4)]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            for _ in range(20):
+                got[i] = step(*sets[i])
+            streams[i].synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(got, want):
+        assert a is not None and all(torch.equal(u, v) for u, v in zip(a, b))
