@@ -367,6 +367,20 @@ int l8_rotary(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, int
  * Requires C % 8 == 0, ldx % 8 == 0, 16-byte aligned x, R <= 1048560. */
 int l8_cast_mxfp4(const void *x, int64_t R, int64_t C, int64_t ldx, void *q, int64_t ldq, void *s, int64_t lds,
                   void *qt, int64_t ldqt, void *st, int64_t ldst, void *stream);
+/* Two such casts, in one launch where the columns of both are wanted and the rows of both or neither. */
+typedef struct {
+  const void *x;
+  int64_t R, C, ldx;
+  void *q;
+  int64_t ldq;
+  void *s;
+  int64_t lds;
+  void *qt;
+  int64_t ldqt;
+  void *st;
+  int64_t ldst;
+} l8_mxfp4_cast;
+int l8_cast_mxfp4_two(const l8_mxfp4_cast *two, void *stream);
 /* Back to bf16 [R,C] (ldy, elements): exact, but infinite from 6 * 2^126 on; a block of scale 255 is NaN. */
 int l8_mxfp4_to_bf16(const void *q, int64_t ldq, const void *s, int64_t lds, int64_t R, int64_t C, void *y, int64_t ldy, void *stream);
 

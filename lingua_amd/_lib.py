@@ -65,6 +65,7 @@ SIGNATURES = {
     "l8_add_rmsnorm_bwd": [_p, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _i64, _p],
     "l8_rotary": [_p, _i64, _i64, _i64, _i64, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _p],
     "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
+    "l8_cast_mxfp4_two": [_p, _p],
     "l8_mxfp4_to_bf16": [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],
     "l8_gemm_mxfp4_nt": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _i64, _p, _i64, _p],
     "l8_gemm_mxfp4_workspace": [_i64, _i64, _i64],

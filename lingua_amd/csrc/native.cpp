@@ -35,7 +35,7 @@ struct Library {
   X(l8_cast_rowwise_many) X(l8_cast_rowwise_cols_many) X(l8_gemm_nt_multi) X(l8_gemm_nt_sum) X(l8_rmsnorm_cast_rowwise)            \
   X(l8_rmsnorm_workspace) X(l8_rmsnorm_bwd_as) X(l8_rmsnorm_bwd_workspace) X(l8_swiglu_cast_rowwise) X(l8_swiglu_workspace)        \
   X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed) X(l8_add_rmsnorm_cast_rowwise) X(l8_add_rmsnorm_bwd) X(l8_rotary)     \
-  X(l8_cast_mxfp4) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
+  X(l8_cast_mxfp4) X(l8_cast_mxfp4_two) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
   L8_ENTRIES(L8_ENTRY)
 #undef L8_ENTRY
 } lib;
@@ -1102,8 +1102,9 @@ Tensor mx_forward(const Tensor &a, const Tensor &w, const Tensor &bias, bool nee
   const Mx qa(ra.rows, ra.cols, o, true), qw(rw.rows, rw.cols, o, true);
   if (need_w) at = Mx(ra.cols, ra.rows, o, true);
   if (need_a) wt = Mx(rw.cols, rw.rows, o, true);
-  cast_mx(ra, qa, at, stream);
-  cast_mx(rw, qw, wt, stream);
+  const l8_mxfp4_cast two[2] = {{ra.p, ra.rows, ra.cols, ra.ld, qa.qp(), qa.ldq(), qa.sp(), qa.lds(), at.qp(), at.ldq(), at.sp(), at.lds()},
+                                {rw.p, rw.rows, rw.cols, rw.ld, qw.qp(), qw.ldq(), qw.sp(), qw.lds(), wt.qp(), wt.ldq(), wt.sp(), wt.lds()}};
+  check(lib.l8_cast_mxfp4_two(two, stream), "l8_cast_mxfp4_two");
   auto sizes = a.sizes().vec();
   sizes.back() = rw.rows;
   const Tensor y = at::empty(sizes, o);

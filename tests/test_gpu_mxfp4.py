@@ -84,6 +84,35 @@ def test_back_to_bf16_of_any_bytes(R, blocks, cols):
     assert torch.equal(back.nan_to_num(7.0), want.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("shapes", [((333, 264), (64, 1040)), ((2500, 4096), (4100, 2056)), ((5, 8), (70000, 64)), ((0, 64), (32, 64))])
+@pytest.mark.parametrize("wanted", [("rows columns", "rows columns"), ("columns", "columns"), ("rows", "rows columns"), ("rows", "rows")])
+def test_two_casts_in_one_call(shapes, wanted):
+    """The bytes of single casts, whichever copies are wanted; what lies between rows stays."""
+    import struct
+    from lingua_amd import _lib, ops
+    pack, kept, pairs = [], [], []
+    for i, ((R, C), want) in enumerate(zip(shapes, wanted)):
+        x = seeded_bf16((R, C), seed=R + C).cuda()
+        copies = []
+        for name, (rows, cols) in (("rows", (R, C)), ("columns", (C, R))):
+            blocks = (cols + 31) // 32
+            q = torch.full((rows, blocks * 16 + 16), 0xA5, dtype=torch.uint8, device="cuda")
+            s = torch.full((rows, (blocks + 7) // 4 * 4), 0xA5, dtype=torch.uint8, device="cuda")
+            copies.append((q, s, blocks) if name in want else None)
+        pack += [x.data_ptr(), R, C, C]
+        for c in copies:
+            pack += [0, 0, 0, 0] if c is None else [c[0].data_ptr(), c[0].stride(0), c[1].data_ptr(), c[1].stride(0)]
+        kept.append(x)
+        pairs.append(copies)
+    _lib.check(_lib.load().l8_cast_mxfp4_two(struct.pack("24q", *pack), torch.cuda.current_stream().cuda_stream), "l8_cast_mxfp4_two")
+    for x, copies in zip(kept, pairs):
+        for c, single in zip(copies, ops.cast_mxfp4(x, transposed=True)):
+            if c is not None:
+                q, s, blocks = c
+                assert torch.equal(q[:, :blocks * 16], single[0].view(torch.uint8)) and torch.equal(s[:, :blocks], single[1].view(torch.uint8))
+                assert bool((q[:, blocks * 16:] == 0xA5).all()) and bool((s[:, blocks:] == 0xA5).all())
+
+
 def operand(rows, blocks, seed, low=126, high=129):
     g = torch.Generator().manual_seed(seed)
     return (torch.randint(0, 256, (rows, blocks * 16), generator=g, dtype=torch.uint8),
