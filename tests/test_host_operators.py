@@ -32,6 +32,15 @@ def test_product_is_refused(change):
     assert refused("l8_gemm_mxfp4_nt", *{**GEMM, **change}.values())
 
 
+def test_two_casts_are_refused():
+    import struct
+    good, bad = [P, 64, 64, 64, P, 32, P, 16, P, 32, P, 16], [P, 64, 60, 64, P, 32, P, 16, P, 32, P, 16]
+    assert refused("l8_cast_mxfp4_two", None, None)
+    assert refused("l8_cast_mxfp4_two", struct.pack("24q", *good, *bad), None) and refused("l8_cast_mxfp4_two", struct.pack("24q", *bad, *good), None)
+    empty = [0, 0, 64, 64] + [0] * 8
+    assert _lib.load().l8_cast_mxfp4_two(struct.pack("24q", *empty, *empty), None) == 0
+
+
 def test_product_workspace():
     lib = _lib.load()
     assert lib.l8_gemm_mxfp4_workspace(64, 64, 4096) == 0 and lib.l8_gemm_mxfp4_workspace(0, 64, 64) == 0 and lib.l8_gemm_mxfp4_workspace(-1, 8192, 8192) == 0
