@@ -860,11 +860,19 @@ PyObject *mxfp4_packed(PyObject *, PyObject *const *args, Py_ssize_t n) {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// Gradients as a pass that is itself differentiated hands them on: an error if anybody asks for more.
-variable_list once(variable_list grads, const char *what) {
+// Gradients as a pass that is itself differentiated hands them on: an error for whoever asks for the derivative of one that `varies` with
+// something that learns.  (They come from kernels, which nothing records: each is made to ask for a gradient, so that the error is
+// what it meets.  One that does not vary is a constant and stays one.)
+variable_list once(variable_list grads, std::initializer_list<bool> varies, const char *what) {
   if (!at::GradMode::is_enabled()) return grads;
-  return torch::autograd::DelayedError(std::string(what) + " is not differentiable twice", (int)grads.size())(std::move(grads));
+  size_t i = 0;
+  for (const bool v : varies) {
+    Tensor &g = grads[i++];
+    if (v && g.defined()) g = torch::autograd::DelayedError(std::string(what) + " is not differentiable twice", 1)({g.detach().set_requires_grad(true)})[0];
+  }
+  return grads;
 }
+bool learns(const Tensor &t) { return t.defined() && t.requires_grad(); }
 // A leaf's gradient is accumulated on the stream that its node was made on, and the node lives as long as a graph that holds it.  One
 // made on the default stream cannot take part in a capture: the captured backward pass would end the process.
 void refuse_captured(std::initializer_list<const Tensor *> inputs, const char *what) {
@@ -917,6 +925,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
                                           want_col ? col.mutable_data_ptr<float>() : nullptr, ws.p(), ws_bytes, stream_of(device)), "l8_add_rmsnorm_cast_rowwise");
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({h, w, rstd});
+    ctx->saved_data["sum learns"] = learns(x) || learns(res);
     variable_list out = {h, y, q, s};
     if (want_col) out.push_back(col);
     ctx->mark_non_differentiable({out.begin() + 2, out.end()});
@@ -944,9 +953,10 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
                                     gw.mutable_data_ptr(), f32, ws.p(), ws_bytes, stream_of(device)), "l8_rmsnorm_bwd");
     } else if (grads[0].defined()) {   // only the sum was used
       TORCH_CHECK(grads[0].scalar_type() == at::kBFloat16, kName, " backward: bf16 gradients required, got ", grads[0].scalar_type());
-      gx = grads[0];
+      return {grads[0], grads[0], Tensor(), Tensor(), Tensor()};
     }
-    return once({gx, gx, gw, Tensor(), Tensor()}, kName);
+    const bool sum_learns = ctx->saved_data["sum learns"].toBool(), gx_varies = sum_learns || learns(w) || learns(grads[0]) || learns(grads[1]);
+    return once({gx, gx, gw, Tensor(), Tensor()}, {gx_varies, gx_varies, sum_learns || learns(grads[1])}, kName);
   }
 };
 
@@ -1053,7 +1063,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
       const Tensor in[2] = {x[0], x[1]};
       rotate(in, g, saved[0], saved[1], saved[2], ctx->saved_data["half"].toBool(), true);
     }
-    return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()}, "rotary");
+    return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()}, {learns(grads[0]), learns(grads[1])}, "rotary");
   }
 };
 
@@ -1159,7 +1169,9 @@ struct Mxfp4Linear : torch::autograd::Function<Mxfp4Linear> {
       const Space ws(gy, bytes);
       check(lib.l8_col_sum(rg.p, rg.rows, rg.cols, rg.ld, gbias.mutable_data_ptr(), ws.p(), bytes, stream), "l8_col_sum");
     }
-    return once({ga, gw, gbias, Tensor(), Tensor()}, "mxfp4_linear");
+    // (what was kept of the one operand says that the other learns)
+    const bool gy_learns = learns(grads[0]);
+    return once({ga, gw, gbias, Tensor(), Tensor()}, {gy_learns || saved[0].defined(), gy_learns || saved[2].defined(), gy_learns}, "mxfp4_linear");
   }
 };
 

@@ -605,6 +605,21 @@ def _refuse_captured(a, b, c, what):
         _lib.native_for(a.get_device()).refuse_captured(a, b, c, what)
 
 
+def _once(what, grads, varies):
+    """Gradients as a backward pass that is itself differentiated hands them on: an error for whoever asks for the derivative of one that
+    varies with something that learns.  ``once_differentiable`` looks at the incoming gradients alone, and lets the derivative with
+    respect to the saved operands go missing where those do not learn."""
+    if not torch.is_grad_enabled():
+        return grads
+    error = torch._C._functions.DelayedError
+    return tuple(error(f"{what} is not differentiable twice".encode(), 1)(g.detach().requires_grad_()) if g is not None and v else g
+                 for g, v in zip(grads, varies))
+
+
+def _learns(t) -> bool:
+    return t is not None and t.requires_grad
+
+
 class Fp8Linear(torch.nn.Linear):
     def forward(self, input: torch.Tensor) -> torch.Tensor:
         weight, bias = self.weight, self.bias

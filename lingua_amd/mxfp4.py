@@ -48,22 +48,23 @@ class Mxfp4LinearFn(torch.autograd.Function):
         return ops.gemm_mxfp4_nt(qa, qw, sa, sw, bias)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
         if gy.dtype != torch.bfloat16:
             raise RuntimeError(f"mxfp4_linear backward: bf16 grad_out required, got {gy.dtype}")
         qat, sat, qwt, swt = ctx.saved_tensors
         need_a, need_w, need_bias = ctx.needs_input_grad
         ga = gw = gbias = None
-        if need_a or need_w:
-            rows, cols = ops.cast_mxfp4(gy, rowwise=need_a, transposed=need_w, on_lines=True)
-            if need_a:
-                ga = ops.gemm_mxfp4_nt(rows[0], qwt, rows[1], swt)
-            if need_w:
-                gw = ops.gemm_mxfp4_nt(cols[0], qat, cols[1], sat)
-        if need_bias:
-            gbias = ops.col_sum(gy) if ops.rows_on_16_bytes(gy) else gy.sum(dim=0)
-        return ga, gw, gbias
+        with torch.no_grad():
+            if need_a or need_w:
+                rows, cols = ops.cast_mxfp4(gy, rowwise=need_a, transposed=need_w, on_lines=True)
+                if need_a:
+                    ga = ops.gemm_mxfp4_nt(rows[0], qwt, rows[1], swt)
+                if need_w:
+                    gw = ops.gemm_mxfp4_nt(cols[0], qat, cols[1], sat)
+            if need_bias:
+                gbias = ops.col_sum(gy) if ops.rows_on_16_bytes(gy) else gy.sum(dim=0)
+        gy_learns = f8._learns(gy)   # (what was kept of the one operand says that the other learns)
+        return f8._once("mxfp4_linear", (ga, gw, gbias), (gy_learns or qat is not None, gy_learns or qwt is not None, gy_learns))
 
 
 def mxfp4_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:

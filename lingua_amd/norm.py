@@ -73,27 +73,29 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(h2d, weight, rstd)
         ctx.x_shape = x.shape
+        ctx.sum_learns = x.requires_grad or residual.requires_grad
         return h2d.unflatten(0, x.shape[:-1]), y2d.unflatten(0, x.shape[:-1])
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gh, gy):
         h2d, weight, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
         for g in (gh, gy):
             if g is not None and g.dtype != torch.bfloat16:
                 raise RuntimeError(f"add_rmsnorm backward: bf16 gradients required, got {g.dtype}")
-        gx = gw = None
         if gy is None:   # only the sum was used
-            gx = gh
-        else:
+            return gh if need[0] else None, gh if need[1] else None, None, None, None
+        gy_learns = f8._learns(gy)
+        gx_varies = ctx.sum_learns or f8._learns(weight) or f8._learns(gh) or gy_learns
+        with torch.no_grad():
             gy2d = gy.flatten(end_dim=-2)
             if gh is None:
                 gx2d, gw = ops.rmsnorm_bwd(gy2d, h2d, weight, rstd, gw_dtype=weight.dtype)
             else:
                 gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh.flatten(end_dim=-2), h2d, weight, rstd, gw_dtype=weight.dtype)
             gx = gx2d.reshape(ctx.x_shape)
-        need = ctx.needs_input_grad
-        return gx if need[0] else None, gx if need[1] else None, gw if need[2] else None, None, None
+        grads = gx if need[0] else None, gx if need[1] else None, gw if need[2] else None
+        return (*f8._once("add_rmsnorm", grads, (gx_varies, gx_varies, ctx.sum_learns or gy_learns)), None, None)
 
 
 def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, eps: float):

@@ -25,17 +25,18 @@ class RotaryFn(torch.autograd.Function):
         return ops.rotary(xq, xk, cos, sin, positions, in_halves)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         for g in (gq, gk):
             if g is not None and g.dtype != torch.bfloat16:
                 raise RuntimeError(f"rotary backward: bf16 gradients required, got {g.dtype}")
         gq = gq if ctx.needs_input_grad[0] else None
         gk = gk if ctx.needs_input_grad[1] else None
+        varies = (f8._learns(gq), f8._learns(gk))
         if gq is not None or gk is not None:
             cos, sin, positions = ctx.saved_tensors
-            gq, gk = ops.rotary(gq, gk, cos, sin, positions, ctx.in_halves, inverse=True)
-        return gq, gk, None, None, None, None
+            with torch.no_grad():
+                gq, gk = ops.rotary(gq, gk, cos, sin, positions, ctx.in_halves, inverse=True)
+        return (*f8._once("rotary", (gq, gk), varies), None, None, None, None)
 
 
 def rotary(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None,

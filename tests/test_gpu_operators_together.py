@@ -7,6 +7,7 @@ import torch.nn.functional as F
 import plain_operators as plain
 from bench_workloads import Attention, Llama
 from conftest import seeded_bf16
+from plain_operators import host  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -247,3 +248,70 @@ def test_threads_at_once():
         t.join()
     for a, b in zip(got, want):
         assert a is not None and all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+def twice(name, x, w, gain, tables):
+    """An operator's output on x [8,64] and the leaves whose gradients a further pass may run into."""
+    from lingua_amd import mxfp4, norm, rope
+    if name == "add_rmsnorm":
+        return norm.add_rmsnorm(x, x.detach(), gain, 1e-5)[1], (x, gain)
+    if name == "rotary":
+        return rope.rotary(x.view(1, 8, 2, 32), x.view(1, 8, 2, 32), *tables)[0].view(8, 64), (x,)
+    return mxfp4.mxfp4_linear(x, w, gain), (x, w, gain)
+
+
+@pytest.mark.parametrize("name", ["add_rmsnorm", "rotary", "mxfp4_linear"])
+def test_second_derivatives_are_refused(name, host):
+    """A gradient that was itself made for differentiation has the bits of an ordinary one, and whoever asks for its derivative gets an
+    error, not the derivative of everything but this operator."""
+    from lingua_amd import rope
+    leaves = [seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (64, 64), (64,)))]
+    tables = [t.cuda() for t in rope.rotary_tables(32, 8)]
+    y, of = twice(name, *leaves, tables)
+    ordinary = torch.autograd.grad(y.float().square().sum(), of)
+    for i, leaf in enumerate(of):
+        y, _ = twice(name, *leaves, tables)
+        loss = y.float().square().sum()
+        grads = torch.autograd.grad(loss, of, create_graph=True)
+        assert all(torch.equal(g, o) for g, o in zip(grads, ordinary))
+        with pytest.raises(RuntimeError, match=f"{name} is not differentiable twice"):
+            (loss + grads[i].float().square().sum()).backward()
+        # the same where only this leaf's gradient was asked for
+        y, _ = twice(name, *leaves, tables)
+        loss = y.float().square().sum()
+        g, = torch.autograd.grad(loss, leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match=f"{name} is not differentiable twice"):
+            (loss + g.float().square().sum()).backward()
+    # a pass that does not run into them goes through
+    y, _ = twice(name, *leaves, tables)
+    loss = y.float().square().sum()
+    torch.autograd.grad(loss, of, create_graph=True)
+    for leaf in leaves:
+        leaf.grad = None
+    loss.backward()
+    assert all(torch.equal(leaf.grad, o) for leaf, o in zip(of, ordinary))
+
+
+def test_second_derivatives_of_a_linear_loss(host):
+    """The gradient that arrives is a constant: what an operator makes of it varies where the operator is not linear in its inputs, and
+    only there."""
+    from lingua_amd import mxfp4, norm, rope
+    x, w, gain = (seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (64, 64), (64,))))
+    tables = [t.cuda() for t in rope.rotary_tables(32, 8)]
+
+    def grads(y, of):
+        return torch.autograd.grad(y, of, torch.ones_like(y), create_graph=True)
+
+    for g in grads(norm.add_rmsnorm(x, x.detach(), gain, 1e-5)[1], (x, gain)) + grads(mxfp4.mxfp4_linear(x, w), (x, w)):
+        with pytest.raises(RuntimeError, match="is not differentiable twice"):
+            g.float().sum().backward()
+    for y, of in ((mxfp4.mxfp4_linear(x, w.detach(), gain), (x, gain)), (mxfp4.mxfp4_linear(x.detach(), w), (w,)),
+                  (rope.rotary(x.view(1, 8, 2, 32), x.view(1, 8, 2, 32).detach(), *tables)[0], (x,)),
+                  (norm.add_rmsnorm(x.detach(), x.detach(), gain, 1e-5)[1], (gain,))):
+        assert not any(g.requires_grad for g in grads(y, of))
+    # the sum alone passes its gradient through, and the derivative of that
+    h, _ = norm.add_rmsnorm(x, x.detach(), gain, 1e-5)
+    scale = torch.tensor(3.0, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad((h * scale).sum(), x, create_graph=True)
+    g.sum().backward()
+    assert float(scale.grad) == x.numel()

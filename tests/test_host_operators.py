@@ -188,3 +188,49 @@ def test_conversion_keeps_parameters_and_refuses_other_modules():
     for other in (copy.deepcopy(model), torch.load(buffer, weights_only=False)):
         assert type(other.layers[0]) is type(model.layers[0]) and list(other.state_dict()) == keys
         assert other.layers[0].ffn_norm is not model.layers[0].ffn_norm
+
+
+def interpreted(monkeypatch):
+    """The Python forms on the CPU, plain torch in the kernels' place: name -> (output, leaves) of fresh leaves."""
+    from lingua_amd import float8, mxfp4, norm, ops, rope
+    g = torch.Generator().manual_seed(0)
+    leaf = lambda *shape: torch.randn(shape, generator=g).to(torch.bfloat16).requires_grad_()   # noqa: E731
+    cos, sin = rope.rotary_tables(16, 4)
+    turn = lambda t, s: None if t is None else plain.rotate(t.detach(), cos[None, :, None], s[None, :, None], False).to(torch.bfloat16)   # noqa: E731
+    monkeypatch.setattr(float8.config, "share_input_casts", False)
+    monkeypatch.setattr(ops, "rotary", lambda q, k, c, s, p, half, inverse=False: (turn(q, -sin if inverse else sin), turn(k, -sin if inverse else sin)))
+    pair = lambda x: (x.detach().clone(), torch.zeros(()))   # noqa: E731
+    monkeypatch.setattr(ops, "cast_mxfp4", lambda x, rowwise=True, transposed=False, on_lines=False: (pair(x) if rowwise else None, pair(x.t()) if transposed else None))
+    monkeypatch.setattr(ops, "gemm_mxfp4_nt", lambda a, b, sa, sb, bias=None: a @ b.t() + (0 if bias is None else bias.detach()))
+    monkeypatch.setattr(ops, "col_sum", lambda t: t.sum(0))
+
+    def forward(x, r, w, eps, col_amax=None, on_lines=False):
+        h, rstd, y = plain.add_rmsnorm(x.detach(), r.detach(), w.detach(), eps)
+        return h.to(torch.bfloat16), y.to(torch.bfloat16), None, None, rstd
+
+    def backward(gy, gh, h, w, rstd, gw_dtype):
+        gx, gw, _, _ = plain.add_rmsnorm_gradients(h.double(), rstd, w.detach().double(), gy.double(), gh.double())
+        return gx.to(torch.bfloat16), gw.to(gw_dtype)
+
+    monkeypatch.setattr(ops, "add_rmsnorm_cast_rowwise", forward)
+    monkeypatch.setattr(ops, "add_rmsnorm_bwd", backward)
+    monkeypatch.setattr(ops, "rmsnorm_bwd", lambda gy, h, w, rstd, gw_dtype: backward(gy, torch.zeros_like(gy), h, w, rstd, gw_dtype))
+    x, w, gain, q = leaf(4, 16), leaf(8, 16), leaf(16), leaf(1, 4, 2, 16)
+    return {"add_rmsnorm": (lambda: norm.Fp8AddRMSNormFn.apply(x, x.detach(), gain, 1e-5, False)[1], (x, gain)),
+            "rotary": (lambda: rope.RotaryFn.apply(q, q, cos, sin, None, False)[0], (q,)),
+            "mxfp4_linear": (lambda: mxfp4.Mxfp4LinearFn.apply(x, w, gain[:8]), (x, w, gain))}
+
+
+@pytest.mark.parametrize("name", ["add_rmsnorm", "rotary", "mxfp4_linear"])
+@pytest.mark.parametrize("linear_loss", [False, True])
+def test_python_forms_refuse_second_derivatives(name, linear_loss, monkeypatch):
+    call, leaves = interpreted(monkeypatch)[name]
+    for leaf in leaves:
+        loss = call().float()
+        loss = loss.sum() if linear_loss else loss.square().sum()
+        grad, = torch.autograd.grad(loss, leaf, create_graph=True)
+        if linear_loss and (name == "rotary" or (name == "mxfp4_linear" and leaf is leaves[2])):
+            assert not grad.requires_grad      # these are linear: the gradient of a constant's is a constant
+            continue
+        with pytest.raises(RuntimeError, match=f"{name} is not differentiable twice"):
+            (loss + grad.float().square().sum()).backward()
