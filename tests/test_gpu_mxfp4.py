@@ -43,6 +43,27 @@ def test_casts_are_the_formats(shape):
     check_cast(alone, x.t().contiguous())
 
 
+# Shapes that give every unit a tile of 256 x 128: a last band of rows and last columns that are not full, 79, 130 and 2188 bands
+@pytest.mark.parametrize("shape", [(2500, 4104), (4129, 2056), (70001, 64)])
+def test_large_casts_are_the_formats(shape):
+    from lingua_amd import ops
+    R, C = shape
+    assert (R + 255) // 256 * ((C + 127) // 128) >= torch.cuda.get_device_properties(0).multi_processor_count
+    x = spread(R, C, seed=R + C)
+    x[40:104, :] = 0.0
+    x[41:104:2, :] = -0.0
+    x[200:264, 8:16] = torch.tensor(2.0 ** -133).to(torch.bfloat16)
+    x[300, :], x[301, 5] = 2.0 ** -133, 0.0
+    x[777, 33], x[R - 1, C - 1], x[1500, 2], x[R - 40, 40] = float("nan"), float("inf"), -float("inf"), float("nan")
+    x = x.cuda()
+    rows, cols = ops.cast_mxfp4(x, rowwise=True, transposed=True)
+    check_cast(rows, x)
+    check_cast(cols, x.t().contiguous())
+    none, alone = ops.cast_mxfp4(x, rowwise=False, transposed=True, on_lines=True)
+    assert none is None
+    check_cast(alone, x.t().contiguous())
+
+
 def test_cast_of_blocks_that_are_zero_or_not_finite_and_of_rows_apart():
     from lingua_amd import ops
     wide = seeded_bf16((70, 256), seed=3)
