@@ -279,6 +279,35 @@ def test_linear_with_a_packed_weight(M, K, N, with_bias):
     assert three.shape == (1, M, N) and torch.equal(three[0], got)
 
 
+# Each form of the few-token kernel, one window of 512 columns a wave and several, shares that differ and waves without any: tokens
+# quantised inside (M up to 8), or before on one or two tiles of weight rows (N from 4896 on) and one, two or four of tokens
+@pytest.mark.parametrize("M,K,N", [(1, 11008, 64), (2, 2048, 48), (2, 11008, 80), (4, 11008, 64), (4, 512, 9872), (5, 8208, 48), (6, 8192, 64), (8, 4096, 272), (8, 48, 64),
+                                   (9, 4624, 64), (12, 11008, 48), (16, 8208, 64), (20, 4624, 48), (24, 528, 5008), (32, 11008, 4912), (32, 8208, 96), (33, 4624, 48),
+                                   (48, 4624, 5008), (64, 11008, 272), (64, 11008, 4912)])
+@pytest.mark.parametrize("with_bias", [False, True])
+def test_few_tokens_are_exact(M, K, N, with_bias):
+    """Both operands are multiples of 1/2 up to 6 times 1/2, 1 or 2, with a 4 or a 6 in every block, so that the cast of x is x.  Products
+    are multiples of 1/16 and their magnitudes add up to less than 2^20: every partial sum is exact in fp32, in any order."""
+    from lingua_amd import mxfp4
+    blocks = (K + 31) // 32
+    (qx, sx), (qw, sw) = operand(M, blocks, M + K), operand(N, blocks, N + K)
+    code = plain.mx_unpack(qx)
+    code[:, ::32] = code[:, ::32] & 8 | 6 + (code[:, ::32] & 1)
+    x = plain.mx_values(code, sx)[:, :K]
+    w = plain.mx_values(plain.mx_unpack(qw), sw)[:, :K].cuda()
+    xb = x.to(torch.bfloat16).cuda()
+    assert torch.equal(xb.cpu().double(), x) and torch.equal(plain.mx_rounded(xb.cpu()), x)
+    if K % 32:
+        qw[:, (K - 1) // 32 * 16 + K % 32 // 2:] = 0     # (codes behind the last column are zeros)
+    bias = torch.randint(-64, 64, (N,), generator=torch.Generator().manual_seed(N)).to(torch.bfloat16).cuda() if with_bias else None
+    got = mxfp4.linear_packed(xb, qw.cuda(), sw.cuda(), bias)
+    want = x.cuda() @ w.t()
+    assert float((x.abs().cuda() @ w.abs().t()).max()) + 64 < 2.0 ** 20
+    if bias is not None:
+        want = want + bias.double()
+    assert torch.equal(got, want.to(torch.bfloat16))
+
+
 @pytest.mark.parametrize("M", [1, 3, 12, 20, 70, 300])
 def test_linear_over_nothing_is_its_bias(M):
     from lingua_amd import mxfp4
