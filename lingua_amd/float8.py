@@ -230,13 +230,17 @@ class _WeightCasts:
     version counter and stream are what they were (an optimizer step advances the version).  A slot holds the
     weight by weak reference only and goes away with it, so the cache never holds more than two bytes per
     parameter of the ``Fp8Linear`` weights that are alive (and an eighth of that for rows on 128-byte lines), and a
-    deleted model releases its copies.  Used only with ``config.cache_weight_casts``."""
+    deleted model releases its copies.  Used only with ``config.cache_weight_casts``.
+
+    A call that is being captured neither takes a copy from here nor leaves one: a graph would go on reading a copy that
+    is dropped when the weight changes, and what it writes itself is there only once it has run.  It quantises the weight
+    in every replay."""
 
     def __init__(self):
         self.entries = {}   # id(weight) -> {"ref": weakref to the weight, "key": ..., "row": ..., "tw": ...}
 
     def _slot(self, w):
-        if w.is_inference():
+        if w.is_inference() or (w.is_cuda and torch.cuda.is_current_stream_capturing()):
             return None
         key = _LastCast._key(w)
         slot = self.entries.get(id(w))

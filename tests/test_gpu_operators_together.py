@@ -315,3 +315,38 @@ def test_second_derivatives_of_a_linear_loss(host):
     g, = torch.autograd.grad((h * scale).sum(), x, create_graph=True)
     g.sum().backward()
     assert float(scale.grad) == x.numel()
+
+
+@pytest.mark.parametrize("kind", ["mxfp4", "fp8"])
+def test_captured_linears_share_no_kept_weight(kind, monkeypatch):
+    """With copies of the weights kept between calls: a warm-up and two captures on one stream.  A weight that has changed since, the second
+    graph replayed without the first, and an eager call on that stream give what a call without kept copies gives."""
+    import lingua_amd
+    from lingua_amd import Fp8Linear, mxfp4
+    monkeypatch.setattr(lingua_amd.config, "cache_weight_casts", True)
+    lin = (mxfp4.Mxfp4Linear if kind == "mxfp4" else Fp8Linear)(256, 128, bias=False, dtype=torch.bfloat16, device="cuda")
+    xs = [seeded_bf16((m, 256), seed=m).cuda() for m in (3, 40)]
+    stream, graphs, ys = torch.cuda.Stream(), [torch.cuda.CUDAGraph() for _ in xs], []
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.no_grad():
+        with torch.cuda.stream(stream):
+            for x in xs:
+                lin(x)
+        torch.cuda.synchronize()
+        for x, graph in zip(xs, graphs):
+            with torch.cuda.graph(graph, stream=stream):
+                ys.append(lin(x))
+        with torch.cuda.stream(stream):
+            eager = lin(xs[1])
+        lin.weight.mul_(-2.0)
+        torch.cuda.synchronize()
+        lingua_amd.clear_cast_memos()
+        want = [lin(x) for x in xs]
+        assert torch.equal(eager * -2.0, want[1])
+        for i in (1, 1, 0):
+            ys[i].zero_()
+            torch.cuda.synchronize()
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(ys[i], want[i])
+    lingua_amd.clear_cast_memos()
