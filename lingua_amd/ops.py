@@ -107,6 +107,10 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def _column_amaxes(t: torch.Tensor, C: int, device) -> bool:
+    return t.dtype == torch.float32 and t.numel() == C and t.is_contiguous() and t.device == device
+
+
 def _empty_fp8(rows: int, cols: int, device, on_lines: bool) -> torch.Tensor:
     """A quantised operand; ``on_lines``: with rows that start on 128-byte lines, which the products read up to 1.6 times as
     fast where they are bound by the L2's requests (figures at fp8_row_stride in csrc/linear.cpp)."""
@@ -142,8 +146,8 @@ def cast_rowwise(x: torch.Tensor, col_amax: Optional[torch.Tensor] = None, want_
     scale_direct = out_scale is not None and (R <= 1 or out_scale.stride(0) == 1)  # the kernel writes a dense vector
     scale = out_scale if scale_direct else torch.empty((R, 1), dtype=torch.float32, device=x.device)
     amax = torch.empty((R, 1), dtype=torch.bfloat16, device=x.device)
-    if col_amax is not None and (col_amax.dtype != torch.float32 or col_amax.numel() != C or not col_amax.is_contiguous()):
-        raise RuntimeError("cast_rowwise: col_amax must be a contiguous fp32 tensor with C elements")
+    if col_amax is not None and not _column_amaxes(col_amax, C, x.device):
+        raise RuntimeError("cast_rowwise: col_amax must be a contiguous fp32 tensor with C elements on the same device")
     ws, ws_bytes = None, 0
     if col_amax is not None:
         ws_bytes = _lib.load().l8_cast_rowwise_workspace(R, C)
@@ -347,8 +351,8 @@ def cast_colwise_transposed(x: torch.Tensor, col_amax_f32: torch.Tensor, pad_to:
     x = _rows_2d(x, torch.bfloat16, "cast_colwise_transposed")
     st = _prep(x, "cast_colwise_transposed")
     R, C = x.shape
-    if col_amax_f32.dtype != torch.float32 or col_amax_f32.numel() != C or not col_amax_f32.is_contiguous():
-        raise RuntimeError("cast_colwise_transposed: col_amax must be a contiguous fp32 tensor with C elements")
+    if not _column_amaxes(col_amax_f32, C, x.device):
+        raise RuntimeError("cast_colwise_transposed: col_amax must be a contiguous fp32 tensor with C elements on the same device")
     if R == 0:
         # no rows: the product over them is zero; one block of zero columns keeps the GEMM's reduction length valid
         q = torch.zeros((C, pad_to), dtype=torch.uint8, device=x.device).view(torch.float8_e4m3fn)
@@ -632,8 +636,8 @@ def swiglu_cast_rowwise(h1: torch.Tensor, h3: torch.Tensor, want_h: bool = True,
     q = _empty_fp8(R, C, dev, on_lines)
     scale = torch.empty((R, 1), dtype=torch.float32, device=dev)
     amax = torch.empty((R, 1), dtype=torch.bfloat16, device=dev)
-    if col_amax is not None and (col_amax.dtype != torch.float32 or col_amax.numel() != C or not col_amax.is_contiguous()):
-        raise RuntimeError("swiglu_cast_rowwise: col_amax must be a contiguous fp32 tensor with C elements")
+    if col_amax is not None and not _column_amaxes(col_amax, C, dev):
+        raise RuntimeError("swiglu_cast_rowwise: col_amax must be a contiguous fp32 tensor with C elements on the same device")
     ws, ws_bytes = _swiglu_ws(R, C, dev, 1) if col_amax is not None else (None, 0)
     with _timed("swiglu_cast_rowwise", R * C * (5 + (2 if want_h else 0)) + 4 * R, dev):
         code = _lib.load().l8_swiglu_cast_rowwise(
@@ -661,8 +665,8 @@ def swiglu_bwd_cast_rowwise(dh: torch.Tensor, h1: torch.Tensor, h3: torch.Tensor
     R, C = dh.shape
     dev = dh.device
     for ca in (col_amax1, col_amax3):
-        if ca is not None and (ca.dtype != torch.float32 or ca.numel() != C or not ca.is_contiguous()):
-            raise RuntimeError("swiglu_bwd_cast_rowwise: column amaxes must be contiguous fp32 tensors with C elements")
+        if ca is not None and not _column_amaxes(ca, C, dev):
+            raise RuntimeError("swiglu_bwd_cast_rowwise: column amaxes must be contiguous fp32 tensors with C elements on the same device")
     g1 = torch.empty((R, C), dtype=torch.bfloat16, device=dev) if want_g else None
     g3 = torch.empty((R, C), dtype=torch.bfloat16, device=dev) if want_g else None
     q1, q3 = _empty_fp8(R, C, dev, on_lines), _empty_fp8(R, C, dev, on_lines)
@@ -698,8 +702,8 @@ def swiglu_bwd_cast_transposed(dh: torch.Tensor, h1: torch.Tensor, h3: torch.Ten
     st = _prep(dh, "swiglu_bwd_cast_transposed")
     R, C = dh.shape
     cols = (col_amax1, col_amax3, col_amax_h)
-    if R == 0 or any(ca.dtype != torch.float32 or ca.numel() != C or ca.device != dh.device or not ca.is_contiguous() for ca in cols):
-        raise RuntimeError("swiglu_bwd_cast_transposed: rows, and contiguous fp32 column amaxes with C elements, required")
+    if R == 0 or any(not _column_amaxes(ca, C, dh.device) for ca in cols):
+        raise RuntimeError("swiglu_bwd_cast_transposed: rows, and contiguous fp32 column amaxes with C elements on the same device, required")
     Rp = (R + 15) // 16 * 16
     qs = [_empty_fp8(C, Rp, dh.device, on_lines) for _ in range(3)]
     ss = [torch.empty((C, 1), dtype=torch.float32, device=dh.device) for _ in range(3)]
@@ -722,8 +726,8 @@ def rmsnorm_cast_rowwise(x: torch.Tensor, weight: torch.Tensor, eps: float, want
     if weight.dtype not in (torch.bfloat16, torch.float32) or weight.numel() != C or weight.device != dev:
         raise RuntimeError("rmsnorm_cast_rowwise: weight must be bf16 or fp32 with C elements on the same device")
     weight = weight.contiguous()
-    if col_amax is not None and (not want_q or col_amax.dtype != torch.float32 or col_amax.numel() != C or not col_amax.is_contiguous()):
-        raise RuntimeError("rmsnorm_cast_rowwise: col_amax needs the cast and must be a contiguous fp32 tensor with C elements")
+    if col_amax is not None and (not want_q or not _column_amaxes(col_amax, C, dev)):
+        raise RuntimeError("rmsnorm_cast_rowwise: col_amax needs the cast and must be a contiguous fp32 tensor with C elements on the same device")
     y = torch.empty((R, C), dtype=torch.bfloat16, device=dev)
     q = _empty_fp8(R, C, dev, on_lines) if want_q else None
     scale = torch.empty((R, 1), dtype=torch.float32, device=dev) if want_q else None
@@ -790,8 +794,8 @@ def add_rmsnorm_cast_rowwise(x: torch.Tensor, residual: torch.Tensor, weight: to
     if weight.dtype not in (torch.bfloat16, torch.float32) or weight.numel() != C or weight.device != dev:
         raise RuntimeError(f"{what}: weight must be bf16 or fp32 with C elements on the same device")
     weight = weight.contiguous()
-    if col_amax is not None and (not want_q or col_amax.dtype != torch.float32 or col_amax.numel() != C or not col_amax.is_contiguous()):
-        raise RuntimeError(f"{what}: col_amax needs the cast and must be a contiguous fp32 tensor with C elements")
+    if col_amax is not None and (not want_q or not _column_amaxes(col_amax, C, dev)):
+        raise RuntimeError(f"{what}: col_amax needs the cast and must be a contiguous fp32 tensor with C elements on the same device")
     h, y = (torch.empty((R, C), dtype=torch.bfloat16, device=dev) for _ in range(2))
     q = _empty_fp8(R, C, dev, on_lines) if want_q else None
     scale = torch.empty((R, 1), dtype=torch.float32, device=dev) if want_q else None

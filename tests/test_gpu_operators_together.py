@@ -350,3 +350,15 @@ def test_captured_linears_share_no_kept_weight(kind, monkeypatch):
             torch.cuda.synchronize()
             assert torch.equal(ys[i], want[i])
     lingua_amd.clear_cast_memos()
+
+
+def test_column_amaxes_elsewhere_are_refused():
+    """A kernel writes (or reads) them through their address: on the host it would be no address of the GPU's."""
+    from lingua_amd import ops
+    x, w, col = seeded_bf16((16, 64), seed=1).cuda(), seeded_bf16((64,), seed=2).cuda(), torch.zeros(64)
+    for call in (lambda c: ops.add_rmsnorm_cast_rowwise(x, x, w, 1e-5, col_amax=c), lambda c: ops.rmsnorm_cast_rowwise(x, w, 1e-5, col_amax=c),
+                 lambda c: ops.cast_rowwise(x, col_amax=c), lambda c: ops.cast_colwise_transposed(x, c), lambda c: ops.swiglu_cast_rowwise(x, x, col_amax=c),
+                 lambda c: ops.swiglu_bwd_cast_rowwise(x, x, x, c, c), lambda c: ops.swiglu_bwd_cast_transposed(x, x, x, c, c, c)):
+        call(col.cuda())
+        with pytest.raises(RuntimeError, match="same device"):
+            call(col)
