@@ -364,7 +364,7 @@ int l8_rotary(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, int
  *   x       bf16 [R,C] (ldx, elements)
  *   q, s    codes and scales of the rows; qt, st of the columns (that is, of x transposed: [C,R]); either pair may be NULL
  *   ldq, lds, ldqt, ldst   bytes from row to row: multiples of 16 for codes and of 4 for scales, pointers aligned alike
- * Requires C % 8 == 0, ldx % 8 == 0, 16-byte aligned x, R <= 1048560. */
+ * Requires C % 8 == 0, ldx % 8 == 0, 16-byte aligned x, R <= 1048560, C <= 2^30; with qt fewer than 2^22 tiles of 256 x 128. */
 int l8_cast_mxfp4(const void *x, int64_t R, int64_t C, int64_t ldx, void *q, int64_t ldq, void *s, int64_t lds,
                   void *qt, int64_t ldqt, void *st, int64_t ldst, void *stream);
 /* Two such casts, in one launch where the columns of both are wanted and the rows of both or neither. */
@@ -397,7 +397,8 @@ int64_t l8_gemm_mxfp4_workspace(int64_t M, int64_t N, int64_t K);
 /* y [M,N] bf16 (ldy) = x [M,K] . w [N,K]^T + bias with x bf16 (ldx, elements) quantised as l8_cast_mxfp4 does and w kept in MXFP4:
  * codes qw (ldqw bytes, a multiple of 16, 16-byte aligned) and scales sw (ldsw bytes, any).  Up to 64 tokens (16, where the weight is
  * wide) run on a kernel of their own, the first few of them in that one launch; more as l8_cast_mxfp4 and l8_gemm_mxfp4_nt, with the
- * scales copied onto 16-byte lines where they do not lie on them.  K % 8 == 0, ldx % 8 == 0, x 16-byte aligned; workspace of l8_mxfp4_linear_workspace(M, N, K) bytes, 16-byte aligned. */
+ * scales copied onto 16-byte lines where they do not lie on them.  K % 8 == 0, ldx % 8 == 0, x 16-byte aligned; M < 2^20 - 16,
+ * N < 2^28 (2^27 - 15 on the kernel of few tokens), K < 2^24; workspace of l8_mxfp4_linear_workspace(M, N, K) bytes, 16-byte aligned. */
 int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx, const void *qw, int64_t ldqw, const void *sw, int64_t ldsw, int64_t N,
                     const void *bias, void *y, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream);
 int64_t l8_mxfp4_linear_workspace(int64_t M, int64_t N, int64_t K);

@@ -612,6 +612,7 @@ static int launch_gemm_mxfp4(MxGemmArgs a, hipStream_t st) {
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32;
   constexpr int lds = NS * (BM + BN) * 128 + (NS / 2 + 1) * (BM + BN) * 16;
   a.tiles_m = (a.M + BM - 1) / BM, a.tiles_n = (a.N + BN - 1) / BN;
+  L8_REQUIRE((int64_t)a.tiles_m * a.tiles_n * (WM * WN * 64) < (1LL << 32), "l8_gemm_mxfp4_nt: more tiles than a grid has");
   a.wide = a.N % TN == 0 && a.ldc % TN == 0 && ((uintptr_t)a.C % (TN * 2)) == 0 && a.ldc < (1 << 22);
   static bool ready[kMaxDev];   // benign race: every thread sets the same attribute
   const int slot = device_slot();
@@ -684,7 +685,7 @@ extern "C" int l8_gemm_mxfp4_nt(const void *A, const void *sa, const void *B, co
   const MxGemmArgs a = {(const uint8_t *)A, (const uint8_t *)B, (const uint8_t *)sa, (const uint8_t *)sb, lda, ldb, ldsa, ldsb,
                         (const uint16_t *)bias, (uint16_t *)C, ldc, (int)M, (int)N, (int)blocks, 0, 0, false};
   hipStream_t st = (hipStream_t)stream;
-  L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");
+  L8_REQUIRE(((M + 255) / 256) * ((N + 255) / 256) < (1 << 24), "l8_gemm_mxfp4_nt: more tiles than a grid has");   // (tiles are counted in 32 bits)
   if (takes_stream(M, N, blocks)) {
     const int64_t need = l8_gemm_mxfp4_workspace(M, N, K);
     L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "l8_gemm_mxfp4_nt: needs a 16-byte aligned workspace of %lld bytes",

@@ -174,6 +174,9 @@ using namespace l8;
 
 namespace l8 {
 
+static int64_t large_tiles(const l8_mxfp4_cast &o) { return (o.C + kMxTileC - 1) / kMxTileC * ((o.R + 255) / 256); }
+constexpr int64_t kMostLargeTiles = (1 << 22) - 1;   // of 1024 threads each: a grid has fewer than 2^32
+
 static int check_cast(const l8_mxfp4_cast &o) {
   L8_REQUIRE(o.R >= 0 && o.C >= 0, "l8_cast_mxfp4: negative shape R=%lld C=%lld", (long long)o.R, (long long)o.C);
   if (o.R == 0 || o.C == 0) return L8_OK;
@@ -185,8 +188,9 @@ static int check_cast(const l8_mxfp4_cast &o) {
              "l8_cast_mxfp4: rows of 16 bytes per block on 16-byte lines and of a scale per block on 4-byte lines are wanted");
   L8_REQUIRE(!o.qt || (o.ldqt % 16 == 0 && o.ldqt >= bands * 16 && ((uintptr_t)o.qt % 16) == 0 && o.ldst % 4 == 0 && o.ldst >= bands && ((uintptr_t)o.st % 4) == 0),
              "l8_cast_mxfp4: transposed rows of 16 bytes per block on 16-byte lines and of a scale per block on 4-byte lines are wanted");
-  L8_REQUIRE(o.R <= (int64_t)65535 * 16 && o.C <= (int64_t)1 << 30 && (o.C + kMxTileC - 1) / kMxTileC * ((o.R + 63) / 64) < (1 << 30),
-             "l8_cast_mxfp4: R=%lld exceeds %d, C=%lld 2^30 or their product what a grid covers", (long long)o.R, 65535 * 16, (long long)o.C);
+  L8_REQUIRE(o.R <= (int64_t)65535 * 16 && o.C <= (int64_t)1 << 30, "l8_cast_mxfp4: R=%lld exceeds %d or C=%lld 2^30", (long long)o.R, 65535 * 16, (long long)o.C);
+  L8_REQUIRE(!o.qt || large_tiles(o) <= kMostLargeTiles, "l8_cast_mxfp4: R=%lld, C=%lld are more tiles of 256 x %d than a grid has threads for", (long long)o.R,
+             (long long)o.C, kMxTileC);
   return L8_OK;
 }
 
@@ -200,7 +204,7 @@ static int launch_tiles(const l8_mxfp4_cast *const *o, int n, hipStream_t st) {
     const l8_mxfp4_cast &c = *o[i];
     t.op[i] = {(const uint16_t *)c.x, c.R, c.C, c.ldx, (uint8_t *)c.q, (uint8_t *)c.s, (uint8_t *)c.qt, (uint8_t *)c.st, c.ldq, c.lds, c.ldqt, c.ldst};
     t.across[i] = (int)across(c.C);
-    large += across(c.C) * down(c.R, 256);
+    large += large_tiles(c);
   }
   const int rows = large >= num_cus() ? 256 : 64;
   t.first = (int)(t.across[0] * down(o[0]->R, rows));
@@ -228,9 +232,10 @@ extern "C" int l8_cast_mxfp4_two(const l8_mxfp4_cast *two, void *stream) {
   hipStream_t st = (hipStream_t)stream;
   auto some = [](const l8_mxfp4_cast &o) { return o.R > 0 && o.C > 0; };
   const l8_mxfp4_cast *const both[2] = {two, two + 1};
-  // one launch where the same copies are wanted of both: [1021,2048] and [2064,2048] 9.6 -> 6.4 us, [4096,4096] and [11008,4096]
+  // one launch where the same copies are wanted of both and a grid holds them: [1021,2048] and [2064,2048] 9.6 -> 6.4 us, [4096,4096] and [11008,4096]
   // 40.9 -> 36.1
-  if (some(two[0]) && some(two[1]) && two[0].qt && two[1].qt && !two[0].q == !two[1].q) return launch_tiles(both, 2, st);
+  if (some(two[0]) && some(two[1]) && two[0].qt && two[1].qt && !two[0].q == !two[1].q && large_tiles(two[0]) + large_tiles(two[1]) <= kMostLargeTiles)
+    return launch_tiles(both, 2, st);
   for (const l8_mxfp4_cast *o : both) {
     const int rc = l8_cast_mxfp4(o->x, o->R, o->C, o->ldx, o->q, o->ldq, o->s, o->lds, o->qt, o->ldqt, o->st, o->ldst, stream);
     if (rc != L8_OK) return rc;

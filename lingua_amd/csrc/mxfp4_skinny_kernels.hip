@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void mxfp4_scales_on_lines_kernel(const uint8_
 }
 
 template <int MT, int NT, bool QX>
-static int launch_few(const MxFewArgs &a, hipStream_t st) {
+static int launch_few(const MxFewArgs &a, hipStream_t st) {   // (fewer than 2^32 threads: the entry sees to it)
   hipLaunchKernelGGL((linear_mxfp4_few_kernel<MT, NT, QX>), dim3((unsigned)((a.N + 16 * NT - 1) / (16 * NT))), dim3(kFewBlock), 0, st, a);
   L8_HIP(hipGetLastError());
   return L8_OK;
@@ -272,10 +272,15 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
   L8_REQUIRE(K == 0 || (x && qw && sw), "l8_mxfp4_linear: null pointer");
   L8_REQUIRE(K == 0 || (K % 8 == 0 && ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0), "l8_mxfp4_linear: K=%lld and ldx must be multiples of 8, x 16-byte aligned", (long long)K);
   L8_REQUIRE(M < (1 << 20) - 16 && N < (1 << 28) && K < (1 << 24), "l8_mxfp4_linear: M < 2^20 - 16, N < 2^28 and K < 2^24 are served");
-  if (K == 0) ldx = ldqw = ldsw = 0;
+  // (a workgroup for 16 weight rows, of 512 threads: fewer than 2^32 of them)
+  L8_REQUIRE(!few_tokens(M, N) || N <= (1 << 27) - 16, "l8_mxfp4_linear: N <= 2^27 - 16 is served for up to 16 tokens");
+  if (K == 0) ldx = ldqw = ldsw = 0, x = qw = sw = nullptr;
   L8_REQUIRE(ldqw % 16 == 0 && ldqw >= blocks * 16 && ldqw <= (1 << 23) - 16 && ((uintptr_t)qw % 16) == 0 && ldsw >= blocks,
              "l8_mxfp4_linear: rows of codes on 16-byte lines less than 2^23 bytes apart, and a scale per block, are wanted");
   const MxLinearPlan plan = plan_of(M, N, K);
+  const bool move_scales = !few_tokens(M, N) && (ldsw % 16 || ldsw > (1 << 23) - 16 || ((uintptr_t)sw % 16));
+  const int64_t pieces = plan.lds / 16, move_groups = (N * pieces + 255) / 256;
+  L8_REQUIRE(!move_scales || move_groups < (1 << 24), "l8_mxfp4_linear: more scales to copy than a grid has threads");
   L8_REQUIRE(plan.total == 0 || (workspace && workspace_bytes >= plan.total && ((uintptr_t)workspace % 16) == 0),
              "l8_mxfp4_linear: needs a 16-byte aligned workspace of %lld bytes", (long long)plan.total);
   hipStream_t st = (hipStream_t)stream;
@@ -291,10 +296,8 @@ extern "C" int l8_mxfp4_linear(const void *x, int64_t M, int64_t K, int64_t ldx,
     a.x = ws + plan.q, a.ldx = plan.ldq, a.sx = ws + plan.s, a.ldsx = plan.lds;
     return mxfp4_few_packed(a, st);
   }
-  if (ldsw % 16 || ldsw > (1 << 23) - 16 || ((uintptr_t)sw % 16)) {   // a launch of 3 us
-    const int64_t pieces = plan.lds / 16, grid = (N * pieces + 255) / 256;
-    L8_REQUIRE(grid < (1LL << 31), "l8_mxfp4_linear: more scales than a grid has threads");
-    hipLaunchKernelGGL(mxfp4_scales_on_lines_kernel, dim3((unsigned)grid), dim3(256), 0, st, (const uint8_t *)sw, ldsw, N, (int)blocks, ws + plan.scales, (int)pieces);
+  if (move_scales) {   // a launch of 3 us
+    hipLaunchKernelGGL(mxfp4_scales_on_lines_kernel, dim3((unsigned)move_groups), dim3(256), 0, st, (const uint8_t *)sw, ldsw, N, (int)blocks, ws + plan.scales, (int)pieces);
     L8_HIP(hipGetLastError());
     sw = ws + plan.scales, ldsw = plan.lds;
   }

@@ -234,3 +234,16 @@ def test_python_forms_refuse_second_derivatives(name, linear_loss, monkeypatch):
             continue
         with pytest.raises(RuntimeError, match=f"{name} is not differentiable twice"):
             (loss + grad.float().square().sum()).backward()
+
+
+# 2^32 threads and more are not a grid: refused before anything is enqueued
+def test_more_threads_than_a_grid_has_are_refused():
+    wide = dict(M=(1 << 20) - 256, N=(1 << 20) - 1, ldc=1 << 20, ws=P, ws_bytes=1 << 60)     # (an odd N: tiles of 128 x 128)
+    assert refused("l8_gemm_mxfp4_nt", *{**GEMM, **wide}.values())
+    assert refused("l8_cast_mxfp4", *{**CAST, **dict(R=1, C=1 << 30, ldx=1 << 30, ldq=1 << 29, lds=1 << 25, ldqt=16, ldst=4)}.values())
+    import struct
+    small, large = [P, 64, 64, 64, P, 32, P, 16, P, 32, P, 16], [P, 1, 1 << 30, 1 << 30, P, 1 << 29, P, 1 << 25, P, 16, P, 4]
+    assert refused("l8_cast_mxfp4_two", struct.pack("24q", *small, *large), None)
+    assert refused("l8_mxfp4_linear", *{**LINEAR, **dict(N=(1 << 27) - 15, K=32, ldx=32, ldqw=16, ldsw=1, ldy=1 << 27)}.values())
+    odd = dict(M=100, N=(1 << 27) - 16, K=(1 << 24) - 32, ldx=1 << 24, ldqw=(1 << 23) - 16, ldsw=(1 << 19) + 1, ldy=1 << 27, ws=P, ws_bytes=1 << 60)
+    assert refused("l8_mxfp4_linear", *{**LINEAR, **odd}.values())
