@@ -41,9 +41,10 @@ struct MxGemmArgs {
   bool wide;                      // TN columns of C can be stored at once
 };
 
-// s_waitcnt vmcnt(n), and lgkmcnt(0), alone
+// s_waitcnt vmcnt(n) alone, and with lgkmcnt(0).  In front of a barrier that hands a ring slot back to the loads it is the second: the
+// wave's fragment reads of that slot must have returned, or a load to LDS overtakes them.
 #define MX_WAIT_VM(n) __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (0x7 << 4) | (0xF << 8) | ((((n) >> 4) & 0x3) << 14))
-#define MX_WAIT_LGKM0() __builtin_amdgcn_s_waitcnt(0xF | (0x7 << 4) | (0x0 << 8) | (0x3 << 14))
+#define MX_WAIT_VM_LGKM0(n) __builtin_amdgcn_s_waitcnt(((n) & 0xF) | (0x7 << 4) | ((((n) >> 4) & 0x3) << 14))
 
 // f(0), f(1), .. as straight code, each with its number as a constant
 template <typename F, int... I>
@@ -188,7 +189,7 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_mxfp4_kernel(const MxGemmArg
       for (int r = (N_RD * i) / N_MMA; r < (N_RD * (i + 1)) / N_MMA; ++r) read_frag(1, r);
       __builtin_amdgcn_sched_barrier(0);
     });
-    __builtin_amdgcn_s_waitcnt((((NS - 2) * (NLA + NLB)) & 0xF) | (0x7 << 4) | ((((NS - 2) * (NLA + NLB)) >> 4) << 14));
+    MX_WAIT_VM_LGKM0((NS - 2) * (NLA + NLB));
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -562,8 +563,8 @@ __global__ __launch_bounds__(256) void gemm_mxfp4_stream_kernel(const MxGemmArgs
     });
     frag_addrs(wrap(s0 + 2) * UNIT, wrap(s0 + 3) * UNIT, ad);
     constexpr int PEND = NL + (ODD ? 0 : NSC);
-    if (!ODD && stores) __builtin_amdgcn_s_waitcnt(((N_STORES + PEND) & 0xF) | (0x7 << 4) | (((N_STORES + PEND) >> 4) << 14));
-    else __builtin_amdgcn_s_waitcnt((PEND & 0xF) | (0x7 << 4) | ((PEND >> 4) << 14));
+    if (!ODD && stores) MX_WAIT_VM_LGKM0(N_STORES + PEND);
+    else MX_WAIT_VM_LGKM0(PEND);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
