@@ -58,27 +58,25 @@ class Fp8RMSNormFn(torch.autograd.Function):
 
 
 class Fp8AddRMSNormFn(torch.autograd.Function):
+    """``add_rmsnorm`` on 2-D operands.  (It returns what it made and no views of it: those could not be written in place.)"""
+
     @staticmethod
     def forward(ctx, x, residual, weight, eps, training):
         if x.dtype != torch.bfloat16 or residual.dtype != torch.bfloat16:
             raise RuntimeError(f"add_rmsnorm: bf16 activations required, got {x.dtype} and {residual.dtype}")
-        if x.shape != residual.shape:
-            raise RuntimeError(f"add_rmsnorm: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
         want_col = bool(training and f8.config.fp8_wgrad)
-        x2d, r2d = x.flatten(end_dim=-2), residual.flatten(end_dim=-2)
-        col = torch.empty(x2d.shape[1], dtype=torch.float32, device=x.device) if want_col else None
-        h2d, y2d, q, s, rstd = ops.add_rmsnorm_cast_rowwise(x2d, r2d, weight, eps, col_amax=col, on_lines=True)
-        if f8.config.share_input_casts:
-            f8._fwd_cast.put(y2d, (q, s, col), "rmsnorm")
+        col = torch.empty(x.shape[1], dtype=torch.float32, device=x.device) if want_col else None
+        h, y, q, s, rstd = ops.add_rmsnorm_cast_rowwise(x, residual, weight, eps, col_amax=col, on_lines=True)
+        if f8.config.share_input_casts:   # (the memo keeps its tensor: not the graph behind it)
+            f8._fwd_cast.put(y.detach(), (q, s, col), "rmsnorm")
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(h2d, weight, rstd)
-        ctx.x_shape = x.shape
+        ctx.save_for_backward(h, weight, rstd)
         ctx.sum_learns = x.requires_grad or residual.requires_grad
-        return h2d.unflatten(0, x.shape[:-1]), y2d.unflatten(0, x.shape[:-1])
+        return h, y
 
     @staticmethod
     def backward(ctx, gh, gy):
-        h2d, weight, rstd = ctx.saved_tensors
+        h, weight, rstd = ctx.saved_tensors
         need = ctx.needs_input_grad
         for g in (gh, gy):
             if g is not None and g.dtype != torch.bfloat16:
@@ -88,12 +86,10 @@ class Fp8AddRMSNormFn(torch.autograd.Function):
         gy_learns = f8._learns(gy)
         gx_varies = ctx.sum_learns or f8._learns(weight) or f8._learns(gh) or gy_learns
         with torch.no_grad():
-            gy2d = gy.flatten(end_dim=-2)
             if gh is None:
-                gx2d, gw = ops.rmsnorm_bwd(gy2d, h2d, weight, rstd, gw_dtype=weight.dtype)
+                gx, gw = ops.rmsnorm_bwd(gy, h, weight, rstd, gw_dtype=weight.dtype)
             else:
-                gx2d, gw = ops.add_rmsnorm_bwd(gy2d, gh.flatten(end_dim=-2), h2d, weight, rstd, gw_dtype=weight.dtype)
-            gx = gx2d.reshape(ctx.x_shape)
+                gx, gw = ops.add_rmsnorm_bwd(gy, gh, h, weight, rstd, gw_dtype=weight.dtype)
         grads = gx if need[0] else None, gx if need[1] else None, gw if need[2] else None
         return (*f8._once("add_rmsnorm", grads, (gx_varies, gx_varies, ctx.sum_learns or gy_learns)), None, None)
 
@@ -112,7 +108,12 @@ def add_rmsnorm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor, e
                 f8._fwd_cast.put(y.detach().flatten(end_dim=-2), (q, s, col), "rmsnorm")
             return h, y
     f8._refuse_captured(x, residual, weight, "add_rmsnorm")
-    return Fp8AddRMSNormFn.apply(x, residual, weight, eps, training)
+    if x.shape != residual.shape:
+        raise RuntimeError(f"add_rmsnorm: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
+    if x.dim() == 2:
+        return Fp8AddRMSNormFn.apply(x, residual, weight, eps, training)
+    h, y = Fp8AddRMSNormFn.apply(x.flatten(end_dim=-2), residual.flatten(end_dim=-2), weight, eps, training)
+    return h.unflatten(0, x.shape[:-1]), y.unflatten(0, x.shape[:-1])
 
 
 class Fp8RMSNorm(torch.nn.Module):

@@ -362,3 +362,21 @@ def test_column_amaxes_elsewhere_are_refused():
         call(col.cuda())
         with pytest.raises(RuntimeError, match="same device"):
             call(col)
+
+
+@pytest.mark.parametrize("shape", [(24, 64), (2, 12, 64)])
+def test_outputs_may_be_written_in_place(shape, host):
+    """As any operator's: the norm and what it is multiplied by in place have the gradients of the product, and a sum that was written
+    over before the backward pass that needs it is an error."""
+    from lingua_amd import norm
+    x, res, gain = (seeded_bf16(s, seed=i).cuda().requires_grad_() for i, s in enumerate((shape, shape, (64,))))
+    h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+    want = torch.autograd.grad((y * 2.0).sum() + h.sum(), (x, res, gain))
+    h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+    y.mul_(2.0)
+    for got, w in zip(torch.autograd.grad(y.sum() + h.sum(), (x, res, gain)), want):
+        assert torch.equal(got, w)
+    h, y = norm.add_rmsnorm(x, res, gain, 1e-5)
+    h.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
