@@ -782,6 +782,13 @@ MxRows rows_of(const Mx &m) {
   return r;
 }
 
+// Rows of bytes that start on 16-byte lines, as the product wants them: `t` where they do, else a copy.  (Hooks on saved tensors hand a
+// kept copy back in any layout.)
+Tensor on_lines_of_16(const Tensor &t) {
+  if (!t.defined() || t.dim() != 2 || !t.is_cuda() || (((uintptr_t)t.const_data_ptr() % 16) == 0 && t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) % 16 == 0))) return t;
+  return at::empty_strided(t.sizes(), {(t.size(1) + 15) / 16 * 16, 1}, t.options()).copy_(t);
+}
+
 // cast_mxfp4(x, rowwise, transposed, on_lines) -> (q, s, qt, st) or None
 PyObject *cast_mxfp4(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -897,11 +904,14 @@ PyObject *refuse_captured_py(PyObject *, PyObject *const *args, Py_ssize_t n) {
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
-// A gradient as the kernels take it: bf16, of `sizes`, dense rows.
+// A bf16 matrix as the kernels take it, or a dense copy.  (Hooks on saved tensors hand a kept one back in any layout, as gradients come.)
+Tensor aligned_rows(const Tensor &t) {
+  Rows r;
+  return as_rows(t, t.get_device(), r) && on_16_bytes(r) ? t : t.clone(at::MemoryFormat::Contiguous);
+}
 Tensor gradient(const Tensor &g, const char *what) {
   TORCH_CHECK(g.scalar_type() == at::kBFloat16, what, " backward: bf16 gradients required, got ", g.scalar_type());
-  Rows r;
-  return as_rows(g, g.get_device(), r) && on_16_bytes(r) ? g : g.clone(at::MemoryFormat::Contiguous);
+  return aligned_rows(g);
 }
 Rows rows_of(const Tensor &t) {
   Rows r;
@@ -933,9 +943,9 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &h = saved[0], &w = saved[1], &rstd = saved[2];
     Tensor gx, gw;
     if (grads[1].defined()) {
+      const Tensor h = aligned_rows(saved[0]), w = saved[1].contiguous(), rstd = saved[2].contiguous();
       const Tensor gy = gradient(grads[1], kName), gh = grads[0].defined() ? gradient(grads[0], kName) : Tensor();
       const Rows rg = rows_of(gy), rh = rows_of(h);
       const Rows ru = gh.defined() ? rows_of(gh) : Rows();
@@ -955,7 +965,7 @@ struct AddRMSNorm : torch::autograd::Function<AddRMSNorm> {
       TORCH_CHECK(grads[0].scalar_type() == at::kBFloat16, kName, " backward: bf16 gradients required, got ", grads[0].scalar_type());
       return {grads[0], grads[0], Tensor(), Tensor(), Tensor()};
     }
-    const bool sum_learns = ctx->saved_data["sum learns"].toBool(), gx_varies = sum_learns || learns(w) || learns(grads[0]) || learns(grads[1]);
+    const bool sum_learns = ctx->saved_data["sum learns"].toBool(), gx_varies = sum_learns || learns(saved[1]) || learns(grads[0]) || learns(grads[1]);
     return once({gx, gx, gw, Tensor(), Tensor()}, {gx_varies, gx_varies, sum_learns || learns(grads[1])}, kName);
   }
 };
@@ -1061,7 +1071,8 @@ struct Rotary : torch::autograd::Function<Rotary> {
     if (x[0].defined() || x[1].defined()) {
       const c10::DeviceGuard guard((x[0].defined() ? x[0] : x[1]).device());
       const Tensor in[2] = {x[0], x[1]};
-      rotate(in, g, saved[0], saved[1], saved[2], ctx->saved_data["half"].toBool(), true);
+      const bool alike = saved[0].strides() == saved[1].strides();   // (hooks may have handed one back in another layout)
+      rotate(in, g, alike ? saved[0] : saved[0].contiguous(), alike ? saved[1] : saved[1].contiguous(), saved[2], ctx->saved_data["half"].toBool(), true);
     }
     return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()}, {learns(grads[0]), learns(grads[1])}, "rotary");
   }
@@ -1139,7 +1150,8 @@ struct Mxfp4Linear : torch::autograd::Function<Mxfp4Linear> {
     return y;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
+    auto saved = ctx->get_saved_variables();
+    for (Tensor &t : saved) t = on_lines_of_16(t);
     const Tensor gy = gradient(grads[0], "mxfp4_linear");
     const int device = gy.get_device();
     const c10::DeviceGuard guard(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));

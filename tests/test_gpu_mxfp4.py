@@ -450,6 +450,27 @@ def test_two_streams_at_once():
     assert all(torch.equal(g, w) for gs, w in zip(got, want) for g in gs)
 
 
+@pytest.mark.parametrize("M,K,N", [(40, 80, 48), (300, 528, 272)])
+@pytest.mark.parametrize("hooks", ["clones", "host", "rows apart"])
+def test_kept_copies_in_other_layouts(M, K, N, hooks, host):
+    """Hooks on saved tensors hand the kept copies back in layouts of their own: the gradients are the same."""
+    from lingua_amd import mxfp4
+
+    def apart(t):
+        return torch.empty_strided(t.shape, (t.shape[1] + 3, 1), dtype=torch.uint8, device=t.device).copy_(t.view(torch.uint8)).view(t.dtype)
+
+    with_hooks = {"clones": lambda: torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), lambda t: t.contiguous()),
+                  "host": torch.autograd.graph.save_on_cpu,
+                  "rows apart": lambda: torch.autograd.graph.saved_tensors_hooks(apart, lambda t: t)}[hooks]
+    leaves = [seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((M, K), (N, K), (N,)))]
+    gy = seeded_bf16((M, N), std=0.01, seed=5).cuda()
+    want = torch.autograd.grad(mxfp4.mxfp4_linear(*leaves), leaves, gy)
+    with with_hooks():
+        y = mxfp4.mxfp4_linear(*leaves)
+    for got, w in zip(torch.autograd.grad(y, leaves, gy), want):
+        assert torch.equal(got, w)
+
+
 def test_rows_off_their_lines(host):
     """Operands and gradients that start at odd elements, an odd number of elements apart: copied, with the results of dense ones."""
     from lingua_amd import mxfp4, ops

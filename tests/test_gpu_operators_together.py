@@ -380,3 +380,33 @@ def test_outputs_may_be_written_in_place(shape, host):
     h.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("name", ["add_rmsnorm", "rotary"])
+def test_kept_operands_in_other_layouts(name, host):
+    """Hooks on saved tensors hand every second operand back with its elements apart: the gradients are the same."""
+    from lingua_amd import rope
+    leaves = [seeded_bf16(s, std=0.1, seed=i).cuda().requires_grad_() for i, s in enumerate(((8, 64), (64, 64), (64,)))]
+    tables = [t.cuda() for t in rope.rotary_tables(32, 8)]
+
+    def run():
+        y, of = twice(name, *leaves, tables)
+        return lambda: torch.autograd.grad(y, of, gy)
+
+    def apart(t):
+        return torch.stack((t, torch.full_like(t, 7.0)), -1)[..., 0]
+
+    gy = seeded_bf16((8, 64), std=0.01, seed=5).cuda()
+    want = run()()
+    for parity in (0, 1):
+        calls_made = []
+
+        def pack(t):
+            calls_made.append(t)
+            return apart(t) if len(calls_made) % 2 == parity else t
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            later = run()
+        assert calls_made
+        for got, w in zip(later(), want):
+            assert torch.equal(got, w)
