@@ -410,3 +410,35 @@ def test_kept_operands_in_other_layouts(name, host):
         assert calls_made
         for got, w in zip(later(), want):
             assert torch.equal(got, w)
+
+
+class Gate(torch.autograd.Function):
+    """silu, whose backward takes the same steps in a pass that is itself differentiated (PyTorch's rounds more often there)."""
+
+    @staticmethod
+    def forward(ctx, x):
+        ctx.save_for_backward(x)
+        return F.silu(x)
+
+    @staticmethod
+    def backward(ctx, g):
+        with torch.no_grad():
+            return torch.ops.aten.silu_backward(g, ctx.saved_tensors[0])
+
+
+def test_a_model_whose_gradients_are_made_for_differentiation(monkeypatch):
+    """The refusal waits until somebody differentiates: a pass with create_graph through every operator and the fp8 ones beside them has the
+    bits of an ordinary one."""
+    model = model_of(True)
+    for layer in model.layers:
+        mlp = layer.feed_forward
+        monkeypatch.setattr(mlp, "forward", lambda x, m=mlp: m.w2(Gate.apply(m.w1(x)) * m.w3(x)))
+    tokens = torch.randint(0, 64, (2, 37), generator=torch.Generator().manual_seed(2)).cuda()
+    names, of = zip(*[(n, p) for n, p in model.named_parameters() if n != "tok_embeddings.weight"])   # (that gradient is added up by atomics)
+
+    def grads(**kwargs):
+        return torch.autograd.grad(F.cross_entropy(model(tokens).flatten(0, 1).float(), tokens.flatten()), of, **kwargs)
+
+    want = grads()
+    for name, got, w in zip(names, grads(create_graph=True), want):
+        assert torch.equal(got, w), name
