@@ -337,6 +337,67 @@ int l8_add_rmsnorm_bwd(const void *gy, const void *gh, const void *h, const void
                        int64_t C, int64_t ldgy, int64_t ldgh, int64_t ldh, void *gx, int64_t ldgx, void *gw, int gw_is_f32,
                        void *workspace, int64_t workspace_bytes, void *stream);
 
+/* Dropout by a counter-based generator, whose mask is never stored: y[i] = residual[i] + (bits(i) >= threshold ? x[i] * 65536 / (65536 -
+ * threshold) : 0), in fp32, rounded once.  bits(i): 16 bits of Philox4x32-10 with counter (i / 8, low and high 32 bits; site; step, low 32
+ * bits) and key seed; element i takes the lower (i even) or upper half of word i % 8 / 2.
+ *   x, y, residual  bf16 [n], dense, any even address; residual NULL: none; y may be x or residual
+ *   numbers         int64 {seed, step} on the GPU, read when the kernel runs
+ *   site            0 .. 2^32 - 1: which of a step's calls this is
+ *   threshold       0 .. 65536, the dropped share in 1/65536; 65536: everything
+ * Requires n < 2^35. */
+int l8_dropout(const void *x, const void *residual, void *y, int64_t n, const int64_t *numbers, int64_t site, int64_t threshold, void *stream);
+
+/* Layer norm with the row-wise cast of its output, of a residual sum and of a sum with a dropped operand; RMSNorm of such a sum.
+ *   h = x, or with residual h = bf16(residual + x), or with numbers h = bf16(residual + dropout(x)), element (r,c) being i = r * C + c
+ *   centred: y = bf16((h - mean) * rstd * w + b), rstd = 1 / sqrt(var + eps); else y = bf16(h * rstd * w), rstd = 1 / sqrt(mean(h^2) + eps)
+ *   w, b            bf16 or (w_is_f32, b_is_f32) fp32 [C]; NULL: ones, zeros
+ *   h               written with residual (else ignored)
+ *   q, scale        as l8_cast_rowwise of y; both NULL: no cast.  col_amax fp32 [C] or NULL, with a workspace of l8_rmsnorm_workspace bytes
+ *   mean, rstd      fp32 [R], kept for the backward pass; either may be NULL
+ * Without `centred` residual, numbers and w are needed and b is NULL (l8_rmsnorm_cast_rowwise and l8_add_rmsnorm_cast_rowwise are the others).
+ * Requires C % 8 == 0, C <= 8192, bf16 operands on 16-byte lines. */
+typedef struct {
+  const void *x, *residual, *w, *b;
+  int64_t w_is_f32, b_is_f32, centred, R, C, ldx, ldr;
+  double eps;
+  const int64_t *numbers;
+  int64_t site, threshold;
+  void *h;
+  int64_t ldh;
+  void *y;
+  int64_t ldy;
+  void *q;
+  int64_t ldq;
+  float *scale, *mean, *rstd, *col_amax;
+  void *workspace;
+  int64_t workspace_bytes;
+  void *stream;
+} l8_norm_fwd_args;
+int l8_norm_fwd(const l8_norm_fwd_args *args);
+/* Its backward pass: gx, the gradient of h (gh, the gradient that arrives at h itself, may be NULL) and with it of x and residual; with
+ * numbers gres is the gradient of h and gx = dropout(gres before rounding).  gw, gb (bf16 or fp32 [C], either may be NULL) are sums over the
+ * rows in a fixed order; with either a workspace of l8_norm_bwd_workspace bytes. */
+typedef struct {
+  const void *gy, *gh, *h, *w;
+  int64_t w_is_f32, centred, R, C, ldgy, ldgh, ldh;
+  const float *mean, *rstd;
+  const int64_t *numbers;
+  int64_t site, threshold;
+  void *gx;
+  int64_t ldgx;
+  void *gres;
+  int64_t ldgres;
+  void *gw;
+  int64_t gw_is_f32;
+  void *gb;
+  int64_t gb_is_f32;
+  void *workspace;
+  int64_t workspace_bytes;
+  void *stream;
+} l8_norm_bwd_args;
+int l8_norm_bwd(const l8_norm_bwd_args *args);
+int64_t l8_norm_bwd_workspace(int64_t R, int64_t C, int64_t centred);
+
 /* Rotary positions of queries and keys (apply_rotary_emb of lingua/transformer.py), both in one launch:
  *   y[b,s,h,:] = x[b,s,h,:] with its first `rot` columns turned: pair i = columns (2 i, 2 i + 1), or with in_halves
  *   (i, i + rot / 2), (a, c) -> (a cos - c sin, a sin + c cos) in fp32, rounded once; the other columns are copied.

@@ -63,6 +63,10 @@ SIGNATURES = {
     "l8_rmsnorm_bwd_as": [_p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _i64, _p],
     "l8_add_rmsnorm_cast_rowwise": [_p, _p, _p, _int, _i64, _i64, _i64, _i64, ctypes.c_float, _p, _i64, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _p],
     "l8_add_rmsnorm_bwd": [_p, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _int, _p, _i64, _p],
+    "l8_dropout": [_p, _p, _p, _i64, _p, _i64, _i64, _p],
+    "l8_norm_fwd": [ctypes.c_char_p],
+    "l8_norm_bwd": [ctypes.c_char_p],
+    "l8_norm_bwd_workspace": [_i64, _i64, _i64],
     "l8_rotary": [_p, _i64, _i64, _i64, _i64, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _p],
     "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
     "l8_cast_mxfp4_two": [_p, _p],
@@ -83,7 +87,7 @@ SIGNATURES = {
     "l8_gemm_pick": [_i64, _i64, _i64],
 }
 _RETURNS_STR = {"l8_last_error", "l8_gemm_algo_name"}
-_RETURNS_I64 = {"l8_cast_rowwise_workspace", "l8_gemm_workspace", "l8_gemm_workspace_gave_up_offset", "l8_swiglu_workspace", "l8_rmsnorm_workspace", "l8_rmsnorm_bwd_workspace",
+_RETURNS_I64 = {"l8_cast_rowwise_workspace", "l8_gemm_workspace", "l8_gemm_workspace_gave_up_offset", "l8_swiglu_workspace", "l8_rmsnorm_workspace", "l8_rmsnorm_bwd_workspace", "l8_norm_bwd_workspace",
                 "l8_linear_fwd_workspace", "l8_linear_fwd_rows_workspace", "l8_col_sum_workspace", "l8_gemm_mxfp4_workspace", "l8_mxfp4_linear_workspace"}
 
 _lib = None

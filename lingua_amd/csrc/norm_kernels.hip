@@ -19,92 +19,9 @@
 // Two layouts, as in the row-wise casts: a wavefront per row for short rows, a
 // 256-thread workgroup per row for the longer ones; both add a row up in the same
 // order, so a row's result does not hang on the layout.
-#include "l8_common.h"
+#include "norm.h"
 
 namespace l8 {
-
-constexpr int kNormBlock = 256;
-constexpr int kNormWaves = kNormBlock / 64;
-
-// sum over the 64 lanes of a wave, result uniform
-L8_DEV float wave_sum_f32(float v) {
-  auto step = [&](int moved) { v += __int_as_float(moved); };
-  step(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xB1, 0xF, 0xF, true));   // quad_perm [1,0,3,2]
-  step(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4E, 0xF, 0xF, true));   // quad_perm [2,3,0,1]
-  step(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x124, 0xF, 0xF, true));  // row_ror:4
-  step(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xF, 0xF, true));  // row_ror:8
-  const float a = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0));
-  const float b = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 16));
-  const float c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32));
-  const float d = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 48));
-  return (a + b) + (c + d);
-}
-
-// The weights of a lane's columns, kept in registers for all rows it sees: packed pairs as they are in memory (bf16),
-// or one register each (fp32).  Zero beyond column C.
-template <int N, bool W_F32>
-struct NormWeights {
-  uint32_t reg[N * (W_F32 ? 8 : 4)];
-  template <typename ColOf>
-  L8_DEV void load(const void *w, int C, ColOf col_of) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const int c = col_of(j);
-#pragma unroll
-      for (int e = 0; e < (W_F32 ? 8 : 4); ++e) {
-        uint32_t v = 0;
-        // a bf16 weight may start at any even address: the copy states two-byte alignment
-        if (c < C) {
-          if (W_F32) v = ((const uint32_t *)w)[c + e];
-          else __builtin_memcpy(&v, (const uint16_t *)w + c + 2 * e, 4);
-        }
-        reg[j * (W_F32 ? 8 : 4) + e] = v;
-      }
-    }
-  }
-  L8_DEV float get(int j, int e) const {
-    if (W_F32) return __uint_as_float(reg[j * 8 + e]);
-    const uint32_t p = reg[j * 4 + (e >> 1)];
-    return __uint_as_float((e & 1) ? (p & 0xffff0000u) : (p << 16));
-  }
-};
-
-#if defined(__HIP_DEVICE_COMPILE__)
-// row r of x; zeros beyond column C and for a row at or beyond R (no branch around a load)
-template <int N, typename ColOf>
-L8_DEV void load_norm_row(v4i (&buf)[N], const uint16_t *x, int64_t r, int64_t R, int64_t ldx, int C, ColOf col_of) {
-  const __amdgpu_buffer_rsrc_t rs = make_rsrc(x + (r < R ? r : 0) * ldx, r < R ? (uint32_t)C * 2u : 0u);
-#pragma unroll
-  for (int j = 0; j < N; ++j) buf[j] = load16_nt(rs, (uint32_t)col_of(j) * 2u, 0);
-}
-L8_DEV void store16_nt(__amdgpu_buffer_rsrc_t rs, uint32_t voff, v4i data) {
-  __builtin_amdgcn_raw_buffer_store_b128(data, rs, (int)voff, 0, 2 /* non-temporal */);
-}
-L8_DEV void store8_nt(__amdgpu_buffer_rsrc_t rs, uint32_t voff, v2i data) {
-  __builtin_amdgcn_raw_buffer_store_b64(data, rs, (int)voff, 0, 2 /* non-temporal */);
-}
-// Eight bf16 plus eight bf16, each sum rounded to nearest even.
-L8_DEV v4i sum_bf16x8(v4i a, v4i b) {
-  v4i out;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float lo = __uint_as_float((uint32_t)a[k] << 16) + __uint_as_float((uint32_t)b[k] << 16);
-    const float hi = __uint_as_float((uint32_t)a[k] & 0xffff0000u) + __uint_as_float((uint32_t)b[k] & 0xffff0000u);
-    out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
-  }
-  return out;
-}
-// The row of x becomes the row of h = bf16(x + residual), which is also written: the norm is that of the sum as it is kept.
-template <int N, typename ColOf>
-L8_DEV void add_residual(v4i (&cur)[N], const v4i (&res)[N], uint16_t *h, int64_t r, int64_t ldh, int C, ColOf col_of) {
-  const __amdgpu_buffer_rsrc_t rsH = make_rsrc(h + r * ldh, (uint32_t)C * 2u);
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    cur[j] = sum_bf16x8(cur[j], res[j]);
-    store16_nt(rsH, (uint32_t)col_of(j) * 2u, cur[j]);
-  }
-}
-#endif
 
 // The residual stream of a block (lingua/transformer.py:497-543: h = x + attention(..), then ffn_norm(h)): kernels with ADD
 // read a second operand of x's shape, write the sum and normalise it.  9 bytes per element, HBM-bound: [16384,4096] 111.6 us,
@@ -441,9 +358,10 @@ __global__ __launch_bounds__(kNormBlock, 2) void rmsnorm_bwd_kernel(
 // time: 16 bytes per thread and load, the next 256 rows in flight under the additions, which come one after the other
 // but read LDS.  (With each addition waiting for its row from memory the fold of 512 rows of 2048 columns took 20 us.)
 // gw leaves as fp32 or, for a bf16 weight, rounded: a conversion of its own was a launch of 4 to 5 us for a few KiB.
+// A layer norm's rows hold its bias's sums too, behind column `first.n`: those leave through `second`.
 constexpr int kGwCols = 32, kGwThreads = 1024, kGwRows = 256, kGwSums = 8;
 __global__ __launch_bounds__(kGwThreads) void rmsnorm_gw_fold_kernel(const float *__restrict__ partials, int n_slots, int C,
-                                                                     void *__restrict__ gw, int gw_f32) {
+                                                                     const GradOut first, const GradOut second) {
   constexpr int QUADS = kGwCols / 4, STEP = kGwThreads / QUADS, LOADS = kGwRows / STEP;  // threads to a row, rows to a load
   __shared__ v4f rows[kGwRows][QUADS];
   __shared__ float sums[kGwSums][kGwCols];
@@ -479,17 +397,26 @@ __global__ __launch_bounds__(kGwThreads) void rmsnorm_gw_fold_kernel(const float
     float t = sums[0][tx];
 #pragma unroll
     for (int k = 1; k < kGwSums; ++k) t += sums[k][tx];
-    if (gw_f32) ((float *)gw)[c] = t;
-    else ((uint16_t *)gw)[c] = (uint16_t)bf16_rne_bits(t);
+    const GradOut &out = c < first.n ? first : second;
+    const int at = c < first.n ? c : c - first.n;
+    if (!out.p) return;
+    if (out.f32) ((float *)out.p)[at] = t;
+    else ((uint16_t *)out.p)[at] = (uint16_t)bf16_rne_bits(t);
   }
 }
 
-static int64_t norm_blocks(int64_t R) {
+int fold_norm_grads(const float *partials, int64_t slots, const GradOut &first, const GradOut &second, hipStream_t st) {
+  const int C = first.n + second.n;
+  if (C == 0) return L8_OK;
+  hipLaunchKernelGGL(rmsnorm_gw_fold_kernel, dim3((unsigned)((C + kGwCols - 1) / kGwCols)), dim3(kGwThreads), 0, st, partials, (int)slots, C, first, second);
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+int64_t norm_blocks(int64_t R) {
   const int64_t cap = (int64_t)num_cus() * 2;
   return R < cap ? R : cap;
 }
-
-constexpr int64_t kNormMaxC = 4 * kNormWaves * 512;  // 8192: the weights of a thread's columns live in registers
 
 // Which layout, forward: a wavefront per row up to 2048 columns, a workgroup per row beyond (up to 8192), where a wave's
 // row, the row requested ahead, the weights and the column maxima no longer fit 256 registers.  Inside a 1B-sized step,
@@ -532,10 +459,7 @@ static int launch_norm_bwd(const void *gy, const void *x, const void *w, const f
   hipLaunchKernelGGL((rmsnorm_bwd_kernel<N, N == 1 ? 4 : 2, W_F32, ADD>), dim3((unsigned)blocks), dim3(kNormBlock), 0, st, (const uint16_t *)gy,
                      (const uint16_t *)x, w, rstd, R, (int)C, ldg, ldx, (uint16_t *)gx, ldgx, (float *)ws, (const uint16_t *)gh, ldgh);
   L8_HIP(hipGetLastError());
-  hipLaunchKernelGGL(rmsnorm_gw_fold_kernel, dim3((unsigned)((C + kGwCols - 1) / kGwCols)), dim3(kGwThreads), 0, st,
-                     (const float *)ws, (int)blocks, (int)C, gw, gw_f32);
-  L8_HIP(hipGetLastError());
-  return L8_OK;
+  return fold_norm_grads((const float *)ws, blocks, GradOut{gw, gw_f32, (int)C}, GradOut{nullptr, 0, 0}, st);
 }
 
 }  // namespace l8
@@ -562,12 +486,8 @@ static int rmsnorm_bwd_impl(const char *who, const void *gy, const void *x, cons
   L8_REQUIRE(R >= 0 && C >= 0, "%s: negative shape R=%lld C=%lld", who, (long long)R, (long long)C);
   if (C == 0) return L8_OK;
   L8_REQUIRE(gw, "%s: null pointer", who);
-  if (R == 0) {  // no rows: gw = 0, written by the fold kernel over zero partial rows
-    hipLaunchKernelGGL(rmsnorm_gw_fold_kernel, dim3((unsigned)((C + kGwCols - 1) / kGwCols)), dim3(kGwThreads), 0, (hipStream_t)stream,
-                       (const float *)nullptr, 0, (int)C, gw, gw_is_f32);
-    L8_HIP(hipGetLastError());
-    return L8_OK;
-  }
+  if (R == 0)  // no rows: gw = 0, written by the fold kernel over zero partial rows
+    return fold_norm_grads(nullptr, 0, GradOut{gw, gw_is_f32, (int)C}, GradOut{nullptr, 0, 0}, (hipStream_t)stream);
   L8_REQUIRE(gy && x && w && rstd && gx, "%s: null pointer", who);
   L8_REQUIRE(C % 8 == 0 && ldg % 8 == 0 && ldx % 8 == 0 && ldgx % 8 == 0 && ldg >= C && ldx >= C && ldgx >= C && (!gh || (ldgh % 8 == 0 && ldgh >= C)),
              "%s: C=%lld and the leading dimensions must be multiples of 8 with ld >= C", who, (long long)C);

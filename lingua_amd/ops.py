@@ -842,6 +842,129 @@ def add_rmsnorm_bwd(gy: torch.Tensor, gh: torch.Tensor, h: torch.Tensor, weight:
     return gx, gw
 
 
+def _drop_args(drop, device, what: str):
+    """(address of seed and step, site, threshold) of a ``lingua_amd.dropout.Drop``; (None, 0, 0) of None."""
+    if drop is None:
+        return None, 0, 0
+    p, numbers, site = drop
+    if not 0 <= p <= 1:
+        raise RuntimeError(f"{what}: a share of 0 to 1 is dropped, got {p}")
+    if not 0 <= site < 1 << 32:
+        raise RuntimeError(f"{what}: a site is a number of 32 bits, got {site}")
+    if numbers.dtype != torch.int64 or numbers.shape != (2,) or not numbers.is_contiguous() or numbers.device != device:
+        raise RuntimeError(f"{what}: the seed and step must be two dense int64 numbers on the input's device, got {numbers.dtype} {tuple(numbers.shape)} on {numbers.device}")
+    return numbers.data_ptr(), site, round(65536 * p)
+
+
+def dropout(x: torch.Tensor, drop, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """bf16 x of any shape with the elements of ``drop`` (a ``lingua_amd.dropout.Drop``) dropped, added to ``residual`` if given."""
+    what = "dropout"
+    if x.dtype != torch.bfloat16 or (residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != x.shape or residual.device != x.device)):
+        raise RuntimeError(f"{what}: bf16 tensors of one shape on one device required, got {x.dtype} {tuple(x.shape)}" +
+                           ("" if residual is None else f" and {residual.dtype} {tuple(residual.shape)}"))
+    st = _prep(x, what)
+    ptr, site, threshold = _drop_args(drop, x.device, what)
+    if ptr is None:
+        raise RuntimeError(f"{what}: nothing says what is dropped")
+    x = x.contiguous()
+    residual = residual.contiguous() if residual is not None else None
+    y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+    n = x.numel()
+    with _timed("dropout", n * (4 if residual is None else 6), x.device):
+        code = _lib.load().l8_dropout(x.data_ptr(), None if residual is None else residual.data_ptr(), y.data_ptr(), n, ptr, site, threshold, st)
+    _lib.check(code, "l8_dropout")
+    return y
+
+
+def _norm_param(t, C: int, device, what: str):
+    if t is None:
+        return None
+    if t.dtype not in (torch.bfloat16, torch.float32) or t.numel() != C or t.device != device:
+        raise RuntimeError(f"{what}: weight and bias must be bf16 or fp32 with C elements on the same device")
+    return t.contiguous()
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+_NORM_FWD = struct.Struct("11qd16q")   # l8_norm_fwd_args: eight bytes per member
+_NORM_BWD = struct.Struct("27q")       # l8_norm_bwd_args
+
+
+def layernorm_cast_rowwise(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor], eps: float,
+                           residual: Optional[torch.Tensor] = None, drop=None, centred: bool = True, want_q: bool = True,
+                           col_amax: Optional[torch.Tensor] = None, want_stats: bool = True, on_lines: bool = False):
+    """h = x, or bf16(residual + x), or with ``drop`` (a ``lingua_amd.dropout.Drop``) bf16(residual + dropout(x)); y the layer norm of h
+    and its row-wise cast, in one pass; bf16 [R,C].  ``centred`` False: the RMSNorm of a sum with a dropped operand.
+    Returns (h | None, y, q fp8 | None, scale [R,1] fp32 | None, stats fp32 [2,R] | None: mean and 1 / deviation)."""
+    what = "layernorm_cast_rowwise"
+    x = _rows_on_lines(x, torch.bfloat16, what)
+    st = _prep(x, what)
+    R, C = x.shape
+    dev = x.device
+    if residual is not None:
+        residual = _rows_on_lines(residual, torch.bfloat16, what)
+        if residual.shape != x.shape or residual.device != dev:
+            raise RuntimeError(f"{what}: x and residual must have the same shape and device, got {tuple(x.shape)} and {tuple(residual.shape)}")
+    weight, bias = _norm_param(weight, C, dev, what), _norm_param(bias, C, dev, what)
+    numbers, site, threshold = _drop_args(drop, dev, what)
+    if col_amax is not None and (not want_q or not _column_amaxes(col_amax, C, dev)):
+        raise RuntimeError(f"{what}: col_amax needs the cast and must be a contiguous fp32 tensor with C elements on the same device")
+    h = torch.empty((R, C), dtype=torch.bfloat16, device=dev) if residual is not None else None
+    y = torch.empty((R, C), dtype=torch.bfloat16, device=dev)
+    q = _empty_fp8(R, C, dev, on_lines) if want_q else None
+    scale = torch.empty((R, 1), dtype=torch.float32, device=dev) if want_q else None
+    stats = torch.empty((2, R), dtype=torch.float32, device=dev) if want_stats else None
+    with _timed(what, R * C * ((4 if residual is None else 8) + want_q) + 12 * R, dev):
+        ws_bytes = _lib.load().l8_rmsnorm_workspace(R, C) if col_amax is not None else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        code = _lib.load().l8_norm_fwd(_NORM_FWD.pack(
+            x.data_ptr(), _addr(residual), _addr(weight), _addr(bias), weight is not None and weight.dtype == torch.float32,
+            bias is not None and bias.dtype == torch.float32, centred, R, C, _ld(x), _ld(residual) if residual is not None else 0, float(eps),
+            numbers or 0, site, threshold, _addr(h), C, y.data_ptr(), C, _addr(q), _ld(q) if want_q else 0, _addr(scale),
+            _addr(stats), stats.data_ptr() + 4 * R if want_stats else 0, _addr(col_amax), _addr(ws), ws_bytes, st or 0))
+    _lib.check(code, "l8_norm_fwd")
+    return h, y, q, scale, stats
+
+
+def layernorm_bwd(gy: torch.Tensor, gh: Optional[torch.Tensor], h: torch.Tensor, weight: Optional[torch.Tensor], stats: torch.Tensor, drop=None,
+                  centred: bool = True, gw_dtype: Optional[torch.dtype] = None, gb_dtype: Optional[torch.dtype] = None):
+    """Backward of ``layernorm_cast_rowwise``: (gx, gres | None, gw | None, gb | None) from the gradients gy of the norm and gh (or None) of h
+    itself.  Without ``drop`` gx is the gradient of both operands of the sum; with it gx is x's and gres the residual's.  ``gw_dtype``,
+    ``gb_dtype``: bf16 or fp32, None where that gradient is not wanted."""
+    what = "layernorm_bwd"
+    gy, h = _rows_on_lines(gy, torch.bfloat16, f"{what}(gy)"), _rows_on_lines(h, torch.bfloat16, f"{what}(h)")
+    gh = None if gh is None else _rows_on_lines(gh, torch.bfloat16, f"{what}(gh)")
+    if gy.shape != h.shape or gy.device != h.device or (gh is not None and (gh.shape != h.shape or gh.device != h.device)):
+        raise RuntimeError(f"{what}: gy, gh and h must have the same shape and device")
+    st = _prep(h, what)
+    R, C = h.shape
+    dev = h.device
+    weight = _norm_param(weight, C, dev, what)
+    if stats.dtype != torch.float32 or stats.shape != (2, R) or stats.device != dev:
+        raise RuntimeError(f"{what}: stats must be fp32 [2,R] on the same device")
+    stats = stats.contiguous()
+    for t in (gw_dtype, gb_dtype):
+        if t not in (None, torch.bfloat16, torch.float32):
+            raise RuntimeError(f"{what}: gw_dtype and gb_dtype must be bf16 or fp32")
+    numbers, site, threshold = _drop_args(drop, dev, what)
+    gx = torch.empty((R, C), dtype=torch.bfloat16, device=dev)
+    gres = torch.empty((R, C), dtype=torch.bfloat16, device=dev) if drop is not None else None
+    gw = torch.empty((C,), dtype=gw_dtype, device=dev) if gw_dtype is not None else None
+    gb = torch.empty((C,), dtype=gb_dtype, device=dev) if gb_dtype is not None else None
+    with _timed(what, R * C * (6 + (2 if gh is not None else 0) + (2 if gres is not None else 0)) + 8 * R, dev):
+        ws_bytes = _lib.load().l8_norm_bwd_workspace(R, C, centred) if gw is not None or gb is not None else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        code = _lib.load().l8_norm_bwd(_NORM_BWD.pack(
+            gy.data_ptr(), _addr(gh), h.data_ptr(), _addr(weight), weight is not None and weight.dtype == torch.float32, centred, R, C,
+            _ld(gy), _ld(gh) if gh is not None else 0, _ld(h), stats.data_ptr(), stats.data_ptr() + 4 * R, numbers or 0, site, threshold,
+            gx.data_ptr(), C, _addr(gres), C, _addr(gw), gw_dtype == torch.float32, _addr(gb), gb_dtype == torch.float32, _addr(ws),
+            ws_bytes, st or 0))
+    _lib.check(code, "l8_norm_bwd")
+    return gx, gres, gw, gb
+
+
 def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
            positions: Optional[torch.Tensor] = None, in_halves: bool = False, inverse: bool = False):
     """Rotary positions of xq [B,S,Hq,D] and xk [B,S,Hk,D] (bf16, either may be None) by the angles whose cosines and sines are

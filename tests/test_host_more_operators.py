@@ -1,0 +1,91 @@
+"""What the host refuses of layer norm, dropout, rotary positions on several axes and low-rank adapters before anything is enqueued: no GPU
+needed."""
+import struct
+
+import pytest
+import torch
+
+from lingua_amd import _lib
+
+P = 1 << 20      # an address that is aligned and never touched
+
+
+def refused(name, *args):
+    lib = _lib.load()
+    return getattr(lib, name)(*args) == -1 and name.encode() in lib.l8_last_error()
+
+
+FWD = dict(x=P, residual=P, w=P, b=P, w_f32=0, b_f32=0, centred=1, R=4, C=64, ldx=64, ldr=64, eps=1e-5, numbers=P, site=0, threshold=100, h=P, ldh=64, y=P, ldy=64, q=P, ldq=64,
+           scale=P, mean=P, rstd=P, col=0, ws=0, ws_bytes=0, stream=0)
+
+
+@pytest.mark.parametrize("change", [dict(R=-1), dict(C=-8), dict(x=0), dict(y=0), dict(h=0), dict(C=60, ldx=64), dict(C=8200, ldx=8200, ldr=8200, ldh=8200, ldy=8200, ldq=8200), dict(ldx=60),
+                                    dict(ldx=56), dict(x=P + 8), dict(residual=P + 8), dict(residual=0), dict(ldr=60), dict(h=P + 2), dict(ldh=32), dict(y=P + 8), dict(ldy=4), dict(q=0),
+                                    dict(scale=0), dict(q=P + 4), dict(ldq=60), dict(w=P + 1), dict(w=P + 2, w_f32=1), dict(b=P + 2, b_f32=1), dict(col=P), dict(col=P, ws=P, ws_bytes=8),
+                                    dict(col=P, q=0, scale=0), dict(site=-1), dict(site=1 << 32), dict(threshold=-1), dict(threshold=65537), dict(numbers=P + 4), dict(centred=0),
+                                    dict(centred=0, b=0, numbers=0), dict(centred=0, b=0, w=0)])
+def test_norm_is_refused(change):
+    assert refused("l8_norm_fwd", struct.pack("11qd16q", *{**FWD, **change}.values()))
+
+
+BWD = dict(gy=P, gh=P, h=P, w=P, w_f32=0, centred=1, R=4, C=64, ldgy=64, ldgh=64, ldh=64, mean=P, rstd=P, numbers=P, site=0, threshold=100, gx=P, ldgx=64, gres=P, ldgres=64, gw=P, gw_f32=1,
+           gb=P, gb_f32=1, ws=P, ws_bytes=1 << 20, stream=0)
+
+
+@pytest.mark.parametrize("change", [dict(R=-1), dict(C=-8), dict(gy=0), dict(h=0), dict(gx=0), dict(rstd=0), dict(mean=0), dict(C=60), dict(C=8200, ldgy=8200, ldgh=8200, ldh=8200, ldgx=8200,
+                                                                                                                                 ldgres=8200), dict(ldgy=60),
+                                    dict(gh=P + 8), dict(ldgh=56), dict(ldh=60), dict(ldgx=4), dict(gres=0), dict(numbers=0), dict(ldgres=60), dict(gres=P + 8), dict(w=P + 1), dict(ws=0),
+                                    dict(ws_bytes=16), dict(ws=P + 8), dict(centred=0), dict(centred=0, gb=0, w=0), dict(threshold=70000)])
+def test_norm_backward_is_refused(change):
+    assert refused("l8_norm_bwd", struct.pack("27q", *{**BWD, **change}.values()))
+
+
+DROP = dict(x=P, residual=P, y=P, n=64, numbers=P, site=0, threshold=1, stream=0)
+
+
+@pytest.mark.parametrize("change", [dict(n=-1), dict(x=None), dict(y=None), dict(numbers=None), dict(x=P + 1), dict(residual=P + 1), dict(site=-1), dict(site=1 << 32), dict(threshold=65537),
+                                    dict(numbers=P + 4), dict(n=1 << 35)])
+def test_dropout_is_refused(change):
+    assert refused("l8_dropout", *{**DROP, **change}.values())
+
+
+def test_empty_calls_do_nothing():
+    lib = _lib.load()
+    assert lib.l8_dropout(None, None, None, 0, None, 0, 0, None) == 0
+    assert lib.l8_norm_fwd(struct.pack("11qd16q", *{**FWD, "R": 0, "x": 0}.values())) == 0
+    assert lib.l8_norm_bwd(struct.pack("27q", *{**BWD, "C": 0, "gy": 0}.values())) == 0
+    assert lib.l8_norm_bwd(struct.pack("27q", *{**BWD, "R": 0, "gw": 0, "gb": 0}.values())) == 0
+    assert lib.l8_norm_bwd_workspace(0, 64, 1) == 0 and lib.l8_norm_bwd_workspace(5, 0, 1) == 0
+
+
+def test_arguments_are_refused():
+    """Before anything asks for a GPU."""
+    from lingua_amd import dropout, norm
+    x, n = torch.zeros(4, 64, dtype=torch.bfloat16), dropout.numbers(1, "cpu")
+    Drop = dropout.Drop
+    for bad in (Drop(-0.1, n), Drop(1.1, n), Drop(float("nan"), n), Drop(0.1, n, -1), Drop(0.1, n, 1 << 32), Drop(0.1, n[:1]), Drop(0.1, n.int()), Drop(0.1, n.repeat(2)[::2]),
+                Drop(0.1, torch.zeros(2, dtype=torch.int64, device="meta"))):
+        for call in (lambda: dropout.dropout(x, bad), lambda: dropout.dropout_add(x, x, bad), lambda: norm.add_layernorm(x, x, dropout=bad),
+                     lambda: norm.add_rmsnorm(x, x, x[0], 1e-5, bad)):
+            with pytest.raises(RuntimeError, match="dropped|32 bits|int64"):
+                call()
+    for call in (lambda: norm.layernorm(x.float()), lambda: norm.layernorm(x[0]), lambda: norm.add_layernorm(x, x[:2]), lambda: norm.add_layernorm(x, x.float()),
+                 lambda: dropout.dropout(x.float(), Drop(0.1, n)), lambda: dropout.dropout_add(x, x[:2], Drop(0.1, n))):
+        with pytest.raises(RuntimeError, match="bf16|same shape|leading dimension"):
+            call()
+
+
+def test_no_cpu_path():
+    from lingua_amd import dropout, norm
+    x, n = torch.zeros(4, 64, dtype=torch.bfloat16), dropout.numbers(1, "cpu")
+    drop = dropout.Drop(0.1, n)
+    for call in (lambda: norm.layernorm(x), lambda: norm.add_layernorm(x, x), lambda: norm.add_layernorm(x, x, dropout=drop), lambda: norm.add_rmsnorm(x, x, x[0], 1e-5, drop),
+                 lambda: dropout.dropout(x, drop), lambda: dropout.dropout_add(x, x, drop), lambda: norm.Fp8LayerNorm(64)(x), lambda: dropout.Dropout(0.1, n)(x)):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
+
+
+def test_seed_is_any_64_bits():
+    from lingua_amd import dropout
+    for seed in (0, 1, -1, 2 ** 63, 2 ** 64 - 1, 2 ** 64 + 5):
+        assert int(dropout.numbers(seed, "cpu")[0]) % 2 ** 64 == seed % 2 ** 64
