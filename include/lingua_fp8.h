@@ -417,6 +417,16 @@ int l8_rotary(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, int
               const float *cos, const float *sin, int64_t table_row, int64_t table_col, int64_t length,
               const void *positions, int positions_i32, int64_t pos_b, int64_t pos_s, void *stream);
 
+/* The same with tokens that stand at a place of several axes (time, height, width): rot / 2 = the sum of sections[0 .. axes - 1], the pairs
+ * that each axis turns; pair i of axis a turns by the angle of row positions[a,b,s], column i of the tables.
+ *   axes        1 to 4
+ *   in_rounds   the pairs go to the axes one after the other in turn, an axis that has its share being passed over; else an axis's pairs lie
+ *               side by side, in the order of the axes
+ *   positions   element (a,b,s) at a * pos_axis + b * pos_b + s * pos_s; a token of which any position lies outside [0, length) becomes NaN */
+int l8_rotary_axes(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D, const int64_t *sections, int64_t axes, int in_rounds,
+                   int in_halves, int inverse, const float *cos, const float *sin, int64_t table_row, int64_t table_col, int64_t length,
+                   const void *positions, int positions_i32, int64_t pos_axis, int64_t pos_b, int64_t pos_s, void *stream);
+
 /* MXFP4 (OCP Microscaling formats 1.0): e2m1 codes in blocks of 32, the last block of a row possibly shorter, with an e8m0 scale each.
  *   byte = max(E - 2, 0), E the biased exponent of the block's amax; 255 (NaN), with codes 0, for a block with an inf or NaN
  *   code = e2m1(x * 2^(127 - byte)), nearest even, saturating at 6

@@ -68,6 +68,7 @@ SIGNATURES = {
     "l8_norm_bwd": [ctypes.c_char_p],
     "l8_norm_bwd_workspace": [_i64, _i64, _i64],
     "l8_rotary": [_p, _i64, _i64, _i64, _i64, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _p],
+    "l8_rotary_axes": [_p, _i64, _i64, _i64, _p, _i64, _int, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _i64, _p],
     "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
     "l8_cast_mxfp4_two": [_p, _p],
     "l8_mxfp4_to_bf16": [_p, _i64, _p, _i64, _i64, _i64, _p, _i64, _p],

@@ -966,12 +966,14 @@ def layernorm_bwd(gy: torch.Tensor, gh: Optional[torch.Tensor], h: torch.Tensor,
 
 
 def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
-           positions: Optional[torch.Tensor] = None, in_halves: bool = False, inverse: bool = False):
+           positions: Optional[torch.Tensor] = None, in_halves: bool = False, inverse: bool = False, sections=None, in_rounds: bool = False):
     """Rotary positions of xq [B,S,Hq,D] and xk [B,S,Hk,D] (bf16, either may be None) by the angles whose cosines and sines are
     cos, sin (fp32 [P, rot / 2]); positions int32 or int64, broadcastable to [B,S] (None: 0 .. S - 1).  ``inverse``: the transposed
-    rotation.  Returns dense tensors of the same shapes.  A token at a position outside [0, P) becomes NaN."""
-    what = "rotary"
-    if kernel_timer is None and cos.is_cuda:   # the same in one call, for operands that need no copies
+    rotation.  Returns dense tensors of the same shapes.  A token at a position outside [0, P) becomes NaN.
+    ``sections`` (pairs per axis, up to four axes): positions broadcastable to [axes,B,S], each axis turning its pairs, side by side or
+    ``in_rounds``."""
+    what = "rotary" if sections is None else "rotary_axes"
+    if kernel_timer is None and cos.is_cuda and sections is None:   # the same in one call, for operands that need no copies
         res = _lib.native_for(cos.get_device()).rotary(xq, xk, cos, sin, positions, in_halves, inverse)
         if res is not None:
             return res
@@ -994,15 +996,23 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
     P, rot = cos.shape[0], 2 * cos.shape[1]
     if rot < 2 or rot > D:
         raise RuntimeError(f"{what}: tables for {rot} columns do not fit heads of {D}")
-    pos_ptr, pos_i32, pos_b, pos_s = None, 0, 0, 0
+    shape = (B, S)
+    if sections is not None:
+        if not 1 <= len(sections) <= 4 or any(n < 0 for n in sections) or 2 * sum(sections) != rot:
+            raise RuntimeError(f"{what}: the pairs of one to four axes must be the tables' {rot // 2}, got {tuple(sections)}")
+        if positions is None:
+            raise RuntimeError(f"{what}: positions are needed")
+        shape = (len(sections), B, S)
+    pos_ptr, pos_i32, pos_b, pos_s, pos_axis = None, 0, 0, 0, 0
     if positions is not None:
         if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
             raise RuntimeError(f"{what}: positions must be int32 or int64 on the inputs' device")
         try:
-            positions = positions.expand(B, S)
+            positions = positions.expand(shape)
         except RuntimeError:
-            raise RuntimeError(f"{what}: positions {tuple(positions.shape)} do not broadcast to [{B}, {S}]") from None
-        pos_ptr, pos_i32, (pos_b, pos_s) = positions.data_ptr(), int(positions.dtype == torch.int32), positions.stride()
+            raise RuntimeError(f"{what}: positions {tuple(positions.shape)} do not broadcast to {list(shape)}") from None
+        pos_ptr, pos_i32, (pos_b, pos_s) = positions.data_ptr(), int(positions.dtype == torch.int32), positions.stride()[-2:]
+        pos_axis = positions.stride(0)
     elif S > P:
         raise RuntimeError(f"{what}: {S} tokens, the tables hold {P} positions")
     outs, items, keep = [], [], []
@@ -1018,10 +1028,15 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
         keep.append(t)
         outs.append(y)
         items += [t.data_ptr(), y.data_ptr(), t.shape[2], t.stride(0), t.stride(1), t.stride(2)]
-    with _timed("rotary", sum(4 * t.numel() for t in xs) + 4 * B * S * rot, dev):
-        code = _lib.load().l8_rotary(struct.pack("12q", *items), B, S, D, rot, int(in_halves), int(inverse), cos.data_ptr(), sin.data_ptr(),
-                                     cos.stride(0), cos.stride(1), P, pos_ptr, pos_i32, pos_b, pos_s, st)
-    _lib.check(code, "l8_rotary")
+    with _timed(what, sum(4 * t.numel() for t in xs) + 4 * B * S * rot, dev):
+        head, tables = (struct.pack("12q", *items), B, S, D), (cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.stride(1), P, pos_ptr, pos_i32)
+        if sections is None:
+            code = _lib.load().l8_rotary(*head, rot, int(in_halves), int(inverse), *tables, pos_b, pos_s, st)
+        else:
+            n = len(sections)
+            code = _lib.load().l8_rotary_axes(*head, struct.pack(f"{n}q", *sections), n, int(in_rounds), int(in_halves), int(inverse), *tables,
+                                              pos_axis, pos_b, pos_s, st)
+    _lib.check(code, f"l8_{what}")
     return tuple(outs)
 
 

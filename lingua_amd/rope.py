@@ -4,9 +4,11 @@
 is the general form: either layout of pairs, a part of the head, tokens at positions given as a tensor, tables from ``rotary_tables``
 for contexts longer than the trained one.  Forward and backward are one kernel launch each (``l8_rotary``) for queries and keys
 together; q and k may be column slices of one product (``lingua_amd.qkv.fuse_qkv``), nothing is copied on the way in.
+
+``rotary_axes`` is the form for images and video: a token stands at a place of up to four axes, and each axis turns its share of the pairs.
 """
 import math
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -14,15 +16,16 @@ from . import _lib, ops
 from . import float8 as f8
 
 LAYOUTS = ("interleaved", "half")
+ORDERS = ("sections", "rounds")
 
 
 class RotaryFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, xq, xk, cos, sin, positions, in_halves):
+    def forward(ctx, xq, xk, cos, sin, positions, in_halves, sections=None, in_rounds=False):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(cos, sin, positions)
-        ctx.in_halves = in_halves
-        return ops.rotary(xq, xk, cos, sin, positions, in_halves)
+        ctx.in_halves, ctx.axes = in_halves, {} if sections is None else {"sections": sections, "in_rounds": in_rounds}
+        return ops.rotary(xq, xk, cos, sin, positions, in_halves, **ctx.axes)
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -35,8 +38,8 @@ class RotaryFn(torch.autograd.Function):
         if gq is not None or gk is not None:
             cos, sin, positions = ctx.saved_tensors
             with torch.no_grad():
-                gq, gk = ops.rotary(gq, gk, cos, sin, positions, ctx.in_halves, inverse=True)
-        return (*f8._once("rotary", (gq, gk), varies), None, None, None, None)
+                gq, gk = ops.rotary(gq, gk, cos, sin, positions, ctx.in_halves, inverse=True, **ctx.axes)
+        return (*f8._once("rotary", (gq, gk), varies), None, None, None, None, None, None)
 
 
 def rotary(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -57,6 +60,26 @@ def rotary(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Ten
             return res
     f8._refuse_captured(xq, xk, None, "rotary")
     return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half")
+
+
+def rotary_axes(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, sections: Sequence[int],
+                order: str = "sections", layout: str = "interleaved"):
+    """``(xq, xk)`` [B,S,H,D] bf16 with pairs of columns turned by the positions of their tokens on several axes: pair i, of axis a, by the
+    angle of row ``positions[a,b,s]``, column i of the tables; the columns behind the last pair are copied.
+
+    ``cos``, ``sin``  fp32 [P, pairs]: ``rotary_tables`` (one run of frequencies over all pairs) or ``axes_tables`` (one for each axis)
+    ``positions``     int32 or int64, broadcastable to [axes,B,S].  A token of which any position is outside [0, P) becomes NaN.
+    ``sections``      pairs that each of up to four axes turns, their sum cos.shape[1]
+    ``order``         "sections": an axis's pairs side by side, the axes in their order; "rounds": a pair to each axis in turn, an axis that
+                      has its share being passed over
+    ``layout``        as in ``rotary``
+    """
+    if layout not in LAYOUTS:
+        raise RuntimeError(f"rotary_axes: unknown layout {layout!r}, one of {LAYOUTS}")
+    if order not in ORDERS:
+        raise RuntimeError(f"rotary_axes: unknown order {order!r}, one of {ORDERS}")
+    f8._refuse_captured(xq, xk, None, "rotary_axes")
+    return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half", tuple(sections), order == "rounds")
 
 
 def apply_rotary_emb(xq: torch.Tensor, xk: torch.Tensor, seq_dim: int, freqs_cis: torch.Tensor):
@@ -112,3 +135,26 @@ def rotary_tables(rot: int, length: int, theta: float = 10000.0, scaling: Option
         size = 0.1 * math.log(factor) + 1.0
     angle = torch.arange(length, device=device, dtype=torch.float64)[:, None] * freq
     return (angle.cos() * size).float(), (angle.sin() * size).float()
+
+
+def pair_axes(sections: Sequence[int], order: str = "sections"):
+    """The axis that each pair of ``rotary_axes`` turns by: a list of sum(sections) numbers."""
+    left = list(sections)
+    if order not in ORDERS or any(n < 0 for n in left):
+        raise RuntimeError(f"pair_axes: shares of pairs and an order of {ORDERS} are wanted, got {left} and {order!r}")
+    if order == "sections":
+        return [a for a, n in enumerate(left) for _ in range(n)]
+    return [a for turn in range(max(left, default=0)) for a, n in enumerate(left) if turn < n]
+
+
+def axes_tables(sections: Sequence[int], length: int, theta: float = 10000.0, order: str = "sections", device=None):
+    """``(cos, sin)`` fp32 [length, sum(sections)] for ``rotary_axes`` with a run of frequencies for each axis, as models of images have
+    them: the j-th of an axis's n pairs turns by p * theta^(-j / n)."""
+    if length < 0:
+        raise RuntimeError(f"axes_tables: a length is wanted, got {length}")
+    cos, sin = (torch.empty((length, sum(sections)), dtype=torch.float32, device=device) for _ in range(2))
+    of = torch.tensor(pair_axes(sections, order), device=device)
+    for a, n in enumerate(sections):
+        if n:
+            cos[:, of == a], sin[:, of == a] = rotary_tables(2 * n, length, theta, device=device)
+    return cos, sin

@@ -49,6 +49,21 @@ def test_dropout_is_refused(change):
     assert refused("l8_dropout", *{**DROP, **change}.values())
 
 
+ROTARY = dict(B=2, S=3, D=64, sections=(16, 8, 8), axes=3, rounds=0, half=0, inverse=0, cos=P, sin=P, row=32, col=1, length=8, pos=P, i32=0, pos_a=6, pos_b=3, pos_s=1, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(B=-1), dict(D=63), dict(D=514), dict(axes=0), dict(axes=5, sections=(4, 4, 4, 4, 4)), dict(sections=(0, 0, 0)), dict(sections=(16, -8, 8)),
+                                    dict(sections=(16, 8, 9)), dict(sections=(1 << 60, 1 << 60, 1 << 60)), dict(sections=(256, 1, 0), D=512), dict(cos=None), dict(sin=P + 2), dict(pos=None),
+                                    dict(pos=P + 4), dict(pos=P + 2, i32=1), dict(length=-1), dict(B=1 << 12, S=1 << 12), dict(x=None), dict(y=P + 1), dict(heads=-1)])
+def test_rotary_axes_is_refused(change):
+    own = {k: change.pop(k) for k in ("x", "y", "heads") if k in change}
+    fields = dict(x=P, y=P, heads=4, ldb=768, lds=256, ldh=64) | own
+    args = {**ROTARY, **change}
+    args["sections"] = struct.pack(f"{len(args['sections'])}q", *args["sections"])
+    two = struct.pack("12q", *[v or 0 for v in fields.values()], P, P, 1, 768, 256, 64)
+    assert refused("l8_rotary_axes", two, *args.values())
+
+
 def test_empty_calls_do_nothing():
     lib = _lib.load()
     assert lib.l8_dropout(None, None, None, 0, None, 0, 0, None) == 0
@@ -75,12 +90,26 @@ def test_arguments_are_refused():
             call()
 
 
+def test_rotary_axes_arguments_are_refused():
+    from lingua_amd import rope
+    q, cos, pos = torch.zeros(1, 2, 4, 16, dtype=torch.bfloat16), torch.zeros(4, 8), torch.zeros(3, 1, 2, dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="layout"):
+        rope.rotary_axes(q, q, cos, cos, pos, (4, 2, 2), layout="whole")
+    with pytest.raises(RuntimeError, match="order"):
+        rope.rotary_axes(q, q, cos, cos, pos, (4, 2, 2), order="turns")
+    with pytest.raises(RuntimeError, match="order|shares"):
+        rope.pair_axes((4, -1))
+    with pytest.raises(RuntimeError, match="length"):
+        rope.axes_tables((4, 4), -1)
+
+
 def test_no_cpu_path():
-    from lingua_amd import dropout, norm
+    from lingua_amd import dropout, norm, rope
     x, n = torch.zeros(4, 64, dtype=torch.bfloat16), dropout.numbers(1, "cpu")
     drop = dropout.Drop(0.1, n)
     for call in (lambda: norm.layernorm(x), lambda: norm.add_layernorm(x, x), lambda: norm.add_layernorm(x, x, dropout=drop), lambda: norm.add_rmsnorm(x, x, x[0], 1e-5, drop),
-                 lambda: dropout.dropout(x, drop), lambda: dropout.dropout_add(x, x, drop), lambda: norm.Fp8LayerNorm(64)(x), lambda: dropout.Dropout(0.1, n)(x)):
+                 lambda: dropout.dropout(x, drop), lambda: dropout.dropout_add(x, x, drop), lambda: norm.Fp8LayerNorm(64)(x), lambda: dropout.Dropout(0.1, n)(x),
+                 lambda: rope.rotary_axes(x.view(1, 4, 1, 64), x.view(1, 4, 1, 64), torch.zeros(4, 32), torch.zeros(4, 32), torch.zeros(2, 1, 4).long(), (16, 16))):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
 
