@@ -427,6 +427,35 @@ int l8_rotary_axes(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D
                    int in_halves, int inverse, const float *cos, const float *sin, int64_t table_row, int64_t table_col, int64_t length,
                    const void *positions, int positions_i32, int64_t pos_axis, int64_t pos_b, int64_t pos_s, void *stream);
 
+/* Low-rank adapters of many requests beside a projection: out_t = y_t + scale_i (x_t A_i^T) B_i, i = index[t], A bf16 [n,r,K], B bf16 [n,r,N].
+ * r a multiple of 8 up to 128, K and N multiples of 8 below 2^24, n up to 2^16, T below 2^24 tokens; rows of tokens and factors on 16-byte
+ * lines; h fp32 [splits,T,r], 16-byte aligned, of which rows of tokens without an adapter are neither written nor read.
+ *
+ * route: tokens by adapter.  index int32 or (index_is_i64) int64 [T]: 0 .. n - 1, -1: none; any other: the token's results are NaN.
+ * order int32 [T], starts int32 [n+3]: adapter i's tokens are order[starts[i] .. starts[i+1]), in their order; then those with none, then the
+ * others. */
+int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, int64_t n, int *order, int *starts, void *stream);
+/* h = x F_i^T, F = A (forward) or, with x the output's gradient, B (backward), without the scale; in `splits` parts (l8_lowrank_splits says how
+ * many pay). */
+int l8_lowrank_shrink(const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const int *order, const int *starts,
+                      float *h, int64_t splits, void *stream);
+int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K);
+/* out = y + scale_i h F_i, bf16 [T,N]; y NULL: zeros, scale NULL: ones.  Tokens without an adapter: out = y.  out may be y. */
+int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
+                      int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream);
+/* grad_i = scale_i sum over the tokens of i of h_t (x) z_t, bf16 [n,r,D], for two sides in one launch (grad NULL: not that one): that of A with h
+ * of the gradient and z = x, that of B with h of the forward and z the gradient.  Sums in a fixed order. */
+typedef struct {
+  const float *h;
+  int64_t splits;
+  const void *z;
+  int64_t ldz, D;
+  void *grad;
+} l8_lowrank_side;
+int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, int64_t T, int64_t n, int64_t r, const int *order, const int *starts,
+                     void *workspace, int64_t workspace_bytes, void *stream);
+int64_t l8_lowrank_outer_workspace(int64_t T, int64_t r, int64_t K, int64_t N);
+
 /* MXFP4 (OCP Microscaling formats 1.0): e2m1 codes in blocks of 32, the last block of a row possibly shorter, with an e8m0 scale each.
  *   byte = max(E - 2, 0), E the biased exponent of the block's amax; 255 (NaN), with codes 0, for a block with an inf or NaN
  *   code = e2m1(x * 2^(127 - byte)), nearest even, saturating at 6

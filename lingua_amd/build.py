@@ -16,7 +16,7 @@ CSRC = os.path.join(_HERE, "csrc")
 # same variable); LINGUA_FP8_HIPCC_EXTRA: more hipcc flags for such a variant, e.g. "-DL8_STRADDLE=3 -DL8_READ_GROUPS1=20".
 LIB_PATH = os.environ.get("LINGUA_FP8_LIB") or os.path.join(_HERE, "liblingua_fp8.so")
 SOURCES = ["api.cpp", "linear.cpp", "cast_kernels.hip", "gemm_kernels.hip", "swiglu_kernels.hip", "norm_kernels.hip", "layernorm_kernels.hip", "dropout_kernels.hip",
-           "skinny_kernels.hip", "rope_kernels.hip", "mxfp4_kernels.hip", "mxfp4_gemm_kernels.hip", "mxfp4_skinny_kernels.hip"]
+           "skinny_kernels.hip", "rope_kernels.hip", "lowrank_kernels.hip", "mxfp4_kernels.hip", "mxfp4_gemm_kernels.hip", "mxfp4_skinny_kernels.hip"]
 
 OBJ_DIR = os.path.join(_HERE, "build")     # object files (ignored by git)
 

@@ -1,0 +1,657 @@
+// Low-rank adapters of many requests at once, beside a projection that they share: token t of adapter i gets
+//
+//   out_t = y_t + s_i (x_t A_i^T) B_i            A [n, r, K], B [n, r, N] bf16, i = index[t]
+//
+// and the backward pass
+//
+//   gh_t = s_i gy_t B_i^T,  gx_t = gh_t A_i,  gA_i = sum over its tokens of gh_t (x) x_t,  gB_i = sum of s_i h_t (x) gy_t.
+//
+// Both factors lie with the rank in front, so that three kernels serve both passes: `shrink` (rows times a factor along its long side),
+// `expand` (h times a factor across it, added to y or not) and `outer` (the factors' gradients).  All of it is bound by memory: r is
+// far below the 300 flop per byte at which the matrix cores would be, so tokens' rows go from memory to the matrix instruction's
+// registers as they lie, in whole lines, and factors, of which there are few, come from the L2.
+//
+// Tokens are grouped by adapter first (`route`: a stable order, so every sum has one order), and a workgroup's tile holds tokens of one
+// adapter: tile s of B tokens belongs to the group g with the largest starts[g] / B + g <= s, since a group of c tokens that begins at
+// starts[g] takes at most ceil(c / B) of the starts[g + 1] / B + g + 1 - (starts[g] / B + g) numbers between its own first and the next
+// one's.  That leaves at most one number a group unused and needs no table of tiles.  Groups n and n + 1 are the tokens without an adapter
+// (out = y) and those whose index is no adapter's (out = NaN: the index is on the GPU, where nothing can be refused).
+//
+// h is held in 32 bits, [splits, T, r]: K is shared out over `splits` workgroups where there are few tokens, and whoever reads h adds the
+// parts up in order.  Where h is an operand of a matrix instruction it goes in as two bf16 numbers, hi + lo, 16 bits of it: the second
+// product costs nothing beside memory (with r <= 16 the two halves even share one instruction), and the result is rounded once, at the end.
+// (An infinity on the other side of such a product makes infinity or NaN: hi and lo may have different signs.)
+#include "l8_common.h"
+
+#include <algorithm>
+
+namespace l8 {
+
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+
+L8_DEV v4f mfma(v4i a, v4i b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0); }
+
+// ---- tokens by adapter ----
+
+constexpr int kRouteBlock = 1024;
+
+// A workgroup per group: how many tokens stand in front of its own, then its own tokens in their order.
+template <typename Index>
+__global__ __launch_bounds__(kRouteBlock) void lowrank_route_kernel(const Index *__restrict__ index, int T, int n, int *__restrict__ order, int *__restrict__ starts) {
+  constexpr int WAVES = kRouteBlock / 64;
+  __shared__ int sums[WAVES], base[WAVES];
+  const int mine = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  auto group_of = [&](int t) {
+    const int64_t i = (int64_t)index[t];
+    return i >= 0 && i < n ? (int)i : i == -1 ? n : n + 1;
+  };
+  int less = 0;
+  for (int t = threadIdx.x; t < T; t += kRouteBlock) less += group_of(t) < mine;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) less += __shfl_xor(less, d);
+  if (lane == 0) sums[wave] = less;
+  __syncthreads();
+  int at = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) at += sums[w];
+  if (threadIdx.x == 0) {
+    starts[mine] = at;
+    if (mine == n + 1) starts[n + 2] = T;
+  }
+  for (int t0 = 0; t0 < T; t0 += kRouteBlock) {
+    const int t = t0 + threadIdx.x;
+    const bool own = t < T && group_of(t) == mine;
+    const uint64_t votes = __ballot(own);
+    if (lane == 0) base[wave] = __popcll(votes);
+    __syncthreads();
+    int before = at, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      if (w < wave) before += base[w];
+      all += base[w];
+    }
+    if (own) order[before + __popcll(votes & ((1ull << lane) - 1))] = t;
+    at += all;
+    __syncthreads();
+  }
+}
+
+struct Tile {
+  int group, first, count;   // tokens order[first .. first + count); count 0: a number that no tile has
+  int piece, tokens;         // which of its group's tiles, and the group's tokens
+};
+// Tile `slot` of at most `size` tokens.  The same for the whole workgroup.
+L8_DEV Tile tile_of(const int *__restrict__ starts, int n, int size, int slot) {
+  const int lane = threadIdx.x & 63;
+  int g = -1;
+  for (int i0 = 0; i0 < n + 2; i0 += 64) {   // the groups whose first number is at most `slot` come first
+    const int i = i0 + lane;
+    const int have = __popcll(__ballot(i < n + 2 && starts[i < n + 2 ? i : 0] / size + i <= slot));
+    g += have;
+    if (have < 64) break;
+  }
+  g = __builtin_amdgcn_readfirstlane(g);
+  Tile t;
+  t.group = g;
+  const int from = starts[g], to = starts[g + 1];
+  t.piece = slot - (from / size + g);
+  t.tokens = to - from;
+  t.first = from + t.piece * size;
+  t.count = min(size, max(0, to - t.first));
+  return t;
+}
+
+// ---- rows times a factor along its long side ----
+
+struct ShrinkArgs {
+  const uint16_t *x, *f;
+  const int *order, *starts;
+  float *h;
+  int64_t ldx;
+  int T, K, n, r, splits;
+};
+
+// MT tiles of 16 tokens by RT of 16 ranks, the W waves share K.  A wave takes 64 columns a step, the waves side by side: lane group g
+// (of 16 lanes) takes columns 16 g .. 16 g + 15 of a step, the first eight into one matrix instruction and the others into a second, so
+// that a row is read in whole lines.  Which column meets which place of the instruction does not matter as long as it is the same for
+// both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
+template <int MT, int RT, int W>
+__global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs p) {
+  __shared__ float red[W / 2][MT * RT * 256];
+  const Tile tile = tile_of(p.starts, p.n, MT * 16, blockIdx.x);
+  if (tile.group >= p.n || tile.count == 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int K = p.K, steps = (K + 63) / 64, rank0 = blockIdx.z * RT * 16;
+  const int lo = (int)((int64_t)steps * blockIdx.y / p.splits), hi = (int)((int64_t)steps * (blockIdx.y + 1) / p.splits);
+  const uint16_t *xr[MT], *fr[RT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xr[m] = p.x + (int64_t)p.order[tile.first + min(m * 16 + row, tile.count - 1)] * p.ldx;
+#pragma unroll
+  for (int j = 0; j < RT; ++j) fr[j] = p.f + ((int64_t)tile.group * p.r + min(rank0 + j * 16 + row, p.r - 1)) * K;
+  v4f acc[MT][RT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int j = 0; j < RT; ++j) acc[m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  v4i a[2][MT][2], b[2][RT][2];
+  auto request = [&](int s, int step) {
+    // the last step may pass the row's end: columns beyond it are read from within the row and zeroed before they are used
+    const int k0 = step * 64 + g * 16, k1 = min(k0, K - 8), k2 = min(k0 + 8, K - 8);
+#pragma unroll
+    for (int m = 0; m < MT; ++m) a[s][m][0] = *(const v4i *)(xr[m] + k1), a[s][m][1] = *(const v4i *)(xr[m] + k2);
+#pragma unroll
+    for (int j = 0; j < RT; ++j) b[s][j][0] = *(const v4i *)(fr[j] + k1), b[s][j][1] = *(const v4i *)(fr[j] + k2);
+  };
+  auto multiply = [&](int s, int step) {
+    if (step * 64 + 64 > K) {
+      const int k0 = step * 64 + g * 16;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        if (k0 + 8 * c >= K) {
+#pragma unroll
+          for (int m = 0; m < MT; ++m) a[s][m][c] = v4i{0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < RT; ++j) b[s][j][c] = v4i{0, 0, 0, 0};
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[m][j] = mfma(a[s][m][c], b[s][j][c], acc[m][j]);
+  };
+  int step = lo + wave;
+  if (step < hi) request(0, step);
+  while (step < hi) {
+    request(1, min(step + W, hi - 1));
+    multiply(0, step);
+    step += W;
+    if (step >= hi) break;
+    request(0, min(step + W, hi - 1));
+    multiply(1, step);
+    step += W;
+  }
+  // the upper half of the waves hands its sums to the lower half, until one has them all
+#pragma unroll
+  for (int half = W / 2; half; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) *(v4f *)&red[wave - half][(m * RT + j) * 256 + lane * 4] = acc[m][j];
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+          const v4f other = *(const v4f *)&red[wave][(m * RT + j) * 256 + lane * 4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[m][j][i] += other[i];
+        }
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+  // a lane has rank `row` of each sixteen, tokens 4 g .. 4 g + 3
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = m * 16 + g * 4 + i;
+      if (at >= tile.count) continue;
+      float *out = p.h + ((int64_t)blockIdx.y * p.T + p.order[tile.first + at]) * p.r;
+#pragma unroll
+      for (int j = 0; j < RT; ++j)
+        if (rank0 + j * 16 + row < p.r) out[rank0 + j * 16 + row] = acc[m][j][i];
+    }
+}
+
+// ---- h times a factor across its long side ----
+
+// Eight values of h, `splits` parts added up in order, times the adapter's scale.
+L8_DEV void load_h(float (&v)[8], const float *__restrict__ h, int64_t part, int splits, float scale) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+  for (int s = 0; s < splits; ++s) {
+    const v4f u = *(const v4f *)(h + s * part), w = *(const v4f *)(h + s * part + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += u[e], v[e + 4] += w[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] *= scale;
+}
+// hi + lo = v to 16 bits, both bf16; a v that is not finite is hi alone.
+L8_DEV uint32_t hi_bits(float v) { return bf16_rne_bits(v); }
+L8_DEV uint32_t lo_bits(float v) {
+  const uint32_t hi = bf16_rne_bits(v);
+  return (hi & 0x7f80u) == 0x7f80u ? 0u : bf16_rne_bits(v - bf16_bits_to_f32(hi));
+}
+L8_DEV v4i pack8(const float (&v)[8], bool low) {
+  v4i out;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t a = low ? lo_bits(v[2 * k]) : hi_bits(v[2 * k]), b = low ? lo_bits(v[2 * k + 1]) : hi_bits(v[2 * k + 1]);
+    out[k] = (int)(a | (b << 16));
+  }
+  return out;
+}
+// Eight rows of eight columns -> for each column the eight rows' values, one v_perm per two values.
+L8_DEV void transpose8(v4i (&out)[8], const v4i (&rows)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      out[j][k] = (int)__builtin_amdgcn_perm((uint32_t)rows[2 * k + 1][j >> 1], (uint32_t)rows[2 * k][j >> 1], (j & 1) ? 0x07060302u : 0x05040100u);
+}
+
+struct ExpandArgs {
+  const uint16_t *y, *f;
+  const float *h, *scale;
+  const int *order, *starts;
+  uint16_t *out;
+  int64_t ldy, ldo;
+  int T, N, n, r, splits;
+};
+
+constexpr int kExpandWaves = 4;
+
+// MT tiles of 16 tokens by 128 columns a wave.  Column 8 c + j of a wave's 128 is column c of matrix instruction j: a lane then reads
+// eight neighbouring columns of eight rows of the factor, turns the block round in registers, and ends up with eight neighbouring
+// columns of four tokens: 16-byte loads and stores, 256 bytes of a row at once, and no LDS.
+// KS steps of 32 ranks, each with the upper and the lower bits of h; KS 0: up to 16 ranks, where one instruction takes both.
+template <int MT, int KS>
+__global__ __launch_bounds__(kExpandWaves * 64) void lowrank_expand_kernel(const ExpandArgs p) {
+  const Tile tile = tile_of(p.starts, p.n, MT * 16, blockIdx.x);
+  if (tile.count == 0) return;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int col = (blockIdx.y * kExpandWaves + wave) * 128 + row * 8;
+  const bool in = col < p.N;
+  if (tile.group >= p.n) {   // no adapter: y as it is; no known adapter: NaN
+#pragma unroll 1
+    for (int at = g; at < tile.count; at += 4) {
+      const int64_t t = p.order[tile.first + at];
+      v4i v = {0, 0, 0, 0};
+      if (p.y && in) v = *(const v4i *)(p.y + t * p.ldy + col);
+      if (tile.group > p.n) v = v4i{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
+      if (in) *(v4i *)(p.out + t * p.ldo + col) = v;
+    }
+    return;
+  }
+  constexpr int STEPS = KS ? KS : 1;
+  const int r = p.r;
+  v4i b[STEPS][8];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int k0 = KS ? s * 32 + g * 8 : (g & 1) * 8;
+    const uint16_t *f = p.f + ((int64_t)tile.group * r + min(k0, r - 8)) * p.N + (in ? col : 0);
+    v4i rows[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) rows[e] = *(const v4i *)(f + (int64_t)e * p.N);
+    transpose8(b[s], rows);
+    if (k0 >= r) {   // (ranks beyond r: h is zero there, and so is the factor, whatever the row that was read holds)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) b[s][j] = v4i{0, 0, 0, 0};
+    }
+  }
+  const float scale = p.scale ? p.scale[tile.group] : 1.0f;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m * 16 >= tile.count) break;
+    const int64_t mine = p.order[tile.first + min(m * 16 + row, tile.count - 1)];
+    int64_t t[4];
+    v4i y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = min(m * 16 + g * 4 + i, tile.count - 1);
+      t[i] = p.order[tile.first + at];
+      y[i] = v4i{0, 0, 0, 0};
+      if (p.y) y[i] = *(const v4i *)(p.y + t[i] * p.ldy + (in ? col : 0));
+    }
+    v4f acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      const int k0 = KS ? s * 32 + g * 8 : (g & 1) * 8;
+      float v[8];
+      load_h(v, p.h + mine * r + min(k0, r - 8), (int64_t)p.T * r, p.splits, scale);
+      if (k0 >= r) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      }
+      if constexpr (KS) {
+        const v4i hi = pack8(v, false), lo = pack8(v, true);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = mfma(hi, b[s][j], acc[j]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = mfma(lo, b[s][j], acc[j]);
+      } else {
+        const v4i both = g < 2 ? pack8(v, false) : pack8(v, true);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = mfma(both, b[s][j], acc[j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v4i out;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float lo = __uint_as_float((uint32_t)y[i][k] << 16) + acc[2 * k][i], hi = __uint_as_float((uint32_t)y[i][k] & 0xffff0000u) + acc[2 * k + 1][i];
+        out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
+      }
+      if (in && m * 16 + g * 4 + i < tile.count) *(v4i *)(p.out + t[i] * p.ldo + col) = out;
+    }
+  }
+}
+
+// ---- gradients of the factors ----
+
+struct OuterSide {           // grad_i [r, D] = sum over the tokens of i of h_t (x) z_t
+  const float *h;
+  const uint16_t *z;
+  uint16_t *grad;
+  float *partials;           // [2 (T / size + 1), r, D]: groups of more than one tile
+  int64_t ldz;
+  int D, splits, chunks;     // chunks of 512 columns
+};
+struct OuterArgs {
+  OuterSide side[2];
+  const float *scale;
+  const int *order, *starts;
+  int T, n, r, size;
+};
+
+constexpr int kOuterWaves = 4, kOuterTokens = 128, kOuterPitch = kOuterTokens + 8;
+
+// Where a tile of a group that has several leaves its sums: the first of a group and the others apart, since a group's last tile and the
+// next group's first may begin within one `size` tokens.
+L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)(first / size) + (piece > 0); }
+
+// RT tiles of 16 ranks by 128 columns a wave, over a tile's tokens.  z is read as `expand` reads the factor: eight neighbouring columns of
+// eight tokens' rows a lane, turned round in registers; h is laid out by rank in LDS, 128 tokens at a time, both halves of its bits.
+template <int RT>
+__global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const OuterArgs p) {
+  __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][kOuterPitch];
+  __shared__ __attribute__((aligned(16))) int toks[kOuterTokens];
+  const Tile tile = tile_of(p.starts, p.n, p.size, blockIdx.x);
+  if (tile.group >= p.n || (tile.count == 0 && tile.piece > 0)) return;
+  const int which = (int)blockIdx.y >= p.side[0].chunks;
+  const OuterSide &sd = p.side[which];
+  const int chunk = blockIdx.y - (which ? p.side[0].chunks : 0);
+  const int rank0 = blockIdx.z * RT * 16, r = p.r, D = sd.D;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int col = (chunk * kOuterWaves + wave) * 128 + row * 8;
+  const bool in = col < D;
+  const uint16_t *z = sd.z + (in ? col : 0);
+  const float scale = p.scale ? p.scale[tile.group] : 1.0f;
+  v4f acc[RT][8];
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int p0 = 0; p0 < tile.count; p0 += kOuterTokens) {
+    const int here = min(kOuterTokens, tile.count - p0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kOuterTokens; i += kOuterWaves * 64) toks[i] = p.order[tile.first + p0 + min(i, here - 1)];
+    for (int i = threadIdx.x; i < kOuterTokens * RT * 2; i += kOuterWaves * 64) {   // eight ranks of a token
+      const int at = i / (RT * 2), k = i % (RT * 2) * 8;
+      float v[8];
+      if (at < here && rank0 + k < r) {
+        load_h(v, sd.h + (int64_t)p.order[tile.first + p0 + at] * r + rank0 + k, (int64_t)p.T * r, sd.splits, scale);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) hs[0][k + e][at] = (uint16_t)hi_bits(v[e]), hs[1][k + e][at] = (uint16_t)lo_bits(v[e]);
+    }
+    __syncthreads();
+    v4i rows[2][8];
+    auto request = [&](int s, int sub) {
+      const v4i t0 = *(const v4i *)&toks[sub * 32 + g * 8], t1 = *(const v4i *)&toks[sub * 32 + g * 8 + 4];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rows[s][e] = *(const v4i *)(z + (int64_t)(e < 4 ? t0[e & 3] : t1[e & 3]) * sd.ldz);
+    };
+    const int subs = (here + 31) / 32;
+    request(0, 0);
+#pragma unroll
+    for (int sub = 0; sub < kOuterTokens / 32; ++sub) {
+      if (sub >= subs) break;
+      if (sub + 1 < kOuterTokens / 32) request((sub + 1) & 1, min(sub + 1, subs - 1));
+      v4i(&z8)[8] = rows[sub & 1];
+      if (sub * 32 + 32 > here) {   // behind the last token stands the last one again: not a number times zero is no zero
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (sub * 32 + g * 8 + e >= here) z8[e] = v4i{0, 0, 0, 0};
+      }
+      v4i b[8];
+      transpose8(b, z8);
+#pragma unroll
+      for (int m = 0; m < RT; ++m)
+#pragma unroll
+        for (int low = 0; low < 2; ++low) {
+          const v4i a = *(const v4i *)&hs[low][m * 16 + row][sub * 32 + g * 8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[m][j] = mfma(a, b[j], acc[m][j]);
+        }
+    }
+  }
+  if (!in) return;
+  // a lane has columns col .. col + 7 of ranks 4 g .. 4 g + 3 of each sixteen
+  const bool alone = tile.tokens <= p.size;
+#pragma unroll
+  for (int m = 0; m < RT; ++m)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int rank = rank0 + m * 16 + g * 4 + i;
+      if (rank >= r) continue;
+      if (alone) {
+        v4i out;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = (int)(bf16_rne_bits(acc[m][2 * k][i]) | (bf16_rne_bits(acc[m][2 * k + 1][i]) << 16));
+        *(v4i *)(sd.grad + ((int64_t)tile.group * r + rank) * D + col) = out;
+      } else {
+        float *out = sd.partials + (outer_part(tile.first, p.size, tile.piece) * r + rank) * D + col;
+        *(v4f *)out = v4f{acc[m][0][i], acc[m][1][i], acc[m][2][i], acc[m][3][i]};
+        *(v4f *)(out + 4) = v4f{acc[m][4][i], acc[m][5][i], acc[m][6][i], acc[m][7][i]};
+      }
+    }
+}
+
+// The sums of a group's tiles, in their order, rounded: groups of more than one tile.
+__global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int64_t blocks0) {
+  const int from = p.starts[blockIdx.y], tokens = p.starts[blockIdx.y + 1] - from;
+  if (tokens <= p.size) return;
+  const int which = (int64_t)blockIdx.x >= blocks0;
+  const OuterSide &sd = p.side[which];
+  const int64_t at = ((int64_t)blockIdx.x - (which ? blocks0 : 0)) * 2048 + threadIdx.x * 8, all = (int64_t)p.r * sd.D;
+  if (at >= all) return;
+  v4f lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+  const int pieces = (tokens + p.size - 1) / p.size;
+  for (int i = 0; i < pieces; ++i) {
+    const float *part = sd.partials + outer_part(from + i * p.size, p.size, i) * all + at;
+    const v4f a = *(const v4f *)part, b = *(const v4f *)(part + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) lo[e] += a[e], hi[e] += b[e];
+  }
+  v4i out;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const float u = k < 2 ? lo[2 * k] : hi[2 * k - 4], w = k < 2 ? lo[2 * k + 1] : hi[2 * k - 3];
+    out[k] = (int)(bf16_rne_bits(u) | (bf16_rne_bits(w) << 16));
+  }
+  *(v4i *)(sd.grad + (int64_t)blockIdx.y * all + at) = out;
+}
+
+// ---- host ----
+
+constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 1 << 16, kMaxCols = 1 << 24;
+
+// Tokens of a tile: 64, which read a factor a quarter as often, where the adapters have that many on average.
+static int tile_tokens(int64_t T, int64_t n) { return T >= 64 * (n + 1) ? 64 : 16; }
+static int64_t tile_slots(int64_t T, int64_t n, int64_t size) { return T / size + n + 2; }
+
+// Tokens of a tile of the factors' gradients: so many tiles that two workgroups a unit have work.
+static int outer_size(int64_t T, int64_t K, int64_t N) {
+  const int64_t chunks = (K + 511) / 512 + (N + 511) / 512, wanted = (2 * (int64_t)num_cus() + chunks - 1) / chunks;
+  int size = kOuterTokens;
+  while (size < 2048 && size * wanted < T) size *= 2;
+  return size;
+}
+
+static bool rows_fit(const void *p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld >= cols; }
+static int check_sizes(const char *who, int64_t T, int64_t n, int64_t r, int64_t D) {
+  L8_REQUIRE(T >= 0 && T < kMaxTokens, "%s: %lld tokens, fewer than 2^24 are wanted", who, (long long)T);
+  L8_REQUIRE(n >= 1 && n <= kMaxAdapters, "%s: %lld adapters, 1 to 2^16 are wanted", who, (long long)n);
+  L8_REQUIRE(r >= 8 && r <= kMaxRank && r % 8 == 0, "%s: rank %lld is not a multiple of 8 up to %lld", who, (long long)r, (long long)kMaxRank);
+  L8_REQUIRE(D >= 8 && D % 8 == 0 && D < kMaxCols, "%s: %lld columns, a multiple of 8 below 2^24 is wanted", who, (long long)D);
+  return L8_OK;
+}
+static int check_grid(const char *who, int64_t x, int64_t y, int64_t z, int64_t threads) {
+  L8_REQUIRE(y <= 65535 && x * y * z * threads < (1ll << 32), "%s: 2^32 threads or more", who);
+  return L8_OK;
+}
+static int check_plan(const char *who, int64_t T, const void *order, const void *starts) {
+  L8_REQUIRE((order || T == 0) && starts && ((uintptr_t)order % 4) == 0 && ((uintptr_t)starts % 4) == 0, "%s: null or misaligned order of tokens", who);
+  return L8_OK;
+}
+#define L8_CALL(expr)              \
+  do {                             \
+    const int code_ = (expr);      \
+    if (code_ != L8_OK) return code_; \
+  } while (0)
+
+}  // namespace l8
+
+using namespace l8;
+
+extern "C" int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, int64_t n, int *order, int *starts, void *stream) {
+  const char *who = "l8_lowrank_route";
+  L8_CALL(check_sizes(who, T, n, 8, 8));
+  L8_CALL(check_plan(who, T, order, starts));
+  L8_REQUIRE(T == 0 || (index && ((uintptr_t)index % (index_is_i64 ? 8 : 4)) == 0), "%s: null or misaligned index", who);
+  const dim3 grid((unsigned)(n + 2)), block(kRouteBlock);
+  hipStream_t st = (hipStream_t)stream;
+  if (index_is_i64) hipLaunchKernelGGL(lowrank_route_kernel<int64_t>, grid, block, 0, st, (const int64_t *)index, (int)T, (int)n, order, starts);
+  else hipLaunchKernelGGL(lowrank_route_kernel<int32_t>, grid, block, 0, st, (const int32_t *)index, (int)T, (int)n, order, starts);
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+// Workgroups that share K: as many as give every unit one, with at least two steps left for each wave.
+extern "C" int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K) {
+  if (T <= 0 || n <= 0 || K <= 0) return 1;
+  const int64_t size = tile_tokens(T, n), tiles = std::min(T, tile_slots(T, n, size)), waves = size == 16 ? 8 : 4;
+  return std::max<int64_t>(1, std::min<int64_t>({num_cus() / tiles, (K + 63) / 64 / (2 * waves), 16}));
+}
+
+extern "C" int l8_lowrank_shrink(const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const int *order, const int *starts,
+                                 float *h, int64_t splits, void *stream) {
+  const char *who = "l8_lowrank_shrink";
+  L8_CALL(check_sizes(who, T, n, r, K));
+  L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
+  if (T == 0) return L8_OK;
+  L8_CALL(check_plan(who, T, order, starts));
+  L8_REQUIRE(rows_fit(x, ldx, K) && rows_fit(f, K, K) && h && ((uintptr_t)h % 16) == 0, "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  const int64_t size = tile_tokens(T, n), slots = tile_slots(T, n, size);
+  const ShrinkArgs p{(const uint16_t *)x, (const uint16_t *)f, order, starts, h, ldx, (int)T, (int)K, (int)n, (int)r, (int)splits};
+  const unsigned ranks = r <= 64 ? 1 : 2;
+  hipStream_t st = (hipStream_t)stream;
+#define L8_SHRINK(MT, RT, W)                                                                                             \
+  do {                                                                                                                   \
+    L8_CALL(check_grid(who, slots, splits, ranks, W * 64));                                                              \
+    hipLaunchKernelGGL((lowrank_shrink_kernel<MT, RT, W>), dim3((unsigned)slots, (unsigned)splits, ranks), dim3(W * 64), 0, st, p); \
+  } while (0)
+  if (size == 16) {
+    if (r <= 16) L8_SHRINK(1, 1, 8);
+    else if (r <= 32) L8_SHRINK(1, 2, 8);
+    else L8_SHRINK(1, 4, 8);
+  } else {
+    if (r <= 16) L8_SHRINK(4, 1, 4);
+    else if (r <= 32) L8_SHRINK(4, 2, 4);
+    else L8_SHRINK(4, 4, 4);
+  }
+#undef L8_SHRINK
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+extern "C" int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
+                                 int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream) {
+  const char *who = "l8_lowrank_expand";
+  L8_CALL(check_sizes(who, T, n, r, N));
+  L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
+  if (T == 0) return L8_OK;
+  L8_CALL(check_plan(who, T, order, starts));
+  L8_REQUIRE((!y || rows_fit(y, ldy, N)) && rows_fit(f, N, N) && rows_fit(out, ldo, N) && h && ((uintptr_t)h % 16) == 0 && ((uintptr_t)scale % 4) == 0,
+             "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  const int64_t size = tile_tokens(T, n), slots = tile_slots(T, n, size), chunks = (N + kExpandWaves * 128 - 1) / (kExpandWaves * 128);
+  L8_CALL(check_grid(who, slots, chunks, 1, kExpandWaves * 64));
+  const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, order, starts, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits};
+  const dim3 grid((unsigned)slots, (unsigned)chunks), block(kExpandWaves * 64);
+  hipStream_t st = (hipStream_t)stream;
+#define L8_EXPAND(MT)                                                                                        \
+  do {                                                                                                       \
+    if (r <= 16) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 0>), grid, block, 0, st, p);                  \
+    else if (r <= 32) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 1>), grid, block, 0, st, p);             \
+    else if (r <= 64) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 2>), grid, block, 0, st, p);             \
+    else hipLaunchKernelGGL((lowrank_expand_kernel<MT, 4>), grid, block, 0, st, p);                          \
+  } while (0)
+  if (size == 16) L8_EXPAND(1);
+  else L8_EXPAND(4);
+#undef L8_EXPAND
+  L8_HIP(hipGetLastError());
+  return L8_OK;
+}
+
+extern "C" int64_t l8_lowrank_outer_workspace(int64_t T, int64_t r, int64_t K, int64_t N) {
+  if (T <= 0 || r <= 0 || K < 0 || N < 0) return 0;
+  const int64_t size = outer_size(T, K, N);
+  return T <= size ? 0 : 2 * (T / size + 1) * r * (K + N) * (int64_t)sizeof(float);
+}
+
+extern "C" int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, int64_t T, int64_t n, int64_t r, const int *order, const int *starts,
+                                void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *who = "l8_lowrank_outer";
+  L8_REQUIRE(two, "%s: null pointer", who);
+  OuterArgs p{};
+  int64_t D[2];
+  for (int i = 0; i < 2; ++i) {   // a side without a gradient has no columns
+    D[i] = two[i].grad ? two[i].D : 0;
+    L8_CALL(check_sizes(who, T, n, r, two[i].grad ? D[i] : 8));
+    if (!two[i].grad) continue;
+    L8_REQUIRE(((uintptr_t)two[i].grad % 16) == 0 && two[i].splits >= 1 && two[i].splits <= 64, "%s: a misaligned gradient, or parts of h that are not 1 to 64", who);
+    L8_REQUIRE(T == 0 || (rows_fit(two[i].z, two[i].ldz, D[i]) && two[i].h && ((uintptr_t)two[i].h % 16) == 0), "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  }
+  if (D[0] + D[1] == 0) return L8_OK;
+  L8_CALL(check_plan(who, T, order, starts));
+  L8_REQUIRE(((uintptr_t)scale % 4) == 0, "%s: misaligned scale", who);
+  const int size = outer_size(T, D[0], D[1]);
+  const int64_t need = l8_lowrank_outer_workspace(T, r, D[0], D[1]);
+  L8_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0), "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+  const int64_t parts = T <= size ? 0 : 2 * (T / size + 1);
+  for (int i = 0; i < 2; ++i) {
+    p.side[i] = OuterSide{two[i].h, (const uint16_t *)two[i].z, (uint16_t *)two[i].grad, (float *)workspace + (i ? parts * r * D[0] : 0), two[i].ldz, (int)D[i], (int)two[i].splits,
+                          (int)((D[i] + 511) / 512)};
+  }
+  p.scale = scale, p.order = order, p.starts = starts, p.T = (int)T, p.n = (int)n, p.r = (int)r, p.size = size;
+  const int64_t slots = tile_slots(T, n, size), chunks = p.side[0].chunks + p.side[1].chunks, ranks = r <= 64 ? 1 : 2;
+  L8_CALL(check_grid(who, slots, chunks, ranks, kOuterWaves * 64));
+  const dim3 grid((unsigned)slots, (unsigned)chunks, (unsigned)ranks), block(kOuterWaves * 64);
+  hipStream_t st = (hipStream_t)stream;
+  if (r <= 16) hipLaunchKernelGGL(lowrank_outer_kernel<1>, grid, block, 0, st, p);
+  else if (r <= 32) hipLaunchKernelGGL(lowrank_outer_kernel<2>, grid, block, 0, st, p);
+  else hipLaunchKernelGGL(lowrank_outer_kernel<4>, grid, block, 0, st, p);
+  L8_HIP(hipGetLastError());
+  if (parts) {
+    const int64_t b0 = (r * D[0] + 2047) / 2048, b1 = (r * D[1] + 2047) / 2048;
+    L8_CALL(check_grid(who, b0 + b1, 1, n, 256));
+    hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)(b0 + b1), (unsigned)n), dim3(256), 0, st, p, b0);
+    L8_HIP(hipGetLastError());
+  }
+  return L8_OK;
+}

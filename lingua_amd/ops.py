@@ -1040,6 +1040,141 @@ def rotary(xq: Optional[torch.Tensor], xk: Optional[torch.Tensor], cos: torch.Te
     return tuple(outs)
 
 
+# ---- low-rank adapters of many requests ----
+
+def _plan_args(plan, T: int, n: int, device, what: str):
+    order, starts = plan
+    if (order.dtype != torch.int32 or starts.dtype != torch.int32 or order.numel() != T or starts.numel() != n + 3 or order.device != device or
+            starts.device != device or not order.is_contiguous() or not starts.is_contiguous()):
+        raise RuntimeError(f"{what}: the tokens' order must be that of {T} tokens and {n} adapters on the inputs' device")
+    return order.data_ptr(), starts.data_ptr()
+
+
+def _factor(f: torch.Tensor, what: str) -> torch.Tensor:
+    if f.dtype != torch.bfloat16 or f.dim() != 3:
+        raise RuntimeError(f"{what}: factors must be bf16 [adapters, rank, features], got {f.dtype} {tuple(f.shape)}")
+    f = f.contiguous()
+    return f if f.data_ptr() % 16 == 0 else f.clone()
+
+
+def _h_arg(h: torch.Tensor, T: int, r: int, device, what: str) -> torch.Tensor:
+    if h.dtype != torch.float32 or h.dim() != 3 or h.shape[1:] != (T, r) or h.device != device:
+        raise RuntimeError(f"{what}: h must be fp32 [parts, {T}, {r}] on the inputs' device, got {h.dtype} {tuple(h.shape)}")
+    h = h.contiguous()
+    return h if h.data_ptr() % 16 == 0 else h.clone()
+
+
+def _scale_arg(scale, n: int, device, what: str):
+    if scale is None:
+        return None
+    if scale.dtype != torch.float32 or scale.shape != (n,) or scale.device != device:
+        raise RuntimeError(f"{what}: scale must be fp32 with {n} elements on the inputs' device")
+    return scale.contiguous()
+
+
+def lowrank_route(index: torch.Tensor, n: int):
+    """Tokens by adapter: (order int32 [T], starts int32 [n + 3]) of an int32 or int64 index [T] of 0 .. n - 1, -1 for none."""
+    what = "lowrank_route"
+    if index.dtype not in (torch.int32, torch.int64) or index.dim() != 1:
+        raise RuntimeError(f"{what}: an int32 or int64 index of one dimension is wanted, got {index.dtype} {tuple(index.shape)}")
+    st = _prep(index, what)
+    index = index.contiguous()
+    T, dev = index.shape[0], index.device
+    order = torch.empty((T,), dtype=torch.int32, device=dev)
+    starts = torch.empty((n + 3,), dtype=torch.int32, device=dev)
+    with _timed(what, 8 * T, dev):
+        code = _lib.load().l8_lowrank_route(index.data_ptr(), int(index.dtype == torch.int64), T, n, order.data_ptr(), starts.data_ptr(), st)
+    _lib.check(code, "l8_lowrank_route")
+    return order, starts
+
+
+def lowrank_shrink(x: torch.Tensor, f: torch.Tensor, plan) -> torch.Tensor:
+    """fp32 [parts, T, r] whose sum over the parts is x_t f_i^T for every token t of an adapter i; x bf16 [T, D], f bf16 [n, r, D].  Rows of
+    tokens without an adapter are left as they were."""
+    what = "lowrank_shrink"
+    x, f = _rows_on_lines(x, torch.bfloat16, what), _factor(f, what)
+    st = _prep(x, what)
+    (T, D), (n, r, D2), dev = x.shape, f.shape, x.device
+    if D != D2 or f.device != dev:
+        raise RuntimeError(f"{what}: rows of {D} and factors of {D2} features on {dev} and {f.device}")
+    order, starts = _plan_args(plan, T, n, dev, what)
+    with _timed(what, 2 * T * D + 2 * f.numel() + 4 * T * r, dev):
+        splits = _lib.load().l8_lowrank_splits(T, n, D)
+        h = torch.empty((splits, T, r), dtype=torch.float32, device=dev)
+        code = _lib.load().l8_lowrank_shrink(x.data_ptr(), T, D, _ld(x), f.data_ptr(), n, r, order, starts, h.data_ptr(), splits, st)
+    _lib.check(code, "l8_lowrank_shrink")
+    return h
+
+
+def lowrank_expand(y: Optional[torch.Tensor], h: torch.Tensor, f: torch.Tensor, scale: Optional[torch.Tensor], plan, out: Optional[torch.Tensor] = None):
+    """bf16 [T, D]: y_t + scale_i h_t f_i for every token of an adapter i, y_t for the others (y None: zeros); NaN where the index was no
+    adapter's.  ``out`` may be y."""
+    what = "lowrank_expand"
+    f = _factor(f, what)
+    st = _prep(f, what)
+    (n, r, D), dev = f.shape, f.device
+    T = h.shape[1] if h.dim() == 3 else -1
+    h, scale = _h_arg(h, T, r, dev, what), _scale_arg(scale, n, dev, what)
+    given = y
+    if y is not None:
+        y = _rows_on_lines(y, torch.bfloat16, what)
+        if y.shape != (T, D) or y.device != dev:
+            raise RuntimeError(f"{what}: y must be [{T}, {D}] on {dev}, got {tuple(y.shape)} on {y.device}")
+    order, starts = _plan_args(plan, T, n, dev, what)
+    user_out = out is not None
+    if user_out and (out.dtype != torch.bfloat16 or out.shape != (T, D) or out.device != dev or (out.numel() and not (_rows_apart(out) and rows_on_16_bytes(out)))):
+        raise RuntimeError(f"{what}: out must be bf16 [{T}, {D}] on the inputs' device, its rows on 16-byte lines")
+    if user_out and out is not given and y is not None and _overlap(out, y):
+        raise RuntimeError(f"{what}: out and y overlap")
+    if not user_out:
+        out = torch.empty((T, D), dtype=torch.bfloat16, device=dev)
+    with _timed(what, 2 * T * D * (1 if y is None else 2) + 2 * f.numel() + 4 * h.numel(), dev):
+        code = _lib.load().l8_lowrank_expand(_addr(y) or None, _ld(y) if y is not None else 0, h.data_ptr(), h.shape[0], _addr(scale) or None, f.data_ptr(), T, D, n, r,
+                                             order, starts, out.data_ptr(), _ld(out), st)
+    _lib.check(code, "l8_lowrank_expand")
+    if user_out:
+        _wrote_into(out)
+    return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Do two matrices of dense rows lie in one stretch of memory?"""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * _ld(t) + t.shape[1]) * t.element_size()) for t in (a, b))
+    return a0 < b1 and b0 < a1
+
+
+def lowrank_outer(sides, scale: Optional[torch.Tensor], n: int, r: int, plan):
+    """Gradients of factors, bf16 [n, r, D], in one launch: ``sides`` is one or two of (h, z), z bf16 [T, D], for the gradient
+    scale_i sum over i's tokens of h_t (x) z_t."""
+    what = "lowrank_outer"
+    dev = sides[0][1].device
+    st = _prep(sides[0][1], what)
+    T = sides[0][1].shape[0]
+    scale = _scale_arg(scale, n, dev, what)
+    order, starts = _plan_args(plan, T, n, dev, what)
+    keep, items, grads, dims = [], [], [], []
+    for h, z in sides:
+        z = _rows_on_lines(z, torch.bfloat16, what)
+        if z.shape[0] != T or z.device != dev:
+            raise RuntimeError(f"{what}: both sides must be of the same tokens on one device")
+        h = _h_arg(h, T, r, dev, what)
+        grad = torch.empty((n, r, z.shape[1]), dtype=torch.bfloat16, device=dev)
+        keep += [z, h]
+        grads.append(grad)
+        dims.append(z.shape[1])
+        items += [h.data_ptr(), h.shape[0], z.data_ptr(), _ld(z), z.shape[1], grad.data_ptr()]
+    dims += [0] * (2 - len(dims))
+    items += [0] * (12 - len(items))
+    with _timed(what, sum(2 * z.numel() for _, z in sides) + sum(2 * g.numel() for g in grads), dev):
+        need = _lib.load().l8_lowrank_outer_workspace(T, r, *dims)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        code = _lib.load().l8_lowrank_outer(struct.pack("12q", *items), _addr(scale) or None, T, n, r, order, starts, _addr(ws) or None, need, st)
+    _lib.check(code, "l8_lowrank_outer")
+    return grads
+
+
 # ---- MXFP4: e2m1 codes, two a byte, in blocks of 32 along a row, with an e8m0 scale each ----
 
 MX_BLOCK = 32

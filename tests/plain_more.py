@@ -78,3 +78,50 @@ def grad_within(got, want, error):
     """A gradient of a parameter, in bf16 or fp32: within `error` and its own rounding."""
     half = torch.finfo(got.dtype).eps / 2
     return bool(((got.double().cpu() - want.cpu()).abs() <= error.cpu() * (1 + half) + want.cpu().abs() * half + 1e-37).all())
+
+
+# ---- low-rank adapters ----
+
+# Rounding errors: a product of two bf16 is exact in 32 bits, a sum of D of them is off by at most D half steps of the sum of magnitudes in
+# whatever order; h enters a product as two bf16 numbers, which leaves 2^-16 of it, and is scaled with one rounding.
+SPLIT = 2.0 ** -16
+
+
+def lowrank(y, x, a, b, index, scale):
+    """fp64 (out, what it may be off by, h times scale, and its error) of one adapter after the other; y may be None."""
+    x, a, b = (t.detach().double().cpu() for t in (x, a, b))
+    index = index.cpu().long()
+    n, r, D = a.shape
+    T, N = x.shape[0], b.shape[2]
+    s = torch.ones(n, dtype=torch.float64) if scale is None else scale.double().cpu()
+    out = torch.zeros((T, N), dtype=torch.float64) if y is None else y.detach().double().cpu().clone()
+    size, h, eh = torch.zeros((T, N), dtype=torch.float64), torch.zeros((T, r), dtype=torch.float64), torch.zeros((T, r), dtype=torch.float64)
+    for i in range(n):
+        at = (index == i).nonzero()[:, 0]
+        if not len(at):
+            continue
+        h[at] = s[i] * (x[at] @ a[i].t())
+        eh[at] = s[i].abs() * (FP32 * (D + 16)) * (x[at].abs() @ a[i].abs().t()) + (SPLIT + 4 * FP32) * h[at].abs()
+        out[at] += h[at] @ b[i]
+        size[at] = eh[at] @ b[i].abs() + FP32 * (2 * r + 4) * (h[at].abs() @ b[i].abs())
+    size += FP32 * out.abs()
+    return out, size, h, eh
+
+
+def lowrank_grads(x, a, b, index, scale, gy):
+    """fp64 (gx, ga, gb) and what each may be off by."""
+    gx, ex, gh, egh = lowrank(None, gy, b, a, index, scale)
+    _, _, h, eh = lowrank(None, x, a, b, index, scale)
+    index = index.cpu().long()
+    x, gy = x.detach().double().cpu(), gy.double().cpu()
+    n, r, K = a.shape
+    ga, gb = torch.zeros(a.shape, dtype=torch.float64), torch.zeros(b.shape, dtype=torch.float64)
+    ea, eb = ga.clone(), gb.clone()
+    for i in range(n):
+        at = (index == i).nonzero()[:, 0]
+        if not len(at):
+            continue
+        for grad, err, u, eu, z in ((ga, ea, gh, egh, x), (gb, eb, h, eh, gy)):
+            grad[i] = u[at].t() @ z[at]
+            err[i] = eu[at].t() @ z[at].abs() + FP32 * (2 * len(at) + 16) * (u[at].abs().t() @ z[at].abs())
+    return (gx, ga, gb), (ex, ea, eb)

@@ -64,8 +64,84 @@ def test_rotary_axes_is_refused(change):
     assert refused("l8_rotary_axes", two, *args.values())
 
 
+ROUTE = dict(index=P, i64=0, T=64, n=4, order=P, starts=P, stream=None)
+SHRINK = dict(x=P, T=64, K=128, ldx=128, f=P, n=4, r=16, order=P, starts=P, h=P, splits=2, stream=None)
+EXPAND = dict(y=P, ldy=128, h=P, splits=2, scale=P, f=P, T=64, N=128, n=4, r=16, order=P, starts=P, out=P, ldo=128, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(n=(1 << 16) + 1), dict(index=None), dict(index=P + 2), dict(index=P + 4, i64=1), dict(order=None), dict(order=P + 2),
+                                    dict(starts=None), dict(starts=P + 1)])
+def test_route_is_refused(change):
+    assert refused("l8_lowrank_route", *{**ROUTE, **change}.values())
+
+
+@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(n=1 << 17), dict(r=0), dict(r=12), dict(r=136), dict(K=0), dict(K=12, ldx=16), dict(K=1 << 24, ldx=1 << 24),
+                                    dict(x=None), dict(x=P + 8), dict(ldx=120), dict(ldx=132), dict(f=None), dict(f=P + 8), dict(h=None), dict(h=P + 4), dict(order=None), dict(starts=None),
+                                    dict(splits=0), dict(splits=65), dict(T=(1 << 24) - 1, n=1 << 16, splits=64)])
+def test_shrink_is_refused(change):
+    assert refused("l8_lowrank_shrink", *{**SHRINK, **change}.values())
+
+
+@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(r=4), dict(r=130), dict(N=0), dict(N=20, ldy=24, ldo=24), dict(y=P + 8), dict(ldy=64), dict(ldy=130), dict(h=None),
+                                    dict(h=P + 8), dict(splits=0), dict(scale=P + 2), dict(f=None), dict(f=P + 2), dict(out=None), dict(out=P + 8), dict(ldo=132), dict(ldo=64), dict(order=None),
+                                    dict(starts=P + 2), dict(T=(1 << 24) - 1, n=1, N=1 << 16, ldy=1 << 16, ldo=1 << 16)])
+def test_expand_is_refused(change):
+    assert refused("l8_lowrank_expand", *{**EXPAND, **change}.values())
+
+
+SIDE = dict(h=P, splits=2, z=P, ldz=128, D=128, grad=P)
+OUTER = dict(scale=P, T=64, n=4, r=16, order=P, starts=P, ws=None, ws_bytes=0, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(r=20), dict(D=0), dict(D=20, ldz=24), dict(h=0), dict(h=P + 8), dict(splits=0), dict(z=0), dict(z=P + 8), dict(ldz=120),
+                                    dict(ldz=132), dict(grad=P + 8), dict(scale=P + 2), dict(order=None), dict(starts=None), dict(T=10000), dict(T=10000, ws=P, ws_bytes=64),
+                                    dict(T=10000, ws=P + 8, ws_bytes=1 << 40), dict(T=(1 << 24) - 1, n=1 << 16, ws=P, ws_bytes=1 << 60, D=1 << 20, ldz=1 << 20)])
+def test_outer_is_refused(change):
+    side = {**SIDE, **{k: v for k, v in change.items() if k in SIDE}}
+    rest = {**OUTER, **{k: v for k, v in change.items() if k in OUTER}}
+    for first in (True, False):
+        both = (side, SIDE) if first else (SIDE, side)
+        assert refused("l8_lowrank_outer", struct.pack("12q", *both[0].values(), *both[1].values()), *rest.values())
+
+
+def test_lowrank_splits_and_workspace():
+    lib = _lib.load()
+    assert lib.l8_lowrank_splits(0, 4, 64) == lib.l8_lowrank_splits(-5, 4, 64) == lib.l8_lowrank_splits(20, 2, 8) == 1
+    assert all(1 <= lib.l8_lowrank_splits(T, n, K) <= 16 for T in (1, 16, 300, 1 << 20) for n in (1, 40, 1 << 16) for K in (8, 4096, 1 << 20))
+    assert lib.l8_lowrank_outer_workspace(100, 16, 128, 128) == 0 and lib.l8_lowrank_outer_workspace(0, 16, 128, 128) == 0
+    assert lib.l8_lowrank_outer_workspace(1 << 20, 16, 128, 256) % (4 * 16 * 384) == 0
+
+
+def test_lowrank_arguments_are_refused():
+    from lingua_amd import adapters
+    bf = torch.bfloat16
+    y, x, a, b, i = torch.zeros(4, 64, dtype=bf), torch.zeros(4, 32, dtype=bf), torch.zeros(2, 8, 32, dtype=bf), torch.zeros(2, 8, 64, dtype=bf), torch.zeros(4, dtype=torch.int32)
+    call = adapters.add_lowrank
+    for args in ((y, x, a[0], b, i), (y, x, a, b[:, :4], i), (y, x, a, b[:1], i), (y, x[:, :24], a, b, i), (y[:, :8], x, a, b, i), (y[:3], x, a, b, i), (y, x, a, b, i[:3]), (y, x, a, b, i[:, None]),
+                 (y.float(), x, a, b, i), (y, x.float(), a, b, i), (y, x, a.float(), b, i), (y, x, a[:, :4], b[:, :4], i), (y, x.repeat(1, 1)[:, :12], a[:, :, :12], b, i),
+                 (y, x, a.repeat(1, 17, 1), b.repeat(1, 17, 1), i), (y.to("meta"), x, a, b, i), (y, x, a, b, i.to("meta")),
+                 (y, x, a, b, adapters.Plan(i, torch.zeros(6, dtype=torch.int32), 3, (4,)))):
+        with pytest.raises(RuntimeError, match="do not fit|bf16|same tokens|rank|operands on|index is on|plan is for"):
+            call(*args)
+    with pytest.raises(RuntimeError, match="bank"):
+        adapters.route(i, 0)
+
+
+def test_adapters_beside_linears_keep_parameters():
+    from lingua_amd import adapters
+    model = torch.nn.ModuleDict({"w1": torch.nn.Linear(32, 64), "norm": torch.nn.LayerNorm(32)}).to(torch.bfloat16)
+    weight = model["w1"].weight
+    adapters.add_adapters(model, adapters.Requests(2), 8, "w1")
+    assert list(model.state_dict()) == ["w1.a", "w1.b", "w1.scale", "w1.linear.weight", "w1.linear.bias", "norm.weight", "norm.bias"] and model["w1"].linear.weight is weight
+    assert not model["w1"].b.any() and float(model["w1"].scale[1]) == 1
+    x = torch.randn(3, 32, dtype=torch.bfloat16)
+    assert torch.equal(model["w1"](x), model["w1"].linear(x))     # no request has one
+
+
 def test_empty_calls_do_nothing():
     lib = _lib.load()
+    assert lib.l8_lowrank_shrink(*{**SHRINK, "T": 0, "x": None}.values()) == 0 and lib.l8_lowrank_expand(*{**EXPAND, "T": 0, "out": None}.values()) == 0
+    assert lib.l8_lowrank_outer(struct.pack("12q", *[0] * 12), *OUTER.values()) == 0
     assert lib.l8_dropout(None, None, None, 0, None, 0, 0, None) == 0
     assert lib.l8_norm_fwd(struct.pack("11qd16q", *{**FWD, "R": 0, "x": 0}.values())) == 0
     assert lib.l8_norm_bwd(struct.pack("27q", *{**BWD, "C": 0, "gy": 0}.values())) == 0
@@ -104,12 +180,13 @@ def test_rotary_axes_arguments_are_refused():
 
 
 def test_no_cpu_path():
-    from lingua_amd import dropout, norm, rope
+    from lingua_amd import adapters, dropout, norm, rope
     x, n = torch.zeros(4, 64, dtype=torch.bfloat16), dropout.numbers(1, "cpu")
     drop = dropout.Drop(0.1, n)
     for call in (lambda: norm.layernorm(x), lambda: norm.add_layernorm(x, x), lambda: norm.add_layernorm(x, x, dropout=drop), lambda: norm.add_rmsnorm(x, x, x[0], 1e-5, drop),
                  lambda: dropout.dropout(x, drop), lambda: dropout.dropout_add(x, x, drop), lambda: norm.Fp8LayerNorm(64)(x), lambda: dropout.Dropout(0.1, n)(x),
-                 lambda: rope.rotary_axes(x.view(1, 4, 1, 64), x.view(1, 4, 1, 64), torch.zeros(4, 32), torch.zeros(4, 32), torch.zeros(2, 1, 4).long(), (16, 16))):
+                 lambda: rope.rotary_axes(x.view(1, 4, 1, 64), x.view(1, 4, 1, 64), torch.zeros(4, 32), torch.zeros(4, 32), torch.zeros(2, 1, 4).long(), (16, 16)),
+                 lambda: adapters.add_lowrank(x, x, torch.zeros(2, 8, 64, dtype=torch.bfloat16), torch.zeros(2, 8, 64, dtype=torch.bfloat16), torch.zeros(4).int())):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
 
