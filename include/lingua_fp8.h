@@ -443,6 +443,11 @@ int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K);
 /* out = y + scale_i h F_i, bf16 [T,N]; y NULL: zeros, scale NULL: ones.  Tokens without an adapter: out = y.  out may be y. */
 int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
                       int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream);
+/* All of it for a pass without gradients: the three above, or two where up to 64 tokens need no order.  workspace: 16-byte aligned, of
+ * l8_lowrank_add_workspace bytes. */
+int l8_lowrank_add(const void *y, int64_t ldy, const void *x, int64_t ldx, const void *a, const void *b, const float *scale, const void *index, int index_is_i64,
+                   int64_t T, int64_t K, int64_t N, int64_t n, int64_t r, void *out, int64_t ldo, void *workspace, int64_t workspace_bytes, void *stream);
+int64_t l8_lowrank_add_workspace(int64_t T, int64_t K, int64_t n, int64_t r);
 /* grad_i = scale_i sum over the tokens of i of h_t (x) z_t, bf16 [n,r,D], for two sides in one launch (grad NULL: not that one): that of A with h
  * of the gradient and z = x, that of B with h of the forward and z the gradient.  Sums in a fixed order. */
 typedef struct {

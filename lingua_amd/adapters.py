@@ -104,6 +104,9 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         raise RuntimeError(f"{what}: the index is on {index.device}, the operands on {x.device}")
     f8._refuse_captured(y, x, a, what)
     f8._refuse_captured(b, None, None, what)
+    if not isinstance(index, Plan) and not (torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, a, b))) and f8._plain_call():
+        out = ops.lowrank_add(y.reshape(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), a, b, index.flatten(), scale)
+        return out.view(y.shape)
     plan = index if isinstance(index, Plan) else route(index, a.shape[0])
     if y.dim() == 2:
         return LowRankFn.apply(y, x, a, b, scale, plan.order, plan.starts)

@@ -33,71 +33,146 @@ L8_DEV v4f mfma(v4i a, v4i b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32
 
 // ---- tokens by adapter ----
 
-constexpr int kRouteBlock = 1024;
+constexpr int kRouteBlock = 1024, kRouteWaves = kRouteBlock / 64, kRouteTimes = 16;
 
-// A workgroup per group: how many tokens stand in front of its own, then its own tokens in their order.
+// A workgroup per group: how many tokens stand in front of its own, then its own tokens in their order.  Sixteen tokens a thread are
+// requested together and stay in registers between the two counts.
 template <typename Index>
 __global__ __launch_bounds__(kRouteBlock) void lowrank_route_kernel(const Index *__restrict__ index, int T, int n, int *__restrict__ order, int *__restrict__ starts) {
-  constexpr int WAVES = kRouteBlock / 64;
-  __shared__ int sums[WAVES], base[WAVES];
+  constexpr int SPAN = kRouteBlock * kRouteTimes, PLACES = kRouteTimes * kRouteWaves;
+  static_assert(PLACES == 256, "four places a lane of one wave");
+  __shared__ int sums[kRouteWaves], place[PLACES + 1];
   const int mine = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  auto group_of = [&](int t) {
-    const int64_t i = (int64_t)index[t];
-    return i >= 0 && i < n ? (int)i : i == -1 ? n : n + 1;
+  int group[kRouteTimes];
+  auto load = [&](int t0) {
+    int64_t i[kRouteTimes];
+#pragma unroll
+    for (int k = 0; k < kRouteTimes; ++k) {
+      const int t = t0 + k * kRouteBlock + (int)threadIdx.x;
+      i[k] = (int64_t)index[min(t, T - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < kRouteTimes; ++k)
+      group[k] = t0 + k * kRouteBlock + (int)threadIdx.x >= T ? n + 2 : i[k] >= 0 && i[k] < n ? (int)i[k] : i[k] == -1 ? n : n + 1;
   };
   int less = 0;
-  for (int t = threadIdx.x; t < T; t += kRouteBlock) less += group_of(t) < mine;
+  for (int t0 = 0; t0 < T; t0 += SPAN) {
+    load(t0);
+#pragma unroll
+    for (int k = 0; k < kRouteTimes; ++k) less += group[k] < mine;
+  }
 #pragma unroll
   for (int d = 32; d; d >>= 1) less += __shfl_xor(less, d);
   if (lane == 0) sums[wave] = less;
   __syncthreads();
   int at = 0;
 #pragma unroll
-  for (int w = 0; w < WAVES; ++w) at += sums[w];
+  for (int w = 0; w < kRouteWaves; ++w) at += sums[w];
   if (threadIdx.x == 0) {
     starts[mine] = at;
     if (mine == n + 1) starts[n + 2] = T;
   }
-  for (int t0 = 0; t0 < T; t0 += kRouteBlock) {
-    const int t = t0 + threadIdx.x;
-    const bool own = t < T && group_of(t) == mine;
-    const uint64_t votes = __ballot(own);
-    if (lane == 0) base[wave] = __popcll(votes);
-    __syncthreads();
-    int before = at, all = 0;
+  for (int t0 = 0; t0 < T; t0 += SPAN) {
+    if (T > SPAN) load(t0);
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      if (w < wave) before += base[w];
-      all += base[w];
+    for (int k = 0; k < kRouteTimes; ++k) {
+      const uint64_t votes = __ballot(group[k] == mine);
+      if (lane == 0) place[k * kRouteWaves + wave] = __popcll(votes);
     }
-    if (own) order[before + __popcll(votes & ((1ull << lane) - 1))] = t;
-    at += all;
+    __syncthreads();
+    if (wave == 0) {   // counts -> how many stand in front
+      int c[4], sum = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum += c[k] = place[lane * 4 + k];
+      int upto = sum;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int other = __shfl_up(upto, d);
+        if (lane >= d) upto += other;
+      }
+      int before = upto - sum;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        place[lane * 4 + k] = before;
+        before += c[k];
+      }
+      if (lane == 63) place[PLACES] = upto;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kRouteTimes; ++k) {
+      const bool own = group[k] == mine;
+      const uint64_t votes = __ballot(own);
+      if (own) order[at + place[k * kRouteWaves + wave] + __popcll(votes & ((1ull << lane) - 1))] = t0 + k * kRouteBlock + (int)threadIdx.x;
+    }
+    at += place[PLACES];
     __syncthreads();
   }
 }
 
+// The tokens by adapter: `route`'s answer, or the index itself where there are few enough tokens for a wave to look at all of them.
+struct Tokens {
+  const int *order, *starts;   // NULL: the index
+  const void *index;
+  int index_i64;
+};
+constexpr int kFewTokens = 64;
+
 struct Tile {
-  int group, first, count;   // tokens order[first .. first + count); count 0: a number that no tile has
-  int piece, tokens;         // which of its group's tiles, and the group's tokens
+  int group, count;            // count 0: a number that no tile has
+  int first, piece, tokens;    // (of `route`) where its tokens begin in the order, which of its group's tiles it is, and the group's tokens
+  int mine;                    // lane m has token m
+  L8_DEV int token(int m) const { return __shfl(mine, min(m, count - 1)); }
 };
 // Tile `slot` of at most `size` tokens.  The same for the whole workgroup.
 L8_DEV Tile tile_of(const int *__restrict__ starts, int n, int size, int slot) {
   const int lane = threadIdx.x & 63;
-  int g = -1;
-  for (int i0 = 0; i0 < n + 2; i0 += 64) {   // the groups whose first number is at most `slot` come first
-    const int i = i0 + lane;
-    const int have = __popcll(__ballot(i < n + 2 && starts[i < n + 2 ? i : 0] / size + i <= slot));
-    g += have;
-    if (have < 64) break;
+  Tile t{};
+  int before = 0;
+  for (int i0 = 0;; i0 += 64) {   // the groups whose first number is at most `slot` come first
+    const int i = i0 + lane, from = starts[min(i, n + 1)], to = starts[min(i, n + 1) + 1];
+    const int have = __popcll(__ballot(i < n + 2 && from / size + i <= slot));
+    if (have) {
+      const int at = have - 1;
+      t.group = i0 + at;
+      before = __builtin_amdgcn_readlane(from, at);
+      t.tokens = __builtin_amdgcn_readlane(to, at) - before;
+    }
+    if (have < 64 || i0 + 64 >= n + 2) break;
   }
-  g = __builtin_amdgcn_readfirstlane(g);
-  Tile t;
-  t.group = g;
-  const int from = starts[g], to = starts[g + 1];
-  t.piece = slot - (from / size + g);
-  t.tokens = to - from;
-  t.first = from + t.piece * size;
-  t.count = min(size, max(0, to - t.first));
+  t.piece = slot - (before / size + t.group);
+  t.first = before + t.piece * size;
+  t.count = min(size, max(0, t.tokens - t.piece * size));
+  return t;
+}
+// The same with its tokens: up to 64.
+L8_DEV Tile tile_with_tokens(const Tokens &tk, int T, int n, int size, int slot) {
+  const int lane = threadIdx.x & 63;
+  if (tk.order) {
+    Tile t = tile_of(tk.starts, n, size, slot);
+    t.mine = t.count ? tk.order[t.first + min(lane, t.count - 1)] : 0;
+    return t;
+  }
+  // few tokens: one group after the other, in the order in which they first appear, until the slot's is found
+  const int64_t i = lane >= T ? -1 : tk.index_i64 ? ((const int64_t *)tk.index)[lane] : (int64_t)((const int32_t *)tk.index)[lane];
+  const int group = i >= 0 && i < n ? (int)i : i == -1 ? n : n + 1;
+  Tile t{};
+  uint64_t left = __ballot(lane < T);
+  while (left) {
+    const int g = __builtin_amdgcn_readlane(group, __builtin_ctzll(left));
+    const uint64_t same = __ballot(group == g && lane < T);
+    const int tokens = __popcll(same), pieces = (tokens + size - 1) / size;
+    if (slot < pieces) {
+      t.group = g, t.count = min(size, tokens - slot * size);
+      const int place = __popcll(same & ((1ull << lane) - 1)) - slot * size;   // of a lane in `same`
+      const bool in = (same >> lane & 1) && place >= 0 && place < size;
+      // every token goes to the lane of its place; the others go where no token of the tile is (a tile of 16: the last lane)
+      t.mine = __builtin_amdgcn_ds_permute((in ? place : 63) * 4, lane);
+      return t;
+    }
+    slot -= pieces;
+    left &= ~same;
+  }
   return t;
 }
 
@@ -105,27 +180,29 @@ L8_DEV Tile tile_of(const int *__restrict__ starts, int n, int size, int slot) {
 
 struct ShrinkArgs {
   const uint16_t *x, *f;
-  const int *order, *starts;
+  Tokens tokens;
   float *h;
   int64_t ldx;
   int T, K, n, r, splits;
 };
 
-// MT tiles of 16 tokens by RT of 16 ranks, the W waves share K.  A wave takes 64 columns a step, the waves side by side: lane group g
+// MT tiles of 16 tokens by RT of 16 ranks a wave; the W waves are SUB parts of a tile's tokens, and W / SUB of them share K.  A wave takes 64 columns a step, the waves side by side: lane group g
 // (of 16 lanes) takes columns 16 g .. 16 g + 15 of a step, the first eight into one matrix instruction and the others into a second, so
 // that a row is read in whole lines.  Which column meets which place of the instruction does not matter as long as it is the same for
 // both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
-template <int MT, int RT, int W>
+template <int MT, int SUB, int RT, int W>
 __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs p) {
-  __shared__ float red[W / 2][MT * RT * 256];
-  const Tile tile = tile_of(p.starts, p.n, MT * 16, blockIdx.x);
+  constexpr int KW = W / SUB;
+  __shared__ float red[SUB * (KW / 2)][MT * RT * 256];
+  const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, MT * SUB * 16, blockIdx.x);
   if (tile.group >= p.n || tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
+  const int part = wave % SUB, part0 = part * MT * 16, kw = wave / SUB;
   const int K = p.K, steps = (K + 63) / 64, rank0 = blockIdx.z * RT * 16;
   const int lo = (int)((int64_t)steps * blockIdx.y / p.splits), hi = (int)((int64_t)steps * (blockIdx.y + 1) / p.splits);
   const uint16_t *xr[MT], *fr[RT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xr[m] = p.x + (int64_t)p.order[tile.first + min(m * 16 + row, tile.count - 1)] * p.ldx;
+  for (int m = 0; m < MT; ++m) xr[m] = p.x + (int64_t)tile.token(part0 + m * 16 + row) * p.ldx;
 #pragma unroll
   for (int j = 0; j < RT; ++j) fr[j] = p.f + ((int64_t)tile.group * p.r + min(rank0 + j * 16 + row, p.r - 1)) * K;
   v4f acc[MT][RT];
@@ -161,48 +238,48 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
 #pragma unroll
         for (int j = 0; j < RT; ++j) acc[m][j] = mfma(a[s][m][c], b[s][j][c], acc[m][j]);
   };
-  int step = lo + wave;
+  int step = lo + kw;
   if (step < hi) request(0, step);
   while (step < hi) {
-    request(1, min(step + W, hi - 1));
+    request(1, min(step + KW, hi - 1));
     multiply(0, step);
-    step += W;
+    step += KW;
     if (step >= hi) break;
-    request(0, min(step + W, hi - 1));
+    request(0, min(step + KW, hi - 1));
     multiply(1, step);
-    step += W;
+    step += KW;
   }
   // the upper half of the waves hands its sums to the lower half, until one has them all
 #pragma unroll
-  for (int half = W / 2; half; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
+  for (int half = KW / 2; half; half /= 2) {
+    if (kw >= half && kw < 2 * half) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) *(v4f *)&red[wave - half][(m * RT + j) * 256 + lane * 4] = acc[m][j];
+        for (int j = 0; j < RT; ++j) *(v4f *)&red[part * (KW / 2) + kw - half][(m * RT + j) * 256 + lane * 4] = acc[m][j];
     }
     __syncthreads();
-    if (wave < half) {
+    if (kw < half) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
-          const v4f other = *(const v4f *)&red[wave][(m * RT + j) * 256 + lane * 4];
+          const v4f other = *(const v4f *)&red[part * (KW / 2) + kw][(m * RT + j) * 256 + lane * 4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][j][i] += other[i];
         }
     }
     __syncthreads();
   }
-  if (wave) return;
+  if (kw) return;
   // a lane has rank `row` of each sixteen, tokens 4 g .. 4 g + 3
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = m * 16 + g * 4 + i;
+      const int at = part0 + m * 16 + g * 4 + i, token = tile.token(at);
       if (at >= tile.count) continue;
-      float *out = p.h + ((int64_t)blockIdx.y * p.T + p.order[tile.first + at]) * p.r;
+      float *out = p.h + ((int64_t)blockIdx.y * p.T + token) * p.r;
 #pragma unroll
       for (int j = 0; j < RT; ++j)
         if (rank0 + j * 16 + row < p.r) out[rank0 + j * 16 + row] = acc[m][j][i];
@@ -250,100 +327,129 @@ L8_DEV void transpose8(v4i (&out)[8], const v4i (&rows)[8]) {
 struct ExpandArgs {
   const uint16_t *y, *f;
   const float *h, *scale;
-  const int *order, *starts;
+  Tokens tokens;
   uint16_t *out;
   int64_t ldy, ldo;
-  int T, N, n, r, splits;
+  int T, N, n, r, splits, chunks;
 };
 
 constexpr int kExpandWaves = 4;
 
-// MT tiles of 16 tokens by 128 columns a wave.  Column 8 c + j of a wave's 128 is column c of matrix instruction j: a lane then reads
-// eight neighbouring columns of eight rows of the factor, turns the block round in registers, and ends up with eight neighbouring
-// columns of four tokens: 16-byte loads and stores, 256 bytes of a row at once, and no LDS.
+// 16 tokens by 128 columns a wave; the workgroup's four waves are PARTS parts of a tile's tokens by 4 / PARTS stretches of columns.  Column
+// 8 c + j of a wave's 128 is column c of matrix instruction j: a lane then reads eight neighbouring columns of eight rows of the factor,
+// turns the block round in registers, and ends up with eight neighbouring columns of four tokens: 16-byte loads and stores, 256 bytes of a
+// row at once.
 // KS steps of 32 ranks, each with the upper and the lower bits of h; KS 0: up to 16 ranks, where one instruction takes both.
-template <int MT, int KS>
-__global__ __launch_bounds__(kExpandWaves * 64) void lowrank_expand_kernel(const ExpandArgs p) {
-  const Tile tile = tile_of(p.starts, p.n, MT * 16, blockIdx.x);
+// Waves of the same columns and more than 16 ranks share the factor's turned blocks through LDS, each making a part of them.
+// Everything that a wave reads is requested before anything is used: a tile waits for memory three times, for its place, for its tokens and
+// for the rest.
+// Up to 16 ranks: five waves a SIMD and not the four that the compiler would make room for, [16384,4096] with y 61 -> 52 us (six: 57).
+template <int PARTS, int KS>
+__global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : 1) void lowrank_expand_kernel(const ExpandArgs p) {
+  constexpr int STEPS = KS ? KS : 1;
+  constexpr bool SHARED = PARTS == kExpandWaves && KS > 0;
+  __shared__ v4i turned[SHARED ? STEPS * 8 * 64 : 1];
+  const int slot = blockIdx.x / p.chunks, chunk = blockIdx.x - slot * p.chunks;
+  const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, PARTS * 16, slot);
   if (tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-  const int col = (blockIdx.y * kExpandWaves + wave) * 128 + row * 8;
+  const int part0 = wave % PARTS * 16;
+  const int col = (chunk * (kExpandWaves / PARTS) + wave / PARTS) * 128 + row * 8;
   const bool in = col < p.N;
+  const int from = in ? col : 0, r = p.r;
+  int64_t t[4];
+  v4i y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    t[i] = tile.token(part0 + g * 4 + i);
+    y[i] = v4i{0, 0, 0, 0};
+    if (p.y) y[i] = __builtin_nontemporal_load((const v4i *)(p.y + t[i] * p.ldy + from));
+  }
+  auto store = [&](int i, v4i v) {
+    if (in && part0 + g * 4 + i < tile.count) __builtin_nontemporal_store(v, (v4i *)(p.out + t[i] * p.ldo + col));
+  };
   if (tile.group >= p.n) {   // no adapter: y as it is; no known adapter: NaN
-#pragma unroll 1
-    for (int at = g; at < tile.count; at += 4) {
-      const int64_t t = p.order[tile.first + at];
-      v4i v = {0, 0, 0, 0};
-      if (p.y && in) v = *(const v4i *)(p.y + t * p.ldy + col);
-      if (tile.group > p.n) v = v4i{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0};
-      if (in) *(v4i *)(p.out + t * p.ldo + col) = v;
-    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) store(i, tile.group > p.n ? v4i{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0} : y[i]);
     return;
   }
-  constexpr int STEPS = KS ? KS : 1;
-  const int r = p.r;
-  v4i b[STEPS][8];
+  auto rank_of = [&](int s) { return KS ? s * 32 + g * 8 : (g & 1) * 8; };
+  const float *h = p.h + (int64_t)tile.token(part0 + row) * r;
+  v4f hp[STEPS][2];   // of h: the first of its parts
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    const int k0 = KS ? s * 32 + g * 8 : (g & 1) * 8;
-    const uint16_t *f = p.f + ((int64_t)tile.group * r + min(k0, r - 8)) * p.N + (in ? col : 0);
+    const int k0 = min(rank_of(s), r - 8);
+    hp[s][0] = *(const v4f *)(h + k0), hp[s][1] = *(const v4f *)(h + k0 + 4);
+  }
+  const float scale = p.scale ? p.scale[tile.group] : 1.0f;
+  auto turn = [&](v4i (&b)[8], int s) {
+    const int k0 = rank_of(s);
+    const uint16_t *f = p.f + ((int64_t)tile.group * r + min(k0, r - 8)) * p.N + from;
     v4i rows[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) rows[e] = *(const v4i *)(f + (int64_t)e * p.N);
-    transpose8(b[s], rows);
-    if (k0 >= r) {   // (ranks beyond r: h is zero there, and so is the factor, whatever the row that was read holds)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) b[s][j] = v4i{0, 0, 0, 0};
+    for (int e = 0; e < 8; ++e)
+      if (k0 >= r) rows[e] = v4i{0, 0, 0, 0};   // (ranks beyond r: zero, whatever the row that was read holds)
+    transpose8(b, rows);
+  };
+  v4i own[SHARED ? 1 : STEPS][8];
+  if constexpr (SHARED) {
+    for (int s = wave; s < STEPS; s += kExpandWaves) {
+      turn(own[0], s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) turned[(s * 8 + j) * 64 + lane] = own[0][j];
+    }
+    __syncthreads();
+  } else {
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) turn(own[s], s);
+  }
+  if (part0 >= tile.count) return;
+  v4f acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {
+    const int k0 = rank_of(s);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = hp[s][e >> 2][e & 3];
+    for (int q = 1; q < p.splits; ++q) {
+      const float *more = h + (int64_t)q * p.T * r + min(k0, r - 8);
+      const v4f u = *(const v4f *)more, w = *(const v4f *)(more + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += u[e], v[e + 4] += w[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = k0 < r ? v[e] * scale : 0.0f;
+    v4i b[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (SHARED) b[j] = turned[(s * 8 + j) * 64 + lane];
+      else b[j] = own[s][j];
+    }
+    if constexpr (KS) {
+      const v4i hi = pack8(v, false), lo = pack8(v, true);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mfma(hi, b[j], acc[j]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mfma(lo, b[j], acc[j]);
+    } else {
+      const v4i both = g < 2 ? pack8(v, false) : pack8(v, true);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mfma(both, b[j], acc[j]);
     }
   }
-  const float scale = p.scale ? p.scale[tile.group] : 1.0f;
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    if (m * 16 >= tile.count) break;
-    const int64_t mine = p.order[tile.first + min(m * 16 + row, tile.count - 1)];
-    int64_t t[4];
-    v4i y[4];
+  for (int i = 0; i < 4; ++i) {
+    v4i out;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int at = min(m * 16 + g * 4 + i, tile.count - 1);
-      t[i] = p.order[tile.first + at];
-      y[i] = v4i{0, 0, 0, 0};
-      if (p.y) y[i] = *(const v4i *)(p.y + t[i] * p.ldy + (in ? col : 0));
+    for (int k = 0; k < 4; ++k) {
+      const float lo = __uint_as_float((uint32_t)y[i][k] << 16) + acc[2 * k][i], hi = __uint_as_float((uint32_t)y[i][k] & 0xffff0000u) + acc[2 * k + 1][i];
+      out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
     }
-    v4f acc[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const int k0 = KS ? s * 32 + g * 8 : (g & 1) * 8;
-      float v[8];
-      load_h(v, p.h + mine * r + min(k0, r - 8), (int64_t)p.T * r, p.splits, scale);
-      if (k0 >= r) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      }
-      if constexpr (KS) {
-        const v4i hi = pack8(v, false), lo = pack8(v, true);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = mfma(hi, b[s][j], acc[j]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = mfma(lo, b[s][j], acc[j]);
-      } else {
-        const v4i both = g < 2 ? pack8(v, false) : pack8(v, true);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = mfma(both, b[s][j], acc[j]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v4i out;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float lo = __uint_as_float((uint32_t)y[i][k] << 16) + acc[2 * k][i], hi = __uint_as_float((uint32_t)y[i][k] & 0xffff0000u) + acc[2 * k + 1][i];
-        out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
-      }
-      if (in && m * 16 + g * 4 + i < tile.count) *(v4i *)(p.out + t[i] * p.ldo + col) = out;
-    }
+    store(i, out);
   }
 }
 
@@ -364,18 +470,20 @@ struct OuterArgs {
   int T, n, r, size;
 };
 
-constexpr int kOuterWaves = 4, kOuterTokens = 128, kOuterPitch = kOuterTokens + 8;
+constexpr int kOuterWaves = 4;
 
 // Where a tile of a group that has several leaves its sums: the first of a group and the others apart, since a group's last tile and the
 // next group's first may begin within one `size` tokens.
 L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)(first / size) + (piece > 0); }
 
 // RT tiles of 16 ranks by 128 columns a wave, over a tile's tokens.  z is read as `expand` reads the factor: eight neighbouring columns of
-// eight tokens' rows a lane, turned round in registers; h is laid out by rank in LDS, 128 tokens at a time, both halves of its bits.
-template <int RT>
-__global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const OuterArgs p) {
-  __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][kOuterPitch];
-  __shared__ __attribute__((aligned(16))) int toks[kOuterTokens];
+// eight tokens' rows a lane, turned round in registers, 32 tokens requested ahead; h is laid out by rank in LDS, TOKENS at a time, both
+// halves of its bits.
+template <int RT, int TOKENS>
+__global__ __launch_bounds__(kOuterWaves * 64, RT <= 2 ? 2 : 1) void lowrank_outer_kernel(const OuterArgs p) {
+  constexpr int PITCH = TOKENS + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][PITCH];
+  __shared__ __attribute__((aligned(16))) int toks[TOKENS];
   const Tile tile = tile_of(p.starts, p.n, p.size, blockIdx.x);
   if (tile.group >= p.n || (tile.count == 0 && tile.piece > 0)) return;
   const int which = (int)blockIdx.y >= p.side[0].chunks;
@@ -386,6 +494,7 @@ __global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const O
   const int col = (chunk * kOuterWaves + wave) * 128 + row * 8;
   const bool in = col < D;
   const uint16_t *z = sd.z + (in ? col : 0);
+  const int64_t ldz = sd.ldz;
   const float scale = p.scale ? p.scale[tile.group] : 1.0f;
   v4f acc[RT][8];
 #pragma unroll
@@ -393,15 +502,16 @@ __global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const O
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-  for (int p0 = 0; p0 < tile.count; p0 += kOuterTokens) {
-    const int here = min(kOuterTokens, tile.count - p0);
+  for (int p0 = 0; p0 < tile.count; p0 += TOKENS) {
+    const int here = min(TOKENS, tile.count - p0), subs = (here + 31) / 32;
     __syncthreads();
-    for (int i = threadIdx.x; i < kOuterTokens; i += kOuterWaves * 64) toks[i] = p.order[tile.first + p0 + min(i, here - 1)];
-    for (int i = threadIdx.x; i < kOuterTokens * RT * 2; i += kOuterWaves * 64) {   // eight ranks of a token
-      const int at = i / (RT * 2), k = i % (RT * 2) * 8;
+    for (int i = threadIdx.x; i < TOKENS * RT * 2; i += kOuterWaves * 64) {   // eight ranks of a token; neighbouring lanes write neighbouring tokens
+      const int at = i % TOKENS, k = i / TOKENS * 8;
+      const int token = p.order[tile.first + p0 + min(at, here - 1)];
+      if (k == 0) toks[at] = token;
       float v[8];
       if (at < here && rank0 + k < r) {
-        load_h(v, sd.h + (int64_t)p.order[tile.first + p0 + at] * r + rank0 + k, (int64_t)p.T * r, sd.splits, scale);
+        load_h(v, sd.h + (int64_t)token * r + rank0 + k, (int64_t)p.T * r, sd.splits, scale);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = 0.0f;
@@ -414,15 +524,10 @@ __global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const O
     auto request = [&](int s, int sub) {
       const v4i t0 = *(const v4i *)&toks[sub * 32 + g * 8], t1 = *(const v4i *)&toks[sub * 32 + g * 8 + 4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) rows[s][e] = *(const v4i *)(z + (int64_t)(e < 4 ? t0[e & 3] : t1[e & 3]) * sd.ldz);
+      for (int e = 0; e < 8; ++e) rows[s][e] = *(const v4i *)(z + (int64_t)(e < 4 ? t0[e & 3] : t1[e & 3]) * ldz);
     };
-    const int subs = (here + 31) / 32;
-    request(0, 0);
-#pragma unroll
-    for (int sub = 0; sub < kOuterTokens / 32; ++sub) {
-      if (sub >= subs) break;
-      if (sub + 1 < kOuterTokens / 32) request((sub + 1) & 1, min(sub + 1, subs - 1));
-      v4i(&z8)[8] = rows[sub & 1];
+    auto multiply = [&](int s, int sub) {
+      v4i(&z8)[8] = rows[s];
       if (sub * 32 + 32 > here) {   // behind the last token stands the last one again: not a number times zero is no zero
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -438,6 +543,15 @@ __global__ __launch_bounds__(kOuterWaves * 64) void lowrank_outer_kernel(const O
 #pragma unroll
           for (int j = 0; j < 8; ++j) acc[m][j] = mfma(a, b[j], acc[m][j]);
         }
+    };
+    request(0, 0);
+#pragma unroll 1
+    for (int sub = 0; sub < subs; sub += 2) {
+      request(1, min(sub + 1, subs - 1));
+      multiply(0, sub);
+      if (sub + 1 >= subs) break;
+      request(0, min(sub + 2, subs - 1));
+      multiply(1, sub + 1);
     }
   }
   if (!in) return;
@@ -498,7 +612,7 @@ static int64_t tile_slots(int64_t T, int64_t n, int64_t size) { return T / size 
 // Tokens of a tile of the factors' gradients: so many tiles that two workgroups a unit have work.
 static int outer_size(int64_t T, int64_t K, int64_t N) {
   const int64_t chunks = (K + 511) / 512 + (N + 511) / 512, wanted = (2 * (int64_t)num_cus() + chunks - 1) / chunks;
-  int size = kOuterTokens;
+  int size = 128;
   while (size < 2048 && size * wanted < T) size *= 2;
   return size;
 }
@@ -549,63 +663,109 @@ extern "C" int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K) {
   return std::max<int64_t>(1, std::min<int64_t>({num_cus() / tiles, (K + 63) / 64 / (2 * waves), 16}));
 }
 
-extern "C" int l8_lowrank_shrink(const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const int *order, const int *starts,
-                                 float *h, int64_t splits, void *stream) {
-  const char *who = "l8_lowrank_shrink";
-  L8_CALL(check_sizes(who, T, n, r, K));
+namespace l8 {
+
+// Tiles that a launch has numbers for.  (Of few tokens each may be a tile of its own, and there are no unused numbers.)
+static int64_t tiles_of(const Tokens &tk, int64_t T, int64_t n, int64_t size) {
+  const int64_t slots = tile_slots(T, n, size);
+  return tk.order ? slots : std::min(T, slots);
+}
+
+static int shrink_impl(const char *who, const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const Tokens &tk, float *h, int64_t splits,
+                       hipStream_t st) {
   L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
-  if (T == 0) return L8_OK;
-  L8_CALL(check_plan(who, T, order, starts));
   L8_REQUIRE(rows_fit(x, ldx, K) && rows_fit(f, K, K) && h && ((uintptr_t)h % 16) == 0, "%s: null or misaligned operand, or rows off 16-byte lines", who);
-  const int64_t size = tile_tokens(T, n), slots = tile_slots(T, n, size);
-  const ShrinkArgs p{(const uint16_t *)x, (const uint16_t *)f, order, starts, h, ldx, (int)T, (int)K, (int)n, (int)r, (int)splits};
+  const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size);
+  const ShrinkArgs p{(const uint16_t *)x, (const uint16_t *)f, tk, h, ldx, (int)T, (int)K, (int)n, (int)r, (int)splits};
   const unsigned ranks = r <= 64 ? 1 : 2;
-  hipStream_t st = (hipStream_t)stream;
-#define L8_SHRINK(MT, RT, W)                                                                                             \
+#define L8_SHRINK(MT, SUB, RT, W)                                                                                        \
   do {                                                                                                                   \
     L8_CALL(check_grid(who, slots, splits, ranks, W * 64));                                                              \
-    hipLaunchKernelGGL((lowrank_shrink_kernel<MT, RT, W>), dim3((unsigned)slots, (unsigned)splits, ranks), dim3(W * 64), 0, st, p); \
+    hipLaunchKernelGGL((lowrank_shrink_kernel<MT, SUB, RT, W>), dim3((unsigned)slots, (unsigned)splits, ranks), dim3(W * 64), 0, st, p); \
   } while (0)
   if (size == 16) {
-    if (r <= 16) L8_SHRINK(1, 1, 8);
-    else if (r <= 32) L8_SHRINK(1, 2, 8);
-    else L8_SHRINK(1, 4, 8);
+    if (r <= 16) L8_SHRINK(1, 1, 1, 8);
+    else if (r <= 32) L8_SHRINK(1, 1, 2, 8);
+    else L8_SHRINK(1, 1, 4, 8);
   } else {
-    if (r <= 16) L8_SHRINK(4, 1, 4);
-    else if (r <= 32) L8_SHRINK(4, 2, 4);
-    else L8_SHRINK(4, 4, 4);
+    if (r <= 16) L8_SHRINK(4, 1, 1, 8);
+    else if (r <= 32) L8_SHRINK(4, 1, 2, 8);
+    else L8_SHRINK(4, 1, 4, 4);
   }
 #undef L8_SHRINK
   L8_HIP(hipGetLastError());
   return L8_OK;
 }
 
-extern "C" int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
-                                 int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream) {
-  const char *who = "l8_lowrank_expand";
-  L8_CALL(check_sizes(who, T, n, r, N));
+static int expand_impl(const char *who, const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n, int64_t r,
+                       const Tokens &tk, void *out, int64_t ldo, hipStream_t st) {
   L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
-  if (T == 0) return L8_OK;
-  L8_CALL(check_plan(who, T, order, starts));
   L8_REQUIRE((!y || rows_fit(y, ldy, N)) && rows_fit(f, N, N) && rows_fit(out, ldo, N) && h && ((uintptr_t)h % 16) == 0 && ((uintptr_t)scale % 4) == 0,
              "%s: null or misaligned operand, or rows off 16-byte lines", who);
-  const int64_t size = tile_tokens(T, n), slots = tile_slots(T, n, size), chunks = (N + kExpandWaves * 128 - 1) / (kExpandWaves * 128);
-  L8_CALL(check_grid(who, slots, chunks, 1, kExpandWaves * 64));
-  const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, order, starts, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits};
-  const dim3 grid((unsigned)slots, (unsigned)chunks), block(kExpandWaves * 64);
-  hipStream_t st = (hipStream_t)stream;
-#define L8_EXPAND(MT)                                                                                        \
+  const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size), cols = size == 16 ? kExpandWaves * 128 : 128, chunks = (N + cols - 1) / cols;
+  L8_CALL(check_grid(who, slots * chunks, 1, 1, kExpandWaves * 64));
+  const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, tk, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits, (int)chunks};
+  const dim3 grid((unsigned)(slots * chunks)), block(kExpandWaves * 64);
+#define L8_EXPAND(PARTS)                                                                                          \
   do {                                                                                                       \
-    if (r <= 16) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 0>), grid, block, 0, st, p);                  \
-    else if (r <= 32) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 1>), grid, block, 0, st, p);             \
-    else if (r <= 64) hipLaunchKernelGGL((lowrank_expand_kernel<MT, 2>), grid, block, 0, st, p);             \
-    else hipLaunchKernelGGL((lowrank_expand_kernel<MT, 4>), grid, block, 0, st, p);                          \
+    if (r <= 16) hipLaunchKernelGGL((lowrank_expand_kernel<PARTS, 0>), grid, block, 0, st, p);                  \
+    else if (r <= 32) hipLaunchKernelGGL((lowrank_expand_kernel<PARTS, 1>), grid, block, 0, st, p);             \
+    else if (r <= 64) hipLaunchKernelGGL((lowrank_expand_kernel<PARTS, 2>), grid, block, 0, st, p);             \
+    else hipLaunchKernelGGL((lowrank_expand_kernel<PARTS, 4>), grid, block, 0, st, p);                          \
   } while (0)
   if (size == 16) L8_EXPAND(1);
   else L8_EXPAND(4);
 #undef L8_EXPAND
   L8_HIP(hipGetLastError());
   return L8_OK;
+}
+
+}  // namespace l8
+
+extern "C" int l8_lowrank_shrink(const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const int *order, const int *starts,
+                                 float *h, int64_t splits, void *stream) {
+  const char *who = "l8_lowrank_shrink";
+  L8_CALL(check_sizes(who, T, n, r, K));
+  if (T == 0) return L8_OK;
+  L8_CALL(check_plan(who, T, order, starts));
+  return shrink_impl(who, x, T, K, ldx, f, n, r, Tokens{order, starts, nullptr, 0}, h, splits, (hipStream_t)stream);
+}
+
+extern "C" int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
+                                 int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream) {
+  const char *who = "l8_lowrank_expand";
+  L8_CALL(check_sizes(who, T, n, r, N));
+  if (T == 0) return L8_OK;
+  L8_CALL(check_plan(who, T, order, starts));
+  return expand_impl(who, y, ldy, h, splits, scale, f, T, N, n, r, Tokens{order, starts, nullptr, 0}, out, ldo, (hipStream_t)stream);
+}
+
+extern "C" int64_t l8_lowrank_add_workspace(int64_t T, int64_t K, int64_t n, int64_t r) {
+  if (T <= 0 || K <= 0 || n <= 0 || r <= 0) return 0;
+  const int64_t plan = T <= kFewTokens ? 0 : (T + n + 3 + 3) / 4 * 16;
+  return plan + l8_lowrank_splits(T, n, K) * T * r * (int64_t)sizeof(float);
+}
+
+extern "C" int l8_lowrank_add(const void *y, int64_t ldy, const void *x, int64_t ldx, const void *a, const void *b, const float *scale, const void *index, int index_is_i64,
+                              int64_t T, int64_t K, int64_t N, int64_t n, int64_t r, void *out, int64_t ldo, void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *who = "l8_lowrank_add";
+  L8_CALL(check_sizes(who, T, n, r, K));
+  L8_CALL(check_sizes(who, T, n, r, N));
+  if (T == 0) return L8_OK;
+  const int64_t need = l8_lowrank_add_workspace(T, K, n, r), splits = l8_lowrank_splits(T, n, K);
+  L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+  L8_REQUIRE(index && ((uintptr_t)index % (index_is_i64 ? 8 : 4)) == 0, "%s: null or misaligned index", who);
+  L8_REQUIRE(rows_fit(b, N, N) && rows_fit(out, ldo, N) && (!y || rows_fit(y, ldy, N)), "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  float *h = (float *)workspace;
+  Tokens tk{nullptr, nullptr, index, index_is_i64};
+  if (T > kFewTokens) {
+    int *starts = (int *)workspace, *order = starts + n + 3;
+    h = (float *)workspace + (T + n + 3 + 3) / 4 * 4;
+    L8_CALL(l8_lowrank_route(index, index_is_i64, T, n, order, starts, stream));
+    tk = Tokens{order, starts, nullptr, 0};
+  }
+  L8_CALL(shrink_impl(who, x, T, K, ldx, a, n, r, tk, h, splits, (hipStream_t)stream));
+  return expand_impl(who, y, ldy, h, splits, scale, b, T, N, n, r, tk, out, ldo, (hipStream_t)stream);
 }
 
 extern "C" int64_t l8_lowrank_outer_workspace(int64_t T, int64_t r, int64_t K, int64_t N) {
@@ -643,9 +803,9 @@ extern "C" int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, 
   L8_CALL(check_grid(who, slots, chunks, ranks, kOuterWaves * 64));
   const dim3 grid((unsigned)slots, (unsigned)chunks, (unsigned)ranks), block(kOuterWaves * 64);
   hipStream_t st = (hipStream_t)stream;
-  if (r <= 16) hipLaunchKernelGGL(lowrank_outer_kernel<1>, grid, block, 0, st, p);
-  else if (r <= 32) hipLaunchKernelGGL(lowrank_outer_kernel<2>, grid, block, 0, st, p);
-  else hipLaunchKernelGGL(lowrank_outer_kernel<4>, grid, block, 0, st, p);
+  if (r <= 16) hipLaunchKernelGGL((lowrank_outer_kernel<1, 256>), grid, block, 0, st, p);
+  else if (r <= 32) hipLaunchKernelGGL((lowrank_outer_kernel<2, 256>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((lowrank_outer_kernel<4, 128>), grid, block, 0, st, p);
   L8_HIP(hipGetLastError());
   if (parts) {
     const int64_t b0 = (r * D[0] + 2047) / 2048, b1 = (r * D[1] + 2047) / 2048;

@@ -1137,6 +1137,29 @@ def lowrank_expand(y: Optional[torch.Tensor], h: torch.Tensor, f: torch.Tensor, 
     return out
 
 
+def lowrank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, index: torch.Tensor, scale: Optional[torch.Tensor] = None):
+    """``lowrank_expand(y, lowrank_shrink(x, a, plan), b, scale, plan)`` with the order of an int32 or int64 index [T], in one call: where no
+    gradient is wanted."""
+    what = "lowrank_add"
+    y, x = _rows_on_lines(y, torch.bfloat16, what), _rows_on_lines(x, torch.bfloat16, what)
+    a, b = _factor(a, what), _factor(b, what)
+    st = _prep(x, what)
+    (T, K), (n, r, _), N, dev = x.shape, a.shape, b.shape[2], x.device
+    if a.shape[2] != K or b.shape[:2] != (n, r) or y.shape != (T, N) or any(t.device != dev for t in (y, a, b, index)):
+        raise RuntimeError(f"{what}: operands {tuple(y.shape)}, {tuple(x.shape)}, {tuple(a.shape)} and {tuple(b.shape)} do not fit or are not on one device")
+    if index.dtype not in (torch.int32, torch.int64) or index.shape != (T,):
+        raise RuntimeError(f"{what}: an int32 or int64 index of {T} tokens is wanted, got {index.dtype} {tuple(index.shape)}")
+    index, scale = index.contiguous(), _scale_arg(scale, n, dev, what)
+    out = torch.empty((T, N), dtype=torch.bfloat16, device=dev)
+    with _timed(what, 2 * T * (K + 2 * N) + 2 * a.numel() + 2 * b.numel(), dev):
+        need = _lib.load().l8_lowrank_add_workspace(T, K, n, r)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        code = _lib.load().l8_lowrank_add(y.data_ptr(), _ld(y), x.data_ptr(), _ld(x), a.data_ptr(), b.data_ptr(), _addr(scale) or None, index.data_ptr(),
+                                          int(index.dtype == torch.int64), T, K, N, n, r, out.data_ptr(), N, _addr(ws) or None, need, st)
+    _lib.check(code, "l8_lowrank_add")
+    return out
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
     """Do two matrices of dense rows lie in one stretch of memory?"""
     if not a.numel() or not b.numel():
