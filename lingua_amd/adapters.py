@@ -16,7 +16,7 @@ from typing import Optional, Union
 
 import torch
 
-from . import ops
+from . import _lib, ops
 from . import float8 as f8
 
 
@@ -86,6 +86,12 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     ``scale``  fp32 [n], or None for ones; no gradient flows to it
     """
     what = "add_lowrank"
+    planned = isinstance(index, Plan)
+    if f8._native_call(x, 0) and f8._plain_call() and (not planned or (index.n == a.shape[0] and index.shape == x.shape[:-1])):
+        at = (None, index.order, index.starts) if planned else (index, None, None)
+        out = _lib.native_for(x.get_device()).add_lowrank(y, x, a, b, scale, *at)
+        if out is not None:
+            return out
     if a.dim() != 3 or b.dim() != 3 or a.shape[:2] != b.shape[:2] or x.dim() < 1 or y.dim() < 1 or x.shape[-1] != a.shape[2] or y.shape[-1] != b.shape[2]:
         raise RuntimeError(f"{what}: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit an input {tuple(x.shape)} and an output {tuple(y.shape)}")
     for t in (y, x, a, b):
@@ -97,17 +103,17 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
         raise RuntimeError(f"{what}: a rank that is a multiple of 8 up to 128 and features that are multiples of 8 are wanted, got {tuple(a.shape)} and {tuple(b.shape)}")
     if x.shape[:-1] != y.shape[:-1] or tuple(index.shape) != x.shape[:-1]:
         raise RuntimeError(f"{what}: x {tuple(x.shape)}, y {tuple(y.shape)} and the index {tuple(index.shape)} are not of the same tokens")
-    if isinstance(index, Plan):
+    if planned:
         if index.n != a.shape[0]:
             raise RuntimeError(f"{what}: the plan is for {index.n} adapters, the bank holds {a.shape[0]}")
     elif index.device != x.device:
         raise RuntimeError(f"{what}: the index is on {index.device}, the operands on {x.device}")
     f8._refuse_captured(y, x, a, what)
     f8._refuse_captured(b, None, None, what)
-    if not isinstance(index, Plan) and not (torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, a, b))) and f8._plain_call():
+    if not planned and not (torch.is_grad_enabled() and any(t.requires_grad for t in (y, x, a, b))) and f8._plain_call():
         out = ops.lowrank_add(y.reshape(-1, y.shape[-1]), x.reshape(-1, x.shape[-1]), a, b, index.flatten(), scale)
         return out.view(y.shape)
-    plan = index if isinstance(index, Plan) else route(index, a.shape[0])
+    plan = index if planned else route(index, a.shape[0])
     if y.dim() == 2:
         return LowRankFn.apply(y, x, a, b, scale, plan.order, plan.starts)
     tokens = y.shape[:-1]

@@ -35,6 +35,8 @@ struct Library {
   X(l8_cast_rowwise_many) X(l8_cast_rowwise_cols_many) X(l8_gemm_nt_multi) X(l8_gemm_nt_sum) X(l8_rmsnorm_cast_rowwise)            \
   X(l8_rmsnorm_workspace) X(l8_rmsnorm_bwd_as) X(l8_rmsnorm_bwd_workspace) X(l8_swiglu_cast_rowwise) X(l8_swiglu_workspace)        \
   X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed) X(l8_add_rmsnorm_cast_rowwise) X(l8_add_rmsnorm_bwd) X(l8_rotary)     \
+  X(l8_rotary_axes) X(l8_dropout) X(l8_norm_fwd) X(l8_norm_bwd) X(l8_norm_bwd_workspace) X(l8_lowrank_route) X(l8_lowrank_shrink) X(l8_lowrank_splits)   \
+  X(l8_lowrank_expand) X(l8_lowrank_outer) X(l8_lowrank_outer_workspace) X(l8_lowrank_add) X(l8_lowrank_add_workspace)                   \
   X(l8_cast_mxfp4) X(l8_cast_mxfp4_two) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
   L8_ENTRIES(L8_ENTRY)
 #undef L8_ENTRY
@@ -995,15 +997,18 @@ PyObject *add_rmsnorm(PyObject *, PyObject *const *args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// Pairs that each axis of a position turns (none: one position a token), side by side or in turn.
+struct Axes {
+  std::vector<int64_t> sections;
+  bool in_rounds = false;
+};
 // Both forms of a rotation: y of x, either of them possibly undefined.
-void rotate(const Tensor (&x)[2], Tensor (&y)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves, bool inverse) {
+void rotate(const Tensor (&x)[2], Tensor (&y)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves, bool inverse, const Axes &axes) {
   const Tensor &one = x[0].defined() ? x[0] : x[1];
   const int64_t B = one.size(0), S = one.size(1), D = one.size(3);
-  int64_t pos_b = 0, pos_s = 0;
-  if (pos.defined()) {
-    pos_s = pos.size(-1) == 1 ? 0 : pos.stride(-1);
-    pos_b = pos.dim() == 1 || pos.size(0) == 1 ? 0 : pos.stride(0);
-  }
+  int64_t at[3] = {0, 0, 0};   // strides of a position: axis, batch, token
+  if (pos.defined())
+    for (int64_t i = 0; i < pos.dim(); ++i) at[3 - pos.dim() + i] = pos.size(i) == 1 ? 0 : pos.stride(i);
   l8_rotary_operand two[2];
   for (int i = 0; i < 2; ++i) {
     two[i] = {nullptr, nullptr, 0, 0, 0, 0};
@@ -1011,8 +1016,14 @@ void rotate(const Tensor (&x)[2], Tensor (&y)[2], const Tensor &cos, const Tenso
     y[i] = at::empty(x[i].sizes(), x[i].options());
     two[i] = {x[i].const_data_ptr(), y[i].mutable_data_ptr(), x[i].size(2), x[i].stride(0), x[i].stride(1), x[i].stride(2)};
   }
-  check(lib.l8_rotary(two, B, S, D, 2 * cos.size(1), in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), cos.size(0),
-                      pos.defined() ? pos.const_data_ptr() : nullptr, pos.defined() && pos.scalar_type() == at::kInt, pos_b, pos_s, stream_of(one.get_device())), "l8_rotary");
+  const void *pos_p = pos.defined() ? pos.const_data_ptr() : nullptr;
+  const bool i32 = pos.defined() && pos.scalar_type() == at::kInt;
+  if (axes.sections.empty())
+    check(lib.l8_rotary(two, B, S, D, 2 * cos.size(1), in_halves, inverse, cos.const_data_ptr<float>(), sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), cos.size(0),
+                        pos_p, i32, at[1], at[2], stream_of(one.get_device())), "l8_rotary");
+  else
+    check(lib.l8_rotary_axes(two, B, S, D, axes.sections.data(), (int64_t)axes.sections.size(), axes.in_rounds, in_halves, inverse, cos.const_data_ptr<float>(),
+                             sin.const_data_ptr<float>(), cos.stride(0), cos.stride(1), cos.size(0), pos_p, i32, at[0], at[1], at[2], stream_of(one.get_device())), "l8_rotary_axes");
 }
 // Dense heads, and for the interleaved layout pairs on 4-byte lines?
 bool heads_fit(const Tensor &t, bool in_halves) {
@@ -1024,7 +1035,7 @@ bool heads_fit(const Tensor &t, bool in_halves) {
   return (odd & 1) == 0;
 }
 // May the extension take these operands?
-bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves) {
+bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const Tensor &pos, bool in_halves, const Axes &axes) {
   const Tensor &one = x[0].defined() ? x[0] : x[1];
   if (!one.is_cuda() || one.dim() != 4) return false;
   const int device = one.get_device();
@@ -1040,24 +1051,37 @@ bool rotates(const Tensor (&x)[2], const Tensor &cos, const Tensor &sin, const T
       return false;
   const int64_t P = cos.size(0), rot = 2 * cos.size(1);
   if (rot < 2 || rot > D || (!pos.defined() && S > P)) return false;
-  if (pos.defined()) {   // [S], [1], [1,S], [B,1] or [B,S]
+  const int64_t count = (int64_t)axes.sections.size();
+  if (count) {
+    int64_t pairs = 0;
+    for (const int64_t n : axes.sections) {
+      if (n < 0 || n > 256) return false;
+      pairs += n;
+    }
+    if (count > 4 || 2 * pairs != rot || !pos.defined()) return false;
+  }
+  if (pos.defined()) {   // broadcastable to [B,S], with axes to [axes,B,S]
     if ((pos.scalar_type() != at::kInt && pos.scalar_type() != at::kLong) || pos.layout() != at::kStrided || !pos.is_cuda() || pos.get_device() != device ||
-        pos.dim() < 1 || pos.dim() > 2)
+        pos.dim() < 1 || pos.dim() > (count ? 3 : 2))
       return false;
-    const int64_t ps = pos.size(-1), pb = pos.dim() == 2 ? pos.size(0) : 1;
-    if ((ps != S && ps != 1) || (pb != B && pb != 1)) return false;
+    const int64_t whole[3] = {count, B, S};
+    for (int64_t i = 0; i < pos.dim(); ++i)
+      if (pos.size(i) != 1 && pos.size(i) != whole[3 - pos.dim() + i]) return false;
   }
   return true;
 }
 
 struct Rotary : torch::autograd::Function<Rotary> {
-  static variable_list forward(AutogradContext *ctx, const Tensor &xq, const Tensor &xk, const Tensor &cos, const Tensor &sin, const std::optional<Tensor> &at, bool in_halves) {
+  static variable_list forward(AutogradContext *ctx, const Tensor &xq, const Tensor &xk, const Tensor &cos, const Tensor &sin, const std::optional<Tensor> &at, bool in_halves,
+                               std::vector<int64_t> sections, bool in_rounds) {
     const Tensor x[2] = {xq, xk}, pos = at.value_or(Tensor());
     Tensor y[2];
-    rotate(x, y, cos, sin, pos, in_halves, false);
+    rotate(x, y, cos, sin, pos, in_halves, false, Axes{sections, in_rounds});
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({cos, sin, pos});
     ctx->saved_data["half"] = in_halves;
+    ctx->saved_data["sections"] = sections;
+    ctx->saved_data["rounds"] = in_rounds;
     return {y[0], y[1]};
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
@@ -1072,9 +1096,10 @@ struct Rotary : torch::autograd::Function<Rotary> {
       const c10::DeviceGuard guard((x[0].defined() ? x[0] : x[1]).device());
       const Tensor in[2] = {x[0], x[1]};
       const bool alike = saved[0].strides() == saved[1].strides();   // (hooks may have handed one back in another layout)
-      rotate(in, g, alike ? saved[0] : saved[0].contiguous(), alike ? saved[1] : saved[1].contiguous(), saved[2], ctx->saved_data["half"].toBool(), true);
+      rotate(in, g, alike ? saved[0] : saved[0].contiguous(), alike ? saved[1] : saved[1].contiguous(), saved[2], ctx->saved_data["half"].toBool(), true,
+             Axes{ctx->saved_data["sections"].toIntVector(), ctx->saved_data["rounds"].toBool()});
     }
-    return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor()}, {learns(grads[0]), learns(grads[1])}, "rotary");
+    return once({g[0], g[1], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, {learns(grads[0]), learns(grads[1])}, "rotary");
   }
 };
 
@@ -1086,32 +1111,407 @@ PyObject *rotary(PyObject *, PyObject *const *args, Py_ssize_t n) {
   const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
   const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
   const bool in_halves = truth(args[5]), inverse = truth(args[6]);
-  if (!rotates(x, cos, sin, pos, in_halves)) Py_RETURN_NONE;
+  const Axes axes;
+  if (!rotates(x, cos, sin, pos, in_halves, axes)) Py_RETURN_NONE;
   Tensor y[2];
   {
     pybind11::gil_scoped_release no_gil;
-    rotate(x, y, cos, sin, pos, in_halves, inverse);
+    rotate(x, y, cos, sin, pos, in_halves, inverse, axes);
   }
   return tuple_of({y[0], y[1]});
   END_HANDLE_TH_ERRORS
 }
 
-// rotary_pair(xq, xk, cos, sin, positions, in_halves) -> (yq, yk), differentiable, or None
+// rotary_pair(xq, xk, cos, sin, positions, in_halves[, sections, in_rounds]) -> (yq, yk), differentiable, or None
 PyObject *rotary_pair(PyObject *, PyObject *const *args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 6) throw std::runtime_error("rotary_pair: 6 arguments");
+  if (n != 6 && n != 8) throw std::runtime_error("rotary_pair: 6 or 8 arguments");
   if (!tensors(args, 5) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
   const Tensor x[2] = {arg(args[0]), arg(args[1])}, pos = arg(args[4]);
   const Tensor &cos = THPVariable_Unpack(args[2]), &sin = THPVariable_Unpack(args[3]);
   const bool in_halves = truth(args[5]);
-  if (!rotates(x, cos, sin, pos, in_halves)) Py_RETURN_NONE;
+  Axes axes;
+  if (n == 8) {
+    if (!PyTuple_Check(args[6]) || PyTuple_GET_SIZE(args[6]) < 1) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(args[6]); ++i) {
+      axes.sections.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(args[6], i)));
+      if (axes.sections.back() == -1 && PyErr_Occurred()) throw python_error();
+    }
+    axes.in_rounds = truth(args[7]);
+  }
+  if (!rotates(x, cos, sin, pos, in_halves, axes)) Py_RETURN_NONE;
   variable_list y;
   {
     pybind11::gil_scoped_release no_gil;
-    if (at::GradMode::is_enabled()) refuse_captured({&x[0], &x[1]}, "rotary");
-    y = Rotary::apply(x[0], x[1], cos, sin, pos.defined() ? std::optional<Tensor>(pos) : std::nullopt, in_halves);
+    if (at::GradMode::is_enabled()) refuse_captured({&x[0], &x[1]}, n == 8 ? "rotary_axes" : "rotary");
+    y = Rotary::apply(x[0], x[1], cos, sin, pos.defined() ? std::optional<Tensor>(pos) : std::nullopt, in_halves, axes.sections, axes.in_rounds);
   }
   return tuple_of({y[0], y[1]});
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- layer norm, dropout ----
+
+// What is dropped of an operand: seed and step, and which call of the step.
+struct Dropped {
+  Tensor numbers;   // undefined: nothing
+  int64_t site = 0, threshold = 0;
+  const int64_t *p() const { return numbers.defined() ? numbers.const_data_ptr<int64_t>() : nullptr; }
+};
+std::optional<Tensor> maybe(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+int64_t number(PyObject *o) {
+  const int64_t v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) throw python_error();
+  return v;
+}
+bool is_param(const Tensor &t, int64_t n, int device) { return !t.defined() || dense(t, t.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16, n, device); }
+bool is_numbers(const Tensor &t, int device) { return !t.defined() || (t.dim() == 1 && dense(t, at::kLong, 2, device)); }
+void *addr(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+const void *caddr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+
+struct NormOut {
+  Tensor h, y, q, s, stats, col;
+};
+NormOut norm_pass(const Tensor &x, const Tensor &res, const Tensor &w, const Tensor &b, const Dropped &drop, double eps, bool centred, bool want_q, bool want_col, bool want_stats,
+                  bool on_lines) {
+  const Rows rx = rows_of(x), rr = res.defined() ? rows_of(res) : Rows();
+  const int64_t R = rx.rows, C = rx.cols;
+  const auto o = x.options(), f32 = o.dtype(at::kFloat);
+  NormOut out;
+  if (res.defined()) out.h = at::empty(x.sizes(), o);
+  out.y = at::empty(x.sizes(), o);
+  if (want_q) out.q = empty_fp8(R, C, o, on_lines), out.s = at::empty({R, 1}, f32);
+  if (want_stats) out.stats = at::empty({2, R}, f32);
+  if (want_col) out.col = at::empty({C}, f32);
+  const int64_t ws_bytes = want_col ? lib.l8_rmsnorm_workspace(R, C) : 0;
+  const Space ws(x, ws_bytes);
+  float *stats = want_stats ? out.stats.mutable_data_ptr<float>() : nullptr;
+  const l8_norm_fwd_args a{rx.p, rr.p, caddr(w), caddr(b), w.defined() && w.scalar_type() == at::kFloat, b.defined() && b.scalar_type() == at::kFloat, centred, R, C, rx.ld, rr.ld, eps,
+                           drop.p(), drop.site, drop.threshold, addr(out.h), C, addr(out.y), C, addr(out.q), want_q ? out.q.stride(0) : 0, (float *)addr(out.s), stats,
+                           stats ? stats + R : nullptr, (float *)addr(out.col), ws.p(), ws_bytes, stream_of(x.get_device())};
+  check(lib.l8_norm_fwd(&a), "l8_norm_fwd");
+  return out;
+}
+
+struct Norm : torch::autograd::Function<Norm> {
+  static const char *name(bool centred, bool added) { return !centred ? "add_rmsnorm" : added ? "add_layernorm" : "layernorm"; }
+  // -> [h,] y[, q, scale[, col amax]]
+  static variable_list forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &res, const std::optional<Tensor> &w, const std::optional<Tensor> &b,
+                               const std::optional<Tensor> &numbers, int64_t site, int64_t threshold, double eps, bool centred, bool want_col, bool quantise) {
+    const Tensor none;
+    const Tensor &r = res ? *res : none, &wt = w ? *w : none, &bt = b ? *b : none, &n = numbers ? *numbers : none;
+    const NormOut out = norm_pass(x, r, wt, bt, Dropped{n, site, threshold}, eps, centred, quantise, want_col, true, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({r.defined() ? out.h : x, wt, out.stats, n});
+    ctx->saved_data["sum learns"] = learns(x) || learns(r);
+    ctx->saved_data["centred"] = centred;
+    ctx->saved_data["has"] = (int64_t)(r.defined() | (wt.defined() << 1) | (bt.defined() << 2));
+    ctx->saved_data["b"] = bt.defined() ? (int64_t)bt.scalar_type() : (int64_t)0;
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["threshold"] = threshold;
+    variable_list all;
+    if (r.defined()) all.push_back(out.h);
+    all.push_back(out.y);
+    const size_t learn = all.size();
+    if (quantise) all.insert(all.end(), {out.q, out.s});
+    if (want_col) all.push_back(out.col);
+    ctx->mark_non_differentiable({all.begin() + learn, all.end()});
+    return all;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const int64_t has = ctx->saved_data["has"].toInt();
+    const bool added = has & 1, has_w = has & 2, has_b = has & 4, centred = ctx->saved_data["centred"].toBool();
+    const char *what = name(centred, added);
+    const Tensor gh_in = added ? grads[0] : Tensor(), gy_in = grads[added ? 1 : 0];
+    for (const Tensor *g : {&gh_in, &gy_in}) TORCH_CHECK(!g->defined() || g->scalar_type() == at::kBFloat16, what, " backward: bf16 gradients required, got ", g->scalar_type());
+    // (asked for operand by operand, in the order in which those that are there were given)
+    int at = 0;
+    const bool need_x = ctx->needs_input_grad(at++), need_r = added && ctx->needs_input_grad(at++);
+    const bool need_w = has_w && ctx->needs_input_grad(at++), need_b = has_b && ctx->needs_input_grad(at++);
+    const Dropped drop{saved[3], ctx->saved_data["site"].toInt(), ctx->saved_data["threshold"].toInt()};
+    Tensor gx, gres, gw, gb;
+    auto all = [&](std::initializer_list<bool> varies) {
+      return once({gx, gres, gw, gb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, varies, what);
+    };
+    if (!gy_in.defined()) {   // only the sum was used, if anything
+      if (!gh_in.defined()) return all({});
+      gx = need_x ? gh_in : Tensor();
+      if (gx.defined() && drop.numbers.defined()) {
+        const c10::DeviceGuard guard(gh_in.device());
+        const Tensor g = gh_in.contiguous(), numbers = drop.numbers.contiguous();
+        gx = at::empty(g.sizes(), g.options());
+        check(lib.l8_dropout(g.const_data_ptr(), nullptr, gx.mutable_data_ptr(), g.numel(), numbers.const_data_ptr<int64_t>(), drop.site, drop.threshold, stream_of(g.get_device())),
+              "l8_dropout");
+        variable_list one = once({gx}, {learns(gh_in)}, what);
+        gx = one[0];
+      }
+      gres = need_r ? gh_in : Tensor();
+      return {gx, gres, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+    const Tensor h = aligned_rows(saved[0]), w = saved[1].defined() ? saved[1].contiguous() : Tensor(), stats = saved[2].contiguous(),
+                 numbers = saved[3].defined() ? saved[3].contiguous() : Tensor();
+    const Tensor gy = gradient(gy_in, what), gh = gh_in.defined() ? gradient(gh_in, what) : Tensor();
+    const Rows rh = rows_of(h), rg = rows_of(gy), ru = gh.defined() ? rows_of(gh) : Rows();
+    const int64_t R = rh.rows, C = rh.cols;
+    const int device = h.get_device();
+    const c10::DeviceGuard guard(h.device());
+    const auto o = h.options();
+    gx = at::empty(h.sizes(), o);
+    if (numbers.defined()) gres = at::empty(h.sizes(), o);
+    if (need_w) gw = at::empty({C}, w.options());
+    if (need_b) gb = at::empty({C}, o.dtype((at::ScalarType)ctx->saved_data["b"].toInt()));
+    const int64_t ws_bytes = need_w || need_b ? lib.l8_norm_bwd_workspace(R, C, centred) : 0;
+    const Space ws(h, ws_bytes);
+    const float *st = stats.const_data_ptr<float>();
+    const l8_norm_bwd_args a{rg.p, ru.p, rh.p, caddr(w), w.defined() && w.scalar_type() == at::kFloat, centred, R, C, rg.ld, ru.ld, rh.ld, st, st + R,
+                             numbers.defined() ? numbers.const_data_ptr<int64_t>() : nullptr, drop.site, drop.threshold, addr(gx), C, addr(gres), C, addr(gw),
+                             gw.defined() && gw.scalar_type() == at::kFloat, addr(gb), gb.defined() && gb.scalar_type() == at::kFloat, ws.p(), ws_bytes, stream_of(device)};
+    check(lib.l8_norm_bwd(&a), "l8_norm_bwd");
+    if (!numbers.defined()) gres = gx;
+    if (!need_x) gx = Tensor();
+    if (!need_r) gres = Tensor();
+    const bool sum_learns = ctx->saved_data["sum learns"].toBool(), gy_learns = learns(gy_in), varies = sum_learns || learns(saved[1]) || learns(gh_in) || gy_learns;
+    return all({varies, varies, sum_learns || gy_learns, gy_learns});
+  }
+};
+
+bool norm_takes(const Tensor &x, const Tensor &res, const Tensor &w, const Tensor &b, const Tensor &numbers) {
+  if (!x.is_cuda()) return false;
+  const int device = x.get_device();
+  Rows rx, rr;
+  return as_rows(x, device, rx) && on_16_bytes(rx) && (!res.defined() || (as_rows(res, device, rr) && on_16_bytes(rr) && res.sizes() == x.sizes())) &&
+         is_param(w, rx.cols, device) && is_param(b, rx.cols, device) && is_numbers(numbers, device) && c10::hip::current_device() == device;
+}
+
+// norm(x, residual, weight, bias, numbers, site, threshold, eps, centred, want_col, quantise) -> (h, y, q, scale, col amax), differentiable, or None
+PyObject *norm(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 11) throw std::runtime_error("norm: 11 arguments");
+  if (!tensors(args, 5) || args[0] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]);
+  const Tensor res = arg(args[1]), w = arg(args[2]), b = arg(args[3]), numbers = arg(args[4]);
+  const int64_t site = number(args[5]), threshold = number(args[6]);
+  const double eps = PyFloat_AsDouble(args[7]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  const bool centred = truth(args[8]), want_col = truth(args[9]), quantise = truth(args[10]);
+  if (!norm_takes(x, res, w, b, numbers)) Py_RETURN_NONE;
+  variable_list out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (at::GradMode::is_enabled()) refuse_captured({&x, &res, &w, &b}, Norm::name(centred, res.defined()));
+    out = Norm::apply(x, maybe(res), maybe(w), maybe(b), maybe(numbers), site, threshold, eps, centred, want_col, quantise);
+  }
+  const size_t y = res.defined();
+  return tuple_of({y ? out[0] : Tensor(), out[y], quantise ? out[y + 1] : Tensor(), quantise ? out[y + 2] : Tensor(), want_col ? out[y + 3] : Tensor()});
+  END_HANDLE_TH_ERRORS
+}
+
+// norm_fwd(x, residual, weight, bias, numbers, site, threshold, eps, centred, want_q, want_stats, on_lines) -> (h, y, q, scale, stats) or None
+PyObject *norm_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 12) throw std::runtime_error("norm_fwd: 12 arguments");
+  if (!tensors(args, 5) || args[0] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]);
+  const Tensor res = arg(args[1]), w = arg(args[2]), b = arg(args[3]), numbers = arg(args[4]);
+  const int64_t site = number(args[5]), threshold = number(args[6]);
+  const double eps = PyFloat_AsDouble(args[7]);
+  if (eps == -1.0 && PyErr_Occurred()) throw python_error();
+  const bool centred = truth(args[8]), want_q = truth(args[9]), want_stats = truth(args[10]), on_lines = truth(args[11]);
+  if (x.dim() != 2 || !norm_takes(x, res, w, b, numbers)) Py_RETURN_NONE;
+  NormOut out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    out = norm_pass(x, res, w, b, Dropped{numbers, site, threshold}, eps, centred, want_q, false, want_stats, on_lines);
+  }
+  return tuple_of({out.h, out.y, out.q, out.s, out.stats});
+  END_HANDLE_TH_ERRORS
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static Tensor pass(const Tensor &x, const Tensor &res, const Tensor &numbers, int64_t site, int64_t threshold) {
+    const Tensor y = at::empty(x.sizes(), x.options());
+    check(lib.l8_dropout(x.const_data_ptr(), caddr(res), y.mutable_data_ptr(), x.numel(), numbers.const_data_ptr<int64_t>(), site, threshold, stream_of(x.get_device())), "l8_dropout");
+    return y;
+  }
+  static Tensor forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &res, const Tensor &numbers, int64_t site, int64_t threshold) {
+    ctx->save_for_backward({numbers});
+    ctx->saved_data["site"] = site;
+    ctx->saved_data["threshold"] = threshold;
+    ctx->saved_data["added"] = res.has_value();
+    return pass(x, res.value_or(Tensor()), numbers, site, threshold);
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const Tensor &g = grads[0];
+    TORCH_CHECK(g.scalar_type() == at::kBFloat16, "dropout backward: bf16 gradients required, got ", g.scalar_type());
+    const Tensor numbers = ctx->get_saved_variables()[0].contiguous();
+    const bool added = ctx->saved_data["added"].toBool();
+    Tensor gx;
+    if (ctx->needs_input_grad(0)) {
+      const c10::DeviceGuard guard(g.device());
+      gx = once({pass(g.contiguous(), Tensor(), numbers, ctx->saved_data["site"].toInt(), ctx->saved_data["threshold"].toInt())}, {learns(g)}, "dropout")[0];
+    }
+    return {gx, added && ctx->needs_input_grad(1) ? g : Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// dropout(x, residual, numbers, site, threshold) -> y, differentiable, or None
+PyObject *dropout(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 5) throw std::runtime_error("dropout: 5 arguments");
+  if (!tensors(args, 3) || args[0] == Py_None || args[2] == Py_None) Py_RETURN_NONE;
+  const Tensor &x = THPVariable_Unpack(args[0]), &numbers = THPVariable_Unpack(args[2]);
+  const Tensor res = arg(args[1]);
+  const int64_t site = number(args[3]), threshold = number(args[4]);
+  if (!x.is_cuda() || x.numel() < 1) Py_RETURN_NONE;
+  const int device = x.get_device();
+  if (!dense(x, at::kBFloat16, x.numel(), device) || (res.defined() && (!dense(res, at::kBFloat16, x.numel(), device) || res.sizes() != x.sizes())) || !is_numbers(numbers, device) ||
+      c10::hip::current_device() != device)
+    Py_RETURN_NONE;
+  Tensor y;
+  {
+    pybind11::gil_scoped_release no_gil;
+    if (at::GradMode::is_enabled()) refuse_captured({&x, &res}, res.defined() ? "dropout_add" : "dropout");
+    y = Dropout::apply(x, maybe(res), numbers, site, threshold);
+  }
+  return wrap(y);
+  END_HANDLE_TH_ERRORS
+}
+
+// ---- low-rank adapters ----
+
+struct Bank {   // one factor, and whoever reads it
+  const void *p;
+  int64_t n, r, cols;
+};
+bool as_bank(const Tensor &t, int device, Bank &f) {
+  if (!t.defined() || t.dim() != 3 || t.numel() < 1 || !dense(t, at::kBFloat16, t.numel(), device) || ((uintptr_t)t.const_data_ptr() % 16) != 0) return false;
+  f = {t.const_data_ptr(), t.size(0), t.size(1), t.size(2)};
+  return f.r % 8 == 0 && f.r >= 8 && f.r <= 128 && f.cols % 8 == 0;
+}
+// Factors as hooks on saved tensors may hand them back: dense and on 16-byte lines, or a copy that is.
+Tensor bank_rows(const Tensor &t) {
+  const Tensor c = t.contiguous();
+  return ((uintptr_t)c.const_data_ptr() % 16) == 0 ? c : c.clone();
+}
+Tensor lowrank_h(const Rows &x, const Tensor &like, const Bank &f, const Tensor &order, const Tensor &starts, void *stream) {
+  const int64_t splits = lib.l8_lowrank_splits(x.rows, f.n, f.cols);
+  const Tensor h = at::empty({splits, x.rows, f.r}, like.options().dtype(at::kFloat));
+  check(lib.l8_lowrank_shrink(x.p, x.rows, f.cols, x.ld, f.p, f.n, f.r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), h.mutable_data_ptr<float>(), splits, stream),
+        "l8_lowrank_shrink");
+  return h;
+}
+void lowrank_out(const Rows &y, const Tensor &h, const Tensor &scale, const Bank &f, const Tensor &order, const Tensor &starts, const Tensor &out, void *stream) {
+  check(lib.l8_lowrank_expand(y.p, y.ld, h.const_data_ptr<float>(), h.size(0), scale.defined() ? scale.const_data_ptr<float>() : nullptr, f.p, h.size(1), f.cols, f.n, f.r,
+                              order.const_data_ptr<int>(), starts.const_data_ptr<int>(), out.mutable_data_ptr(), f.cols, stream), "l8_lowrank_expand");
+}
+
+struct LowRank : torch::autograd::Function<LowRank> {
+  static constexpr const char *kName = "add_lowrank";
+  static Tensor forward(AutogradContext *ctx, const Tensor &y, const Tensor &x, const Tensor &a, const Tensor &b, const std::optional<Tensor> &scale, const Tensor &order,
+                        const Tensor &starts, bool learn_x, bool learn_a, bool learn_b) {
+    Bank fa, fb;
+    TORCH_CHECK(as_bank(a, a.get_device(), fa) && as_bank(b, b.get_device(), fb), "add_lowrank: factors");
+    void *stream = stream_of(x.get_device());
+    const Tensor s = scale.value_or(Tensor()), h = lowrank_h(rows_of(x), x, fa, order, starts, stream), out = at::empty(y.sizes(), y.options());
+    lowrank_out(rows_of(y), h, s, fb, order, starts, out, stream);
+    ctx->save_for_backward({learn_a ? x : Tensor(), learn_x ? a : Tensor(), learn_x || learn_a ? b : Tensor(), learn_b ? h : Tensor(), s, order, starts});
+    ctx->saved_data["like"] = x.sizes().vec();
+    ctx->saved_data["bank"] = std::vector<int64_t>{fa.n, fa.r, fa.cols, fb.cols};
+    ctx->saved_data["learns"] = (int64_t)(learn_x | (learn_a << 1) | (learn_b << 2));
+    return out;
+  }
+  static variable_list backward(AutogradContext *ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor gy = gradient(grads[0], kName);
+    const int device = gy.get_device();
+    const c10::DeviceGuard guard(gy.device());
+    void *stream = stream_of(device);
+    const auto sizes = ctx->saved_data["bank"].toIntVector();
+    const int64_t n = sizes[0], r = sizes[1], K = sizes[2], N = sizes[3], learnt = ctx->saved_data["learns"].toInt();
+    const bool need_y = ctx->needs_input_grad(0), need_x = ctx->needs_input_grad(1) && saved[1].defined(), need_a = ctx->needs_input_grad(2) && saved[0].defined(),
+               need_b = ctx->needs_input_grad(3) && saved[3].defined();
+    const Rows rg = rows_of(gy);
+    const Tensor scale = saved[4].defined() ? saved[4].contiguous() : Tensor(), order = saved[5].contiguous(), starts = saved[6].contiguous();
+    const Tensor x = need_a ? aligned_rows(saved[0]) : Tensor(), a = need_x ? bank_rows(saved[1]) : Tensor(), b = need_x || need_a ? bank_rows(saved[2]) : Tensor(),
+                 h = need_b ? bank_rows(saved[3]) : Tensor();
+    Tensor gh, gx, ga, gb;
+    Bank f;
+    if (need_x || need_a) {
+      TORCH_CHECK(as_bank(b, device, f), "add_lowrank backward: factors");
+      gh = lowrank_h(rg, gy, f, order, starts, stream);
+    }
+    if (need_x) {
+      TORCH_CHECK(as_bank(a, device, f), "add_lowrank backward: factors");
+      gx = at::empty(ctx->saved_data["like"].toIntVector(), gy.options());
+      lowrank_out(Rows(), gh, scale, f, order, starts, gx, stream);
+    }
+    if (need_a || need_b) {
+      l8_lowrank_side two[2] = {};
+      if (need_a) {
+        ga = at::empty({n, r, K}, gy.options());
+        const Rows rx = rows_of(x);
+        two[0] = {gh.const_data_ptr<float>(), gh.size(0), rx.p, rx.ld, K, ga.mutable_data_ptr()};
+      }
+      if (need_b) {
+        gb = at::empty({n, r, N}, gy.options());
+        two[1] = {h.const_data_ptr<float>(), h.size(0), rg.p, rg.ld, N, gb.mutable_data_ptr()};
+      }
+      const int64_t bytes = lib.l8_lowrank_outer_workspace(rg.rows, r, need_a ? K : 0, need_b ? N : 0);
+      const Space ws(gy, bytes);
+      check(lib.l8_lowrank_outer(two, scale.defined() ? scale.const_data_ptr<float>() : nullptr, rg.rows, n, r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), ws.p(), bytes,
+                                 stream), "l8_lowrank_outer");
+    }
+    const bool g = learns(grads[0]), lx = learnt & 1, la = learnt & 2, lb = learnt & 4;
+    const variable_list made = once({gx, ga, gb}, {g || la || lb, g || lx || lb, g || lx || la}, kName);
+    return {need_y ? grads[0] : Tensor(), made[0], made[1], made[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// add_lowrank(y, x, a, b, scale, index, order, starts) -> out, differentiable, or None; order and starts (of one index): None where the index is to
+// be looked at now
+PyObject *add_lowrank(PyObject *, PyObject *const *args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  if (n != 8) throw std::runtime_error("add_lowrank: 8 arguments");
+  if (!tensors(args, 8) || args[0] == Py_None || args[1] == Py_None || args[2] == Py_None || args[3] == Py_None) Py_RETURN_NONE;
+  const Tensor &y = THPVariable_Unpack(args[0]), &x = THPVariable_Unpack(args[1]), &a = THPVariable_Unpack(args[2]), &b = THPVariable_Unpack(args[3]);
+  const Tensor scale = arg(args[4]), index = arg(args[5]);
+  Tensor order = arg(args[6]), starts = arg(args[7]);
+  if (!x.is_cuda()) Py_RETURN_NONE;
+  const int device = x.get_device();
+  Rows rx, ry;
+  Bank fa, fb;
+  if (!as_rows(x, device, rx) || !as_rows(y, device, ry) || !on_16_bytes(rx) || !on_16_bytes(ry) || rx.rows != ry.rows || !as_bank(a, device, fa) || !as_bank(b, device, fb) ||
+      fa.n != fb.n || fa.r != fb.r || fa.cols != rx.cols || fb.cols != ry.cols || x.dim() != y.dim() || x.sizes().slice(0, x.dim() - 1) != y.sizes().slice(0, y.dim() - 1) ||
+      (scale.defined() && (scale.dim() != 1 || !dense(scale, at::kFloat, fa.n, device))) || c10::hip::current_device() != device)
+    Py_RETURN_NONE;
+  const int64_t T = rx.rows;
+  const bool planned = order.defined();
+  if (planned ? !dense(order, at::kInt, T, device) || !starts.defined() || !dense(starts, at::kInt, fa.n + 3, device)
+              : !index.defined() || !dense(index, index.scalar_type() == at::kLong ? at::kLong : at::kInt, T, device) || index.sizes() != x.sizes().slice(0, x.dim() - 1))
+    Py_RETURN_NONE;
+  Tensor out;
+  {
+    pybind11::gil_scoped_release no_gil;
+    const bool grad = at::GradMode::is_enabled() && (learns(y) || learns(x) || learns(a) || learns(b));
+    void *stream = stream_of(device);
+    if (!grad && !planned) {
+      out = at::empty(y.sizes(), y.options());
+      const int64_t bytes = lib.l8_lowrank_add_workspace(T, fa.cols, fa.n, fa.r);
+      const Space ws(x, bytes);
+      check(lib.l8_lowrank_add(ry.p, ry.ld, rx.p, rx.ld, fa.p, fb.p, scale.defined() ? scale.const_data_ptr<float>() : nullptr, index.const_data_ptr(), index.scalar_type() == at::kLong,
+                               T, fa.cols, fb.cols, fa.n, fa.r, out.mutable_data_ptr(), fb.cols, ws.p(), bytes, stream), "l8_lowrank_add");
+    } else {
+      if (grad) refuse_captured({&y, &x, &a, &b}, LowRank::kName);
+      if (!planned) {
+        order = at::empty({T}, x.options().dtype(at::kInt)), starts = at::empty({fa.n + 3}, x.options().dtype(at::kInt));
+        check(lib.l8_lowrank_route(index.const_data_ptr(), index.scalar_type() == at::kLong, T, fa.n, order.mutable_data_ptr<int>(), starts.mutable_data_ptr<int>(), stream),
+              "l8_lowrank_route");
+      }
+      out = LowRank::apply(y, x, a, b, maybe(scale), order, starts, grad && learns(x), grad && learns(a), grad && learns(b));
+    }
+  }
+  return wrap(out);
   END_HANDLE_TH_ERRORS
 }
 
@@ -1257,6 +1657,10 @@ PyMethodDef methods[] = {
     {"mxfp4_to_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_to_bf16)), METH_FASTCALL, nullptr},
     {"add_rmsnorm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_rmsnorm)), METH_FASTCALL, nullptr},
     {"rotary_pair", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rotary_pair)), METH_FASTCALL, nullptr},
+    {"norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm)), METH_FASTCALL, nullptr},
+    {"norm_fwd", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(norm_fwd)), METH_FASTCALL, nullptr},
+    {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dropout)), METH_FASTCALL, nullptr},
+    {"add_lowrank", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(add_lowrank)), METH_FASTCALL, nullptr},
     {"refuse_captured", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(refuse_captured_py)), METH_FASTCALL, nullptr},
     {"mxfp4_packed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_packed)), METH_FASTCALL, nullptr},
     {"mxfp4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(mxfp4_linear)), METH_FASTCALL, nullptr},

@@ -15,7 +15,7 @@ from typing import NamedTuple
 
 import torch
 
-from . import ops
+from . import _lib, ops
 from . import float8 as f8
 
 
@@ -54,18 +54,24 @@ class DropoutFn(torch.autograd.Function):
         return gx, (g if ctx.needs_input_grad[1] else None), None, None, None
 
 
+def _dropout(x, residual, drop, what):
+    threshold = ops._drop_args(drop, x.device, what)[2]
+    if f8._native_call(x, 0) and f8._plain_call():
+        y = _lib.native_for(x.get_device()).dropout(x, residual, drop.numbers, drop.site, threshold)
+        if y is not None:
+            return y
+    f8._refuse_captured(x, residual, None, what)
+    return DropoutFn.apply(x, residual, drop.numbers, drop.p, drop.site)
+
+
 def dropout(x: torch.Tensor, drop: Drop) -> torch.Tensor:
     """x, bf16 of any shape, with a share of its elements dropped and the others scaled up; differentiable."""
-    ops._drop_args(drop, x.device, "dropout")
-    f8._refuse_captured(x, None, None, "dropout")
-    return DropoutFn.apply(x, None, drop.numbers, drop.p, drop.site)
+    return _dropout(x, None, drop, "dropout")
 
 
 def dropout_add(x: torch.Tensor, residual: torch.Tensor, drop: Drop) -> torch.Tensor:
     """``residual + dropout(x, drop)`` in one pass, rounded once; differentiable."""
-    ops._drop_args(drop, x.device, "dropout_add")
-    f8._refuse_captured(x, residual, None, "dropout_add")
-    return DropoutFn.apply(x, residual, drop.numbers, drop.p, drop.site)
+    return _dropout(x, residual, drop, "dropout_add")
 
 
 class Dropout(torch.nn.Module):

@@ -159,12 +159,19 @@ def _norm(x, residual, weight, bias, eps, drop, centred, quantise):
             raise RuntimeError(f"{what}: bf16 activations required, got {t.dtype}")
     if residual is not None and x.shape != residual.shape:
         raise RuntimeError(f"{what}: x and residual must have the same shape, got {tuple(x.shape)} and {tuple(residual.shape)}")
-    ops._drop_args(drop, x.device, what)
+    threshold = ops._drop_args(drop, x.device, what)[2]
     p, numbers, site = (0.0, None, 0) if drop is None else drop
+    want_col = quantise and torch.is_grad_enabled() and bool(f8.config.fp8_wgrad)
+    if f8._native_call(x, 0) and f8._plain_call():
+        res = _lib.native_for(x.get_device()).norm(x, residual, weight, bias, numbers, site, threshold, eps, centred, want_col, quantise)
+        if res is not None:
+            h, y, q, s, col = res
+            if quantise and f8.config.share_input_casts:   # (the memo keeps its tensor: not the graph behind it)
+                f8._fwd_cast.put(y.detach().flatten(end_dim=-2), (q, s, col), "norm")
+            return y if h is None else (h, y)
     f8._refuse_captured(x, residual, weight, what)
     if bias is not None:
         f8._refuse_captured(bias, None, None, what)
-    want_col = quantise and torch.is_grad_enabled() and bool(f8.config.fp8_wgrad)
     args = weight, bias, numbers, p, site, eps, centred, want_col, quantise
     if x.dim() == 2:
         return NormFn.apply(x, residual, *args)

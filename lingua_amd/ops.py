@@ -899,6 +899,12 @@ def layernorm_cast_rowwise(x: torch.Tensor, weight: Optional[torch.Tensor], bias
     and its row-wise cast, in one pass; bf16 [R,C].  ``centred`` False: the RMSNorm of a sum with a dropped operand.
     Returns (h | None, y, q fp8 | None, scale [R,1] fp32 | None, stats fp32 [2,R] | None: mean and 1 / deviation)."""
     what = "layernorm_cast_rowwise"
+    if kernel_timer is None and x.is_cuda and col_amax is None:   # the same in one call, for operands that need no copies
+        threshold = _drop_args(drop, x.device, what)[2]
+        res = _lib.native_for(x.get_device()).norm_fwd(x, residual, weight, bias, None if drop is None else drop.numbers, 0 if drop is None else drop.site, threshold, eps,
+                                                       centred, want_q, want_stats, on_lines)
+        if res is not None:
+            return res
     x = _rows_on_lines(x, torch.bfloat16, what)
     st = _prep(x, what)
     R, C = x.shape

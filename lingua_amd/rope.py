@@ -78,8 +78,13 @@ def rotary_axes(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torc
         raise RuntimeError(f"rotary_axes: unknown layout {layout!r}, one of {LAYOUTS}")
     if order not in ORDERS:
         raise RuntimeError(f"rotary_axes: unknown order {order!r}, one of {ORDERS}")
+    sections = tuple(sections)
+    if f8._native_call(xq, 0) and f8._plain_call():
+        res = _lib.native_for(xq.get_device()).rotary_pair(xq, xk, cos, sin, positions, layout == "half", sections, order == "rounds")
+        if res is not None:
+            return res
     f8._refuse_captured(xq, xk, None, "rotary_axes")
-    return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half", tuple(sections), order == "rounds")
+    return RotaryFn.apply(xq, xk, cos, sin, positions, layout == "half", sections, order == "rounds")
 
 
 def apply_rotary_emb(xq: torch.Tensor, xk: torch.Tensor, seq_dim: int, freqs_cis: torch.Tensor):

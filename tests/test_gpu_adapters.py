@@ -4,7 +4,7 @@ import torch
 
 import plain_more as plain
 from conftest import seeded_bf16
-from plain_operators import within
+from plain_operators import host, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -50,7 +50,7 @@ def run(T, n, r, K, N, how, seed=0, dtype=torch.int32, scaled=True):
 
 @pytest.mark.parametrize("T", [1, 2, 16, 17, 63, 100, 257, 700])
 @pytest.mark.parametrize("n, how", [(1, "one"), (3, "mixed"), (5, "runs"), (70, "mixed"), (2, "none")])
-def test_tokens(T, n, how):
+def test_tokens(T, n, how, host):
     if how == "runs" and T < 6:
         how = "mixed"
     run(T, n, 16, 200, 328, how, seed=T + n)
@@ -58,18 +58,18 @@ def test_tokens(T, n, how):
 
 @pytest.mark.parametrize("r", [8, 16, 24, 32, 40, 48, 56, 64, 72, 96, 104, 128])
 @pytest.mark.parametrize("T, n", [(37, 4), (330, 2)])
-def test_ranks(r, T, n):
+def test_ranks(r, T, n, host):
     run(T, n, r, 264, 520, "mixed", seed=r)
 
 
 @pytest.mark.parametrize("K, N", [(8, 8), (8, 4104), (2064, 8), (56, 72), (64, 128), (136, 512), (1024, 1032), (4096, 40)])
 @pytest.mark.parametrize("T", [5, 200])
-def test_features(K, N, T):
+def test_features(K, N, T, host):
     run(T, 2, 16, K, N, "mixed", seed=K + T, dtype=torch.int64, scaled=T == 5)
 
 
 @pytest.mark.parametrize("T, n, how", [(3000, 2, "runs"), (2900, 1, "one"), (4200, 3, "mixed"), (1500, 9, "runs")])
-def test_groups_of_several_tiles(T, n, how):
+def test_groups_of_several_tiles(T, n, how, host):
     """Factors' gradients whose sums meet over several workgroups, and small ones beside large ones."""
     run(T, n, 8, 72, 136, how, seed=T)
     run(T, n, 40, 520, 16, how, seed=T)
@@ -93,7 +93,7 @@ def test_route(T, n, dtype):
 
 
 @pytest.mark.parametrize("T", [40, 400])
-def test_strangers_and_values_that_are_not_finite(T):
+def test_strangers_and_values_that_are_not_finite(T, host):
     """An index of no adapter makes its token NaN, an infinite or NaN token itself, and neither anything else; factors' gradients leave
     strangers out."""
     from lingua_amd import adapters
@@ -136,7 +136,7 @@ def test_strangers_and_values_that_are_not_finite(T):
     assert not bool(gb2[0][:, 3].isfinite().any())
 
 
-def test_strides_shapes_and_plans():
+def test_strides_shapes_and_plans(host):
     from lingua_amd import adapters, ops
     n, r, K, N, T = 3, 16, 72, 136, 60
     a, b, scale = bank(n, r, K, N)
@@ -175,7 +175,7 @@ def test_strides_shapes_and_plans():
         ops.lowrank_expand(big[1:T + 1, :N], h, b, scale, (plan.order, plan.starts), out=out)
 
 
-def test_no_tokens_and_repeated_runs():
+def test_no_tokens_and_repeated_runs(host):
     from lingua_amd import adapters
     n, r, K, N = 4, 16, 264, 520
     a, b, scale = (t.requires_grad_(t.dtype == torch.bfloat16) for t in bank(n, r, K, N))
@@ -197,7 +197,7 @@ def test_no_tokens_and_repeated_runs():
 
 
 @pytest.mark.parametrize("which", ["y", "x", "a", "b", "xa", "ab", "none"])
-def test_parts_of_the_gradient(which):
+def test_parts_of_the_gradient(which, host):
     from lingua_amd import adapters
     T, n, r, K, N = 70, 2, 24, 72, 136
     a, b, scale = bank(n, r, K, N)

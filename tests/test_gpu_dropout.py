@@ -5,7 +5,7 @@ import torch
 import plain_more as plain
 import plain_operators
 from conftest import seeded_bf16
-from plain_operators import within
+from plain_operators import host, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -29,7 +29,7 @@ def test_generator_is_the_published_one():
 @pytest.mark.parametrize("shape", [(1,), (7,), (8,), (9,), (333, 2064), (3, 5, 11), (4096,)])
 @pytest.mark.parametrize("p", [0.0, 0.1, 0.5, 1.0])
 @pytest.mark.parametrize("added", [False, True])
-def test_bits(shape, p, added):
+def test_bits(shape, p, added, host):
     from lingua_amd import dropout
     n = numbers(seed=-3, step=2 ** 40 + 7)
     drop = dropout.Drop(p, n, site=9 if p == 0.1 else 2 ** 32 - 1)
@@ -64,7 +64,7 @@ def test_share_and_independence():
         assert abs(float((masks[0][:-d] & masks[0][d:]).double().mean()) - 0.0625) < 5 * (0.0625 * 0.9375 / x.numel()) ** 0.5
 
 
-def test_what_is_dropped_is_gone():
+def test_what_is_dropped_is_gone(host):
     from lingua_amd import dropout
     n = numbers()
     x = torch.full((4096,), float("nan"), dtype=torch.bfloat16, device="cuda")
@@ -75,7 +75,7 @@ def test_what_is_dropped_is_gone():
     assert not bool(dropout.dropout(x, dropout.Drop(1.0, n)).any())
 
 
-def test_elements_off_lines():
+def test_elements_off_lines(host):
     from lingua_amd import dropout
     x = seeded_bf16((1001,), seed=1).cuda()
     drop = dropout.Drop(0.3, numbers())
@@ -92,7 +92,7 @@ NORM_SIZES = [(1, 8), (3, 1152), (5, 2056), (2, 4104), (4, 6152), (3, 8192), (10
 
 @pytest.mark.parametrize("R, C", NORM_SIZES)
 @pytest.mark.parametrize("centred", [True, False])
-def test_inside_the_norms(R, C, centred):
+def test_inside_the_norms(R, C, centred, host):
     """The sum is dropout_add's bit for bit; y, the copy, its scales and the column amaxes are those of the norm of that sum; gradients are
     within their rounding of 64 bits and dropped where forward dropped."""
     from lingua_amd import dropout, norm, ops
@@ -154,7 +154,7 @@ def test_far_elements():
     assert torch.equal((y[first:] != 0).cpu(), keep)
 
 
-def test_numbers_changed_between_the_passes_are_an_error():
+def test_numbers_changed_between_the_passes_are_an_error(host):
     from lingua_amd import dropout, norm
     n = numbers()
     x, res = (seeded_bf16((16, 64), seed=i).cuda().requires_grad_() for i in range(2))
