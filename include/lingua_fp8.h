@@ -439,7 +439,7 @@ int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, int64_t n, 
  * many pay). */
 int l8_lowrank_shrink(const void *x, int64_t T, int64_t K, int64_t ldx, const void *f, int64_t n, int64_t r, const int *order, const int *starts,
                       float *h, int64_t splits, void *stream);
-int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K);
+int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t r, int64_t K);
 /* out = y + scale_i h F_i, bf16 [T,N]; y NULL: zeros, scale NULL: ones.  Tokens without an adapter: out = y.  out may be y. */
 int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int64_t splits, const float *scale, const void *f, int64_t T, int64_t N, int64_t n,
                       int64_t r, const int *order, const int *starts, void *out, int64_t ldo, void *stream);

@@ -71,7 +71,7 @@ SIGNATURES = {
     "l8_rotary_axes": [_p, _i64, _i64, _i64, _p, _i64, _int, _int, _int, _p, _p, _i64, _i64, _i64, _p, _int, _i64, _i64, _i64, _p],
     "l8_lowrank_route": [_p, _int, _i64, _i64, _p, _p, _p],
     "l8_lowrank_shrink": [_p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _p],
-    "l8_lowrank_splits": [_i64, _i64, _i64],
+    "l8_lowrank_splits": [_i64, _i64, _i64, _i64],
     "l8_lowrank_expand": [_p, _i64, _p, _i64, _p, _p, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
     "l8_lowrank_add": [_p, _i64, _p, _i64, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p],
     "l8_lowrank_add_workspace": [_i64, _i64, _i64, _i64],

@@ -330,47 +330,55 @@ struct ExpandArgs {
   Tokens tokens;
   uint16_t *out;
   int64_t ldy, ldo;
-  int T, N, n, r, splits, chunks;
+  int T, N, n, r, splits, chunks, per;   // (of 128 columns in a row: a workgroup's)
 };
 
 constexpr int kExpandWaves = 4;
 
-// 16 tokens by 128 columns a wave; the workgroup's four waves are PARTS parts of a tile's tokens by 4 / PARTS stretches of columns.  Column
-// 8 c + j of a wave's 128 is column c of matrix instruction j: a lane then reads eight neighbouring columns of eight rows of the factor,
-// turns the block round in registers, and ends up with eight neighbouring columns of four tokens: 16-byte loads and stores, 256 bytes of a
-// row at once.
+// 16 tokens by 128 columns a wave and step; the workgroup's four waves are PARTS parts of a tile's tokens by 4 / PARTS stretches of columns.
+// Column 8 c + j of a wave's 128 is column c of matrix instruction j: a lane then reads eight neighbouring columns of eight rows of the
+// factor, turns the block round in registers, and ends up with eight neighbouring columns of four tokens: 16-byte loads and stores, 256 bytes
+// of a row at once.
 // KS steps of 32 ranks, each with the upper and the lower bits of h; KS 0: up to 16 ranks, where one instruction takes both.
-// Waves of the same columns and more than 16 ranks share the factor's turned blocks through LDS, each making a part of them.
-// Everything that a wave reads is requested before anything is used: a tile waits for memory three times, for its place, for its tokens and
-// for the rest.
-// Up to 16 ranks: five waves a SIMD and not the four that the compiler would make room for, [16384,4096] with y 61 -> 52 us (six: 57).
+// Waves of the same columns and more than 16 ranks share the factor's turned blocks through LDS, each making a part of them, and go on to the
+// next 128 columns `per` times: h, 4 r bytes a token and more in parts, is then read once for all of them.  The next step's y and factor are
+// requested before the present one is multiplied.
+// A tile waits for memory three times: for its place, for its tokens, for everything else.
+// us at [16384,4096] with y: up to 16 ranks with five waves a SIMD 52, with four 61, with six 57; 64 ranks one step a workgroup 70, up to eight 58,
+// of h in three parts 100 and 63; 128 ranks 104 and 68.
 template <int PARTS, int KS>
-__global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : 1) void lowrank_expand_kernel(const ExpandArgs p) {
+__global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : PARTS == 1 ? 1 : 2) void lowrank_expand_kernel(const ExpandArgs p) {
   constexpr int STEPS = KS ? KS : 1;
   constexpr bool SHARED = PARTS == kExpandWaves && KS > 0;
-  __shared__ v4i turned[SHARED ? STEPS * 8 * 64 : 1];
+  __shared__ v4i turned[2][SHARED ? STEPS * 8 * 64 : 1];
   const int slot = blockIdx.x / p.chunks, chunk = blockIdx.x - slot * p.chunks;
   const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, PARTS * 16, slot);
   if (tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
   const int part0 = wave % PARTS * 16;
-  const int col = (chunk * (kExpandWaves / PARTS) + wave / PARTS) * 128 + row * 8;
-  const bool in = col < p.N;
-  const int from = in ? col : 0, r = p.r;
+  const int N = p.N, r = p.r, per = SHARED ? p.per : 1;
+  const int col0 = SHARED ? chunk * per * 128 + row * 8 : (chunk * (kExpandWaves / PARTS) + wave / PARTS) * 128 + row * 8;
   int64_t t[4];
-  v4i y[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    t[i] = tile.token(part0 + g * 4 + i);
-    y[i] = v4i{0, 0, 0, 0};
-    if (p.y) y[i] = __builtin_nontemporal_load((const v4i *)(p.y + t[i] * p.ldy + from));
-  }
-  auto store = [&](int i, v4i v) {
-    if (in && part0 + g * 4 + i < tile.count) __builtin_nontemporal_store(v, (v4i *)(p.out + t[i] * p.ldo + col));
+  for (int i = 0; i < 4; ++i) t[i] = tile.token(part0 + g * 4 + i);
+  v4i y[SHARED ? 2 : 1][4];
+  auto request_y = [&](int s, int col) {   // (beyond the last column: the first ones, which nobody stores)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[s][i] = v4i{0, 0, 0, 0};
+      if (p.y) y[s][i] = __builtin_nontemporal_load((const v4i *)(p.y + t[i] * p.ldy + (col < N ? col : 0)));
+    }
   };
+  auto store = [&](int i, int col, v4i v) {
+    if (col < N && part0 + g * 4 + i < tile.count) __builtin_nontemporal_store(v, (v4i *)(p.out + t[i] * p.ldo + col));
+  };
+  request_y(0, col0);
   if (tile.group >= p.n) {   // no adapter: y as it is; no known adapter: NaN
+    for (int c = 0; c < per; ++c) {
+      if (c) request_y(0, col0 + c * 128);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) store(i, tile.group > p.n ? v4i{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0} : y[i]);
+      for (int i = 0; i < 4; ++i) store(i, col0 + c * 128, tile.group > p.n ? v4i{0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0, 0x7fc07fc0} : y[0][i]);
+    }
     return;
   }
   auto rank_of = [&](int s) { return KS ? s * 32 + g * 8 : (g & 1) * 8; };
@@ -382,74 +390,109 @@ __global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : 1) void lowrank_ex
     hp[s][0] = *(const v4f *)(h + k0), hp[s][1] = *(const v4f *)(h + k0 + 4);
   }
   const float scale = p.scale ? p.scale[tile.group] : 1.0f;
-  auto turn = [&](v4i (&b)[8], int s) {
-    const int k0 = rank_of(s);
-    const uint16_t *f = p.f + ((int64_t)tile.group * r + min(k0, r - 8)) * p.N + from;
-    v4i rows[8];
+  auto request_f = [&](v4i (&rows)[8], int s, int col) {
+    const uint16_t *f = p.f + ((int64_t)tile.group * r + min(rank_of(s), r - 8)) * N + (col < N ? col : 0);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rows[e] = *(const v4i *)(f + (int64_t)e * p.N);
+    for (int e = 0; e < 8; ++e) rows[e] = *(const v4i *)(f + (int64_t)e * N);
+  };
+  auto turn = [&](v4i (&b)[8], v4i (&rows)[8], int s) {
+    if (rank_of(s) >= r) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (k0 >= r) rows[e] = v4i{0, 0, 0, 0};   // (ranks beyond r: zero, whatever the row that was read holds)
+      for (int e = 0; e < 8; ++e) rows[e] = v4i{0, 0, 0, 0};   // (ranks beyond r: zero, whatever the row that was read holds)
+    }
     transpose8(b, rows);
   };
-  v4i own[SHARED ? 1 : STEPS][8];
+  constexpr int MINE = SHARED ? (STEPS + kExpandWaves - 1) / kExpandWaves : STEPS;   // blocks of the factor that a wave reads
+  static_assert(!SHARED || MINE == 1, "a wave turns one block");
+  v4i rows[MINE][8];
   if constexpr (SHARED) {
-    for (int s = wave; s < STEPS; s += kExpandWaves) {
-      turn(own[0], s);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) turned[(s * 8 + j) * 64 + lane] = own[0][j];
-    }
-    __syncthreads();
+    if (wave < STEPS) request_f(rows[0], wave, col0);
   } else {
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) turn(own[s], s);
+    for (int s = 0; s < STEPS; ++s) request_f(rows[s], s, col0);
   }
-  if (part0 >= tile.count) return;
-  v4f acc[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  v4i hi[STEPS], lo[STEPS];
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
     const int k0 = rank_of(s);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = hp[s][e >> 2][e & 3];
-    for (int q = 1; q < p.splits; ++q) {
-      const float *more = h + (int64_t)q * p.T * r + min(k0, r - 8);
-      const v4f u = *(const v4f *)more, w = *(const v4f *)(more + 4);
+    for (int q0 = 1; q0 < p.splits; q0 += 3) {   // three parts at a time: what stands in for one that is not there is not added
+      v4f u[3], w[3];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] += u[e], v[e + 4] += w[e];
+      for (int q = 0; q < 3; ++q) {
+        const float *more = h + (int64_t)min(q0 + q, p.splits - 1) * p.T * r + min(k0, r - 8);
+        u[q] = *(const v4f *)more, w[q] = *(const v4f *)(more + 4);
+      }
+#pragma unroll
+      for (int q = 0; q < 3; ++q)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (q0 + q < p.splits) v[e] += u[q][e], v[e + 4] += w[q][e];
+        }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = k0 < r ? v[e] * scale : 0.0f;
-    v4i b[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (SHARED) b[j] = turned[(s * 8 + j) * 64 + lane];
-      else b[j] = own[s][j];
-    }
     if constexpr (KS) {
-      const v4i hi = pack8(v, false), lo = pack8(v, true);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = mfma(hi, b[j], acc[j]);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = mfma(lo, b[j], acc[j]);
+      hi[s] = pack8(v, false), lo[s] = pack8(v, true);
     } else {
-      const v4i both = g < 2 ? pack8(v, false) : pack8(v, true);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = mfma(both, b[j], acc[j]);
+      hi[s] = g < 2 ? pack8(v, false) : pack8(v, true);
     }
   }
+  auto step = [&](int s, int c) {   // step c of the columns, with y in y[s]
+    const int col = col0 + c * 128;
+    v4f acc[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v4i out;
+    for (int j = 0; j < 8; ++j) acc[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    v4i own[8];
+    if constexpr (SHARED) {
+      if (wave < STEPS) {
+        turn(own, rows[0], wave);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float lo = __uint_as_float((uint32_t)y[i][k] << 16) + acc[2 * k][i], hi = __uint_as_float((uint32_t)y[i][k] & 0xffff0000u) + acc[2 * k + 1][i];
-      out[k] = (int)(bf16_rne_bits(lo) | (bf16_rne_bits(hi) << 16));
+        for (int j = 0; j < 8; ++j) turned[s][(wave * 8 + j) * 64 + lane] = own[j];
+      }
+      __syncthreads();   // (the other buffer: whoever reads it has not passed the next barrier)
+      if (c + 1 < per) {
+        request_y(SHARED ? s ^ 1 : 0, col + 128);
+        if (wave < STEPS) request_f(rows[0], wave, col + 128);
+      }
     }
-    store(i, out);
+#pragma unroll
+    for (int k = 0; k < STEPS; ++k) {
+      v4i b[8];
+      if constexpr (SHARED) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) b[j] = turned[s][(k * 8 + j) * 64 + lane];
+      } else {
+        turn(b, rows[k], k);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = mfma(hi[k], b[j], acc[j]);
+      if constexpr (KS > 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = mfma(lo[k], b[j], acc[j]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v4i out;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float u = __uint_as_float((uint32_t)y[s][i][k] << 16) + acc[2 * k][i], v = __uint_as_float((uint32_t)y[s][i][k] & 0xffff0000u) + acc[2 * k + 1][i];
+        out[k] = (int)(bf16_rne_bits(u) | (bf16_rne_bits(v) << 16));
+      }
+      store(i, col, out);
+    }
+  };
+  if constexpr (!SHARED) {
+    step(0, 0);
+  } else {
+#pragma unroll 1
+    for (int c = 0; c < per; c += 2) {
+      step(0, c);
+      if (c + 1 < per) step(1, c + 1);
+    }
   }
 }
 
@@ -478,9 +521,9 @@ L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)
 
 // RT tiles of 16 ranks by 128 columns a wave, over a tile's tokens.  z is read as `expand` reads the factor: eight neighbouring columns of
 // eight tokens' rows a lane, turned round in registers, 32 tokens requested ahead; h is laid out by rank in LDS, TOKENS at a time, both
-// halves of its bits.
+// halves of its bits.  Two waves a SIMD: 64 ranks of [16384,4096] and [16384,4096] 130 us where the compiler made room for one, 107.
 template <int RT, int TOKENS>
-__global__ __launch_bounds__(kOuterWaves * 64, RT <= 2 ? 2 : 1) void lowrank_outer_kernel(const OuterArgs p) {
+__global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(const OuterArgs p) {
   constexpr int PITCH = TOKENS + 8;
   __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][PITCH];
   __shared__ __attribute__((aligned(16))) int toks[TOKENS];
@@ -607,6 +650,13 @@ constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 1 << 16, 
 
 // Tokens of a tile: 64, which read a factor a quarter as often, where the adapters have that many on average.
 static int tile_tokens(int64_t T, int64_t n) { return T >= 64 * (n + 1) ? 64 : 16; }
+// The same of `shrink`: with more than 32 ranks, where four tiles of 16 tokens fill a SIMD's registers with one wave, tiles of 32 tokens on twice
+// the waves unless the larger ones give every unit one ([2055,4096] rank 64 in two parts 17.7 us and 23.1, [16384,4096] 56 and 41).
+static int64_t tile_slots(int64_t T, int64_t n, int64_t size);
+static int shrink_tokens(int64_t T, int64_t n, int64_t r) {
+  const int size = tile_tokens(T, n);
+  return size == 64 && r > 32 && tile_slots(T, n, 64) < num_cus() ? 32 : size;
+}
 static int64_t tile_slots(int64_t T, int64_t n, int64_t size) { return T / size + n + 2; }
 
 // Tokens of a tile of the factors' gradients: so many tiles that two workgroups a unit have work.
@@ -657,9 +707,9 @@ extern "C" int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, 
 }
 
 // Workgroups that share K: as many as give every unit one, with at least two steps left for each wave.
-extern "C" int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t K) {
+extern "C" int64_t l8_lowrank_splits(int64_t T, int64_t n, int64_t r, int64_t K) {
   if (T <= 0 || n <= 0 || K <= 0) return 1;
-  const int64_t size = tile_tokens(T, n), tiles = std::min(T, tile_slots(T, n, size)), waves = size == 16 ? 8 : 4;
+  const int64_t size = shrink_tokens(T, n, r), tiles = std::min(T, tile_slots(T, n, size)), waves = size == 64 && r > 32 ? 4 : 8;
   return std::max<int64_t>(1, std::min<int64_t>({num_cus() / tiles, (K + 63) / 64 / (2 * waves), 16}));
 }
 
@@ -675,7 +725,7 @@ static int shrink_impl(const char *who, const void *x, int64_t T, int64_t K, int
                        hipStream_t st) {
   L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
   L8_REQUIRE(rows_fit(x, ldx, K) && rows_fit(f, K, K) && h && ((uintptr_t)h % 16) == 0, "%s: null or misaligned operand, or rows off 16-byte lines", who);
-  const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size);
+  const int64_t size = shrink_tokens(T, n, r), slots = tiles_of(tk, T, n, size);
   const ShrinkArgs p{(const uint16_t *)x, (const uint16_t *)f, tk, h, ldx, (int)T, (int)K, (int)n, (int)r, (int)splits};
   const unsigned ranks = r <= 64 ? 1 : 2;
 #define L8_SHRINK(MT, SUB, RT, W)                                                                                        \
@@ -690,6 +740,7 @@ static int shrink_impl(const char *who, const void *x, int64_t T, int64_t K, int
   } else {
     if (r <= 16) L8_SHRINK(4, 1, 1, 8);
     else if (r <= 32) L8_SHRINK(4, 1, 2, 8);
+    else if (size == 32) L8_SHRINK(2, 1, 4, 8);
     else L8_SHRINK(4, 1, 4, 4);
   }
 #undef L8_SHRINK
@@ -702,9 +753,12 @@ static int expand_impl(const char *who, const void *y, int64_t ldy, const float 
   L8_REQUIRE(splits >= 1 && splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)splits);
   L8_REQUIRE((!y || rows_fit(y, ldy, N)) && rows_fit(f, N, N) && rows_fit(out, ldo, N) && h && ((uintptr_t)h % 16) == 0 && ((uintptr_t)scale % 4) == 0,
              "%s: null or misaligned operand, or rows off 16-byte lines", who);
-  const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size), cols = size == 16 ? kExpandWaves * 128 : 128, chunks = (N + cols - 1) / cols;
+  const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size);
+  // waves that share the factor take as many steps as leave four workgroups a unit
+  const int64_t per = size == 16 || r <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(8, slots * ((N + 127) / 128) / (4 * num_cus())));
+  const int64_t cols = size == 16 ? kExpandWaves * 128 : per * 128, chunks = (N + cols - 1) / cols;
   L8_CALL(check_grid(who, slots * chunks, 1, 1, kExpandWaves * 64));
-  const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, tk, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits, (int)chunks};
+  const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, tk, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits, (int)chunks, (int)per};
   const dim3 grid((unsigned)(slots * chunks)), block(kExpandWaves * 64);
 #define L8_EXPAND(PARTS)                                                                                          \
   do {                                                                                                       \
@@ -743,7 +797,7 @@ extern "C" int l8_lowrank_expand(const void *y, int64_t ldy, const float *h, int
 extern "C" int64_t l8_lowrank_add_workspace(int64_t T, int64_t K, int64_t n, int64_t r) {
   if (T <= 0 || K <= 0 || n <= 0 || r <= 0) return 0;
   const int64_t plan = T <= kFewTokens ? 0 : (T + n + 3 + 3) / 4 * 16;
-  return plan + l8_lowrank_splits(T, n, K) * T * r * (int64_t)sizeof(float);
+  return plan + l8_lowrank_splits(T, n, r, K) * T * r * (int64_t)sizeof(float);
 }
 
 extern "C" int l8_lowrank_add(const void *y, int64_t ldy, const void *x, int64_t ldx, const void *a, const void *b, const float *scale, const void *index, int index_is_i64,
@@ -752,7 +806,7 @@ extern "C" int l8_lowrank_add(const void *y, int64_t ldy, const void *x, int64_t
   L8_CALL(check_sizes(who, T, n, r, K));
   L8_CALL(check_sizes(who, T, n, r, N));
   if (T == 0) return L8_OK;
-  const int64_t need = l8_lowrank_add_workspace(T, K, n, r), splits = l8_lowrank_splits(T, n, K);
+  const int64_t need = l8_lowrank_add_workspace(T, K, n, r), splits = l8_lowrank_splits(T, n, r, K);
   L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
   L8_REQUIRE(index && ((uintptr_t)index % (index_is_i64 ? 8 : 4)) == 0, "%s: null or misaligned index", who);
   L8_REQUIRE(rows_fit(b, N, N) && rows_fit(out, ldo, N) && (!y || rows_fit(y, ldy, N)), "%s: null or misaligned operand, or rows off 16-byte lines", who);

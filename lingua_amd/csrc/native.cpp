@@ -1395,7 +1395,7 @@ Tensor bank_rows(const Tensor &t) {
   return ((uintptr_t)c.const_data_ptr() % 16) == 0 ? c : c.clone();
 }
 Tensor lowrank_h(const Rows &x, const Tensor &like, const Bank &f, const Tensor &order, const Tensor &starts, void *stream) {
-  const int64_t splits = lib.l8_lowrank_splits(x.rows, f.n, f.cols);
+  const int64_t splits = lib.l8_lowrank_splits(x.rows, f.n, f.r, f.cols);
   const Tensor h = at::empty({splits, x.rows, f.r}, like.options().dtype(at::kFloat));
   check(lib.l8_lowrank_shrink(x.p, x.rows, f.cols, x.ld, f.p, f.n, f.r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), h.mutable_data_ptr<float>(), splits, stream),
         "l8_lowrank_shrink");

@@ -1105,7 +1105,7 @@ def lowrank_shrink(x: torch.Tensor, f: torch.Tensor, plan) -> torch.Tensor:
         raise RuntimeError(f"{what}: rows of {D} and factors of {D2} features on {dev} and {f.device}")
     order, starts = _plan_args(plan, T, n, dev, what)
     with _timed(what, 2 * T * D + 2 * f.numel() + 4 * T * r, dev):
-        splits = _lib.load().l8_lowrank_splits(T, n, D)
+        splits = _lib.load().l8_lowrank_splits(T, n, r, D)
         h = torch.empty((splits, T, r), dtype=torch.float32, device=dev)
         code = _lib.load().l8_lowrank_shrink(x.data_ptr(), T, D, _ld(x), f.data_ptr(), n, r, order, starts, h.data_ptr(), splits, st)
     _lib.check(code, "l8_lowrank_shrink")

@@ -106,8 +106,8 @@ def test_outer_is_refused(change):
 
 def test_lowrank_splits_and_workspace():
     lib = _lib.load()
-    assert lib.l8_lowrank_splits(0, 4, 64) == lib.l8_lowrank_splits(-5, 4, 64) == lib.l8_lowrank_splits(20, 2, 8) == 1
-    assert all(1 <= lib.l8_lowrank_splits(T, n, K) <= 16 for T in (1, 16, 300, 1 << 20) for n in (1, 40, 1 << 16) for K in (8, 4096, 1 << 20))
+    assert lib.l8_lowrank_splits(0, 4, 16, 64) == lib.l8_lowrank_splits(-5, 4, 16, 64) == lib.l8_lowrank_splits(20, 2, 64, 8) == 1
+    assert all(1 <= lib.l8_lowrank_splits(T, n, r, K) <= 16 for r in (8, 128) for T in (1, 16, 300, 1 << 20) for n in (1, 40, 1 << 16) for K in (8, 4096, 1 << 20))
     assert lib.l8_lowrank_outer_workspace(100, 16, 128, 128) == 0 and lib.l8_lowrank_outer_workspace(0, 16, 128, 128) == 0
     assert lib.l8_lowrank_outer_workspace(1 << 20, 16, 128, 256) % (4 * 16 * 384) == 0
 
