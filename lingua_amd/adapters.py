@@ -53,7 +53,7 @@ class LowRankFn(torch.autograd.Function):
         if gy.dtype != torch.bfloat16:
             raise RuntimeError(f"add_lowrank backward: bf16 gradients required, got {gy.dtype}")
         x, a, b, h, scale, order, starts = ctx.saved_tensors
-        plan, (n, r) = (order, starts), ctx.sizes
+        plan, (n, r) = (order.contiguous(), starts.contiguous()), ctx.sizes   # (hooks hand them back in any layout)
         need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
         gx = ga = gb = None
         varies = f8._learns(gy)

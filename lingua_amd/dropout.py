@@ -49,7 +49,7 @@ class DropoutFn(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             varies = f8._learns(g)
             with torch.no_grad():
-                gx = ops.dropout(g, Drop(ctx.p, numbers, ctx.site))
+                gx = ops.dropout(g, Drop(ctx.p, numbers.contiguous(), ctx.site))   # (hooks hand it back in any layout)
             gx, = f8._once("dropout", (gx,), (varies,))
         return gx, (g if ctx.needs_input_grad[1] else None), None, None, None
 

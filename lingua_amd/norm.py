@@ -124,7 +124,7 @@ class NormFn(torch.autograd.Function):
         for g in (gh, gy):
             if g is not None and g.dtype != torch.bfloat16:
                 raise RuntimeError(f"{_name(ctx.centred, ctx.added)} backward: bf16 gradients required, got {g.dtype}")
-        drop = None if numbers is None else dr.Drop(ctx.p, numbers, ctx.site)
+        drop = None if numbers is None else dr.Drop(ctx.p, numbers.contiguous(), ctx.site)   # (hooks hand it back in any layout)
         rest = (None,) * 7
         what = _name(ctx.centred, ctx.added)
         if gy is None:   # only the sum was used, if anything
