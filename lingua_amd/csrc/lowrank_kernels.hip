@@ -153,26 +153,28 @@ L8_DEV Tile tile_with_tokens(const Tokens &tk, int T, int n, int size, int slot)
     t.mine = t.count ? tk.order[t.first + min(lane, t.count - 1)] : 0;
     return t;
   }
-  // few tokens: one group after the other, in the order in which they first appear, until the slot's is found
+  // few tokens: every lane finds the tokens of its own group, bit by bit of the group's number; every sixteenth of a group begins a tile
   const int64_t i = lane >= T ? -1 : tk.index_i64 ? ((const int64_t *)tk.index)[lane] : (int64_t)((const int32_t *)tk.index)[lane];
   const int group = i >= 0 && i < n ? (int)i : i == -1 ? n : n + 1;
-  Tile t{};
-  uint64_t left = __ballot(lane < T);
-  while (left) {
-    const int g = __builtin_amdgcn_readlane(group, __builtin_ctzll(left));
-    const uint64_t same = __ballot(group == g && lane < T);
-    const int tokens = __popcll(same), pieces = (tokens + size - 1) / size;
-    if (slot < pieces) {
-      t.group = g, t.count = min(size, tokens - slot * size);
-      const int place = __popcll(same & ((1ull << lane) - 1)) - slot * size;   // of a lane in `same`
-      const bool in = (same >> lane & 1) && place >= 0 && place < size;
-      // every token goes to the lane of its place; the others go where no token of the tile is (a tile of 16: the last lane)
-      t.mine = __builtin_amdgcn_ds_permute((in ? place : 63) * 4, lane);
-      return t;
-    }
-    slot -= pieces;
-    left &= ~same;
+  uint64_t same = __ballot(lane < T);
+  for (int bit = 0; (n + 1) >> bit; ++bit) {
+    const bool set = group >> bit & 1;
+    const uint64_t votes = __ballot(set);
+    same &= set ? votes : ~votes;
   }
+  const uint64_t below = (1ull << lane) - 1;
+  const int place = __popcll(same & below);
+  const uint64_t firsts = __ballot(lane < T && place % size == 0);
+  Tile t{};
+  const uint64_t mine = __ballot((firsts >> lane & 1) && __popcll(firsts & below) == slot);
+  if (!mine) return t;
+  const int lead = __builtin_ctzll(mine);
+  t.group = __builtin_amdgcn_readlane(group, lead);
+  const int from = __builtin_amdgcn_readlane(place, lead);
+  const bool in = lane < T && group == t.group && place >= from && place < from + size;
+  t.count = __popcll(__ballot(in));
+  // every token goes to the lane of its place; the others go where no token of the tile is (a tile of 16: the last lane)
+  t.mine = __builtin_amdgcn_ds_permute((in ? place - from : 63) * 4, lane);
   return t;
 }
 
@@ -809,7 +811,7 @@ extern "C" int l8_lowrank_add(const void *y, int64_t ldy, const void *x, int64_t
   const int64_t need = l8_lowrank_add_workspace(T, K, n, r), splits = l8_lowrank_splits(T, n, r, K);
   L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
   L8_REQUIRE(index && ((uintptr_t)index % (index_is_i64 ? 8 : 4)) == 0, "%s: null or misaligned index", who);
-  L8_REQUIRE(rows_fit(b, N, N) && rows_fit(out, ldo, N) && (!y || rows_fit(y, ldy, N)), "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  L8_REQUIRE(rows_fit(b, N, N) && rows_fit(out, ldo, N) && rows_fit(y, ldy, N), "%s: null or misaligned operand, or rows off 16-byte lines", who);
   float *h = (float *)workspace;
   Tokens tk{nullptr, nullptr, index, index_is_i64};
   if (T > kFewTokens) {
