@@ -756,8 +756,9 @@ static int expand_impl(const char *who, const void *y, int64_t ldy, const float 
   L8_REQUIRE((!y || rows_fit(y, ldy, N)) && rows_fit(f, N, N) && rows_fit(out, ldo, N) && h && ((uintptr_t)h % 16) == 0 && ((uintptr_t)scale % 4) == 0,
              "%s: null or misaligned operand, or rows off 16-byte lines", who);
   const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size);
-  // waves that share the factor take as many steps as leave four workgroups a unit
-  const int64_t per = size == 16 || r <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(8, slots * ((N + 127) / 128) / (4 * num_cus())));
+  // waves that share the factor take as many steps as leave two workgroups a unit ([2055,11008] rank 64, h in three parts, us: 31.0, four a
+  // unit 37.0; [16384,4096] up to eight steps 61, up to sixteen 77)
+  const int64_t per = size == 16 || r <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(8, slots * ((N + 127) / 128) / (2 * num_cus())));
   const int64_t cols = size == 16 ? kExpandWaves * 128 : per * 128, chunks = (N + cols - 1) / cols;
   L8_CALL(check_grid(who, slots * chunks, 1, 1, kExpandWaves * 64));
   const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, tk, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits, (int)chunks, (int)per};
