@@ -428,7 +428,7 @@ int l8_rotary_axes(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D
                    const void *positions, int positions_i32, int64_t pos_axis, int64_t pos_b, int64_t pos_s, void *stream);
 
 /* Low-rank adapters of many requests beside a projection: out_t = y_t + scale_i (x_t A_i^T) B_i, i = index[t], A bf16 [n,r,K], B bf16 [n,r,N].
- * r a multiple of 8 up to 128, K and N multiples of 8 below 2^24, n up to 2^16, T below 2^24 tokens; rows of tokens and factors on 16-byte
+ * r a multiple of 8 up to 128, K and N multiples of 8 below 2^24, n up to 65535, T below 2^24 tokens, (n + 2) T below 2^36; rows of tokens and factors on 16-byte
  * lines; h fp32 [splits,T,r], 16-byte aligned, of which rows of tokens without an adapter are neither written nor read.
  *
  * route: tokens by adapter.  index int32 or (index_is_i64) int64 [T]: 0 .. n - 1, -1: none; any other: the token's results are NaN.

@@ -122,15 +122,28 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
 
 
 class Requests:
-    """Which adapter each token of the running batch has, shared by the banks of a model: ``set`` it before a forward pass.  Without an index
-    (``set(None)``) the adapters are left out."""
+    """Which adapter each token of the running batch has, shared by the banks of a model: ``set`` it before a forward pass, and not again before
+    that pass's backward pass is done (which would be an error).  Without an index (``set(None)``) the adapters are left out.
+
+    The order of the tokens is written to the same memory for every batch of one shape, so that a captured forward pass that is replayed
+    after a ``set`` sees it."""
 
     def __init__(self, n: int):
         self.n, self.plan = n, None
+        self._plans = {}    # a plan for each shape of tokens: a graph may go on reading one
 
     def set(self, index: Optional[torch.Tensor]) -> None:
         """``index`` int32 or int64 on the GPU, of the shape of the batch's tokens."""
-        self.plan = None if index is None else route(index, self.n)
+        if index is None:
+            self.plan = None
+            return
+        key = index.shape, index.device
+        plan = self._plans.get(key)
+        if plan is None:
+            plan = self._plans[key] = route(index, self.n)
+        else:
+            ops.lowrank_route(index.flatten(), self.n, out=(plan.order, plan.starts))
+        self.plan = plan
 
 
 class AdaptedLinear(torch.nn.Module):
@@ -160,7 +173,7 @@ class AdaptedLinear(torch.nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         y = self.linear(x)
         plan = self.requests.plan
-        return y if plan is None else add_lowrank(y, x, self.a, self.b, plan, self.scale)
+        return y if plan is None else add_lowrank(y, x, self.a, self.b, plan, self.scale.float())   # (a model's `to` may have rounded it)
 
     def extra_repr(self):
         return f"adapters={self.a.shape[0]}, rank={self.a.shape[1]}"

@@ -648,7 +648,7 @@ __global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, in
 
 // ---- host ----
 
-constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 1 << 16, kMaxCols = 1 << 24;
+constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 65535, kMaxCols = 1 << 24;
 
 // Tokens of a tile: 64, which read a factor a quarter as often, where the adapters have that many on average.
 static int tile_tokens(int64_t T, int64_t n) { return T >= 64 * (n + 1) ? 64 : 16; }
@@ -672,7 +672,7 @@ static int outer_size(int64_t T, int64_t K, int64_t N) {
 static bool rows_fit(const void *p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld >= cols; }
 static int check_sizes(const char *who, int64_t T, int64_t n, int64_t r, int64_t D) {
   L8_REQUIRE(T >= 0 && T < kMaxTokens, "%s: %lld tokens, fewer than 2^24 are wanted", who, (long long)T);
-  L8_REQUIRE(n >= 1 && n <= kMaxAdapters, "%s: %lld adapters, 1 to 2^16 are wanted", who, (long long)n);
+  L8_REQUIRE(n >= 1 && n <= kMaxAdapters, "%s: %lld adapters, 1 to 65535 are wanted", who, (long long)n);
   L8_REQUIRE(r >= 8 && r <= kMaxRank && r % 8 == 0, "%s: rank %lld is not a multiple of 8 up to %lld", who, (long long)r, (long long)kMaxRank);
   L8_REQUIRE(D >= 8 && D % 8 == 0 && D < kMaxCols, "%s: %lld columns, a multiple of 8 below 2^24 is wanted", who, (long long)D);
   return L8_OK;
@@ -700,6 +700,7 @@ extern "C" int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, 
   L8_CALL(check_sizes(who, T, n, 8, 8));
   L8_CALL(check_plan(who, T, order, starts));
   L8_REQUIRE(T == 0 || (index && ((uintptr_t)index % (index_is_i64 ? 8 : 4)) == 0), "%s: null or misaligned index", who);
+  L8_REQUIRE((n + 2) * T < (1ll << 36), "%s: %lld tokens and %lld adapters: each group's workgroup reads the whole index, 2^36 times or more in all", who, (long long)T, (long long)n);
   const dim3 grid((unsigned)(n + 2)), block(kRouteBlock);
   hipStream_t st = (hipStream_t)stream;
   if (index_is_i64) hipLaunchKernelGGL(lowrank_route_kernel<int64_t>, grid, block, 0, st, (const int64_t *)index, (int)T, (int)n, order, starts);

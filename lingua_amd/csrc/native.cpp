@@ -1164,7 +1164,7 @@ int64_t number(PyObject *o) {
   if (v == -1 && PyErr_Occurred()) throw python_error();
   return v;
 }
-bool is_param(const Tensor &t, int64_t n, int device) { return !t.defined() || dense(t, t.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16, n, device); }
+bool is_param(const Tensor &t, int64_t n, int device) { return !t.defined() || (t.dim() == 1 && dense(t, t.scalar_type() == at::kFloat ? at::kFloat : at::kBFloat16, n, device)); }
 bool is_numbers(const Tensor &t, int device) { return !t.defined() || (t.dim() == 1 && dense(t, at::kLong, 2, device)); }
 void *addr(const Tensor &t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
 const void *caddr(const Tensor &t) { return t.defined() ? t.const_data_ptr() : nullptr; }

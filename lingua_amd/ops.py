@@ -879,8 +879,8 @@ def dropout(x: torch.Tensor, drop, residual: Optional[torch.Tensor] = None) -> t
 def _norm_param(t, C: int, device, what: str):
     if t is None:
         return None
-    if t.dtype not in (torch.bfloat16, torch.float32) or t.numel() != C or t.device != device:
-        raise RuntimeError(f"{what}: weight and bias must be bf16 or fp32 with C elements on the same device")
+    if t.dtype not in (torch.bfloat16, torch.float32) or t.shape != (C,) or t.device != device:
+        raise RuntimeError(f"{what}: weight and bias must be bf16 or fp32 [{C}] on the same device, got {t.dtype} {tuple(t.shape)} on {t.device}")
     return t.contiguous()
 
 
@@ -1078,19 +1078,27 @@ def _scale_arg(scale, n: int, device, what: str):
     return scale.contiguous()
 
 
-def lowrank_route(index: torch.Tensor, n: int):
-    """Tokens by adapter: (order int32 [T], starts int32 [n + 3]) of an int32 or int64 index [T] of 0 .. n - 1, -1 for none."""
+def lowrank_route(index: torch.Tensor, n: int, out=None):
+    """Tokens by adapter: (order int32 [T], starts int32 [n + 3]) of an int32 or int64 index [T] of 0 .. n - 1, -1 for none.  ``out``: such a
+    pair that receives them."""
     what = "lowrank_route"
     if index.dtype not in (torch.int32, torch.int64) or index.dim() != 1:
         raise RuntimeError(f"{what}: an int32 or int64 index of one dimension is wanted, got {index.dtype} {tuple(index.shape)}")
     st = _prep(index, what)
     index = index.contiguous()
     T, dev = index.shape[0], index.device
-    order = torch.empty((T,), dtype=torch.int32, device=dev)
-    starts = torch.empty((n + 3,), dtype=torch.int32, device=dev)
+    if out is None:
+        order = torch.empty((T,), dtype=torch.int32, device=dev)
+        starts = torch.empty((n + 3,), dtype=torch.int32, device=dev)
+    else:
+        order, starts = out
+        _plan_args(out, T, n, dev, what)
     with _timed(what, 8 * T, dev):
         code = _lib.load().l8_lowrank_route(index.data_ptr(), int(index.dtype == torch.int64), T, n, order.data_ptr(), starts.data_ptr(), st)
     _lib.check(code, "l8_lowrank_route")
+    if out is not None:
+        _wrote_into(order)
+        _wrote_into(starts)
     return order, starts
 
 

@@ -313,3 +313,62 @@ def test_modules(kind):
     assert not grads[0][1].any() and grads[0][2].any()      # adapter 1 has no request; the first's b is zero, and its a learns nothing yet
     with pytest.raises(RuntimeError, match="do not fit"):
         w1.load(3, down, up)
+
+
+def test_requests_of_a_captured_model():
+    """A captured forward pass of an adapted linear sees the requests that are set between its replays; another batch size in between leaves it
+    alone; setting requests between a forward and its backward pass is an error; a model that was rounded to bf16 as a whole still runs."""
+    from lingua_amd import adapters
+    requests = adapters.Requests(3)
+    lin = adapters.AdaptedLinear(torch.nn.Linear(64, 128, bias=False, dtype=torch.bfloat16, device="cuda"), requests, 8)
+    with torch.no_grad():
+        lin.b.copy_(seeded_bf16((3, 8, 128), std=0.3, seed=1))
+    lin.to(torch.bfloat16)
+    assert lin.scale.dtype == torch.bfloat16
+    x = seeded_bf16((40, 64), seed=2).cuda()
+    first = torch.arange(40, device="cuda") % 4 - 1
+    requests.set(first)
+    with torch.no_grad():
+        lin(x)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = lin(x)
+        for i in range(3):
+            requests.set(torch.zeros(7 + i, dtype=torch.int32, device="cuda"))
+            lin(x[:7 + i])
+            index = first.roll(i)
+            requests.set(index)
+            want = adapters.add_lowrank(lin.linear(x), x, lin.a, lin.b, index, lin.scale.float())
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(lin(x), want)
+    y = lin(x)
+    requests.set(first)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_inference_mode():
+    """Tensors without version counters go through every operator."""
+    from lingua_amd import adapters, dropout, norm, rope
+    n, r, K, N, T = 3, 16, 64, 128, 100
+    a, b, scale = bank(n, r, K, N)
+    x, y, w = seeded_bf16((T, K), seed=2).cuda(), seeded_bf16((T, N), seed=3).cuda(), seeded_bf16((K,), seed=4).cuda()
+    index, drop = tokens_of(T, n, "mixed"), dropout.Drop(0.2, dropout.numbers(1))
+    cos, sin = (t.cuda() for t in rope.rotary_tables(32, 200))
+    pos = torch.arange(2 * T, device="cuda").view(2, 1, T)
+
+    def run():
+        requests = adapters.Requests(n)
+        requests.set(index)
+        requests.set(index)
+        return (adapters.add_lowrank(y, x, a, b, index, scale), adapters.add_lowrank(y, x, a, b, requests.plan, scale), norm.layernorm(x, w, w, quantise=True),
+                *norm.add_layernorm(x, x, w, dropout=drop), *norm.add_rmsnorm(x, x, w, 1e-5, drop), dropout.dropout(x, drop),
+                *rope.rotary_axes(x.view(1, T, 2, 32), x.view(1, T, 2, 32), cos, sin, pos, (8, 8)))
+
+    want = run()
+    with torch.inference_mode():
+        x, y = x.clone(), y.clone()
+        assert all(torch.equal(u, v) for u, v in zip(run(), want))
