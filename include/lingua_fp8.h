@@ -428,7 +428,7 @@ int l8_rotary_axes(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D
                    const void *positions, int positions_i32, int64_t pos_axis, int64_t pos_b, int64_t pos_s, void *stream);
 
 /* Low-rank adapters of many requests beside a projection: out_t = y_t + scale_i (x_t A_i^T) B_i, i = index[t], A bf16 [n,r,K], B bf16 [n,r,N].
- * r a multiple of 8 up to 128, K and N multiples of 8 below 2^24, n up to 65535, T below 2^24 tokens, (n + 2) T below 2^36; rows of tokens and factors on 16-byte
+ * r a multiple of 8 up to 128, K and N multiples of 8 below 2^24, n up to 65534, T below 2^24 tokens, (n + 2) T below 2^36; rows of tokens and factors on 16-byte
  * lines; h fp32 [splits,T,r], 16-byte aligned, of which rows of tokens without an adapter are neither written nor read.
  *
  * route: tokens by adapter.  index int32 or (index_is_i64) int64 [T]: 0 .. n - 1, -1: none; any other: the token's results are NaN.
@@ -460,6 +460,12 @@ typedef struct {
 int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, int64_t T, int64_t n, int64_t r, const int *order, const int *starts,
                      void *workspace, int64_t workspace_bytes, void *stream);
 int64_t l8_lowrank_outer_workspace(int64_t T, int64_t r, int64_t K, int64_t N);
+/* One such side and, from the same reading of z, also = z F_i^T, fp32 [T,r], without the scale: outer of the factor B and shrink of the gradient.
+ * r up to 16, at least one token; l8_lowrank_outer_shrink_pays says (1 or 0) whether one reading is faster than two. */
+int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *scale, const void *f, float *also, int64_t T, int64_t n, int64_t r, const int *order,
+                            const int *starts, void *workspace, int64_t workspace_bytes, void *stream);
+int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r);
+int64_t l8_lowrank_outer_shrink_workspace(int64_t T, int64_t r, int64_t D);
 
 /* MXFP4 (OCP Microscaling formats 1.0): e2m1 codes in blocks of 32, the last block of a row possibly shorter, with an e8m0 scale each.
  *   byte = max(E - 2, 0), E the biased exponent of the block's amax; 255 (NaN), with codes 0, for a block with an inf or NaN

@@ -76,6 +76,9 @@ SIGNATURES = {
     "l8_lowrank_add": [_p, _i64, _p, _i64, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _i64, _p, _i64, _p, _i64, _p],
     "l8_lowrank_add_workspace": [_i64, _i64, _i64, _i64],
     "l8_lowrank_outer": [_p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
+    "l8_lowrank_outer_shrink": [_p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
+    "l8_lowrank_outer_shrink_pays": [_i64, _i64],
+    "l8_lowrank_outer_shrink_workspace": [_i64, _i64, _i64],
     "l8_lowrank_outer_workspace": [_i64, _i64, _i64, _i64],
     "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],
     "l8_cast_mxfp4_two": [_p, _p],
@@ -96,7 +99,7 @@ SIGNATURES = {
     "l8_gemm_pick": [_i64, _i64, _i64],
 }
 _RETURNS_STR = {"l8_last_error", "l8_gemm_algo_name"}
-_RETURNS_I64 = {"l8_cast_rowwise_workspace", "l8_gemm_workspace", "l8_gemm_workspace_gave_up_offset", "l8_swiglu_workspace", "l8_rmsnorm_workspace", "l8_rmsnorm_bwd_workspace", "l8_norm_bwd_workspace", "l8_lowrank_splits", "l8_lowrank_add_workspace", "l8_lowrank_outer_workspace",
+_RETURNS_I64 = {"l8_cast_rowwise_workspace", "l8_gemm_workspace", "l8_gemm_workspace_gave_up_offset", "l8_swiglu_workspace", "l8_rmsnorm_workspace", "l8_rmsnorm_bwd_workspace", "l8_norm_bwd_workspace", "l8_lowrank_splits", "l8_lowrank_add_workspace", "l8_lowrank_outer_shrink_workspace", "l8_lowrank_outer_workspace",
                 "l8_linear_fwd_workspace", "l8_linear_fwd_rows_workspace", "l8_col_sum_workspace", "l8_gemm_mxfp4_workspace", "l8_mxfp4_linear_workspace"}
 
 _lib = None

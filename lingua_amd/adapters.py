@@ -59,17 +59,21 @@ class LowRankFn(torch.autograd.Function):
         varies = f8._learns(gy)
         with torch.no_grad():
             sides = []
+            together = need_b and (need_x or need_a) and ops.lowrank_outer_shrink_pays(gy.shape[0], r)
             if need_x or need_a:
-                gh = ops.lowrank_shrink(gy, b, plan)
+                if together:
+                    gb, gh = ops.lowrank_outer_shrink(h, gy, b, scale, plan)
+                else:
+                    gh = ops.lowrank_shrink(gy, b, plan)
                 if need_x:
                     gx = ops.lowrank_expand(None, gh, a, scale, plan)
                 if need_a:
                     sides.append((gh, x))
-            if need_b:
+            if need_b and not together:
                 sides.append((h, gy))
             if sides:
                 grads = ops.lowrank_outer(sides, scale, n, r, plan)
-                gb = grads.pop() if need_b else None
+                gb = grads.pop() if need_b and not together else gb
                 ga = grads.pop() if need_a else None
         lx, la, lb = ctx.learns
         gx, ga, gb = f8._once("add_lowrank", (gx, ga, gb), (varies or la or lb, varies or lx or lb, varies or lx or la))

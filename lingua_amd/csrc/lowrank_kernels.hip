@@ -513,6 +513,8 @@ struct OuterArgs {
   const float *scale;
   const int *order, *starts;
   int T, n, r, size;
+  const uint16_t *f;         // with ALSO_H: the factor that z is multiplied with, [n, r, D]
+  float *also;               //              and where that goes, [chunks, T, r], a part for each 512 columns
 };
 
 constexpr int kOuterWaves = 4;
@@ -524,9 +526,15 @@ L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)
 // RT tiles of 16 ranks by 128 columns a wave, over a tile's tokens.  z is read as `expand` reads the factor: eight neighbouring columns of
 // eight tokens' rows a lane, turned round in registers, 32 tokens requested ahead; h is laid out by rank in LDS, TOKENS at a time, both
 // halves of its bits.  Two waves a SIMD: 64 ranks of [16384,4096] and [16384,4096] 130 us where the compiler made room for one, 107.
-template <int RT, int TOKENS>
+//
+// With ALSO_H the kernel also does `shrink`'s work on z, which both read whole: 32 tokens by a wave's 128 columns go through LDS of the wave's
+// own, whose rows are what the matrix instruction wants them to be, and meet the factor's 128 columns, which stay in registers; every 64
+// tokens the waves' sums are added up.  Up to 16 ranks, whose registers leave room for that.
+template <int RT, int TOKENS, bool ALSO_H>
 __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(const OuterArgs p) {
-  constexpr int PITCH = TOKENS + 8;
+  constexpr int PITCH = TOKENS + 8, ZPITCH = 128 + 8;
+  __shared__ __attribute__((aligned(16))) uint16_t zs[ALSO_H ? kOuterWaves : 1][ALSO_H ? 32 : 1][ZPITCH];
+  static_assert(!ALSO_H || 64 * RT * 16 * 4 <= 32 * ZPITCH * 2, "a wave's sums of 64 tokens take the place of its z");
   __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][PITCH];
   __shared__ __attribute__((aligned(16))) int toks[TOKENS];
   const Tile tile = tile_of(p.starts, p.n, p.size, blockIdx.x);
@@ -546,6 +554,19 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
   for (int m = 0; m < RT; ++m)
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+  [[maybe_unused]] v4i f[ALSO_H ? 4 : 1][RT];
+  [[maybe_unused]] v4f sums[2][ALSO_H ? 2 : 1][RT];   // of 64 tokens: by 32, by 16
+  if constexpr (ALSO_H) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = (chunk * kOuterWaves + wave) * 128 + k * 32 + g * 8;
+#pragma unroll
+      for (int j = 0; j < RT; ++j) {
+        f[k][j] = *(const v4i *)(p.f + ((int64_t)tile.group * r + min(j * 16 + row, r - 1)) * D + (at < D ? at : 0));
+        if (at >= D) f[k][j] = v4i{0, 0, 0, 0};
+      }
+    }
+  }
 #pragma unroll 1
   for (int p0 = 0; p0 < tile.count; p0 += TOKENS) {
     const int here = min(TOKENS, tile.count - p0), subs = (here + 31) / 32;
@@ -578,6 +599,23 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
         for (int e = 0; e < 8; ++e)
           if (sub * 32 + g * 8 + e >= here) z8[e] = v4i{0, 0, 0, 0};
       }
+      if constexpr (ALSO_H) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) *(v4i *)&zs[wave][g * 8 + e][row * 8] = in ? z8[e] : v4i{0, 0, 0, 0};   // (columns that are not there: both factors zero)
+        __builtin_amdgcn_wave_barrier();   // one wave's own LDS: it keeps the order of what it issues
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+          for (int j = 0; j < RT; ++j) sums[s][m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const v4i a = *(const v4i *)&zs[wave][m * 16 + row][k * 32 + g * 8];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) sums[s][m][j] = mfma(a, f[k][j], sums[s][m][j]);
+          }
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
       v4i b[8];
       transpose8(b, z8);
 #pragma unroll
@@ -589,14 +627,42 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
           for (int j = 0; j < 8; ++j) acc[m][j] = mfma(a, b[j], acc[m][j]);
         }
     };
+    [[maybe_unused]] auto hand_over = [&](int sub, int count) {   // the sums of `count` times 32 tokens from 32 sub on
+      if constexpr (ALSO_H) {
+        float *mine = (float *)&zs[wave][0][0];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h >= count) break;
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int j = 0; j < RT; ++j)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mine[(h * 32 + m * 16 + g * 4 + i) * (RT * 16) + j * 16 + row] = sums[h][m][j][i];
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < count * 32 * RT * 16; i += kOuterWaves * 64) {
+          const int at = sub * 32 + i / (RT * 16), rank = i % (RT * 16);
+          float v = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kOuterWaves; ++w) v += ((const float *)&zs[w][0][0])[i];
+          if (at < here && rank < r) p.also[((int64_t)chunk * p.T + toks[at]) * r + rank] = v;
+        }
+        __syncthreads();
+      }
+    };
     request(0, 0);
 #pragma unroll 1
     for (int sub = 0; sub < subs; sub += 2) {
       request(1, min(sub + 1, subs - 1));
       multiply(0, sub);
-      if (sub + 1 >= subs) break;
+      if (sub + 1 >= subs) {
+        hand_over(sub, 1);
+        break;
+      }
       request(0, min(sub + 2, subs - 1));
       multiply(1, sub + 1);
+      hand_over(sub, 2);
     }
   }
   if (!in) return;
@@ -621,8 +687,23 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
     }
 }
 
-// The sums of a group's tiles, in their order, rounded: groups of more than one tile.
-__global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int64_t blocks0) {
+// h = the sum of its parts, in their order: the workgroups of row n of `fold`'s grid.
+L8_DEV void sum_parts(const float *__restrict__ parts, int count, int64_t n, float *__restrict__ h) {
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < n; at += (int64_t)gridDim.x * 1024) {
+    v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (int i = 0; i < count; ++i) {
+      const v4f u = *(const v4f *)(parts + i * n + at);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += u[e];
+    }
+    *(v4f *)(h + at) = v;
+  }
+}
+
+// The sums of a group's tiles, in their order, rounded: groups of more than one tile.  (And with `h`, row n: the sum of its parts.)
+__global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int64_t blocks0, float *__restrict__ h) {
+  if ((int)blockIdx.y == p.n) return sum_parts(p.also, p.side[1].chunks, (int64_t)p.T * p.r, h);
   const int from = p.starts[blockIdx.y], tokens = p.starts[blockIdx.y + 1] - from;
   if (tokens <= p.size) return;
   const int which = (int64_t)blockIdx.x >= blocks0;
@@ -648,7 +729,7 @@ __global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, in
 
 // ---- host ----
 
-constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 65535, kMaxCols = 1 << 24;
+constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 65534, kMaxCols = 1 << 24;
 
 // Tokens of a tile: 64, which read a factor a quarter as often, where the adapters have that many on average.
 static int tile_tokens(int64_t T, int64_t n) { return T >= 64 * (n + 1) ? 64 : 16; }
@@ -672,7 +753,7 @@ static int outer_size(int64_t T, int64_t K, int64_t N) {
 static bool rows_fit(const void *p, int64_t ld, int64_t cols) { return p && ((uintptr_t)p % 16) == 0 && ld % 8 == 0 && ld >= cols; }
 static int check_sizes(const char *who, int64_t T, int64_t n, int64_t r, int64_t D) {
   L8_REQUIRE(T >= 0 && T < kMaxTokens, "%s: %lld tokens, fewer than 2^24 are wanted", who, (long long)T);
-  L8_REQUIRE(n >= 1 && n <= kMaxAdapters, "%s: %lld adapters, 1 to 65535 are wanted", who, (long long)n);
+  L8_REQUIRE(n >= 1 && n <= kMaxAdapters, "%s: %lld adapters, 1 to 65534 are wanted", who, (long long)n);
   L8_REQUIRE(r >= 8 && r <= kMaxRank && r % 8 == 0, "%s: rank %lld is not a multiple of 8 up to %lld", who, (long long)r, (long long)kMaxRank);
   L8_REQUIRE(D >= 8 && D % 8 == 0 && D < kMaxCols, "%s: %lld columns, a multiple of 8 below 2^24 is wanted", who, (long long)D);
   return L8_OK;
@@ -861,15 +942,57 @@ extern "C" int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, 
   L8_CALL(check_grid(who, slots, chunks, ranks, kOuterWaves * 64));
   const dim3 grid((unsigned)slots, (unsigned)chunks, (unsigned)ranks), block(kOuterWaves * 64);
   hipStream_t st = (hipStream_t)stream;
-  if (r <= 16) hipLaunchKernelGGL((lowrank_outer_kernel<1, 256>), grid, block, 0, st, p);
-  else if (r <= 32) hipLaunchKernelGGL((lowrank_outer_kernel<2, 256>), grid, block, 0, st, p);
-  else hipLaunchKernelGGL((lowrank_outer_kernel<4, 128>), grid, block, 0, st, p);
+  if (r <= 16) hipLaunchKernelGGL((lowrank_outer_kernel<1, 256, false>), grid, block, 0, st, p);
+  else if (r <= 32) hipLaunchKernelGGL((lowrank_outer_kernel<2, 256, false>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((lowrank_outer_kernel<4, 128, false>), grid, block, 0, st, p);
   L8_HIP(hipGetLastError());
   if (parts) {
     const int64_t b0 = (r * D[0] + 2047) / 2048, b1 = (r * D[1] + 2047) / 2048;
     L8_CALL(check_grid(who, b0 + b1, 1, n, 256));
-    hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)(b0 + b1), (unsigned)n), dim3(256), 0, st, p, b0);
+    hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)(b0 + b1), (unsigned)n), dim3(256), 0, st, p, b0, (float *)nullptr);
     L8_HIP(hipGetLastError());
   }
+  return L8_OK;
+}
+
+// Does one reading of z for both pay?  Wherever its registers allow it, us, one reading and two: [16384,11008] 108 and 177, [4096,4096] 19.5 and
+// 28.3, [1021,2064] 12.5 and 18.1, [256,1024] 11.4 and 18.5 (the parts of h are summed up in the launch that folds the factor's gradients).
+extern "C" int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r) { return T >= 1 && r <= 16; }
+
+extern "C" int64_t l8_lowrank_outer_shrink_workspace(int64_t T, int64_t r, int64_t D) {
+  if (T <= 0 || r <= 0 || D <= 0) return 0;
+  return (D + 511) / 512 * T * r * (int64_t)sizeof(float) + l8_lowrank_outer_workspace(T, r, 0, D);
+}
+
+extern "C" int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *scale, const void *f, float *also, int64_t T, int64_t n, int64_t r, const int *order, const int *starts,
+                                       void *workspace, int64_t workspace_bytes, void *stream) {
+  const char *who = "l8_lowrank_outer_shrink";
+  L8_REQUIRE(one && one->grad && ((uintptr_t)one->grad % 16) == 0, "%s: null or misaligned gradient", who);
+  const int64_t D = one->D;
+  L8_CALL(check_sizes(who, T, n, r, D));
+  L8_REQUIRE(r <= 16, "%s: rank %lld, up to 16 are wanted", who, (long long)r);
+  L8_REQUIRE(T >= 1, "%s: no tokens", who);
+  L8_CALL(check_plan(who, T, order, starts));
+  L8_REQUIRE(one->splits >= 1 && one->splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)one->splits);
+  L8_REQUIRE(rows_fit(one->z, one->ldz, D) && rows_fit(f, D, D) && one->h && ((uintptr_t)one->h % 16) == 0 && also && ((uintptr_t)also % 16) == 0 && ((uintptr_t)scale % 4) == 0,
+             "%s: null or misaligned operand, or rows off 16-byte lines", who);
+  const int64_t need = l8_lowrank_outer_shrink_workspace(T, r, D);
+  L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
+  OuterArgs p{};
+  const int size = outer_size(T, 0, D);
+  const int64_t chunks = (D + 511) / 512, parts = T <= size ? 0 : 2 * (T / size + 1), slots = tile_slots(T, n, size), b1 = (r * D + 2047) / 2048;
+  p.side[1] = OuterSide{one->h, (const uint16_t *)one->z, (uint16_t *)one->grad, (float *)workspace + chunks * T * r, one->ldz, (int)D, (int)one->splits, (int)chunks};
+  p.scale = scale, p.order = order, p.starts = starts, p.T = (int)T, p.n = (int)n, p.r = (int)r, p.size = size;
+  p.f = (const uint16_t *)f, p.also = (float *)workspace;
+  // one launch for both sums: row n is that of h's parts; without groups of several tiles the other rows end at once
+  const int64_t sums = (T * r + 1023) / 1024, x = std::max<int64_t>(parts ? b1 : 1, std::min<int64_t>(sums, 4 * num_cus()));
+  L8_CALL(check_grid(who, slots, chunks, 1, kOuterWaves * 64));
+  L8_CALL(check_grid(who, x, 1, n + 1, 256));
+  const dim3 grid((unsigned)slots, (unsigned)chunks), block(kOuterWaves * 64);
+  hipStream_t st = (hipStream_t)stream;
+  hipLaunchKernelGGL((lowrank_outer_kernel<1, 128, true>), grid, block, 0, st, p);
+  L8_HIP(hipGetLastError());
+  hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)x, (unsigned)(n + 1)), dim3(256), 0, st, p, (int64_t)0, also);
+  L8_HIP(hipGetLastError());
   return L8_OK;
 }

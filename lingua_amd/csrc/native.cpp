@@ -36,7 +36,7 @@ struct Library {
   X(l8_rmsnorm_workspace) X(l8_rmsnorm_bwd_as) X(l8_rmsnorm_bwd_workspace) X(l8_swiglu_cast_rowwise) X(l8_swiglu_workspace)        \
   X(l8_swiglu_bwd_cast_rowwise_q) X(l8_swiglu_bwd_cast_transposed) X(l8_add_rmsnorm_cast_rowwise) X(l8_add_rmsnorm_bwd) X(l8_rotary)     \
   X(l8_rotary_axes) X(l8_dropout) X(l8_norm_fwd) X(l8_norm_bwd) X(l8_norm_bwd_workspace) X(l8_lowrank_route) X(l8_lowrank_shrink) X(l8_lowrank_splits)   \
-  X(l8_lowrank_expand) X(l8_lowrank_outer) X(l8_lowrank_outer_workspace) X(l8_lowrank_add) X(l8_lowrank_add_workspace)                   \
+  X(l8_lowrank_expand) X(l8_lowrank_outer) X(l8_lowrank_outer_workspace) X(l8_lowrank_outer_shrink) X(l8_lowrank_outer_shrink_pays) X(l8_lowrank_outer_shrink_workspace) X(l8_lowrank_add) X(l8_lowrank_add_workspace)                   \
   X(l8_cast_mxfp4) X(l8_cast_mxfp4_two) X(l8_mxfp4_to_bf16) X(l8_gemm_mxfp4_nt) X(l8_gemm_mxfp4_workspace) X(l8_mxfp4_linear) X(l8_mxfp4_linear_workspace)
   L8_ENTRIES(L8_ENTRY)
 #undef L8_ENTRY
@@ -1437,29 +1437,41 @@ struct LowRank : torch::autograd::Function<LowRank> {
                  h = need_b ? bank_rows(saved[3]) : Tensor();
     Tensor gh, gx, ga, gb;
     Bank f;
+    const float *sp = scale.defined() ? scale.const_data_ptr<float>() : nullptr;
+    const bool together = need_b && (need_x || need_a) && lib.l8_lowrank_outer_shrink_pays(rg.rows, r);
     if (need_x || need_a) {
       TORCH_CHECK(as_bank(b, device, f), "add_lowrank backward: factors");
-      gh = lowrank_h(rg, gy, f, order, starts, stream);
+      if (together) {
+        gb = at::empty({n, r, N}, gy.options()), gh = at::empty({1, rg.rows, r}, gy.options().dtype(at::kFloat));
+        const l8_lowrank_side one = {h.const_data_ptr<float>(), h.size(0), rg.p, rg.ld, N, gb.mutable_data_ptr()};
+        const int64_t bytes = lib.l8_lowrank_outer_shrink_workspace(rg.rows, r, N);
+        const Space ws(gy, bytes);
+        check(lib.l8_lowrank_outer_shrink(&one, sp, f.p, gh.mutable_data_ptr<float>(), rg.rows, n, r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), ws.p(), bytes, stream),
+              "l8_lowrank_outer_shrink");
+      } else {
+        gh = lowrank_h(rg, gy, f, order, starts, stream);
+      }
     }
     if (need_x) {
       TORCH_CHECK(as_bank(a, device, f), "add_lowrank backward: factors");
       gx = at::empty(ctx->saved_data["like"].toIntVector(), gy.options());
       lowrank_out(Rows(), gh, scale, f, order, starts, gx, stream);
     }
-    if (need_a || need_b) {
+    const bool side_b = need_b && !together;
+    if (need_a || side_b) {
       l8_lowrank_side two[2] = {};
       if (need_a) {
         ga = at::empty({n, r, K}, gy.options());
         const Rows rx = rows_of(x);
         two[0] = {gh.const_data_ptr<float>(), gh.size(0), rx.p, rx.ld, K, ga.mutable_data_ptr()};
       }
-      if (need_b) {
+      if (side_b) {
         gb = at::empty({n, r, N}, gy.options());
         two[1] = {h.const_data_ptr<float>(), h.size(0), rg.p, rg.ld, N, gb.mutable_data_ptr()};
       }
-      const int64_t bytes = lib.l8_lowrank_outer_workspace(rg.rows, r, need_a ? K : 0, need_b ? N : 0);
+      const int64_t bytes = lib.l8_lowrank_outer_workspace(rg.rows, r, need_a ? K : 0, side_b ? N : 0);
       const Space ws(gy, bytes);
-      check(lib.l8_lowrank_outer(two, scale.defined() ? scale.const_data_ptr<float>() : nullptr, rg.rows, n, r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), ws.p(), bytes,
+      check(lib.l8_lowrank_outer(two, sp, rg.rows, n, r, order.const_data_ptr<int>(), starts.const_data_ptr<int>(), ws.p(), bytes,
                                  stream), "l8_lowrank_outer");
     }
     const bool g = learns(grads[0]), lx = learnt & 1, la = learnt & 2, lb = learnt & 4;

@@ -1212,6 +1212,33 @@ def lowrank_outer(sides, scale: Optional[torch.Tensor], n: int, r: int, plan):
     return grads
 
 
+def lowrank_outer_shrink_pays(T: int, r: int) -> bool:
+    """Is ``lowrank_outer_shrink`` faster than its two parts one after the other?"""
+    return bool(_lib.load().l8_lowrank_outer_shrink_pays(T, r))
+
+
+def lowrank_outer_shrink(h: torch.Tensor, z: torch.Tensor, f: torch.Tensor, scale: Optional[torch.Tensor], plan):
+    """``lowrank_outer([(h, z)], scale, n, r, plan)[0]`` and ``lowrank_shrink(z, f, plan)`` from one reading of z; ranks up to 16, at least one
+    token."""
+    what = "lowrank_outer_shrink"
+    z, f = _rows_on_lines(z, torch.bfloat16, what), _factor(f, what)
+    st = _prep(z, what)
+    (T, D), (n, r, D2), dev = z.shape, f.shape, z.device
+    if D != D2 or f.device != dev:
+        raise RuntimeError(f"{what}: rows of {D} and factors of {D2} features on {dev} and {f.device}")
+    h, scale = _h_arg(h, T, r, dev, what), _scale_arg(scale, n, dev, what)
+    order, starts = _plan_args(plan, T, n, dev, what)
+    grad = torch.empty((n, r, D), dtype=torch.bfloat16, device=dev)
+    also = torch.empty((1, T, r), dtype=torch.float32, device=dev)
+    with _timed(what, 2 * T * D + 4 * f.numel() + 8 * T * r, dev):
+        need = _lib.load().l8_lowrank_outer_shrink_workspace(T, r, D)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        code = _lib.load().l8_lowrank_outer_shrink(struct.pack("6q", h.data_ptr(), h.shape[0], z.data_ptr(), _ld(z), D, grad.data_ptr()), _addr(scale) or None, f.data_ptr(),
+                                                   also.data_ptr(), T, n, r, order, starts, _addr(ws) or None, need, st)
+    _lib.check(code, "l8_lowrank_outer_shrink")
+    return grad, also
+
+
 # ---- MXFP4: e2m1 codes, two a byte, in blocks of 32 along a row, with an e8m0 scale each ----
 
 MX_BLOCK = 32

@@ -75,6 +75,48 @@ def test_groups_of_several_tiles(T, n, how, host):
     run(T, n, 40, 520, 16, how, seed=T)
 
 
+@pytest.mark.parametrize("T, n, how", [(300, 2, "mixed"), (1000, 1, "one"), (70, 5, "runs"), (2900, 3, "mixed"), (1, 1, "one"), (65, 2, "none")])
+@pytest.mark.parametrize("r, D", [(8, 8), (16, 136), (8, 520), (16, 1160), (16, 512)])
+def test_gradient_and_product_from_one_reading(T, n, how, r, D):
+    """The factor's gradient is `outer`'s, the product within its error of 64 bits, rows of no adapter aside; values that are not finite stay in
+    their tokens."""
+    from lingua_amd import ops
+    _, b, scale = bank(n, r, 8, D, seed=T)
+    z = seeded_bf16((T, D), seed=1).cuda()
+    h = torch.randn((2, T, r), generator=torch.Generator().manual_seed(2)).cuda()
+    index = tokens_of(T, n, how, seed=T)
+    plan = ops.lowrank_route(index, n)
+    z[T // 2, D - 1] = float("inf")
+    grad, also = ops.lowrank_outer_shrink(h, z, b, scale, plan)
+    want, = ops.lowrank_outer([(h, z)], scale, n, r, plan)
+    # (tiles of other sizes: sums in another order)
+    bad = ~want.isfinite()
+    assert torch.equal(bad, ~grad.isfinite())
+    plain_sum = torch.zeros(b.shape, dtype=torch.float64)
+    size = plain_sum.clone()
+    hd, zd = h.double().sum(0).cpu(), z.double().cpu()
+    for i in range(n):
+        at = (index == i).nonzero()[:, 0].cpu()
+        plain_sum[i] = float(scale[i]) * (hd[at].t() @ zd[at])
+        size[i] = float(scale[i]) * (plain.SPLIT + plain.FP32 * (2 * len(at) + 24)) * (hd[at].abs().t() @ zd[at].abs())
+    assert within(grad[~bad], plain_sum[~bad.cpu()], size[~bad.cpu()])
+    for i in range(n):
+        at = (index == i).nonzero()[:, 0].cpu()
+        got, x, f = also[0].double().cpu()[at], zd[at], b[i].double().cpu()
+        want = x @ f.t()
+        fine = x.isfinite().all(1)
+        assert bool(((got - want).abs() <= plain.FP32 * (D + 16) * (x.abs() @ f.abs().t()))[fine].all()) and not bool(got[~fine].isfinite().any())
+
+
+@pytest.mark.parametrize("T, n", [(4300, 2), (9000, 7)])
+def test_large_backward(T, n, host):
+    """A pass that reads the gradient once for both."""
+    from lingua_amd import ops
+    K, N = 72, 4104
+    assert ops.lowrank_outer_shrink_pays(T, 16) and not ops.lowrank_outer_shrink_pays(T, 24)
+    run(T, n, 16, K, N, "mixed", seed=T)
+
+
 @pytest.mark.parametrize("T", [1, 5, 64, 1023, 1024, 1025, 5000])
 @pytest.mark.parametrize("n", [1, 3, 64, 200])
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])

@@ -69,7 +69,7 @@ SHRINK = dict(x=P, T=64, K=128, ldx=128, f=P, n=4, r=16, order=P, starts=P, h=P,
 EXPAND = dict(y=P, ldy=128, h=P, splits=2, scale=P, f=P, T=64, N=128, n=4, r=16, order=P, starts=P, out=P, ldo=128, stream=None)
 
 
-@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(n=1 << 16), dict(T=1 << 23, n=8191), dict(index=None), dict(index=P + 2), dict(index=P + 4, i64=1), dict(order=None), dict(order=P + 2),
+@pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(n=65535), dict(T=1 << 23, n=8191), dict(index=None), dict(index=P + 2), dict(index=P + 4, i64=1), dict(order=None), dict(order=P + 2),
                                     dict(starts=None), dict(starts=P + 1)])
 def test_route_is_refused(change):
     assert refused("l8_lowrank_route", *{**ROUTE, **change}.values())
@@ -77,7 +77,7 @@ def test_route_is_refused(change):
 
 @pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(n=1 << 17), dict(r=0), dict(r=12), dict(r=136), dict(K=0), dict(K=12, ldx=16), dict(K=1 << 24, ldx=1 << 24),
                                     dict(x=None), dict(x=P + 8), dict(ldx=120), dict(ldx=132), dict(f=None), dict(f=P + 8), dict(h=None), dict(h=P + 4), dict(order=None), dict(starts=None),
-                                    dict(splits=0), dict(splits=65), dict(T=(1 << 24) - 1, n=65535, splits=64)])
+                                    dict(splits=0), dict(splits=65), dict(T=(1 << 24) - 1, n=65534, splits=64)])
 def test_shrink_is_refused(change):
     assert refused("l8_lowrank_shrink", *{**SHRINK, **change}.values())
 
@@ -95,13 +95,24 @@ OUTER = dict(scale=P, T=64, n=4, r=16, order=P, starts=P, ws=None, ws_bytes=0, s
 
 @pytest.mark.parametrize("change", [dict(T=-1), dict(T=1 << 24), dict(n=0), dict(r=20), dict(D=0), dict(D=20, ldz=24), dict(h=0), dict(h=P + 8), dict(splits=0), dict(z=0), dict(z=P + 8), dict(ldz=120),
                                     dict(ldz=132), dict(grad=P + 8), dict(scale=P + 2), dict(order=None), dict(starts=None), dict(T=10000), dict(T=10000, ws=P, ws_bytes=64),
-                                    dict(T=10000, ws=P + 8, ws_bytes=1 << 40), dict(T=(1 << 24) - 1, n=65535, ws=P, ws_bytes=1 << 60, D=1 << 20, ldz=1 << 20)])
+                                    dict(T=10000, ws=P + 8, ws_bytes=1 << 40), dict(T=(1 << 24) - 1, n=65534, ws=P, ws_bytes=1 << 60, D=1 << 20, ldz=1 << 20)])
 def test_outer_is_refused(change):
     side = {**SIDE, **{k: v for k, v in change.items() if k in SIDE}}
     rest = {**OUTER, **{k: v for k, v in change.items() if k in OUTER}}
     for first in (True, False):
         both = (side, SIDE) if first else (SIDE, side)
         assert refused("l8_lowrank_outer", struct.pack("12q", *both[0].values(), *both[1].values()), *rest.values())
+
+
+BOTH = dict(scale=P, f=P, also=P, T=64, n=4, r=16, order=P, starts=P, ws=P, ws_bytes=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize("change", [dict(T=0), dict(T=-1), dict(n=0), dict(r=24), dict(r=4), dict(D=20, ldz=24), dict(h=0), dict(splits=65), dict(z=P + 8), dict(ldz=120), dict(grad=0), dict(grad=P + 8),
+                                    dict(f=None), dict(f=P + 8), dict(also=None), dict(also=P + 4), dict(scale=P + 2), dict(order=None), dict(starts=None), dict(ws=None), dict(ws=P + 8),
+                                    dict(ws_bytes=64)])
+def test_outer_with_shrink_is_refused(change):
+    side = {**SIDE, **{k: v for k, v in change.items() if k in SIDE}}
+    assert refused("l8_lowrank_outer_shrink", struct.pack("6q", *side.values()), *{**BOTH, **{k: v for k, v in change.items() if k in BOTH}}.values())
 
 
 def test_lowrank_splits_and_workspace():
