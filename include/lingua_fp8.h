@@ -433,7 +433,7 @@ int l8_rotary_axes(const l8_rotary_operand *two, int64_t B, int64_t S, int64_t D
  *
  * route: tokens by adapter.  index int32 or (index_is_i64) int64 [T]: 0 .. n - 1, -1: none; any other: the token's results are NaN.
  * order int32 [T], starts int32 [n+3]: adapter i's tokens are order[starts[i] .. starts[i+1]), in their order; then those with none, then the
- * others. */
+ * others.  (Whoever reads them holds what he reads to its range: other contents make undefined results, no access out of bounds.) */
 int l8_lowrank_route(const void *index, int index_is_i64, int64_t T, int64_t n, int *order, int *starts, void *stream);
 /* h = x F_i^T, F = A (forward) or, with x the output's gradient, B (backward), without the scale; in `splits` parts (l8_lowrank_splits says how
  * many pay). */

@@ -144,7 +144,8 @@ class Requests:
         key = index.shape, index.device
         plan = self._plans.get(key)
         if plan is None:
-            plan = self._plans[key] = route(index, self.n)
+            with torch.inference_mode(False):   # (a training step may be the next to want it)
+                plan = self._plans[key] = route(index, self.n)
         else:
             ops.lowrank_route(index.flatten(), self.n, out=(plan.order, plan.starts))
         self.plan = plan

@@ -124,13 +124,16 @@ struct Tile {
   int mine;                    // lane m has token m
   L8_DEV int token(int m) const { return __shfl(mine, min(m, count - 1)); }
 };
+// What is read of `order` and `starts` is held to their range, so that memory that `route` has not written yet (it was captured and not replayed,
+// or runs on another stream) makes wrong results and no access out of bounds.
+L8_DEV int within(int v, int top) { return (int)min((unsigned)v, (unsigned)top); }
 // Tile `slot` of at most `size` tokens.  The same for the whole workgroup.
-L8_DEV Tile tile_of(const int *__restrict__ starts, int n, int size, int slot) {
+L8_DEV Tile tile_of(const int *__restrict__ starts, int T, int n, int size, int slot) {
   const int lane = threadIdx.x & 63;
   Tile t{};
   int before = 0;
   for (int i0 = 0;; i0 += 64) {   // the groups whose first number is at most `slot` come first
-    const int i = i0 + lane, from = starts[min(i, n + 1)], to = starts[min(i, n + 1) + 1];
+    const int i = i0 + lane, from = within(starts[min(i, n + 1)], T), to = within(starts[min(i, n + 1) + 1], T);
     const int have = __popcll(__ballot(i < n + 2 && from / size + i <= slot));
     if (have) {
       const int at = have - 1;
@@ -143,14 +146,15 @@ L8_DEV Tile tile_of(const int *__restrict__ starts, int n, int size, int slot) {
   t.piece = slot - (before / size + t.group);
   t.first = before + t.piece * size;
   t.count = min(size, max(0, t.tokens - t.piece * size));
+  if (t.piece < 0) t.count = 0, t.piece = 1;   // (starts that do not ascend)
   return t;
 }
 // The same with its tokens: up to 64.
 L8_DEV Tile tile_with_tokens(const Tokens &tk, int T, int n, int size, int slot) {
   const int lane = threadIdx.x & 63;
   if (tk.order) {
-    Tile t = tile_of(tk.starts, n, size, slot);
-    t.mine = t.count ? tk.order[t.first + min(lane, t.count - 1)] : 0;
+    Tile t = tile_of(tk.starts, T, n, size, slot);
+    t.mine = t.count ? within(tk.order[t.first + min(lane, t.count - 1)], T - 1) : 0;
     return t;
   }
   // few tokens: every lane finds the tokens of its own group, bit by bit of the group's number; every sixteenth of a group begins a tile
@@ -537,7 +541,7 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
   static_assert(!ALSO_H || 64 * RT * 16 * 4 <= 32 * ZPITCH * 2, "a wave's sums of 64 tokens take the place of its z");
   __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][PITCH];
   __shared__ __attribute__((aligned(16))) int toks[TOKENS];
-  const Tile tile = tile_of(p.starts, p.n, p.size, blockIdx.x);
+  const Tile tile = tile_of(p.starts, p.T, p.n, p.size, blockIdx.x);
   if (tile.group >= p.n || (tile.count == 0 && tile.piece > 0)) return;
   const int which = (int)blockIdx.y >= p.side[0].chunks;
   const OuterSide &sd = p.side[which];
@@ -573,7 +577,7 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
     __syncthreads();
     for (int i = threadIdx.x; i < TOKENS * RT * 2; i += kOuterWaves * 64) {   // eight ranks of a token; neighbouring lanes write neighbouring tokens
       const int at = i % TOKENS, k = i / TOKENS * 8;
-      const int token = p.order[tile.first + p0 + min(at, here - 1)];
+      const int token = within(p.order[tile.first + p0 + min(at, here - 1)], p.T - 1);
       if (k == 0) toks[at] = token;
       float v[8];
       if (at < here && rank0 + k < r) {
@@ -704,7 +708,7 @@ L8_DEV void sum_parts(const float *__restrict__ parts, int count, int64_t n, flo
 // The sums of a group's tiles, in their order, rounded: groups of more than one tile.  (And with `h`, row n: the sum of its parts.)
 __global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int64_t blocks0, float *__restrict__ h) {
   if ((int)blockIdx.y == p.n) return sum_parts(p.also, p.side[1].chunks, (int64_t)p.T * p.r, h);
-  const int from = p.starts[blockIdx.y], tokens = p.starts[blockIdx.y + 1] - from;
+  const int from = within(p.starts[blockIdx.y], p.T), tokens = within(p.starts[blockIdx.y + 1], p.T) - from;
   if (tokens <= p.size) return;
   const int which = (int64_t)blockIdx.x >= blocks0;
   const OuterSide &sd = p.side[which];

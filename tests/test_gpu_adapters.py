@@ -414,3 +414,48 @@ def test_inference_mode():
     with torch.inference_mode():
         x, y = x.clone(), y.clone()
         assert all(torch.equal(u, v) for u, v in zip(run(), want))
+
+
+def test_requests_first_set_in_inference_mode():
+    """A batch shape that an evaluation in inference mode had first is trained on afterwards, and the other way round."""
+    from lingua_amd import adapters
+    n, r, K, N, T = 3, 16, 64, 128, 100
+    a, b, scale = bank(n, r, K, N)
+    x, y, index = seeded_bf16((T, K), seed=2).cuda(), seeded_bf16((T, N), seed=3).cuda(), tokens_of(T, n, "mixed")
+    want = adapters.add_lowrank(y, x, a, b, index, scale)
+    requests = adapters.Requests(n)
+    with torch.inference_mode():
+        requests.set(index.clone())
+        assert torch.equal(adapters.add_lowrank(y, x, a, b, requests.plan, scale), want)
+    for k in range(2):
+        requests.set(index.roll(k))
+        leaf = a.clone().requires_grad_()
+        got = adapters.add_lowrank(y, x, leaf, b, requests.plan, scale)
+        assert torch.equal(got, adapters.add_lowrank(y, x, a, b, index.roll(k), scale))
+        got.float().sum().backward()
+        assert leaf.grad.isfinite().all()
+        with torch.inference_mode():
+            requests.set(index)
+            assert torch.equal(adapters.add_lowrank(y, x, a, b, requests.plan, scale), want)
+
+
+@pytest.mark.parametrize("r", [16, 32, 64])
+@pytest.mark.parametrize("T, n", [(40, 3), (300, 2), (1000, 70)])
+def test_an_order_that_route_did_not_make(T, n, r):
+    """Contents of an order that has not been written yet: results are whatever they are, and what lies around the outputs stays as it was."""
+    from lingua_amd import ops
+    K, N, guard = 72, 136, 64
+    a, b, scale = bank(n, r, K, N)
+    x, y = seeded_bf16((T, K), seed=2).cuda(), seeded_bf16((T, N), seed=3).cuda()
+    g = torch.Generator().manual_seed(T + r)
+    for k in range(4):
+        low, high = [(-2 ** 31, 2 ** 31), (-5, T + 5), (0, 1), (T, T + 1)][k]
+        plan = tuple(torch.randint(low, high, (m,), generator=g).int().cuda() for m in (T, n + 3))
+        h = ops.lowrank_shrink(x, a, plan)
+        out = torch.full((T + 2 * guard, N), 7.0, dtype=torch.bfloat16, device="cuda")
+        ops.lowrank_expand(y, torch.zeros_like(h), b, scale, plan, out[guard:guard + T])
+        grads = ops.lowrank_outer([(h, x), (h, y)], scale, n, r, plan)
+        if ops.lowrank_outer_shrink_pays(T, r):
+            ops.lowrank_outer_shrink(h, y, b, scale, plan)
+        torch.cuda.synchronize()
+        assert (out[:guard] == 7).all() and (out[guard + T:] == 7).all() and [t.shape for t in grads] == [a.shape, b.shape]
