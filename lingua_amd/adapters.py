@@ -18,6 +18,7 @@ import torch
 
 from . import _lib, ops
 from . import float8 as f8
+from .swiglu import Fp8FeedForward
 
 
 class Plan:
@@ -186,8 +187,14 @@ class AdaptedLinear(torch.nn.Module):
 
 def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, filter: str, alpha: Optional[float] = None) -> torch.nn.Module:
     """Put a bank of ``requests.n`` adapters beside every ``nn.Linear`` (or ``Fp8Linear``, ``Mxfp4Linear``) whose dotted name matches
-    ``filter``; the linears keep their parameters, under ``linear.`` in the state dict."""
+    ``filter``; the linears keep their parameters, under ``linear.`` in the state dict.  Fused feed-forwards multiply by their linears' weights
+    themselves, so those take no adapters: an error."""
     filter_re = re.compile(filter)
+    for name, module in root_module.named_modules():
+        if isinstance(module, Fp8FeedForward):
+            for child in ("w1", "w2", "w3"):
+                if filter_re.search(f"{name}.{child}" if name else child):
+                    raise RuntimeError(f"add_adapters: {name!r} is a fused feed-forward, whose {child} is not called (leave it out of fuse_feed_forward)")
 
     def replace(module: torch.nn.Module, name: str) -> torch.nn.Module:
         if not isinstance(module, torch.nn.Linear) or not filter_re.search(name) or name.endswith(".linear") and name[:-7] in banks:

@@ -149,6 +149,18 @@ def test_adapters_beside_linears_keep_parameters():
     assert torch.equal(model["w1"](x), model["w1"].linear(x))     # no request has one
 
 
+def test_adapters_inside_a_fused_feed_forward_are_refused():
+    """It multiplies by its linears' weights and never calls them: their adapters would be lost."""
+    from lingua_amd import adapters, swiglu
+    lin = [torch.nn.Linear(*s, bias=False, dtype=torch.bfloat16) for s in ((32, 64), (32, 64), (64, 32))]
+    model = torch.nn.ModuleDict({"feed_forward": swiglu.Fp8FeedForward(*lin), "wo": torch.nn.Linear(32, 32)}).to(torch.bfloat16)
+    for match in ("w2$", "w", "feed_forward"):
+        with pytest.raises(RuntimeError, match="fused feed-forward"):
+            adapters.add_adapters(model, adapters.Requests(2), 8, match)
+    adapters.add_adapters(model, adapters.Requests(2), 8, "wo")
+    assert isinstance(model["wo"], adapters.AdaptedLinear) and model["feed_forward"].w1 is lin[0]
+
+
 def test_empty_calls_do_nothing():
     lib = _lib.load()
     assert lib.l8_lowrank_shrink(*{**SHRINK, "T": 0, "x": None}.values()) == 0 and lib.l8_lowrank_expand(*{**EXPAND, "T": 0, "out": None}.values()) == 0
