@@ -294,17 +294,22 @@ struct NormBwd {
 // A workgroup per row; the sums for gw and gb stay in registers over the rows that a workgroup sees and leave as one row of partial sums
 // per workgroup, folded in order (rmsnorm_gw_fold_kernel).  Rows are requested AHEAD - 1 rows before they are used.
 // Four waves of up to three chunks; longer rows take eight waves of two, one workgroup per compute unit: the parameter, its two sums and
-// two rows of four chunks a lane are more than 256 registers.
-template <int N, int WAVES, int AHEAD, bool CENTRED, bool GH, bool DROP>
-__global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void norm_bwd_kernel(const NormBwd p) {
+// two rows of four chunks a lane are more than 256 registers.  Rows of up to three chunks, where there are more of them than workgroups, have
+// a wave each: no barrier and no idle waves; us at [16384,256] 32.3 -> 15.1, [16384,1024] 37.5 -> 29.0, [16384,1152] 38.4 -> 33.0 (with gh, folds
+// included), [2048,1536] 13.7 and 14.6.  (A wave of four chunks would need more than 256 registers.)
+constexpr int bwd_waves(int wpr) { return wpr == 1 ? kNormWaves : wpr; }
+template <int N, int WPR, int AHEAD, bool CENTRED, bool GH, bool DROP>
+__global__ __launch_bounds__(bwd_waves(WPR) * 64, 8 / bwd_waves(WPR)) void norm_bwd_kernel(const NormBwd p) {
 #if defined(__HIP_DEVICE_COMPILE__)
   static_assert(AHEAD % 2 == 0, "a buffer meets the same half of `red` every time");
+  constexpr int WAVES = bwd_waves(WPR), ROWS = WAVES / WPR;
   __shared__ float red_t[2][WAVES], red_x[2][WAVES];
+  __shared__ __attribute__((aligned(16))) float meet[WPR == 1 ? (CENTRED ? 2 : 1) * N * 512 : 4];
   const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int C = p.C;
-  const int64_t R = p.R;
-  auto col_of = [&](int j) { return (j * WAVES + wave) * 512 + lane * 8; };
+  const int64_t R = p.R, stride = (int64_t)gridDim.x * ROWS;
+  auto col_of = [&](int j) { return (j * WPR + (WPR == 1 ? 0 : wave)) * 512 + lane * 8; };
   float w[N][8];
   load_param<N>(w, p.w, p.w_f32, 1.0f, C, col_of);
   float gw[N][8], gb[CENTRED ? N : 1][8];
@@ -328,21 +333,21 @@ __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void norm_bwd_kernel(const N
     load_norm_row<N>(gyb[a], p.gy, r, R, p.ldgy, C, col_of);
   };
 #pragma unroll
-  for (int a = 0; a < AHEAD - 1; ++a) request(a, blockIdx.x + a * (int64_t)gridDim.x);
-  for (int64_t r0 = blockIdx.x; r0 < R; r0 += (int64_t)AHEAD * gridDim.x) {
+  for (int a = 0; a < AHEAD - 1; ++a) request(a, (int64_t)blockIdx.x * ROWS + (WPR == 1 ? wave : 0) + a * stride);
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS + (WPR == 1 ? wave : 0); r0 < R; r0 += AHEAD * stride) {
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const int64_t r = r0 + a * (int64_t)gridDim.x;
-      if (r >= R) break;  // the same for the whole workgroup
+      const int64_t r = r0 + a * stride;
+      if (r >= R) break;  // the same for all waves of a row
       if constexpr (GH) load_norm_row<N>(hb, p.gh, r, R, p.ldgh, C, col_of);
-      request((a + AHEAD - 1) % AHEAD, r + (AHEAD - 1) * (int64_t)gridDim.x);
+      request((a + AHEAD - 1) % AHEAD, r + (AHEAD - 1) * stride);
       const v4i(&xc)[N] = xb[a], (&gc)[N] = gyb[a];
       const float rinv = rb[a], mean = mb[a];
       auto value = [](const v4i(&v)[N], int j, int e) { return (e & 1) ? hi_of(v[j][e >> 1]) : lo_of(v[j][e >> 1]); };
       auto xhat = [&](int j, int e) { return (value(xc, j, e) - mean) * rinv; };
-      float st = 0.0f, sx = 0.0f;
+      float st = 0.0f, sx = 0.0f, tot_x = 0.0f, tot_t = 0.0f;
 #pragma unroll
-      for (int j = 0; j < N; ++j)
+      for (int j = 0; j < N; ++j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const float ge = value(gc, j, e), xh = xhat(j, e);
@@ -352,18 +357,25 @@ __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void norm_bwd_kernel(const N
           if constexpr (CENTRED) st += t;
           sx += t * xh;
         }
-      sx = wave_sum_f32(sx);
-      if constexpr (CENTRED) st = wave_sum_f32(st);
-      if (lane == 0) {
-        red_x[a & 1][wave] = sx;
-        if constexpr (CENTRED) red_t[a & 1][wave] = st;
+        if constexpr (WPR == 1) {   // chunk by chunk, as the waves of the other layout meet
+          tot_x += wave_sum_f32(sx);
+          if constexpr (CENTRED) tot_t += wave_sum_f32(st);
+          st = sx = 0.0f;
+        }
       }
-      __syncthreads();
-      float tot_x = 0.0f, tot_t = 0.0f;
+      if constexpr (WPR > 1) {
+        sx = wave_sum_f32(sx);
+        if constexpr (CENTRED) st = wave_sum_f32(st);
+        if (lane == 0) {
+          red_x[a & 1][wave] = sx;
+          if constexpr (CENTRED) red_t[a & 1][wave] = st;
+        }
+        __syncthreads();
 #pragma unroll
-      for (int wv = 0; wv < WAVES; ++wv) {
-        tot_x += red_x[a & 1][wv];
-        if constexpr (CENTRED) tot_t += red_t[a & 1][wv];
+        for (int wv = 0; wv < WAVES; ++wv) {
+          tot_x += red_x[a & 1][wv];
+          if constexpr (CENTRED) tot_t += red_t[a & 1][wv];
+        }
       }
       const float cx = tot_x * inv_c, ct = tot_t * inv_c;
       const __amdgpu_buffer_rsrc_t rsG = make_rsrc(p.gx + r * p.ldgx, (uint32_t)C * 2u);
@@ -396,6 +408,29 @@ __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void norm_bwd_kernel(const N
     }
   }
   if (!p.partials) return;
+  if constexpr (WPR == 1) {   // the waves' sums meet in LDS, one wave after the other; the last one has them all
+    for (int wv = 0; wv < WAVES; ++wv) {
+      if (wave == wv) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+          for (int part = 0; part < (CENTRED ? 2 : 1); ++part) {
+            float(&mine)[8] = part ? gb[CENTRED ? j : 0] : gw[j];
+            float *at = &meet[(part * N + j) * 512 + lane * 8];
+            if (wv > 0) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) mine[e] = at[e] + mine[e];
+            }
+            if (wv < WAVES - 1) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) at[e] = mine[e];
+            }
+          }
+      }
+      __syncthreads();
+    }
+    if (wave != WAVES - 1) return;
+  }
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     const int c = col_of(j);
@@ -425,24 +460,34 @@ static int launch_fwd(const NormFwd &p, float *col_amax, hipStream_t st) {
 template <bool CENTRED, bool ADD, bool DROP>
 static int launch_fwd_for(const NormFwd &p, float *col_amax, hipStream_t st) {
   const int nch = (p.C + 511) / 512, n = (nch + kNormWaves - 1) / kNormWaves;
-  if (nch <= 4 && p.R > norm_blocks(p.R)) return launch_fwd<4, 1, CENTRED, ADD, DROP>(p, col_amax, st);
+  if (nch <= 4 && p.R > norm_blocks(p.R)) {
+    if (nch <= 1) return launch_fwd<1, 1, CENTRED, ADD, DROP>(p, col_amax, st);
+    if (nch <= 2) return launch_fwd<2, 1, CENTRED, ADD, DROP>(p, col_amax, st);
+    if (nch <= 3) return launch_fwd<3, 1, CENTRED, ADD, DROP>(p, col_amax, st);
+    return launch_fwd<4, 1, CENTRED, ADD, DROP>(p, col_amax, st);
+  }
   if (n <= 1) return launch_fwd<1, kNormWaves, CENTRED, ADD, DROP>(p, col_amax, st);
   if (n <= 2) return launch_fwd<2, kNormWaves, CENTRED, ADD, DROP>(p, col_amax, st);
   if (n <= 3) return launch_fwd<3, kNormWaves, CENTRED, ADD, DROP>(p, col_amax, st);
   return launch_fwd<4, kNormWaves, CENTRED, ADD, DROP>(p, col_amax, st);
 }
 
-template <int N, int WAVES, bool CENTRED, bool GH, bool DROP>
+template <int N, int WPR, bool CENTRED, bool GH, bool DROP>
 static int launch_bwd(const NormBwd &p, const GradOut &gw, const GradOut &gb, hipStream_t st) {
-  const int64_t most = norm_blocks(p.R), blocks = WAVES > kNormWaves && most > num_cus() ? num_cus() : most;
-  hipLaunchKernelGGL((norm_bwd_kernel<N, WAVES, N == 1 ? 4 : 2, CENTRED, GH, DROP>), dim3((unsigned)blocks), dim3(WAVES * 64), 0, st, p);
+  const int64_t most = norm_blocks(WPR == 1 ? (p.R + kNormWaves - 1) / kNormWaves : p.R), blocks = WPR > kNormWaves && most > num_cus() ? num_cus() : most;
+  hipLaunchKernelGGL((norm_bwd_kernel<N, WPR, N == 1 ? 4 : 2, CENTRED, GH, DROP>), dim3((unsigned)blocks), dim3(bwd_waves(WPR) * 64), 0, st, p);
   L8_HIP(hipGetLastError());
   return p.partials ? fold_norm_grads(p.partials, blocks, gw, gb, st) : L8_OK;
 }
 
 template <bool CENTRED, bool GH, bool DROP>
 static int launch_bwd_for(const NormBwd &p, const GradOut &gw, const GradOut &gb, hipStream_t st) {
-  const int n = ((p.C + 511) / 512 + kNormWaves - 1) / kNormWaves;
+  const int nch = (p.C + 511) / 512, n = (nch + kNormWaves - 1) / kNormWaves;
+  if (nch <= 3 && p.R > norm_blocks(p.R)) {
+    if (nch <= 1) return launch_bwd<1, 1, CENTRED, GH, DROP>(p, gw, gb, st);
+    if (nch <= 2) return launch_bwd<2, 1, CENTRED, GH, DROP>(p, gw, gb, st);
+    return launch_bwd<3, 1, CENTRED, GH, DROP>(p, gw, gb, st);
+  }
   if (n <= 1) return launch_bwd<1, kNormWaves, CENTRED, GH, DROP>(p, gw, gb, st);
   if (n <= 2) return launch_bwd<2, kNormWaves, CENTRED, GH, DROP>(p, gw, gb, st);
   if (n <= 3) return launch_bwd<3, kNormWaves, CENTRED, GH, DROP>(p, gw, gb, st);
