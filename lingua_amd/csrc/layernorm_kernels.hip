@@ -10,6 +10,7 @@
 // that a workgroup shares meets at one barrier.  Everything in fp32.
 // Two layouts, as in the RMSNorm: a wavefront per row for short rows, a workgroup for the longer ones; both join the same chunks of 512
 // columns in the same order up to 2048 columns, so a row's result does not hang on how many rows come with it.
+#include <algorithm>
 #include "dropout.h"
 #include "norm.h"
 
@@ -449,7 +450,10 @@ __global__ __launch_bounds__(bwd_waves(WPR) * 64, 8 / bwd_waves(WPR)) void norm_
 
 template <int N, int WPR, bool CENTRED, bool ADD, bool DROP>
 static int launch_fwd(const NormFwd &p, float *col_amax, hipStream_t st) {
-  const int64_t blocks = norm_blocks(WPR == 1 ? (p.R + kNormWaves - 1) / kNormWaves : p.R);
+  int64_t blocks = norm_blocks(WPR == 1 ? (p.R + kNormWaves - 1) / kNormWaves : p.R);
+  // (three a unit, where no row of partial maxima goes with each and the registers allow it; us at [16384,1152] 23.9 -> 21.6 with the cast,
+  // [16384,256] 12.4 -> 10.7; four a unit 21.4 but 31.5 and not 29.2 with a residual)
+  if (WPR == 1 && N <= 3 && !col_amax) blocks = std::min<int64_t>((p.R + kNormWaves - 1) / kNormWaves, 3 * (int64_t)num_cus());
   auto go = [&](auto kernel, size_t lds) { hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(kNormBlock), lds, st, p); };
   if (col_amax) go(norm_fwd_kernel<N, WPR, CENTRED, ADD, DROP, true>, WPR == 1 ? (size_t)p.C * 2 : 0);
   else go(norm_fwd_kernel<N, WPR, CENTRED, ADD, DROP, false>, 0);
