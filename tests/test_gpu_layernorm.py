@@ -122,6 +122,29 @@ def test_gradients(R, C, added, dtype, host):
     assert plain.grad_within(gw, want[1], err[1]) and plain.grad_within(gb, want[2], err[2])
 
 
+@pytest.mark.parametrize("R", [513, 1027, 3001])
+@pytest.mark.parametrize("C", [8, 504, 512, 520, 1024, 1032, 1152, 1536, 1544, 2048])
+def test_gradients_of_many_short_rows(R, C):
+    """Rows of one to four chunks of 512 columns, more of them than workgroups: the gradients against 64 bits, and those of x what they are
+    for a few of the rows alone, with and without a gradient of the sum and a dropped operand."""
+    from lingua_amd import dropout, ops
+    x, res = operands(R, C, seed=C)
+    gy, gh = seeded_bf16((R, C), std=0.1, seed=5).cuda(), seeded_bf16((R, C), std=0.1, seed=6).cuda()
+    w, b = param(C, torch.float32, 1, 1.0), param(C, torch.bfloat16, 2, 0.0)
+    drop = dropout.Drop(0.3, dropout.numbers(8), 2)
+    for centred, d, gsum in ((True, None, None), (True, None, gh), (True, drop, gh), (False, drop, gh), (False, drop, None)):
+        h, _, _, _, stats = ops.layernorm_cast_rowwise(x, w, b if centred else None, EPS, res, d, centred, want_q=False)
+        gx, gres, gw, gb = ops.layernorm_bwd(gy, gsum, h, w, stats, d, centred, torch.float32, torch.float32 if centred else None)
+        whole = gx if gres is None else gres
+        if centred:
+            hat, r, _ = plain.layernorm(h, w.double(), b.double(), EPS)
+            want, err = plain.layernorm_grads(h, hat, r, w.double(), gy, None if gsum is None else gsum.double())
+            assert within(whole, want[0], err[0])
+            assert plain.grad_within(gw, want[1], err[1]) and plain.grad_within(gb, want[2], err[2])
+        few = ops.layernorm_bwd(gy[:5], None if gsum is None else gsum[:5], h[:5], w, stats[:, :5], d, centred)
+        assert torch.equal(gx[:5], few[0]) and (gres is None or torch.equal(gres[:5], few[1]))
+
+
 def test_gradients_against_differences():
     """The gradient of a weighted sum of outputs against central differences of the 64-bit form along random directions."""
     from lingua_amd import norm
