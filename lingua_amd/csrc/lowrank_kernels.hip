@@ -716,8 +716,10 @@ __global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, in
   if (at >= all) return;
   v4f lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
   const int pieces = (tokens + p.size - 1) / p.size;
+  const int64_t part0 = outer_part(from, p.size, 0);   // and piece i > 0 at part0 + 2 i + 1
+#pragma unroll 8
   for (int i = 0; i < pieces; ++i) {
-    const float *part = sd.partials + outer_part(from + i * p.size, p.size, i) * all + at;
+    const float *part = sd.partials + (part0 + 2 * i + (i > 0)) * all + at;
     const v4f a = *(const v4f *)part, b = *(const v4f *)(part + 4);
 #pragma unroll
     for (int e = 0; e < 4; ++e) lo[e] += a[e], hi[e] += b[e];
