@@ -192,25 +192,33 @@ struct ShrinkArgs {
   int T, K, n, r, splits;
 };
 
-// MT tiles of 16 tokens by RT of 16 ranks a wave; the W waves are SUB parts of a tile's tokens, and W / SUB of them share K.  A wave takes 64 columns a step, the waves side by side: lane group g
-// (of 16 lanes) takes columns 16 g .. 16 g + 15 of a step, the first eight into one matrix instruction and the others into a second, so
-// that a row is read in whole lines.  Which column meets which place of the instruction does not matter as long as it is the same for
-// both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
+// MT tiles of 16 tokens by RT of 16 ranks a wave; the W waves are SUB parts of a tile's tokens, and W / SUB of them share K.  A wave takes 64
+// columns a step, the waves side by side.  Eight neighbouring lanes read a row's 128 bytes: the matrix instruction wants neighbouring rows in
+// neighbouring lanes, and read like that every 16 bytes are a line of their own to the cache, 64 of them an instruction.  So what was read goes
+// through LDS of the wave's own, chunk c of a row at place c ^ (row % 8), where neither side meets a bank twice.  Which column meets which place of
+// the instruction does not matter as long as it is the same for both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
 template <int MT, int SUB, int RT, int W>
 __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs p) {
-  constexpr int KW = W / SUB;
-  __shared__ float red[SUB * (KW / 2)][MT * RT * 256];
+  constexpr int KW = W / SUB, BOTH = MT > RT ? MT : RT, RED = MT * RT * 64;
+  constexpr int ROOM = W * BOTH * 128 > SUB * (KW / 2) * RED ? W * BOTH * 128 : SUB * (KW / 2) * RED;
+  __shared__ v4i room[ROOM];   // of a wave: one operand's tiles, 16 rows of eight chunks each; at the end: sums
   const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, MT * SUB * 16, blockIdx.x);
   if (tile.group >= p.n || tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
   const int part = wave % SUB, part0 = part * MT * 16, kw = wave / SUB;
   const int K = p.K, steps = (K + 63) / 64, rank0 = blockIdx.z * RT * 16;
   const int lo = (int)((int64_t)steps * blockIdx.y / p.splits), hi = (int)((int64_t)steps * (blockIdx.y + 1) / p.splits);
-  const uint16_t *xr[MT], *fr[RT];
+  v4i *mine = room + wave * BOTH * 128;
+  const int r8 = lane >> 3, chunk = ((lane & 7) ^ r8) * 8;   // this lane reads rows r8 and r8 + 8 of a tile, from column `chunk` of a step on
+  const uint16_t *xr[MT][2], *fr[RT][2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xr[m] = p.x + (int64_t)tile.token(part0 + m * 16 + row) * p.ldx;
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-  for (int j = 0; j < RT; ++j) fr[j] = p.f + ((int64_t)tile.group * p.r + min(rank0 + j * 16 + row, p.r - 1)) * K;
+    for (int i = 0; i < 2; ++i) xr[m][i] = p.x + (int64_t)tile.token(part0 + m * 16 + i * 8 + r8) * p.ldx;
+#pragma unroll
+  for (int j = 0; j < RT; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) fr[j][i] = p.f + ((int64_t)tile.group * p.r + min(rank0 + j * 16 + i * 8 + r8, p.r - 1)) * K;
   v4f acc[MT][RT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -219,30 +227,51 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
   v4i a[2][MT][2], b[2][RT][2];
   auto request = [&](int s, int step) {
     // the last step may pass the row's end: columns beyond it are read from within the row and zeroed before they are used
-    const int k0 = step * 64 + g * 16, k1 = min(k0, K - 8), k2 = min(k0 + 8, K - 8);
+    const int k = min(step * 64 + chunk, K - 8);
 #pragma unroll
-    for (int m = 0; m < MT; ++m) a[s][m][0] = *(const v4i *)(xr[m] + k1), a[s][m][1] = *(const v4i *)(xr[m] + k2);
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int j = 0; j < RT; ++j) b[s][j][0] = *(const v4i *)(fr[j] + k1), b[s][j][1] = *(const v4i *)(fr[j] + k2);
-  };
-  auto multiply = [&](int s, int step) {
-    if (step * 64 + 64 > K) {
-      const int k0 = step * 64 + g * 16;
+      for (int j = 0; j < RT; ++j) b[s][j][i] = *(const v4i *)(fr[j][i] + k);
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (k0 + 8 * c >= K) {
-#pragma unroll
-          for (int m = 0; m < MT; ++m) a[s][m][c] = v4i{0, 0, 0, 0};
-#pragma unroll
-          for (int j = 0; j < RT; ++j) b[s][j][c] = v4i{0, 0, 0, 0};
-        }
+      for (int m = 0; m < MT; ++m) a[s][m][i] = *(const v4i *)(xr[m][i] + k);
     }
+  };
+  auto fragment = [&](int t, int c) { return mine[t * 128 + row * 8 + ((c * 4 + g) ^ (row & 7))]; };
+  auto multiply = [&](int s, int step) {
+    if (step * 64 + chunk >= K) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+      for (int i = 0; i < 2; ++i) {
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+        for (int m = 0; m < MT; ++m) a[s][m][i] = v4i{0, 0, 0, 0};
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[m][j] = mfma(a[s][m][c], b[s][j][c], acc[m][j]);
+        for (int j = 0; j < RT; ++j) b[s][j][i] = v4i{0, 0, 0, 0};
+      }
+    }
+    v4i f[RT][2];
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mine[(j * 2 + i) * 64 + lane] = b[s][j][i];
+    __builtin_amdgcn_wave_barrier();   // one wave's own LDS: it keeps the order of what it issues
+#pragma unroll
+    for (int j = 0; j < RT; ++j)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) f[j][c] = fragment(j, c);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mine[(m * 2 + i) * 64 + lane] = a[s][m][i];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const v4i x = fragment(m, c);
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[m][j] = mfma(x, f[j][c], acc[m][j]);
+      }
+    __builtin_amdgcn_wave_barrier();
   };
   int step = lo + kw;
   if (step < hi) request(0, step);
@@ -256,13 +285,14 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
     step += KW;
   }
   // the upper half of the waves hands its sums to the lower half, until one has them all
+  if (KW > 1) __syncthreads();   // (they take the tiles' place)
 #pragma unroll
   for (int half = KW / 2; half; half /= 2) {
     if (kw >= half && kw < 2 * half) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) *(v4f *)&red[part * (KW / 2) + kw - half][(m * RT + j) * 256 + lane * 4] = acc[m][j];
+        for (int j = 0; j < RT; ++j) *(v4f *)&room[(part * (KW / 2) + kw - half) * RED + (m * RT + j) * 64 + lane] = acc[m][j];
     }
     __syncthreads();
     if (kw < half) {
@@ -270,7 +300,7 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
-          const v4f other = *(const v4f *)&red[part * (KW / 2) + kw][(m * RT + j) * 256 + lane * 4];
+          const v4f other = *(const v4f *)&room[(part * (KW / 2) + kw) * RED + (m * RT + j) * 64 + lane];
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][j][i] += other[i];
         }
