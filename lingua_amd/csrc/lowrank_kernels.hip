@@ -192,20 +192,19 @@ struct ShrinkArgs {
   int T, K, n, r, splits;
 };
 
-// MT tiles of 16 tokens by RT of 16 ranks a wave; the W waves are SUB parts of a tile's tokens, and W / SUB of them share K.  A wave takes 64
-// columns a step, the waves side by side.  Eight neighbouring lanes read a row's 128 bytes: the matrix instruction wants neighbouring rows in
-// neighbouring lanes, and read like that every 16 bytes are a line of their own to the cache, 64 of them an instruction.  So what was read goes
-// through LDS of the wave's own, chunk c of a row at place c ^ (row % 8), where neither side meets a bank twice.  Which column meets which place of
-// the instruction does not matter as long as it is the same for both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
-template <int MT, int SUB, int RT, int W>
+// MT tiles of 16 tokens by RT of 16 ranks; the W waves share K.  A wave takes 64 columns a step, the waves side by side.  Eight neighbouring
+// lanes read a row's 128 bytes: the matrix instruction wants neighbouring rows in neighbouring lanes, and read like that every 16 bytes are a
+// line of their own to the cache, 64 of them an instruction.  So what was read goes through LDS of the wave's own, chunk c of a row at place c
+// ^ (row % 8), where neither side meets a bank twice.  Which column meets which place of the instruction does not matter as long as it is the
+// same for both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
+template <int MT, int RT, int W>
 __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs p) {
-  constexpr int KW = W / SUB, BOTH = MT > RT ? MT : RT, RED = MT * RT * 64;
-  constexpr int ROOM = W * BOTH * 128 > SUB * (KW / 2) * RED ? W * BOTH * 128 : SUB * (KW / 2) * RED;
+  constexpr int BOTH = MT > RT ? MT : RT, RED = MT * RT * 64;
+  constexpr int ROOM = W * BOTH * 128 > W / 2 * RED ? W * BOTH * 128 : W / 2 * RED;
   __shared__ v4i room[ROOM];   // of a wave: one operand's tiles, 16 rows of eight chunks each; at the end: sums
-  const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, MT * SUB * 16, blockIdx.x);
+  const Tile tile = tile_with_tokens(p.tokens, p.T, p.n, MT * 16, blockIdx.x);
   if (tile.group >= p.n || tile.count == 0) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
-  const int part = wave % SUB, part0 = part * MT * 16, kw = wave / SUB;
   const int K = p.K, steps = (K + 63) / 64, rank0 = blockIdx.z * RT * 16;
   const int lo = (int)((int64_t)steps * blockIdx.y / p.splits), hi = (int)((int64_t)steps * (blockIdx.y + 1) / p.splits);
   v4i *mine = room + wave * BOTH * 128;
@@ -214,7 +213,7 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) xr[m][i] = p.x + (int64_t)tile.token(part0 + m * 16 + i * 8 + r8) * p.ldx;
+    for (int i = 0; i < 2; ++i) xr[m][i] = p.x + (int64_t)tile.token(m * 16 + i * 8 + r8) * p.ldx;
 #pragma unroll
   for (int j = 0; j < RT; ++j)
 #pragma unroll
@@ -273,47 +272,47 @@ __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs
       }
     __builtin_amdgcn_wave_barrier();
   };
-  int step = lo + kw;
+  int step = lo + wave;
   if (step < hi) request(0, step);
   while (step < hi) {
-    request(1, min(step + KW, hi - 1));
+    request(1, min(step + W, hi - 1));
     multiply(0, step);
-    step += KW;
+    step += W;
     if (step >= hi) break;
-    request(0, min(step + KW, hi - 1));
+    request(0, min(step + W, hi - 1));
     multiply(1, step);
-    step += KW;
+    step += W;
   }
   // the upper half of the waves hands its sums to the lower half, until one has them all
-  if (KW > 1) __syncthreads();   // (they take the tiles' place)
+  __syncthreads();   // (they take the tiles' place)
 #pragma unroll
-  for (int half = KW / 2; half; half /= 2) {
-    if (kw >= half && kw < 2 * half) {
+  for (int half = W / 2; half; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) *(v4f *)&room[(part * (KW / 2) + kw - half) * RED + (m * RT + j) * 64 + lane] = acc[m][j];
+        for (int j = 0; j < RT; ++j) *(v4f *)&room[(wave - half) * RED + (m * RT + j) * 64 + lane] = acc[m][j];
     }
     __syncthreads();
-    if (kw < half) {
+    if (wave < half) {
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int j = 0; j < RT; ++j) {
-          const v4f other = *(const v4f *)&room[(part * (KW / 2) + kw) * RED + (m * RT + j) * 64 + lane];
+          const v4f other = *(const v4f *)&room[wave * RED + (m * RT + j) * 64 + lane];
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[m][j][i] += other[i];
         }
     }
     __syncthreads();
   }
-  if (kw) return;
+  if (wave) return;
   // a lane has rank `row` of each sixteen, tokens 4 g .. 4 g + 3
 #pragma unroll
   for (int m = 0; m < MT; ++m)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = part0 + m * 16 + g * 4 + i, token = tile.token(at);
+      const int at = m * 16 + g * 4 + i, token = tile.token(at);
       if (at >= tile.count) continue;
       float *out = p.h + ((int64_t)blockIdx.y * p.T + token) * p.r;
 #pragma unroll
@@ -770,11 +769,11 @@ constexpr int64_t kMaxRank = 128, kMaxTokens = 1 << 24, kMaxAdapters = 65534, kM
 // Tokens of a tile: 64, which read a factor a quarter as often, where the adapters have that many on average.
 static int tile_tokens(int64_t T, int64_t n) { return T >= 64 * (n + 1) ? 64 : 16; }
 // The same of `shrink`: with more than 32 ranks, where four tiles of 16 tokens fill a SIMD's registers with one wave, tiles of 32 tokens on twice
-// the waves unless the larger ones give every unit one ([2055,4096] rank 64 in two parts 17.7 us and 23.1, [16384,4096] 56 and 41).
-static int64_t tile_slots(int64_t T, int64_t n, int64_t size);
+// the waves up to one a unit; us, rank 64, 32 tokens and 64: [2055,4096] in three parts 13.5 and 16.0, [8192,4096] 23.3 and 28.8, [12000,4096]
+// 40.6 and 31.7.
 static int shrink_tokens(int64_t T, int64_t n, int64_t r) {
   const int size = tile_tokens(T, n);
-  return size == 64 && r > 32 && tile_slots(T, n, 64) < num_cus() ? 32 : size;
+  return size == 64 && r > 32 && T <= 32 * (int64_t)num_cus() ? 32 : size;
 }
 static int64_t tile_slots(int64_t T, int64_t n, int64_t size) { return T / size + n + 2; }
 
@@ -848,20 +847,20 @@ static int shrink_impl(const char *who, const void *x, int64_t T, int64_t K, int
   const int64_t size = shrink_tokens(T, n, r), slots = tiles_of(tk, T, n, size);
   const ShrinkArgs p{(const uint16_t *)x, (const uint16_t *)f, tk, h, ldx, (int)T, (int)K, (int)n, (int)r, (int)splits};
   const unsigned ranks = r <= 64 ? 1 : 2;
-#define L8_SHRINK(MT, SUB, RT, W)                                                                                        \
+#define L8_SHRINK(MT, RT, W)                                                                                             \
   do {                                                                                                                   \
     L8_CALL(check_grid(who, slots, splits, ranks, W * 64));                                                              \
-    hipLaunchKernelGGL((lowrank_shrink_kernel<MT, SUB, RT, W>), dim3((unsigned)slots, (unsigned)splits, ranks), dim3(W * 64), 0, st, p); \
+    hipLaunchKernelGGL((lowrank_shrink_kernel<MT, RT, W>), dim3((unsigned)slots, (unsigned)splits, ranks), dim3(W * 64), 0, st, p); \
   } while (0)
   if (size == 16) {
-    if (r <= 16) L8_SHRINK(1, 1, 1, 8);
-    else if (r <= 32) L8_SHRINK(1, 1, 2, 8);
-    else L8_SHRINK(1, 1, 4, 8);
+    if (r <= 16) L8_SHRINK(1, 1, 8);
+    else if (r <= 32) L8_SHRINK(1, 2, 8);
+    else L8_SHRINK(1, 4, 8);
   } else {
-    if (r <= 16) L8_SHRINK(4, 1, 1, 8);
-    else if (r <= 32) L8_SHRINK(4, 1, 2, 8);
-    else if (size == 32) L8_SHRINK(2, 1, 4, 8);
-    else L8_SHRINK(4, 1, 4, 4);
+    if (r <= 16) L8_SHRINK(4, 1, 8);
+    else if (r <= 32) L8_SHRINK(4, 2, 8);
+    else if (size == 32) L8_SHRINK(2, 4, 8);
+    else L8_SHRINK(4, 4, 4);
   }
 #undef L8_SHRINK
   L8_HIP(hipGetLastError());
