@@ -379,8 +379,8 @@ constexpr int kExpandWaves = 4;
 // next 128 columns `per` times: h, 4 r bytes a token and more in parts, is then read once for all of them.  The next step's y and factor are
 // requested before the present one is multiplied.
 // A tile waits for memory three times: for its place, for its tokens, for everything else.
-// us at [16384,4096] with y: up to 16 ranks with five waves a SIMD 52, with four 61, with six 57; 64 ranks one step a workgroup 70, up to eight 58,
-// of h in three parts 100 and 63; 128 ranks 104 and 68.
+// us at [16384,4096] with y, 402 MB: up to 16 ranks with five waves a SIMD 52 (7.7 TB/s, a part of it from the caches), with four 61, with six 57;
+// 64 ranks 67, one step a workgroup 75, and of h in three parts 100 and 77 for one step and for eight.  [16384,11008] of rank 16: 131, 5.5 TB/s.
 template <int PARTS, int KS>
 __global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : PARTS == 1 ? 1 : 2) void lowrank_expand_kernel(const ExpandArgs p) {
   constexpr int STEPS = KS ? KS : 1;
@@ -873,9 +873,11 @@ static int expand_impl(const char *who, const void *y, int64_t ldy, const float 
   L8_REQUIRE((!y || rows_fit(y, ldy, N)) && rows_fit(f, N, N) && rows_fit(out, ldo, N) && h && ((uintptr_t)h % 16) == 0 && ((uintptr_t)scale % 4) == 0,
              "%s: null or misaligned operand, or rows off 16-byte lines", who);
   const int64_t size = tile_tokens(T, n), slots = tiles_of(tk, T, n, size);
-  // waves that share the factor take as many steps as leave two workgroups a unit ([2055,11008] rank 64, h in three parts, us: 31.0, four a
-  // unit 37.0; [16384,4096] up to eight steps 61, up to sixteen 77)
-  const int64_t per = size == 16 || r <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(8, slots * ((N + 127) / 128) / (2 * num_cus())));
+  // waves that share the factor take as many steps as leave two workgroups a unit ([2055,11008] rank 64, h in three parts, us: 30.7, four a
+  // unit 35.5), of an h that is whole up to four, since long ones end unevenly: rank 64, up to four and up to eight, [4096,11008] 46.7 and 55.8,
+  // [6000,4096] 27.4 and 35.5, [8192,4096] 35.4 and 41.4, [16384,4096] 69.0 and 70.4
+  const int64_t most = splits == 1 ? 4 : 8;
+  const int64_t per = size == 16 || r <= 16 ? 1 : std::max<int64_t>(1, std::min<int64_t>(most, slots * ((N + 127) / 128) / (2 * num_cus())));
   const int64_t cols = size == 16 ? kExpandWaves * 128 : per * 128, chunks = (N + cols - 1) / cols;
   L8_CALL(check_grid(who, slots * chunks, 1, 1, kExpandWaves * 64));
   const ExpandArgs p{(const uint16_t *)y, (const uint16_t *)f, h, scale, tk, (uint16_t *)out, ldy, ldo, (int)T, (int)N, (int)n, (int)r, (int)splits, (int)chunks, (int)per};
