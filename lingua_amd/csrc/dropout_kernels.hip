@@ -2,7 +2,8 @@
 // gradient (the residual's gradient is the sum's).  What the generator is: dropout.h.
 //
 // A thread takes a group of eight elements, one 16-byte load and store and one call of the generator.  Bound by memory where the tensor
-// is large, 4 bytes an element and 6 with a residual.
+// is large, 4 bytes an element and 6 with a residual: [16384,4096] 41 us, 6.6 TB/s (a part of it from the caches), and 70 us, 5.7 TB/s.
+// [333,2064] 2.7 us, a launch.
 #include "dropout.h"
 
 namespace l8 {

@@ -36,7 +36,8 @@ L8_DEV v4f mfma(v4i a, v4i b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32
 constexpr int kRouteBlock = 1024, kRouteWaves = kRouteBlock / 64, kRouteTimes = 16;
 
 // A workgroup per group: how many tokens stand in front of its own, then its own tokens in their order.  Sixteen tokens a thread are
-// requested together and stay in registers between the two counts.
+// requested together and stay in registers between the two counts.  Every workgroup reads the whole index, so that none waits for another:
+// 16384 tokens and 8 adapters 6.5 us, 2055 and 12 5.0 (a launch that does nothing: 2 to 3), one launch in place of a count, a sum and a scatter.
 template <typename Index>
 __global__ __launch_bounds__(kRouteBlock) void lowrank_route_kernel(const Index *__restrict__ index, int T, int n, int *__restrict__ order, int *__restrict__ starts) {
   constexpr int SPAN = kRouteBlock * kRouteTimes, PLACES = kRouteTimes * kRouteWaves;
@@ -197,6 +198,9 @@ struct ShrinkArgs {
 // line of their own to the cache, 64 of them an instruction.  So what was read goes through LDS of the wave's own, chunk c of a row at place c
 // ^ (row % 8), where neither side meets a bank twice.  Which column meets which place of the instruction does not matter as long as it is the
 // same for both operands.  blockIdx.z: which 16 RT of more than 64 ranks.
+// us, rank 16: [16384,4096] 29.8 (134 MB, 4.5 TB/s), [16384,11008] 78 (4.6 TB/s), [1500,4096] in four parts 8.6 (10.3 without the turn through LDS);
+// rank 64: [16384,4096] 36.7, [2055,4096] in three parts 14.2.  A unit takes in no more than some 45 bytes a ns (all of them twice the memory's
+// rate): few tiles are bound by that, hence the parts, many by memory.
 template <int MT, int RT, int W>
 __global__ __launch_bounds__(W * 64) void lowrank_shrink_kernel(const ShrinkArgs p) {
   constexpr int BOTH = MT > RT ? MT : RT, RED = MT * RT * 64;
@@ -380,7 +384,8 @@ constexpr int kExpandWaves = 4;
 // requested before the present one is multiplied.
 // A tile waits for memory three times: for its place, for its tokens, for everything else.
 // us at [16384,4096] with y, 402 MB: up to 16 ranks with five waves a SIMD 52 (7.7 TB/s, a part of it from the caches), with four 61, with six 57;
-// 64 ranks 67, one step a workgroup 75, and of h in three parts 100 and 77 for one step and for eight.  [16384,11008] of rank 16: 131, 5.5 TB/s.
+// 64 ranks 67, up to two steps a workgroup 75, and of h in three parts 91 for up to two and 77 for up to eight.  [16384,11008] of rank 16: 131,
+// 5.5 TB/s.
 template <int PARTS, int KS>
 __global__ __launch_bounds__(kExpandWaves * 64, KS == 0 ? 5 : PARTS == 1 ? 1 : 2) void lowrank_expand_kernel(const ExpandArgs p) {
   constexpr int STEPS = KS ? KS : 1;
@@ -563,6 +568,8 @@ L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)
 // With ALSO_H the kernel also does `shrink`'s work on z, which both read whole: 32 tokens by a wave's 128 columns go through LDS of the wave's
 // own, whose rows are what the matrix instruction wants them to be, and meet the factor's 128 columns, which stay in registers; every 64
 // tokens the waves' sums are added up.  Up to 16 ranks, whose registers leave room for that.
+// us: [16384,4096] of rank 16 33 (134 MB, 4.1 TB/s), of rank 64 two such sides 90 (3.0; and 67 MB of sums of tiles, written and read); with
+// ALSO_H [16384,11008] 97 (361 MB, 3.7 TB/s) where both by themselves take 177.
 template <int RT, int TOKENS, bool ALSO_H>
 __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(const OuterArgs p) {
   constexpr int PITCH = TOKENS + 8, ZPITCH = 128 + 8;
