@@ -3,7 +3,7 @@ mask is stored -- forward and backward compute the same bits, and so does a forw
 
 ``numbers(seed, device)`` makes the two numbers {seed, step} that a program keeps on the GPU; it adds one to the step between two training
 steps (``n[1] += 1``, which a captured graph may do by itself: its replays then drop other elements).  Changed between a forward pass and its
-backward pass they are an error, as every saved tensor's in-place change is.  ``Drop(p, numbers, site)`` says what a call drops; calls of
+backward pass they are an error, as every saved tensor's in-place change is.  Ranks that hold other tokens take other seeds.  ``Drop(p, numbers, site)`` says what a call drops; calls of
 one step that are to drop independently have sites of their own.  The norms of ``lingua_amd.norm`` take a ``Drop`` for the operand that they
 add to the residual.  ``Dropout`` stands in for ``nn.Dropout``; ``convert_dropouts(model, numbers)`` swaps the modules and numbers their sites.
 
