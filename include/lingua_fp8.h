@@ -461,10 +461,10 @@ int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, int64_t T, 
                      void *workspace, int64_t workspace_bytes, void *stream);
 int64_t l8_lowrank_outer_workspace(int64_t T, int64_t r, int64_t K, int64_t N);
 /* One such side and, from the same reading of z, also = z F_i^T, fp32 [T,r], without the scale: outer of the factor B and shrink of the gradient.
- * r up to 16, at least one token; l8_lowrank_outer_shrink_pays says (1 or 0) whether one reading is faster than two. */
+ * r up to 32, at least one token; l8_lowrank_outer_shrink_pays says (1 or 0) whether one reading is faster than two. */
 int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *scale, const void *f, float *also, int64_t T, int64_t n, int64_t r, const int *order,
                             const int *starts, void *workspace, int64_t workspace_bytes, void *stream);
-int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r);
+int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r, int64_t D);
 int64_t l8_lowrank_outer_shrink_workspace(int64_t T, int64_t r, int64_t D);
 
 /* MXFP4 (OCP Microscaling formats 1.0): e2m1 codes in blocks of 32, the last block of a row possibly shorter, with an e8m0 scale each.

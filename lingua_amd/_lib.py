@@ -77,7 +77,7 @@ SIGNATURES = {
     "l8_lowrank_add_workspace": [_i64, _i64, _i64, _i64],
     "l8_lowrank_outer": [_p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
     "l8_lowrank_outer_shrink": [_p, _p, _p, _p, _i64, _i64, _i64, _p, _p, _p, _i64, _p],
-    "l8_lowrank_outer_shrink_pays": [_i64, _i64],
+    "l8_lowrank_outer_shrink_pays": [_i64, _i64, _i64],
     "l8_lowrank_outer_shrink_workspace": [_i64, _i64, _i64],
     "l8_lowrank_outer_workspace": [_i64, _i64, _i64, _i64],
     "l8_cast_mxfp4": [_p, _i64, _i64, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p],

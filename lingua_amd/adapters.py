@@ -60,7 +60,7 @@ class LowRankFn(torch.autograd.Function):
         varies = f8._learns(gy)
         with torch.no_grad():
             sides = []
-            together = need_b and (need_x or need_a) and ops.lowrank_outer_shrink_pays(gy.shape[0], r)
+            together = need_b and (need_x or need_a) and ops.lowrank_outer_shrink_pays(gy.shape[0], r, gy.shape[1])
             if need_x or need_a:
                 if together:
                     gb, gh = ops.lowrank_outer_shrink(h, gy, b, scale, plan)

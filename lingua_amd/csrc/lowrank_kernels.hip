@@ -567,21 +567,26 @@ L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)
 //
 // With ALSO_H the kernel also does `shrink`'s work on z, which both read whole: 32 tokens by a wave's 128 columns go through LDS of the wave's
 // own, whose rows are what the matrix instruction wants them to be, and meet the factor's 128 columns, which stay in registers; every 64
-// tokens the waves' sums are added up.  Up to 16 ranks, whose registers leave room for that.
+// tokens (32 with more than 16 ranks) the waves' sums are added up.  Up to 32 ranks, whose registers leave room for that.
+// A tile's columns are neighbouring workgroups, so that its rows are read as whole lines of memory at one time: [16384,8192] 72 us, the tiles being
+// neighbours 94; the gradients alone do better with neighbouring tiles (both sides of [16384,4096] to [16384,4096] a whole pass of 127 and 134).
 // us: [16384,4096] of rank 16 33 (134 MB, 4.1 TB/s), of rank 64 two such sides 90 (3.0; and 67 MB of sums of tiles, written and read); with
 // ALSO_H [16384,11008] 97 (361 MB, 3.7 TB/s) where both by themselves take 177.
 template <int RT, int TOKENS, bool ALSO_H>
 __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(const OuterArgs p) {
   constexpr int PITCH = TOKENS + 8, ZPITCH = 128 + 8;
   __shared__ __attribute__((aligned(16))) uint16_t zs[ALSO_H ? kOuterWaves : 1][ALSO_H ? 32 : 1][ZPITCH];
-  static_assert(!ALSO_H || 64 * RT * 16 * 4 <= 32 * ZPITCH * 2, "a wave's sums of 64 tokens take the place of its z");
+  constexpr int HELD = RT == 1 ? 2 : 1;   // times 32 tokens whose sums a wave keeps until the waves' are added up
+  static_assert(!ALSO_H || HELD * 32 * RT * 16 * 4 <= 32 * ZPITCH * 2, "these sums take the place of its z");
   __shared__ __attribute__((aligned(16))) uint16_t hs[2][RT * 16][PITCH];
   __shared__ __attribute__((aligned(16))) int toks[TOKENS];
-  const Tile tile = tile_of(p.starts, p.T, p.n, p.size, blockIdx.x);
+  const int chunks = p.side[1].chunks;
+  const int slot = ALSO_H ? (int)blockIdx.x / chunks : (int)blockIdx.x, place = ALSO_H ? (int)blockIdx.x - slot * chunks : (int)blockIdx.y;
+  const Tile tile = tile_of(p.starts, p.T, p.n, p.size, slot);
   if (tile.group >= p.n || (tile.count == 0 && tile.piece > 0)) return;
-  const int which = (int)blockIdx.y >= p.side[0].chunks;
+  const int which = place >= p.side[0].chunks;
   const OuterSide &sd = p.side[which];
-  const int chunk = blockIdx.y - (which ? p.side[0].chunks : 0);
+  const int chunk = place - (which ? p.side[0].chunks : 0);
   const int rank0 = blockIdx.z * RT * 16, r = p.r, D = sd.D;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, g = lane >> 4;
   const int col = (chunk * kOuterWaves + wave) * 128 + row * 8;
@@ -595,7 +600,7 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
 #pragma unroll
     for (int j = 0; j < 8; ++j) acc[m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   [[maybe_unused]] v4i f[ALSO_H ? 4 : 1][RT];
-  [[maybe_unused]] v4f sums[2][ALSO_H ? 2 : 1][RT];   // of 64 tokens: by 32, by 16
+  [[maybe_unused]] v4f sums[HELD][ALSO_H ? 2 : 1][RT];   // by 32 tokens, by 16
   if constexpr (ALSO_H) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -646,12 +651,12 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
 #pragma unroll
-          for (int j = 0; j < RT; ++j) sums[s][m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+          for (int j = 0; j < RT; ++j) sums[s % HELD][m][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const v4i a = *(const v4i *)&zs[wave][m * 16 + row][k * 32 + g * 8];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) sums[s][m][j] = mfma(a, f[k][j], sums[s][m][j]);
+            for (int j = 0; j < RT; ++j) sums[s % HELD][m][j] = mfma(a, f[k][j], sums[s % HELD][m][j]);
           }
         }
         __builtin_amdgcn_wave_barrier();
@@ -671,7 +676,7 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
       if constexpr (ALSO_H) {
         float *mine = (float *)&zs[wave][0][0];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < HELD; ++h) {
           if (h >= count) break;
 #pragma unroll
           for (int m = 0; m < 2; ++m)
@@ -696,13 +701,11 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
     for (int sub = 0; sub < subs; sub += 2) {
       request(1, min(sub + 1, subs - 1));
       multiply(0, sub);
-      if (sub + 1 >= subs) {
-        hand_over(sub, 1);
-        break;
-      }
+      if (HELD == 1 || sub + 1 >= subs) hand_over(sub, 1);
+      if (sub + 1 >= subs) break;
       request(0, min(sub + 2, subs - 1));
       multiply(1, sub + 1);
-      hand_over(sub, 2);
+      hand_over(HELD == 1 ? sub + 1 : sub, HELD);
     }
   }
   if (!in) return;
@@ -999,9 +1002,12 @@ extern "C" int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, 
   return L8_OK;
 }
 
-// Does one reading of z for both pay?  Wherever its registers allow it, us, one reading and two: [16384,11008] 108 and 177, [4096,4096] 19.5 and
-// 28.3, [1021,2064] 12.5 and 18.1, [256,1024] 11.4 and 18.5 (the parts of h are summed up in the launch that folds the factor's gradients).
-extern "C" int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r) { return T >= 1 && r <= 16; }
+// Does one reading of z for both pay?  It costs two launches more in a backward pass, which else has both factors' gradients in one, so it
+// does where z is large, above all where the caches do not hold it for the second reading.  us of the whole backward pass, one reading and two:
+// rank 16, [16384,4096] to [16384,11008] 184 and 227, [2055,4096] to [2055,11008] 42.5 and 47.2, [8192,2048] to [8192,8192] 77 and 88, but
+// [16384,4096] to [16384,4096] 136 and 126, [6000,2048] to [6000,5632] 58 and 52, [2048,2048] to [2048,2048] 29 and 25; rank 32, [16384,4096] to
+// [16384,8192] 191 and 201, [8192,4096] to [8192,11008] 133 and 156, [16384,4096] to [16384,4096] 173 and 160.
+extern "C" int l8_lowrank_outer_shrink_pays(int64_t T, int64_t r, int64_t D) { return T >= 2048 && D >= 8192 && r <= 32; }
 
 extern "C" int64_t l8_lowrank_outer_shrink_workspace(int64_t T, int64_t r, int64_t D) {
   if (T <= 0 || r <= 0 || D <= 0) return 0;
@@ -1014,7 +1020,7 @@ extern "C" int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *
   L8_REQUIRE(one && one->grad && ((uintptr_t)one->grad % 16) == 0, "%s: null or misaligned gradient", who);
   const int64_t D = one->D;
   L8_CALL(check_sizes(who, T, n, r, D));
-  L8_REQUIRE(r <= 16, "%s: rank %lld, up to 16 are wanted", who, (long long)r);
+  L8_REQUIRE(r <= 32, "%s: rank %lld, up to 32 are wanted", who, (long long)r);
   L8_REQUIRE(T >= 1, "%s: no tokens", who);
   L8_CALL(check_plan(who, T, order, starts));
   L8_REQUIRE(one->splits >= 1 && one->splits <= 64, "%s: 1 to 64 parts, got %lld", who, (long long)one->splits);
@@ -1030,11 +1036,12 @@ extern "C" int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *
   p.f = (const uint16_t *)f, p.also = (float *)workspace;
   // one launch for both sums: row n is that of h's parts; without groups of several tiles the other rows end at once
   const int64_t sums = (T * r + 1023) / 1024, x = std::max<int64_t>(parts ? b1 : 1, std::min<int64_t>(sums, 4 * num_cus()));
-  L8_CALL(check_grid(who, slots, chunks, 1, kOuterWaves * 64));
+  L8_CALL(check_grid(who, slots * chunks, 1, 1, kOuterWaves * 64));
   L8_CALL(check_grid(who, x, 1, n + 1, 256));
-  const dim3 grid((unsigned)slots, (unsigned)chunks), block(kOuterWaves * 64);
+  const dim3 grid((unsigned)(slots * chunks)), block(kOuterWaves * 64);
   hipStream_t st = (hipStream_t)stream;
-  hipLaunchKernelGGL((lowrank_outer_kernel<1, 128, true>), grid, block, 0, st, p);
+  if (r <= 16) hipLaunchKernelGGL((lowrank_outer_kernel<1, 128, true>), grid, block, 0, st, p);
+  else hipLaunchKernelGGL((lowrank_outer_kernel<2, 128, true>), grid, block, 0, st, p);
   L8_HIP(hipGetLastError());
   hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)x, (unsigned)(n + 1)), dim3(256), 0, st, p, (int64_t)0, also);
   L8_HIP(hipGetLastError());

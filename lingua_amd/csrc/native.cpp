@@ -1438,7 +1438,7 @@ struct LowRank : torch::autograd::Function<LowRank> {
     Tensor gh, gx, ga, gb;
     Bank f;
     const float *sp = scale.defined() ? scale.const_data_ptr<float>() : nullptr;
-    const bool together = need_b && (need_x || need_a) && lib.l8_lowrank_outer_shrink_pays(rg.rows, r);
+    const bool together = need_b && (need_x || need_a) && lib.l8_lowrank_outer_shrink_pays(rg.rows, r, N);
     if (need_x || need_a) {
       TORCH_CHECK(as_bank(b, device, f), "add_lowrank backward: factors");
       if (together) {

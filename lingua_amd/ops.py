@@ -1212,13 +1212,13 @@ def lowrank_outer(sides, scale: Optional[torch.Tensor], n: int, r: int, plan):
     return grads
 
 
-def lowrank_outer_shrink_pays(T: int, r: int) -> bool:
-    """Is ``lowrank_outer_shrink`` faster than its two parts one after the other?"""
-    return bool(_lib.load().l8_lowrank_outer_shrink_pays(T, r))
+def lowrank_outer_shrink_pays(T: int, r: int, D: int) -> bool:
+    """Is a backward pass with ``lowrank_outer_shrink`` faster than one with its two parts?"""
+    return bool(_lib.load().l8_lowrank_outer_shrink_pays(T, r, D))
 
 
 def lowrank_outer_shrink(h: torch.Tensor, z: torch.Tensor, f: torch.Tensor, scale: Optional[torch.Tensor], plan):
-    """``lowrank_outer([(h, z)], scale, n, r, plan)[0]`` and ``lowrank_shrink(z, f, plan)`` from one reading of z; ranks up to 16, at least one
+    """``lowrank_outer([(h, z)], scale, n, r, plan)[0]`` and ``lowrank_shrink(z, f, plan)`` from one reading of z; ranks up to 32, at least one
     token."""
     what = "lowrank_outer_shrink"
     z, f = _rows_on_lines(z, torch.bfloat16, what), _factor(f, what)

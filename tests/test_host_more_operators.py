@@ -107,7 +107,7 @@ def test_outer_is_refused(change):
 BOTH = dict(scale=P, f=P, also=P, T=64, n=4, r=16, order=P, starts=P, ws=P, ws_bytes=1 << 30, stream=None)
 
 
-@pytest.mark.parametrize("change", [dict(T=0), dict(T=-1), dict(n=0), dict(r=24), dict(r=4), dict(D=20, ldz=24), dict(h=0), dict(splits=65), dict(z=P + 8), dict(ldz=120), dict(grad=0), dict(grad=P + 8),
+@pytest.mark.parametrize("change", [dict(T=0), dict(T=-1), dict(n=0), dict(r=40), dict(r=4), dict(D=20, ldz=24), dict(h=0), dict(splits=65), dict(z=P + 8), dict(ldz=120), dict(grad=0), dict(grad=P + 8),
                                     dict(f=None), dict(f=P + 8), dict(also=None), dict(also=P + 4), dict(scale=P + 2), dict(order=None), dict(starts=None), dict(ws=None), dict(ws=P + 8),
                                     dict(ws_bytes=64)])
 def test_outer_with_shrink_is_refused(change):
