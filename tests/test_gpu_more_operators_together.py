@@ -405,3 +405,62 @@ def test_more_than_two_to_the_31st():
     # (few tokens alone share K out differently: the sums' last bits may differ)
     want, size, _, _ = plain.lowrank(x[-tail:], x[-tail:], a, b, index[-tail:], None)
     assert within(out[-tail:], want, size) and torch.equal(out[:-tail], x[:-tail])
+
+
+def test_broadcast_and_transposed_operands(host):
+    """Operands whose rows are one row, and whose rows lie apart: results those of dense copies, gradients summed over what was broadcast."""
+    from lingua_amd import adapters, dropout, norm, rope
+    R, C = 24, 64
+    drop = dropout.Drop(0.3, dropout.numbers(4))
+    a, b = (seeded_bf16((3, 8, C), std=0.3, seed=5 + i).cuda() for i in range(2))
+    w, gy = seeded_bf16((C,), seed=8).cuda(), seeded_bf16((R, C), **GY).cuda()
+    index = torch.tensor([1], device="cuda").expand(R)
+    cos, sin = (t.cuda() for t in rope.rotary_tables(32, 50))
+    pos = torch.tensor([3], device="cuda").expand(2, 1, R)
+    heads = lambda t: t.view(1, R, 2, 32) if t.stride(0) else t.unflatten(1, (2, 32))[None]  # noqa: E731
+    calls = {"layernorm": lambda x, r: norm.layernorm(x, w, w), "add_layernorm": lambda x, r: norm.add_layernorm(x, r, w, dropout=drop)[1],
+             "add_rmsnorm": lambda x, r: norm.add_rmsnorm(x, r, w, 1e-5, drop)[1], "dropout": lambda x, r: dropout.dropout(x, drop),
+             "dropout_add": lambda x, r: dropout.dropout_add(x, r, drop), "add_lowrank": lambda x, r: adapters.add_lowrank(r, x, a, b, index),
+             "rotary_axes": lambda x, r: rope.rotary_axes(heads(x), heads(r), cos, sin, pos, (8, 8))[0].reshape(R, C)}
+    leaf, wide = seeded_bf16((1, C), seed=1).cuda().requires_grad_(), seeded_bf16((C, R), seed=2).cuda().requires_grad_()
+    for name, call in calls.items():
+        for x, r in ((leaf.expand(R, C), wide.t()), (wide.t(), leaf.expand(R, C))):
+            dense = [t.detach().clone(memory_format=torch.contiguous_format).requires_grad_() for t in (x, r)]
+            y, want = call(x if name != "rotary_axes" else x.contiguous(), r if name != "rotary_axes" else r.contiguous()), call(*dense)
+            assert torch.equal(y, want), name
+            got = torch.autograd.grad(y, (leaf, wide), gy, allow_unused=True)
+            ref = torch.autograd.grad(want, dense, gy, allow_unused=True)
+            ref = ref if x.shape == (R, C) and x.stride(0) == 0 else ref[::-1]
+            for g, d, t in zip(got, ref, (leaf, wide)):
+                if d is None:
+                    assert g is None or not g.any()
+                elif t is wide:
+                    assert torch.equal(g, d.t()), name
+                else:   # 24 rows added up in torch's order, rounded once
+                    total = d.double().sum(0, keepdim=True)
+                    assert bool(((g.double() - total).abs() <= 2.0 ** -8 * total.abs() + 25 * 2.0 ** -8 * 2.0 ** -8 * d.double().abs().sum(0)).all()), name
+
+
+def test_copied_models():
+    """A deep copy has its own numbers and requests, and computes what the model does."""
+    import copy
+    from lingua_amd import adapters, dropout
+    numbers, requests = dropout.numbers(3), adapters.Requests(2)
+    model = torch.nn.Sequential(torch.nn.Linear(64, 64, bias=False, dtype=torch.bfloat16, device="cuda"), torch.nn.Dropout(0.5))
+    adapters.add_adapters(model, requests, 8, "0")
+    dropout.convert_dropouts(model, numbers)
+    with torch.no_grad():
+        model[0].b.copy_(seeded_bf16((2, 8, 64), seed=1))
+    x = seeded_bf16((10, 64), seed=2).cuda()
+    index = torch.arange(10, device="cuda") % 3 - 1
+    requests.set(index)
+    other = copy.deepcopy(model)
+    want = model(x)
+    assert torch.equal(other(x), want)
+    requests.set(None)
+    numbers[1] += 1
+    assert torch.equal(other(x), want) and not torch.equal(model(x), want)
+    other[0].requests.set(index.roll(1))
+    requests.set(index)
+    numbers[1] -= 1
+    assert torch.equal(model(x), want)
