@@ -131,25 +131,38 @@ class Requests:
     that pass's backward pass is done (which would be an error).  Without an index (``set(None)``) the adapters are left out.
 
     The order of the tokens is written to the same memory for every batch of one shape, so that a captured forward pass that is replayed
-    after a ``set`` sees it."""
+    after a ``set`` sees it.  That memory is kept for the shapes that a capture asked for and the last 64 others."""
 
     def __init__(self, n: int):
-        self.n, self.plan = n, None
-        self._plans = {}    # a plan for each shape of tokens: a graph may go on reading one
+        self.n, self._plan = n, None
+        self._plans = {}        # of each shape of tokens, the latest last
+        self._captured = set()  # those that a graph goes on reading
+
+    @property
+    def plan(self) -> Optional[Plan]:
+        """The running batch's."""
+        if self._plan is not None and torch.cuda.is_current_stream_capturing():
+            self._captured.add((self._plan.shape, self._plan.order.device))
+        return self._plan
 
     def set(self, index: Optional[torch.Tensor]) -> None:
         """``index`` int32 or int64 on the GPU, of the shape of the batch's tokens."""
         if index is None:
-            self.plan = None
+            self._plan = None
             return
-        key = index.shape, index.device
-        plan = self._plans.get(key)
+        key = tuple(index.shape), index.device
+        plan = self._plans.pop(key, None)
         if plan is None:
             with torch.inference_mode(False):   # (a training step may be the next to want it)
-                plan = self._plans[key] = route(index, self.n)
+                plan = route(index, self.n)
+            others = [k for k in self._plans if k not in self._captured]
+            if len(others) >= 64:
+                del self._plans[others[0]]
         else:
             ops.lowrank_route(index.flatten(), self.n, out=(plan.order, plan.starts))
-        self.plan = plan
+        self._plans[key] = self._plan = plan
+        if torch.cuda.is_current_stream_capturing():
+            self._captured.add(key)
 
 
 class AdaptedLinear(torch.nn.Module):

@@ -459,3 +459,33 @@ def test_an_order_that_route_did_not_make(T, n, r):
             ops.lowrank_outer_shrink(h, y, b, scale, plan)
         torch.cuda.synchronize()
         assert (out[:guard] == 7).all() and (out[guard + T:] == 7).all() and [t.shape for t in grads] == [a.shape, b.shape]
+
+
+def test_requests_of_many_shapes():
+    """Batches of ever other sizes do not pile up memory; the shape that a captured pass reads stays."""
+    from lingua_amd import adapters
+    requests = adapters.Requests(3)
+    lin = adapters.AdaptedLinear(torch.nn.Linear(64, 128, bias=False, dtype=torch.bfloat16, device="cuda"), requests, 8)
+    x = seeded_bf16((300, 64), seed=2).cuda()
+    with torch.no_grad():
+        lin.b.copy_(seeded_bf16((3, 8, 128), std=0.3, seed=1))
+        index = torch.arange(40, device="cuda") % 4 - 1
+        requests.set(index)
+        lin(x[:40])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = lin(x[:40])
+        for T in range(1, 300):
+            requests.set(torch.full((T,), T % 3, dtype=torch.int32, device="cuda"))
+            if T % 50 == 0:
+                want = adapters.add_lowrank(lin.linear(x[:T]), x[:T], lin.a, lin.b, torch.full((T,), T % 3, device="cuda"), lin.scale)
+                assert torch.equal(lin(x[:T]), want)
+        assert len(requests._plans) <= 66
+        for i in range(2):
+            requests.set(index.roll(i))
+            want = adapters.add_lowrank(lin.linear(x[:40]), x[:40], lin.a, lin.b, index.roll(i), lin.scale)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
