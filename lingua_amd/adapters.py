@@ -151,7 +151,7 @@ class Requests:
             self._plan = None
             return
         key = tuple(index.shape), index.device
-        plan = self._plans.pop(key, None)
+        plan = self._plans.get(key)
         if plan is None:
             with torch.inference_mode(False):   # (a training step may be the next to want it)
                 plan = route(index, self.n)
@@ -160,6 +160,7 @@ class Requests:
                 del self._plans[others[0]]
         else:
             ops.lowrank_route(index.flatten(), self.n, out=(plan.order, plan.starts))
+            del self._plans[key]
         self._plans[key] = self._plan = plan
         if torch.cuda.is_current_stream_capturing():
             self._captured.add(key)

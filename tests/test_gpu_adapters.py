@@ -482,6 +482,9 @@ def test_requests_of_many_shapes():
                 want = adapters.add_lowrank(lin.linear(x[:T]), x[:T], lin.a, lin.b, torch.full((T,), T % 3, device="cuda"), lin.scale)
                 assert torch.equal(lin(x[:T]), want)
         assert len(requests._plans) <= 66
+        with pytest.raises(RuntimeError, match="int32 or int64"):
+            requests.set(index.float())     # (and what the graph reads is still there)
+        assert (40,) in [k[0] for k in requests._plans]
         for i in range(2):
             requests.set(index.roll(i))
             want = adapters.add_lowrank(lin.linear(x[:40]), x[:40], lin.a, lin.b, index.roll(i), lin.scale)
@@ -489,3 +492,19 @@ def test_requests_of_many_shapes():
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want)
+
+
+def test_compiled_module():
+    from lingua_amd import adapters
+    requests = adapters.Requests(3)
+    lin = adapters.AdaptedLinear(torch.nn.Linear(64, 128, bias=False, dtype=torch.bfloat16, device="cuda"), requests, 8)
+    with torch.no_grad():
+        lin.b.copy_(seeded_bf16((3, 8, 128), std=0.3, seed=1))
+    x = seeded_bf16((40, 64), seed=2).cuda()
+    compiled = torch.compile(lin, backend="eager")
+    for i in range(2):
+        requests.set((torch.arange(40, device="cuda") + i) % 4 - 1)
+        want, got = lin(x), compiled(x)
+        assert torch.equal(got, want)
+        for u, v in zip(torch.autograd.grad(got.float().sum(), (lin.a, lin.b)), torch.autograd.grad(want.float().sum(), (lin.a, lin.b))):
+            assert torch.equal(u, v)
