@@ -730,9 +730,10 @@ __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(cons
     }
 }
 
-// h = the sum of its parts, in their order: the workgroups of row n of `fold`'s grid.
-L8_DEV void sum_parts(const float *__restrict__ parts, int count, int64_t n, float *__restrict__ h) {
-  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < n; at += (int64_t)gridDim.x * 1024) {
+// h = the sum of its parts, in their order: the workgroups of `fold`'s grid from row `row0` on.
+L8_DEV void sum_parts(const float *__restrict__ parts, int count, int64_t n, float *__restrict__ h, int row0) {
+  const int64_t mine = (int64_t)((int)blockIdx.y - row0) * gridDim.x + blockIdx.x, all = (int64_t)((int)gridDim.y - row0) * gridDim.x;
+  for (int64_t at = (mine * 256 + threadIdx.x) * 4; at < n; at += all * 1024) {
     v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 8
     for (int i = 0; i < count; ++i) {
@@ -744,32 +745,36 @@ L8_DEV void sum_parts(const float *__restrict__ parts, int count, int64_t n, flo
   }
 }
 
-// The sums of a group's tiles, in their order, rounded: groups of more than one tile.  (And with `h`, row n: the sum of its parts.)
-__global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int64_t blocks0, float *__restrict__ h) {
-  if ((int)blockIdx.y == p.n) return sum_parts(p.also, p.side[1].chunks, (int64_t)p.T * p.r, h);
+// The sums of a group's tiles, in their order, rounded: groups of more than one tile, a row of the grid each.  (And with `h`, in the rows behind
+// them: the sum of its parts.)
+__global__ __launch_bounds__(256) void lowrank_fold_kernel(const OuterArgs p, int groups, int64_t blocks0, int64_t blocks, float *__restrict__ h) {
+  if ((int)blockIdx.y >= groups) return sum_parts(p.also, p.side[1].chunks, (int64_t)p.T * p.r, h, groups);
   const int from = within(p.starts[blockIdx.y], p.T), tokens = within(p.starts[blockIdx.y + 1], p.T) - from;
   if (tokens <= p.size) return;
-  const int which = (int64_t)blockIdx.x >= blocks0;
-  const OuterSide &sd = p.side[which];
-  const int64_t at = ((int64_t)blockIdx.x - (which ? blocks0 : 0)) * 2048 + threadIdx.x * 8, all = (int64_t)p.r * sd.D;
-  if (at >= all) return;
-  v4f lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
   const int pieces = (tokens + p.size - 1) / p.size;
   const int64_t part0 = outer_part(from, p.size, 0);   // and piece i > 0 at part0 + 2 i + 1
+#pragma unroll 1
+  for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+    const int which = block >= blocks0;
+    const OuterSide &sd = p.side[which];
+    const int64_t at = (block - (which ? blocks0 : 0)) * 2048 + threadIdx.x * 8, all = (int64_t)p.r * sd.D;
+    if (at >= all) continue;
+    v4f lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
 #pragma unroll 8
-  for (int i = 0; i < pieces; ++i) {
-    const float *part = sd.partials + (part0 + 2 * i + (i > 0)) * all + at;
-    const v4f a = *(const v4f *)part, b = *(const v4f *)(part + 4);
+    for (int i = 0; i < pieces; ++i) {
+      const float *part = sd.partials + (part0 + 2 * i + (i > 0)) * all + at;
+      const v4f a = *(const v4f *)part, b = *(const v4f *)(part + 4);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) lo[e] += a[e], hi[e] += b[e];
-  }
-  v4i out;
+      for (int e = 0; e < 4; ++e) lo[e] += a[e], hi[e] += b[e];
+    }
+    v4i out;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const float u = k < 2 ? lo[2 * k] : hi[2 * k - 4], w = k < 2 ? lo[2 * k + 1] : hi[2 * k - 3];
-    out[k] = (int)(bf16_rne_bits(u) | (bf16_rne_bits(w) << 16));
+    for (int k = 0; k < 4; ++k) {
+      const float u = k < 2 ? lo[2 * k] : hi[2 * k - 4], w = k < 2 ? lo[2 * k + 1] : hi[2 * k - 3];
+      out[k] = (int)(bf16_rne_bits(u) | (bf16_rne_bits(w) << 16));
+    }
+    *(v4i *)(sd.grad + (int64_t)blockIdx.y * all + at) = out;
   }
-  *(v4i *)(sd.grad + (int64_t)blockIdx.y * all + at) = out;
 }
 
 // ---- host ----
@@ -809,6 +814,16 @@ static int check_grid(const char *who, int64_t x, int64_t y, int64_t z, int64_t 
 }
 static int check_plan(const char *who, int64_t T, const void *order, const void *starts) {
   L8_REQUIRE((order || T == 0) && starts && ((uintptr_t)order % 4) == 0 && ((uintptr_t)starts % 4) == 0, "%s: null or misaligned order of tokens", who);
+  return L8_OK;
+}
+// The fold of a launch of `outer`: with `groups` those of several tiles, with h and `sums` workgroups of elements the sum of its parts.  Each does
+// as many blocks as it takes to stay within a launch's 2^32 threads: whatever `outer` takes has a fold.
+static int fold(const OuterArgs &p, int groups, float *h, int64_t sums, hipStream_t st) {
+  const int64_t blocks0 = ((int64_t)p.r * p.side[0].D + 2047) / 2048, blocks = blocks0 + ((int64_t)p.r * p.side[1].D + 2047) / 2048;
+  const int64_t rows = !h ? 0 : groups ? std::min<int64_t>((sums + blocks - 1) / blocks, 65535 - groups) : 1, y = groups + rows;
+  const int64_t x = std::min<int64_t>(groups ? blocks : sums, ((1 << 24) - 1) / y);
+  hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)x, (unsigned)y), dim3(256), 0, st, p, groups, blocks0, blocks, h);
+  L8_HIP(hipGetLastError());
   return L8_OK;
 }
 #define L8_CALL(expr)              \
@@ -993,13 +1008,7 @@ extern "C" int l8_lowrank_outer(const l8_lowrank_side *two, const float *scale, 
   else if (r <= 32) hipLaunchKernelGGL((lowrank_outer_kernel<2, 256, false>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((lowrank_outer_kernel<4, 128, false>), grid, block, 0, st, p);
   L8_HIP(hipGetLastError());
-  if (parts) {
-    const int64_t b0 = (r * D[0] + 2047) / 2048, b1 = (r * D[1] + 2047) / 2048;
-    L8_CALL(check_grid(who, b0 + b1, 1, n, 256));
-    hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)(b0 + b1), (unsigned)n), dim3(256), 0, st, p, b0, (float *)nullptr);
-    L8_HIP(hipGetLastError());
-  }
-  return L8_OK;
+  return parts ? fold(p, (int)n, nullptr, 0, st) : L8_OK;
 }
 
 // Does one reading of z for both pay?  It costs two launches more in a backward pass, which else has both factors' gradients in one, so it
@@ -1030,20 +1039,16 @@ extern "C" int l8_lowrank_outer_shrink(const l8_lowrank_side *one, const float *
   L8_REQUIRE(workspace && workspace_bytes >= need && ((uintptr_t)workspace % 16) == 0, "%s: needs a 16-byte aligned workspace of %lld bytes", who, (long long)need);
   OuterArgs p{};
   const int size = outer_size(T, 0, D);
-  const int64_t chunks = (D + 511) / 512, parts = T <= size ? 0 : 2 * (T / size + 1), slots = tile_slots(T, n, size), b1 = (r * D + 2047) / 2048;
+  const int64_t chunks = (D + 511) / 512, parts = T <= size ? 0 : 2 * (T / size + 1), slots = tile_slots(T, n, size);
   p.side[1] = OuterSide{one->h, (const uint16_t *)one->z, (uint16_t *)one->grad, (float *)workspace + chunks * T * r, one->ldz, (int)D, (int)one->splits, (int)chunks};
   p.scale = scale, p.order = order, p.starts = starts, p.T = (int)T, p.n = (int)n, p.r = (int)r, p.size = size;
   p.f = (const uint16_t *)f, p.also = (float *)workspace;
-  // one launch for both sums: row n is that of h's parts; without groups of several tiles the other rows end at once
-  const int64_t sums = (T * r + 1023) / 1024, x = std::max<int64_t>(parts ? b1 : 1, std::min<int64_t>(sums, 4 * num_cus()));
   L8_CALL(check_grid(who, slots * chunks, 1, 1, kOuterWaves * 64));
-  L8_CALL(check_grid(who, x, 1, n + 1, 256));
   const dim3 grid((unsigned)(slots * chunks)), block(kOuterWaves * 64);
   hipStream_t st = (hipStream_t)stream;
   if (r <= 16) hipLaunchKernelGGL((lowrank_outer_kernel<1, 128, true>), grid, block, 0, st, p);
   else hipLaunchKernelGGL((lowrank_outer_kernel<2, 128, true>), grid, block, 0, st, p);
   L8_HIP(hipGetLastError());
-  hipLaunchKernelGGL(lowrank_fold_kernel, dim3((unsigned)x, (unsigned)(n + 1)), dim3(256), 0, st, p, (int64_t)0, also);
-  L8_HIP(hipGetLastError());
-  return L8_OK;
+  // one launch for both sums
+  return fold(p, parts ? (int)n : 0, also, std::min<int64_t>((T * r + 1023) / 1024, 4 * num_cus()), st);
 }
