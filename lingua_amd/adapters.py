@@ -46,7 +46,7 @@ class LowRankFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         ctx.save_for_backward(x if need[2] else None, a if need[1] else None, b if need[1] or need[2] else None, h if need[3] else None, scale, order, starts)
         ctx.learns = tuple(f8._learns(t) for t in (x, a, b))
-        ctx.sizes = a.shape[0], a.shape[1]
+        ctx.sizes, ctx.order = (a.shape[0], a.shape[1]), f8._stamp(order)
         return ops.lowrank_expand(y, h, b, scale, plan)
 
     @staticmethod
@@ -54,6 +54,7 @@ class LowRankFn(torch.autograd.Function):
         if gy.dtype != torch.bfloat16:
             raise RuntimeError(f"add_lowrank backward: bf16 gradients required, got {gy.dtype}")
         x, a, b, h, scale, order, starts = ctx.saved_tensors
+        f8._unchanged(ctx.order, order, "add_lowrank", "the order of the tokens was")
         plan, (n, r) = (order.contiguous(), starts.contiguous()), ctx.sizes   # (hooks hand them back in any layout)
         need_y, need_x, need_a, need_b = ctx.needs_input_grad[:4]
         gx = ga = gb = None
@@ -128,7 +129,8 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
 
 class Requests:
     """Which adapter each token of the running batch has, shared by the banks of a model: ``set`` it before a forward pass, and not again before
-    that pass's backward pass is done (which would be an error).  Without an index (``set(None)``) the adapters are left out.
+    that pass's backward pass is done (which would be an error, also where ``torch.utils.checkpoint`` with ``use_reentrant=False`` computes the
+    forward pass again).  Without an index (``set(None)``) the adapters are left out.
 
     The order of the tokens is written to the same memory for every batch of one shape, so that a captured forward pass that is replayed
     after a ``set`` sees it.  That memory is kept for the shapes that a capture asked for and the last 64 others."""

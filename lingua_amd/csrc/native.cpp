@@ -882,6 +882,15 @@ variable_list once(variable_list grads, std::initializer_list<bool> varies, cons
   return grads;
 }
 bool learns(const Tensor &t) { return t.defined() && t.requires_grad(); }
+// Where an operand that says which elements or adapters a pass is about stood, and in which version.  A saved tensor's own check does not run
+// under hooks, so a forward pass that is computed again (activation checkpointing) after the operand has changed would hand the backward pass the
+// new contents: the same memory in another version.  (Hooks that kept a copy hand back other memory, with the contents of the forward pass.)
+std::vector<int64_t> stamp(const Tensor &t) { return {(int64_t)(uintptr_t)t.const_data_ptr(), t.is_inference() ? -1 : (int64_t)t._version()}; }
+void unchanged(const c10::IValue &then, const Tensor &now, const char *what, const char *name) {
+  const auto was = then.toIntVector();
+  TORCH_CHECK(was[1] < 0 || now.is_inference() || was[0] != (int64_t)(uintptr_t)now.const_data_ptr() || was[1] == (int64_t)now._version(), what, ": ", name,
+              " modified by an inplace operation between the forward pass and its recomputation");
+}
 // A leaf's gradient is accumulated on the stream that its node was made on, and the node lives as long as a graph that holds it.  One
 // made on the default stream cannot take part in a capture: the captured backward pass would end the process.
 void refuse_captured(std::initializer_list<const Tensor *> inputs, const char *what) {
@@ -1193,6 +1202,7 @@ NormOut norm_pass(const Tensor &x, const Tensor &res, const Tensor &w, const Ten
   return out;
 }
 
+constexpr const char *kNumbers = "the seed and step were";
 struct Norm : torch::autograd::Function<Norm> {
   static const char *name(bool centred, bool added) { return !centred ? "add_rmsnorm" : added ? "add_layernorm" : "layernorm"; }
   // -> [h,] y[, q, scale[, col amax]]
@@ -1209,6 +1219,7 @@ struct Norm : torch::autograd::Function<Norm> {
     ctx->saved_data["b"] = bt.defined() ? (int64_t)bt.scalar_type() : (int64_t)0;
     ctx->saved_data["site"] = site;
     ctx->saved_data["threshold"] = threshold;
+    if (n.defined()) ctx->saved_data["numbers"] = stamp(n);
     variable_list all;
     if (r.defined()) all.push_back(out.h);
     all.push_back(out.y);
@@ -1230,6 +1241,7 @@ struct Norm : torch::autograd::Function<Norm> {
     const bool need_x = ctx->needs_input_grad(at++), need_r = added && ctx->needs_input_grad(at++);
     const bool need_w = has_w && ctx->needs_input_grad(at++), need_b = has_b && ctx->needs_input_grad(at++);
     const Dropped drop{saved[3], ctx->saved_data["site"].toInt(), ctx->saved_data["threshold"].toInt()};
+    if (saved[3].defined()) unchanged(ctx->saved_data["numbers"], saved[3], what, kNumbers);
     Tensor gx, gres, gw, gb;
     auto all = [&](std::initializer_list<bool> varies) {
       return once({gx, gres, gw, gb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, varies, what);
@@ -1339,13 +1351,15 @@ struct Dropout : torch::autograd::Function<Dropout> {
     ctx->saved_data["site"] = site;
     ctx->saved_data["threshold"] = threshold;
     ctx->saved_data["added"] = res.has_value();
+    ctx->saved_data["numbers"] = stamp(numbers);
     return pass(x, res.value_or(Tensor()), numbers, site, threshold);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor &g = grads[0];
     TORCH_CHECK(g.scalar_type() == at::kBFloat16, "dropout backward: bf16 gradients required, got ", g.scalar_type());
-    const Tensor numbers = ctx->get_saved_variables()[0].contiguous();
+    const Tensor kept = ctx->get_saved_variables()[0], numbers = kept.contiguous();
     const bool added = ctx->saved_data["added"].toBool();
+    unchanged(ctx->saved_data["numbers"], kept, added ? "dropout_add" : "dropout", kNumbers);
     Tensor gx;
     if (ctx->needs_input_grad(0)) {
       const c10::DeviceGuard guard(g.device());
@@ -1419,10 +1433,12 @@ struct LowRank : torch::autograd::Function<LowRank> {
     ctx->saved_data["like"] = x.sizes().vec();
     ctx->saved_data["bank"] = std::vector<int64_t>{fa.n, fa.r, fa.cols, fb.cols};
     ctx->saved_data["learns"] = (int64_t)(learn_x | (learn_a << 1) | (learn_b << 2));
+    ctx->saved_data["order"] = stamp(order);
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    unchanged(ctx->saved_data["order"], saved[5], kName, "the order of the tokens was");
     const Tensor gy = gradient(grads[0], kName);
     const int device = gy.get_device();
     const c10::DeviceGuard guard(gy.device());

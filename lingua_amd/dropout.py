@@ -3,8 +3,9 @@ mask is stored -- forward and backward compute the same bits, and so does a forw
 
 ``numbers(seed, device)`` makes the two numbers {seed, step} that a program keeps on the GPU; it adds one to the step between two training
 steps (``n[1] += 1``, which a captured graph may do by itself: its replays then drop other elements).  Changed between a forward pass and its
-backward pass they are an error, as every saved tensor's in-place change is.  Ranks that hold other tokens take other seeds.  ``Drop(p, numbers, site)`` says what a call drops; calls of
-one step that are to drop independently have sites of their own.  The norms of ``lingua_amd.norm`` take a ``Drop`` for the operand that they
+backward pass they are an error, as every saved tensor's in-place change is, also where ``torch.utils.checkpoint`` (``use_reentrant=False``) computes
+the forward pass again; the replay of a graph that changes them is not seen by the host.  Ranks that hold other tokens take other seeds.
+``Drop(p, numbers, site)`` says what a call drops; calls of one step that are to drop independently have sites of their own.  The norms of ``lingua_amd.norm`` take a ``Drop`` for the operand that they
 add to the residual.  ``Dropout`` stands in for ``nn.Dropout``; ``convert_dropouts(model, numbers)`` swaps the modules and numbers their sites.
 
 The share that is dropped is the multiple of 2^-16 next to ``p``, and what stays is scaled by that share.  A dropped element is zero whatever
@@ -37,7 +38,7 @@ class DropoutFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, numbers, p, site):
         ctx.save_for_backward(numbers)
-        ctx.p, ctx.site = p, site
+        ctx.p, ctx.site, ctx.added, ctx.numbers = p, site, residual is not None, f8._stamp(numbers)
         return ops.dropout(x, Drop(p, numbers, site), residual)
 
     @staticmethod
@@ -45,6 +46,7 @@ class DropoutFn(torch.autograd.Function):
         if g.dtype != torch.bfloat16:
             raise RuntimeError(f"dropout backward: bf16 gradients required, got {g.dtype}")
         numbers, = ctx.saved_tensors
+        f8._unchanged(ctx.numbers, numbers, "dropout_add" if ctx.added else "dropout", "the seed and step were")
         gx = None
         if ctx.needs_input_grad[0]:
             varies = f8._learns(g)

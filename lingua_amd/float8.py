@@ -620,6 +620,19 @@ def _once(what, grads, varies):
                  for g, v in zip(grads, varies))
 
 
+def _stamp(t):
+    """Where an operand stood and in which version: for ``_unchanged``."""
+    return None if t is None or t.is_inference() else (t.data_ptr(), t._version)
+
+
+def _unchanged(stamp, t, what, name):
+    """An error where a backward pass is handed an operand that changed after the forward pass.  A saved tensor's own check does not run under
+    hooks: a forward pass that is computed again (activation checkpointing) saves the same memory in another version.  (Hooks that kept a copy
+    hand back other memory, with the contents of the forward pass.)"""
+    if stamp is not None and not t.is_inference() and t.data_ptr() == stamp[0] and t._version != stamp[1]:
+        raise RuntimeError(f"{what}: {name} modified by an inplace operation between the forward pass and its recomputation")
+
+
 def _learns(t) -> bool:
     return t is not None and t.requires_grad
 

@@ -112,7 +112,7 @@ class NormFn(torch.autograd.Function):
             f8._fwd_cast.put(y.detach(), (q, s, col), "norm")
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x if h is None else h, weight, bias, stats, numbers)
-        ctx.p, ctx.site, ctx.centred, ctx.added = p, site, centred, h is not None
+        ctx.p, ctx.site, ctx.centred, ctx.added, ctx.numbers = p, site, centred, h is not None, f8._stamp(numbers)
         ctx.sum_learns = x.requires_grad or f8._learns(residual)
         return y if h is None else (h, y)
 
@@ -127,6 +127,7 @@ class NormFn(torch.autograd.Function):
         drop = None if numbers is None else dr.Drop(ctx.p, numbers.contiguous(), ctx.site)   # (hooks hand it back in any layout)
         rest = (None,) * 7
         what = _name(ctx.centred, ctx.added)
+        f8._unchanged(ctx.numbers, numbers, what, "the seed and step were")
         if gy is None:   # only the sum was used, if anything
             gx = gh if need[0] else None
             if gx is not None and drop is not None:
