@@ -129,8 +129,8 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
 
 class Requests:
     """Which adapter each token of the running batch has, shared by the banks of a model: ``set`` it before a forward pass, and not again before
-    that pass's backward pass is done (which would be an error, also where ``torch.utils.checkpoint`` with ``use_reentrant=False`` computes the
-    forward pass again).  Without an index (``set(None)``) the adapters are left out.
+    that pass's backward pass is done (which would be an error, also where ``torch.utils.checkpoint`` computes the forward pass again; with
+    ``use_reentrant=True`` nothing is kept of that pass, and what the last one went by has to do).  Without an index (``set(None)``) the adapters are left out.
 
     The order of the tokens is written to the same memory for every batch of one shape, so that a captured forward pass that is replayed
     after a ``set`` sees it.  That memory is kept for the shapes that a capture asked for and the last 64 others."""
@@ -139,10 +139,17 @@ class Requests:
         self.n, self._plan = n, None
         self._plans = {}        # of each shape of tokens, the latest last
         self._captured = set()  # those that a graph goes on reading
+        self._read = None       # what the last forward pass went by: a plan and its version
 
     @property
     def plan(self) -> Optional[Plan]:
         """The running batch's."""
+        if not torch.compiler.is_compiling():
+            now = self._plan, 0 if self._plan is None else self._plan.order._version
+            if not f8._in_backward():
+                self._read = now
+            elif self._read not in (None, now):
+                raise RuntimeError("Requests: set between a forward pass and its recomputation")
         if self._plan is not None and torch.cuda.is_current_stream_capturing():
             self._captured.add((self._plan.shape, self._plan.order.device))
         return self._plan

@@ -620,6 +620,11 @@ def _once(what, grads, varies):
                  for g, v in zip(grads, varies))
 
 
+def _in_backward() -> bool:
+    """Does a backward pass make this call?  A forward pass that is made there is a recomputation."""
+    return torch._C._current_graph_task_id() >= 0
+
+
 def _stamp(t):
     """Where an operand stood and in which version: for ``_unchanged``."""
     return None if t is None or t.is_inference() else (t.data_ptr(), t._version)

@@ -70,3 +70,33 @@ def test_copies_kept_on_the_host(name, host):
         y = call(x)
     advance()
     assert torch.equal(torch.autograd.grad(y, x, g)[0], want)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_modules_of_requests(reentrant, host):
+    """Of an adapted linear under either kind of checkpointing: the plain gradients, and an error where other requests, or none, were set before
+    the backward pass.  (A recomputation that is stopped when all saved tensors are there again does not ask for requests that the forward pass
+    did not have: its gradients are right.)"""
+    from lingua_amd import adapters
+    requests = adapters.Requests(3)
+    lin = adapters.AdaptedLinear(torch.nn.Linear(64, 128, bias=False, dtype=torch.bfloat16, device="cuda"), requests, 8)
+    torch.nn.init.normal_(lin.b, std=0.3)
+    x, g = seeded_bf16((48, 64), seed=1).cuda().requires_grad_(), seeded_bf16((48, 128), std=0.1, seed=2).cuda()
+    index = torch.arange(48, device="cuda") % 4 - 1
+    call = lambda t: lin(t) * 2.0  # noqa: E731
+    for i in (index, index.roll(1), None):
+        requests.set(i)
+        want = torch.autograd.grad(call(x), x, g)[0]
+        x.grad = None
+        checkpoint(call, x, use_reentrant=reentrant).backward(g)
+        assert torch.equal(x.grad, want)
+    for first, second in ((index, index.roll(1)), (index, None), (None, index), (index, index[:8])):
+        requests.set(first)
+        want = torch.autograd.grad(call(x), x, g)[0]
+        y = checkpoint(call, x, use_reentrant=reentrant)
+        requests.set(second)
+        if first is None and not reentrant:
+            assert torch.equal(torch.autograd.grad(y, x, g)[0], want)
+            continue
+        with pytest.raises(RuntimeError, match="Requests: set between a forward pass and its recomputation"):
+            y.backward(g)
