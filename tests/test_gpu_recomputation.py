@@ -100,3 +100,68 @@ def test_modules_of_requests(reentrant, host):
             continue
         with pytest.raises(RuntimeError, match="Requests: set between a forward pass and its recomputation"):
             y.backward(g)
+
+
+class Twice(torch.nn.Module):
+    def __init__(self, both):
+        super().__init__()
+        self.drop, self.both = torch.nn.Dropout(0.5), both
+
+    def forward(self, x, reentrant=None):
+        def part(t):
+            t = self.drop(t)
+            return self.drop(t * 1.5) if self.both else t * 1.5
+        return part(x) if reentrant is None else checkpoint(part, x, use_reentrant=reentrant)
+
+
+def test_a_module_that_is_called_twice(host):
+    """Its two calls drop independently, forward and backward alike, and the pass repeated drops the same again."""
+    from lingua_amd import dropout
+    model = dropout.convert_dropouts(Twice(True), dropout.numbers(3))
+    x = torch.ones(1 << 20, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    y = model(x)
+    gx, = torch.autograd.grad(y, x, torch.ones_like(y))
+    stays = float((y != 0).double().mean())    # of two independent draws of a half: a quarter
+    assert abs(stays - 0.25) < 5 * (0.25 * 0.75 / x.numel()) ** 0.5
+    assert torch.equal(gx, y.detach()) and torch.equal(model(x), y)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_modules_of_dropout(reentrant, host):
+    """Under either kind of checkpointing: the plain gradients of a module that is called once, an error for one that is called twice and for a
+    step that was advanced before the backward pass."""
+    from lingua_amd import dropout
+    n = dropout.numbers(3)
+    x, g = seeded_bf16((48, 64), seed=1).cuda().requires_grad_(), seeded_bf16((48, 64), std=0.1, seed=2).cuda()
+    model = dropout.convert_dropouts(Twice(False), n)
+    for _ in range(2):
+        want, = torch.autograd.grad(model(x), x, g)
+        x.grad = None
+        model(x, reentrant).backward(g)
+        assert torch.equal(x.grad, want)
+        n[1] += 1
+    y = model(x, reentrant)
+    n[1] += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation between the forward pass and its recomputation"):
+        y.backward(g)
+    model = dropout.convert_dropouts(Twice(True), n)
+    y = model(x, reentrant)
+    model.eval()
+    model(x)
+    model.train()
+    with pytest.raises(RuntimeError, match="several times in a forward pass"):
+        y.backward(g)
+
+
+def test_compiled_model():
+    from lingua_amd import dropout
+    n = dropout.numbers(3)
+    x, g = seeded_bf16((48, 64), seed=1).cuda().requires_grad_(), seeded_bf16((48, 64), std=0.1, seed=2).cuda()
+    model = dropout.convert_dropouts(Twice(True), n)
+    torch._dynamo.reset()
+    compiled = torch.compile(model, backend="eager")
+    for _ in range(3):
+        want, got = model(x), compiled(x)
+        assert torch.equal(got, want) and torch.equal(torch.autograd.grad(got, x, g)[0], torch.autograd.grad(want, x, g)[0])
+        n[1] += 1
+    torch._dynamo.reset()

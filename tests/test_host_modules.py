@@ -1,0 +1,86 @@
+"""What the modules of dropout and adapters do with a model's structure: no GPU needed."""
+import copy
+import io
+
+import pytest
+import torch
+
+from lingua_amd import adapters, dropout
+
+
+class Twice(torch.nn.Module):
+    """A dropout that is called twice in a forward pass, and one that is called once."""
+
+    def __init__(self):
+        super().__init__()
+        self.drop, self.last = torch.nn.Dropout(0.1), torch.nn.Dropout(0.2)
+
+    def forward(self, fail=False):
+        sites = [self.drop.drop().site, self.last.drop().site, self.drop.drop().site]
+        if fail:
+            raise ValueError
+        return sites
+
+
+def test_calls_of_a_forward_pass_drop_other_elements():
+    """And a forward pass that is repeated drops the same again, also one behind a pass that ended early, and in a copy of the model."""
+    numbers = dropout.numbers(1, "cpu")
+    model = dropout.convert_dropouts(Twice(), numbers)
+    want = [0, 1, 1 << 20]
+    assert model() == want and model() == want
+    with pytest.raises(ValueError):
+        model(fail=True)
+    assert model() == want
+    other = copy.deepcopy(model)
+    assert other() == want and other.drop._pass is not model.drop._pass and other.drop.numbers is not numbers
+    buffer = io.BytesIO()
+    torch.save(model, buffer)
+    assert torch.load(io.BytesIO(buffer.getvalue()), weights_only=False)() == want
+    # outside a pass nothing is counted
+    assert [model.drop.drop().site for _ in range(3)] == [0, 0, 0]
+    model.eval()
+    assert model.drop.drop() is None
+
+
+def test_shared_parents():
+    """A block that stands at two places: one dropout, whose calls are told apart where the model has a forward pass, and refused where it has
+    none."""
+    block = torch.nn.Sequential(torch.nn.Identity(), torch.nn.Dropout(0.1))
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.first, self.second = block, block
+
+        def forward(self):
+            return [part[1].drop().site for part in (self.first, self.second)]
+
+    with pytest.raises(RuntimeError, match="several places of a ModuleList"):
+        dropout.convert_dropouts(torch.nn.ModuleList([block, block]), dropout.numbers(1, "cpu"))
+    assert type(block[1]) is torch.nn.Dropout
+    model = dropout.convert_dropouts(Model(), dropout.numbers(1, "cpu"))
+    assert model.first[1] is model.second[1] and model() == [0, 1 << 20]
+
+
+def test_sites_that_are_taken():
+    """By modules made by hand, also as a later call of a lower site."""
+    n = dropout.numbers(1, "cpu")
+    model = torch.nn.ModuleList([dropout.Dropout(0.1, n, 0), dropout.Dropout(0.1, n, (5 << 20) + 1), torch.nn.Dropout(0.3), torch.nn.Dropout(0.3)])
+    dropout.convert_dropouts(model, n)
+    assert [m.site for m in model] == [0, (5 << 20) + 1, 2, 3]
+
+    class Model(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.drop = torch.nn.Dropout(0.5)
+
+        def forward(self, times):
+            return [self.drop.drop().site for _ in range(times)]
+
+    model = dropout.convert_dropouts(Model(), n)
+    assert model(4096) == [k << 20 for k in range(4096)]
+    with pytest.raises(RuntimeError, match="4096"):
+        model(4097)
+    model.drop.site = 1 << 20
+    with pytest.raises(RuntimeError, match="sites below"):
+        model(2)
