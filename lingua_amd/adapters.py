@@ -89,10 +89,12 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     ``x``      bf16 [..., K], its input
     ``a, b``   bf16 [n, r, K] and [n, r, N]; r a multiple of 8 up to 128, K and N multiples of 8
     ``index``  int32 or int64 of the tokens' shape, or the ``Plan`` that ``route`` made of it; a token with -1 has no adapter
-    ``scale``  fp32 [n], or None for ones; no gradient flows to it
+    ``scale``  fp32 [n], or None for ones; no gradient flows to it: one that asks for a gradient is an error
     """
     what = "add_lowrank"
     planned = isinstance(index, Plan)
+    if scale is not None and scale.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: the scale asks for a gradient, and none flows to it")
     if f8._native_call(x, 0) and f8._plain_call() and (not planned or (index.n == a.shape[0] and index.shape == x.shape[:-1])):
         at = (None, index.order, index.starts) if planned else (index, None, None)
         out = _lib.native_for(x.get_device()).add_lowrank(y, x, a, b, scale, *at)

@@ -84,3 +84,14 @@ def test_sites_that_are_taken():
     model.drop.site = 1 << 20
     with pytest.raises(RuntimeError, match="sites below"):
         model(2)
+
+
+def test_a_scale_that_asks_for_a_gradient_is_refused():
+    """It would learn nothing."""
+    y, x = torch.zeros(4, 64, dtype=torch.bfloat16), torch.zeros(4, 32, dtype=torch.bfloat16)
+    a, b, index = torch.zeros(2, 8, 32, dtype=torch.bfloat16), torch.zeros(2, 8, 64, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int32)
+    scale = torch.ones(2, requires_grad=True)
+    with pytest.raises(RuntimeError, match="scale asks for a gradient"):
+        adapters.add_lowrank(y, x, a, b, index, scale)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):    # (without gradients it is as good as any)
+        adapters.add_lowrank(y, x, a, b, index, scale)
