@@ -67,7 +67,8 @@ def rotary_axes(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torc
     """``(xq, xk)`` [B,S,H,D] bf16 with pairs of columns turned by the positions of their tokens on several axes: pair i, of axis a, by the
     angle of row ``positions[a,b,s]``, column i of the tables; the columns behind the last pair are copied.
 
-    ``cos``, ``sin``  fp32 [P, pairs]: ``rotary_tables`` (one run of frequencies over all pairs) or ``axes_tables`` (one for each axis)
+    ``cos``, ``sin``  fp32 [P, pairs]: ``rotary_tables`` (one run of frequencies over all pairs) or ``axes_tables`` (one for each axis); no
+                      gradient flows to them: tables that ask for one are an error
     ``positions``     int32 or int64, broadcastable to [axes,B,S].  A token of which any position is outside [0, P) becomes NaN.
     ``sections``      pairs that each of up to four axes turns, their sum cos.shape[1]
     ``order``         "sections": an axis's pairs side by side, the axes in their order; "rounds": a pair to each axis in turn, an axis that
@@ -78,6 +79,8 @@ def rotary_axes(xq: torch.Tensor, xk: torch.Tensor, cos: torch.Tensor, sin: torc
         raise RuntimeError(f"rotary_axes: unknown layout {layout!r}, one of {LAYOUTS}")
     if order not in ORDERS:
         raise RuntimeError(f"rotary_axes: unknown order {order!r}, one of {ORDERS}")
+    if (cos.requires_grad or sin.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("rotary_axes: the tables ask for a gradient, and none flows to them")
     sections = tuple(sections)
     if f8._native_call(xq, 0) and f8._plain_call():
         res = _lib.native_for(xq.get_device()).rotary_pair(xq, xk, cos, sin, positions, layout == "half", sections, order == "rounds")

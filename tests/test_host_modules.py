@@ -5,7 +5,7 @@ import io
 import pytest
 import torch
 
-from lingua_amd import adapters, dropout
+from lingua_amd import adapters, dropout, rope
 
 
 class Twice(torch.nn.Module):
@@ -95,3 +95,12 @@ def test_a_scale_that_asks_for_a_gradient_is_refused():
         adapters.add_lowrank(y, x, a, b, index, scale)
     with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):    # (without gradients it is as good as any)
         adapters.add_lowrank(y, x, a, b, index, scale)
+
+
+def test_tables_that_ask_for_a_gradient_are_refused():
+    """Of positions on several axes: they would learn nothing."""
+    q, pos = torch.zeros(1, 2, 4, 16, dtype=torch.bfloat16), torch.zeros(3, 1, 2, dtype=torch.int64)
+    table, learnt = torch.zeros(4, 8), torch.zeros(4, 8, requires_grad=True)
+    for cos, sin in ((learnt, table), (table, learnt)):
+        with pytest.raises(RuntimeError, match="tables ask for a gradient"):
+            rope.rotary_axes(q, q, cos, sin, pos, (4, 2, 2))
