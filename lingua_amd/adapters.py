@@ -212,7 +212,8 @@ class AdaptedLinear(torch.nn.Module):
 
 def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, filter: str, alpha: Optional[float] = None) -> torch.nn.Module:
     """Put a bank of ``requests.n`` adapters beside every ``nn.Linear`` (or ``Fp8Linear``, ``Mxfp4Linear``) whose dotted name matches
-    ``filter``; the linears keep their parameters, under ``linear.`` in the state dict.  Fused feed-forwards multiply by their linears' weights
+    ``filter``; the linears keep their parameters, under ``linear.`` in the state dict.  A linear that stands at several places gets a bank at
+    each (one in a shared parent: one bank).  Fused feed-forwards multiply by their linears' weights
     themselves, so those take no adapters: an error."""
     filter_re = re.compile(filter)
     for name, module in root_module.named_modules():
@@ -221,10 +222,12 @@ def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, fi
                 if filter_re.search(f"{name}.{child}" if name else child):
                     raise RuntimeError(f"add_adapters: {name!r} is a fused feed-forward, whose {child} is not called (leave it out of fuse_feed_forward)")
 
-    def replace(module: torch.nn.Module, name: str) -> torch.nn.Module:
-        if not isinstance(module, torch.nn.Linear) or not filter_re.search(name) or name.endswith(".linear") and name[:-7] in banks:
+    def walk(module: torch.nn.Module, name: str) -> torch.nn.Module:
+        if isinstance(module, AdaptedLinear):   # (the linear inside is not adapted twice)
             return module
-        return AdaptedLinear(module, requests, rank, alpha)
+        for child_name, child in list(module._modules.items()):
+            if child is not None:
+                setattr(module, child_name, walk(child, f"{name}.{child_name}" if name else child_name))
+        return AdaptedLinear(module, requests, rank, alpha) if isinstance(module, torch.nn.Linear) and filter_re.search(name) else module
 
-    banks = {name for name, m in root_module.named_modules() if isinstance(m, AdaptedLinear)}
-    return f8.named_replace(replace, root_module)
+    return walk(root_module, "")

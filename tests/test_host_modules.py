@@ -104,3 +104,23 @@ def test_tables_that_ask_for_a_gradient_are_refused():
     for cos, sin in ((learnt, table), (table, learnt)):
         with pytest.raises(RuntimeError, match="tables ask for a gradient"):
             rope.rotary_axes(q, q, cos, sin, pos, (4, 2, 2))
+
+
+def test_a_linear_at_several_places():
+    """A bank at each place, also below one parent; one in a shared parent has one."""
+    lin = torch.nn.Linear(16, 16, bias=False)
+    model = torch.nn.ModuleDict({"stack": torch.nn.Sequential(lin, torch.nn.ReLU(), lin), "other": lin, "none": None})
+    block = torch.nn.Sequential(torch.nn.Linear(16, 16))
+    model["a"], model["b"] = block, block
+    requests = adapters.Requests(2)
+    for _ in range(2):      # (and not one in another)
+        adapters.add_adapters(model, requests, 8, "")
+        banks = [model["stack"][0], model["stack"][2], model["other"]]
+        assert all(type(m) is adapters.AdaptedLinear and m.linear is lin for m in banks) and len({id(m) for m in banks}) == 3
+        assert type(block[0]) is adapters.AdaptedLinear and type(block[0].linear) is torch.nn.Linear and model["a"][0] is model["b"][0]
+    assert model["none"] is None
+
+
+def test_a_linear_that_has_a_bank_already():
+    model = adapters.add_adapters(torch.nn.Linear(16, 16), adapters.Requests(2), 8, "")
+    assert adapters.add_adapters(model, model.requests, 8, "") is model and type(model.linear) is torch.nn.Linear
