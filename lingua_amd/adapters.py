@@ -213,7 +213,7 @@ class AdaptedLinear(torch.nn.Module):
 def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, filter: str, alpha: Optional[float] = None) -> torch.nn.Module:
     """Put a bank of ``requests.n`` adapters beside every ``nn.Linear`` (or ``Fp8Linear``, ``Mxfp4Linear``) whose dotted name matches
     ``filter``; the linears keep their parameters, under ``linear.`` in the state dict.  A linear that stands at several places gets a bank at
-    each (one in a shared parent: one bank).  Fused feed-forwards multiply by their linears' weights
+    each (one in a shared parent: one bank).  A filter that names no linear is an error.  Fused feed-forwards multiply by their linears' weights
     themselves, so those take no adapters: an error."""
     filter_re = re.compile(filter)
     for name, module in root_module.named_modules():
@@ -221,6 +221,9 @@ def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, fi
             for child in ("w1", "w2", "w3"):
                 if filter_re.search(f"{name}.{child}" if name else child):
                     raise RuntimeError(f"add_adapters: {name!r} is a fused feed-forward, whose {child} is not called (leave it out of fuse_feed_forward)")
+
+    if not any(isinstance(m, (torch.nn.Linear, AdaptedLinear)) and filter_re.search(name) for name, m in root_module.named_modules(remove_duplicate=False)):
+        raise RuntimeError(f"add_adapters: the filter {filter!r} names no linear")
 
     def walk(module: torch.nn.Module, name: str) -> torch.nn.Module:
         if isinstance(module, AdaptedLinear):   # (the linear inside is not adapted twice)

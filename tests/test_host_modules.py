@@ -124,3 +124,11 @@ def test_a_linear_at_several_places():
 def test_a_linear_that_has_a_bank_already():
     model = adapters.add_adapters(torch.nn.Linear(16, 16), adapters.Requests(2), 8, "")
     assert adapters.add_adapters(model, model.requests, 8, "") is model and type(model.linear) is torch.nn.Linear
+
+
+def test_a_filter_that_names_no_linear_is_refused():
+    model = torch.nn.ModuleDict({"w1": torch.nn.Linear(16, 16), "norm": torch.nn.LayerNorm(16)})
+    for match in ("w2", "norm", "w1.weight"):
+        with pytest.raises(RuntimeError, match="names no linear"):
+            adapters.add_adapters(model, adapters.Requests(2), 8, match)
+    assert type(model["w1"]) is torch.nn.Linear
