@@ -216,12 +216,11 @@ def add_adapters(root_module: torch.nn.Module, requests: Requests, rank: int, fi
     each (one in a shared parent: one bank).  A filter that names no linear is an error.  Fused feed-forwards multiply by their linears' weights
     themselves, so those take no adapters: an error."""
     filter_re = re.compile(filter)
-    for name, module in root_module.named_modules():
+    for name, module in root_module.named_modules(remove_duplicate=False):
         if isinstance(module, Fp8FeedForward):
             for child in ("w1", "w2", "w3"):
                 if filter_re.search(f"{name}.{child}" if name else child):
                     raise RuntimeError(f"add_adapters: {name!r} is a fused feed-forward, whose {child} is not called (leave it out of fuse_feed_forward)")
-
     if not any(isinstance(m, (torch.nn.Linear, AdaptedLinear)) and filter_re.search(name) for name, m in root_module.named_modules(remove_duplicate=False)):
         raise RuntimeError(f"add_adapters: the filter {filter!r} names no linear")
 

@@ -132,3 +132,14 @@ def test_a_filter_that_names_no_linear_is_refused():
         with pytest.raises(RuntimeError, match="names no linear"):
             adapters.add_adapters(model, adapters.Requests(2), 8, match)
     assert type(model["w1"]) is torch.nn.Linear
+
+
+def test_a_fused_feed_forward_at_several_places_is_refused():
+    """By any of its names."""
+    from lingua_amd import swiglu
+    fused = swiglu.Fp8FeedForward(*(torch.nn.Linear(*s, bias=False, dtype=torch.bfloat16) for s in ((32, 64), (32, 64), (64, 32))))
+    model = torch.nn.ModuleDict({"first": fused, "second": fused})
+    for match in ("first.w1", "second.w2"):
+        with pytest.raises(RuntimeError, match="fused feed-forward"):
+            adapters.add_adapters(model, adapters.Requests(2), 8, match)
+    assert type(fused.w2) is torch.nn.Linear
