@@ -93,13 +93,13 @@ def add_lowrank(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tens
     """
     what = "add_lowrank"
     planned = isinstance(index, Plan)
-    if scale is not None and scale.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError(f"{what}: the scale asks for a gradient, and none flows to it")
     if f8._native_call(x, 0) and f8._plain_call() and (not planned or (index.n == a.shape[0] and index.shape == x.shape[:-1])):
         at = (None, index.order, index.starts) if planned else (index, None, None)
         out = _lib.native_for(x.get_device()).add_lowrank(y, x, a, b, scale, *at)
         if out is not None:
             return out
+    if scale is not None and scale.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{what}: the scale asks for a gradient, and none flows to it")
     if a.dim() != 3 or b.dim() != 3 or a.shape[:2] != b.shape[:2] or x.dim() < 1 or y.dim() < 1 or x.shape[-1] != a.shape[2] or y.shape[-1] != b.shape[2]:
         raise RuntimeError(f"{what}: factors {tuple(a.shape)} and {tuple(b.shape)} do not fit an input {tuple(x.shape)} and an output {tuple(y.shape)}")
     for t in (y, x, a, b):

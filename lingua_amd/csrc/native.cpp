@@ -885,12 +885,15 @@ bool learns(const Tensor &t) { return t.defined() && t.requires_grad(); }
 // Where an operand that says which elements or adapters a pass is about stood, and in which version.  A saved tensor's own check does not run
 // under hooks, so a forward pass that is computed again (activation checkpointing) after the operand has changed would hand the backward pass the
 // new contents: the same memory in another version.  (Hooks that kept a copy hand back other memory, with the contents of the forward pass.)
-std::vector<int64_t> stamp(const Tensor &t) { return {(int64_t)(uintptr_t)t.const_data_ptr(), t.is_inference() ? -1 : (int64_t)t._version()}; }
-void unchanged(const c10::IValue &then, const Tensor &now, const char *what, const char *name) {
-  const auto was = then.toIntVector();
-  TORCH_CHECK(was[1] < 0 || now.is_inference() || was[0] != (int64_t)(uintptr_t)now.const_data_ptr() || was[1] == (int64_t)now._version(), what, ": ", name,
-              " modified by an inplace operation between the forward pass and its recomputation");
-}
+struct Stamp {
+  int64_t at, version;
+  explicit Stamp(const Tensor &t) : Stamp((int64_t)(uintptr_t)t.const_data_ptr(), t.is_inference() ? -1 : (int64_t)t._version()) {}
+  Stamp(int64_t at, int64_t version) : at(at), version(version) {}
+  void unchanged(const Tensor &now, const char *what, const char *name) const {
+    TORCH_CHECK(version < 0 || now.is_inference() || at != (int64_t)(uintptr_t)now.const_data_ptr() || version == (int64_t)now._version(), what, ": ", name,
+                " modified by an inplace operation between the forward pass and its recomputation");
+  }
+};
 // A leaf's gradient is accumulated on the stream that its node was made on, and the node lives as long as a graph that holds it.  One
 // made on the default stream cannot take part in a capture: the captured backward pass would end the process.
 void refuse_captured(std::initializer_list<const Tensor *> inputs, const char *what) {
@@ -1219,7 +1222,10 @@ struct Norm : torch::autograd::Function<Norm> {
     ctx->saved_data["b"] = bt.defined() ? (int64_t)bt.scalar_type() : (int64_t)0;
     ctx->saved_data["site"] = site;
     ctx->saved_data["threshold"] = threshold;
-    if (n.defined()) ctx->saved_data["numbers"] = stamp(n);
+    if (n.defined()) {
+      const Stamp s(n);
+      ctx->saved_data["numbers"] = std::vector<int64_t>{s.at, s.version};
+    }
     variable_list all;
     if (r.defined()) all.push_back(out.h);
     all.push_back(out.y);
@@ -1241,7 +1247,10 @@ struct Norm : torch::autograd::Function<Norm> {
     const bool need_x = ctx->needs_input_grad(at++), need_r = added && ctx->needs_input_grad(at++);
     const bool need_w = has_w && ctx->needs_input_grad(at++), need_b = has_b && ctx->needs_input_grad(at++);
     const Dropped drop{saved[3], ctx->saved_data["site"].toInt(), ctx->saved_data["threshold"].toInt()};
-    if (saved[3].defined()) unchanged(ctx->saved_data["numbers"], saved[3], what, kNumbers);
+    if (saved[3].defined()) {
+      const auto then = ctx->saved_data["numbers"].toIntVector();
+      Stamp(then[0], then[1]).unchanged(saved[3], what, kNumbers);
+    }
     Tensor gx, gres, gw, gb;
     auto all = [&](std::initializer_list<bool> varies) {
       return once({gx, gres, gw, gb, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, varies, what);
@@ -1341,6 +1350,12 @@ PyObject *norm_fwd(PyObject *, PyObject *const *args, Py_ssize_t n) {
 }
 
 struct Dropout : torch::autograd::Function<Dropout> {
+  struct Kept : torch::CustomClassHolder {   // of the forward pass: one entry of the context, where every one costs the host
+    int64_t site, threshold;
+    bool added;
+    Stamp numbers;
+    Kept(int64_t site, int64_t threshold, bool added, const Tensor &n) : site(site), threshold(threshold), added(added), numbers(n) {}
+  };
   static Tensor pass(const Tensor &x, const Tensor &res, const Tensor &numbers, int64_t site, int64_t threshold) {
     const Tensor y = at::empty(x.sizes(), x.options());
     check(lib.l8_dropout(x.const_data_ptr(), caddr(res), y.mutable_data_ptr(), x.numel(), numbers.const_data_ptr<int64_t>(), site, threshold, stream_of(x.get_device())), "l8_dropout");
@@ -1348,24 +1363,22 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
   static Tensor forward(AutogradContext *ctx, const Tensor &x, const std::optional<Tensor> &res, const Tensor &numbers, int64_t site, int64_t threshold) {
     ctx->save_for_backward({numbers});
-    ctx->saved_data["site"] = site;
-    ctx->saved_data["threshold"] = threshold;
-    ctx->saved_data["added"] = res.has_value();
-    ctx->saved_data["numbers"] = stamp(numbers);
+    ctx->saved_data["kept"] = c10::IValue::make_capsule(c10::make_intrusive<Kept>(site, threshold, res.has_value(), numbers));
     return pass(x, res.value_or(Tensor()), numbers, site, threshold);
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const Tensor &g = grads[0];
     TORCH_CHECK(g.scalar_type() == at::kBFloat16, "dropout backward: bf16 gradients required, got ", g.scalar_type());
-    const Tensor kept = ctx->get_saved_variables()[0], numbers = kept.contiguous();
-    const bool added = ctx->saved_data["added"].toBool();
-    unchanged(ctx->saved_data["numbers"], kept, added ? "dropout_add" : "dropout", kNumbers);
+    const auto held = ctx->saved_data["kept"].toCapsule();
+    const Kept &kept = static_cast<const Kept &>(*held);
+    const Tensor saved = ctx->get_saved_variables()[0], numbers = saved.contiguous();
+    kept.numbers.unchanged(saved, kept.added ? "dropout_add" : "dropout", kNumbers);
     Tensor gx;
     if (ctx->needs_input_grad(0)) {
       const c10::DeviceGuard guard(g.device());
-      gx = once({pass(g.contiguous(), Tensor(), numbers, ctx->saved_data["site"].toInt(), ctx->saved_data["threshold"].toInt())}, {learns(g)}, "dropout")[0];
+      gx = once({pass(g.contiguous(), Tensor(), numbers, kept.site, kept.threshold)}, {learns(g)}, "dropout")[0];
     }
-    return {gx, added && ctx->needs_input_grad(1) ? g : Tensor(), Tensor(), Tensor(), Tensor()};
+    return {gx, kept.added && ctx->needs_input_grad(1) ? g : Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -1431,19 +1444,19 @@ struct LowRank : torch::autograd::Function<LowRank> {
     lowrank_out(rows_of(y), h, s, fb, order, starts, out, stream);
     ctx->save_for_backward({learn_a ? x : Tensor(), learn_x ? a : Tensor(), learn_x || learn_a ? b : Tensor(), learn_b ? h : Tensor(), s, order, starts});
     ctx->saved_data["like"] = x.sizes().vec();
-    ctx->saved_data["bank"] = std::vector<int64_t>{fa.n, fa.r, fa.cols, fb.cols};
+    const Stamp stamp(order);
+    ctx->saved_data["bank"] = std::vector<int64_t>{fa.n, fa.r, fa.cols, fb.cols, stamp.at, stamp.version};
     ctx->saved_data["learns"] = (int64_t)(learn_x | (learn_a << 1) | (learn_b << 2));
-    ctx->saved_data["order"] = stamp(order);
     return out;
   }
   static variable_list backward(AutogradContext *ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    unchanged(ctx->saved_data["order"], saved[5], kName, "the order of the tokens was");
+    const auto sizes = ctx->saved_data["bank"].toIntVector();
+    Stamp(sizes[4], sizes[5]).unchanged(saved[5], kName, "the order of the tokens was");
     const Tensor gy = gradient(grads[0], kName);
     const int device = gy.get_device();
     const c10::DeviceGuard guard(gy.device());
     void *stream = stream_of(device);
-    const auto sizes = ctx->saved_data["bank"].toIntVector();
     const int64_t n = sizes[0], r = sizes[1], K = sizes[2], N = sizes[3], learnt = ctx->saved_data["learns"].toInt();
     const bool need_y = ctx->needs_input_grad(0), need_x = ctx->needs_input_grad(1) && saved[1].defined(), need_a = ctx->needs_input_grad(2) && saved[0].defined(),
                need_b = ctx->needs_input_grad(3) && saved[3].defined();
@@ -1511,7 +1524,7 @@ PyObject *add_lowrank(PyObject *, PyObject *const *args, Py_ssize_t n) {
   Bank fa, fb;
   if (!as_rows(x, device, rx) || !as_rows(y, device, ry) || !on_16_bytes(rx) || !on_16_bytes(ry) || rx.rows != ry.rows || !as_bank(a, device, fa) || !as_bank(b, device, fb) ||
       fa.n != fb.n || fa.r != fb.r || fa.cols != rx.cols || fb.cols != ry.cols || x.dim() != y.dim() || x.sizes().slice(0, x.dim() - 1) != y.sizes().slice(0, y.dim() - 1) ||
-      (scale.defined() && (scale.dim() != 1 || !dense(scale, at::kFloat, fa.n, device))) || c10::hip::current_device() != device)
+      (scale.defined() && (scale.dim() != 1 || !dense(scale, at::kFloat, fa.n, device) || (scale.requires_grad() && at::GradMode::is_enabled()))) || c10::hip::current_device() != device)
     Py_RETURN_NONE;
   const int64_t T = rx.rows;
   const bool planned = order.defined();

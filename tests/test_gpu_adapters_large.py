@@ -106,3 +106,15 @@ def test_generation_with_an_adapter_a_token(T, n, host):
     index[5] = -1
     for r in (8, 64):
         against_64_bits(T, n, r, 520, 264, index, False, seed=T)
+
+
+def test_a_scale_that_asks_for_a_gradient_is_refused(host):
+    from lingua_amd import adapters
+    x, a, b = normal(40, 64), normal(2, 8, 64), normal(2, 8, 64)
+    index, scale = torch.zeros(40, dtype=torch.int32, device="cuda"), torch.ones(2, device="cuda", requires_grad=True)
+    for i in (index, adapters.route(index, 2)):
+        for leaf in (x, x.clone().requires_grad_()):
+            with pytest.raises(RuntimeError, match="scale asks for a gradient"):
+                adapters.add_lowrank(leaf, leaf, a, b, i, scale)
+            with torch.no_grad():
+                assert torch.equal(adapters.add_lowrank(leaf, leaf, a, b, i, scale), adapters.add_lowrank(leaf, leaf, a, b, i))
