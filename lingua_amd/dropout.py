@@ -128,8 +128,8 @@ class Dropout(torch.nn.Module):
                 self._version = f8._stamp(self.numbers)
         elif self._several:
             raise RuntimeError("Dropout: called several times in a forward pass, of which one is computed again: use a module for each call")
-        else:
-            f8._unchanged(self._version, self.numbers, "Dropout", "the seed and step were")
+        elif self._version not in (None, f8._stamp(self.numbers)):   # (others in their place as well)
+            raise RuntimeError("Dropout: the seed and step were modified by an inplace operation between the forward pass and its recomputation, or exchanged")
         if call and (self.site >= _SITES or call >= _CALLS):
             raise RuntimeError(f"Dropout: call {call} of site {self.site} in one forward pass; sites below 2^20 have 4096")
         return Drop(self.p, self.numbers, self.site + call * _SITES)

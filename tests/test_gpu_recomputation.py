@@ -144,6 +144,10 @@ def test_modules_of_dropout(reentrant, host):
     n[1] += 1
     with pytest.raises(RuntimeError, match="modified by an inplace operation between the forward pass and its recomputation"):
         y.backward(g)
+    y = model(x, reentrant)
+    model.drop.numbers = n.clone()
+    with pytest.raises(RuntimeError, match="exchanged"):
+        y.backward(g)
     model = dropout.convert_dropouts(Twice(True), n)
     y = model(x, reentrant)
     model.eval()
