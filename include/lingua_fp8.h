@@ -355,7 +355,7 @@ int l8_dropout(const void *x, const void *residual, void *y, int64_t n, const in
  *   q, scale        as l8_cast_rowwise of y; both NULL: no cast.  col_amax fp32 [C] or NULL, with a workspace of l8_rmsnorm_workspace bytes
  *   mean, rstd      fp32 [R], kept for the backward pass; either may be NULL
  * Without `centred` residual, numbers and w are needed and b is NULL (l8_rmsnorm_cast_rowwise and l8_add_rmsnorm_cast_rowwise are the others).
- * Requires C % 8 == 0, C <= 8192, bf16 operands on 16-byte lines. */
+ * Requires C % 8 == 0, C <= 8192, bf16 operands on 16-byte lines; h, y and q overlap nothing (x and residual may be one tensor). */
 typedef struct {
   const void *x, *residual, *w, *b;
   int64_t w_is_f32, b_is_f32, centred, R, C, ldx, ldr;
@@ -376,7 +376,7 @@ typedef struct {
 int l8_norm_fwd(const l8_norm_fwd_args *args);
 /* Its backward pass: gx, the gradient of h (gh, the gradient that arrives at h itself, may be NULL) and with it of x and residual; with
  * numbers gres is the gradient of h and gx = dropout(gres before rounding).  gw, gb (bf16 or fp32 [C], either may be NULL) are sums over the
- * rows in a fixed order; with either a workspace of l8_norm_bwd_workspace bytes. */
+ * rows in a fixed order; with either a workspace of l8_norm_bwd_workspace bytes.  gx and gres overlap nothing. */
 typedef struct {
   const void *gy, *gh, *h, *w;
   int64_t w_is_f32, centred, R, C, ldgy, ldgh, ldh;

@@ -18,10 +18,9 @@ int drop_of(const char *who, const int64_t *numbers, int64_t site, int64_t thres
   return L8_OK;
 }
 
-// LINES: the pointers are on 16-byte lines; else every element goes by itself.
+// LINES: the pointers are on 16-byte lines; else every element goes by itself.  (y may be x or residual: an element is read before it is written.)
 template <bool ADD, bool LINES>
-__global__ __launch_bounds__(kDropBlock) void dropout_kernel(const uint16_t *__restrict__ x, const uint16_t *__restrict__ residual, uint16_t *__restrict__ y,
-                                                             int64_t n, const Drop drop) {
+__global__ __launch_bounds__(kDropBlock) void dropout_kernel(const uint16_t *x, const uint16_t *residual, uint16_t *y, int64_t n, const Drop drop) {
   const int64_t group = (int64_t)blockIdx.x * kDropBlock + threadIdx.x, at = group * 8;
   if (at >= n) return;
   uint32_t words[4];

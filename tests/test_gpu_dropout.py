@@ -217,3 +217,21 @@ def test_replayed_steps_drop_other_elements():
         want = (h, y, *torch.autograd.grad((h, y), (x2, res2, w2), (g, g)))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert not torch.equal(seen[0][0], seen[1][0])
+
+
+@pytest.mark.parametrize("count", [4096, 1001])
+@pytest.mark.parametrize("off", [0, 1])
+def test_in_place(count, off):
+    """The library's entry with the output over either operand."""
+    from lingua_amd import _lib, dropout
+    n, lib, stream = numbers(), _lib.load(), torch.cuda.current_stream().cuda_stream
+    x, res = (seeded_bf16((count + off,), seed=i).cuda()[off:] for i in range(2))
+    drop = dropout.Drop(0.3, n, 7)
+    for residual, into in ((None, "x"), (res, "x"), (res, "residual")):
+        want = dropout.dropout(x, drop) if residual is None else dropout.dropout_add(x, residual, drop)
+        ops = {"x": x, "residual": residual}
+        room = torch.full((count + off + 8,), 7.0, dtype=torch.bfloat16, device="cuda")
+        y = room[off:off + count].copy_(ops[into])
+        ops[into] = y
+        assert lib.l8_dropout(ops["x"].data_ptr(), None if residual is None else ops["residual"].data_ptr(), y.data_ptr(), count, n.data_ptr(), 7, round(65536 * 0.3), stream) == 0
+        assert torch.equal(y, want) and bool((room[off + count:] == 7).all())
