@@ -570,7 +570,7 @@ L8_DEV int64_t outer_part(int first, int size, int piece) { return 2 * (int64_t)
 // tokens (32 with more than 16 ranks) the waves' sums are added up.  Up to 32 ranks, whose registers leave room for that.
 // A tile's columns are neighbouring workgroups, so that its rows are read as whole lines of memory at one time: [16384,8192] 72 us, the tiles being
 // neighbours 94; the gradients alone do better with neighbouring tiles (both sides of [16384,4096] to [16384,4096] a whole pass of 127 and 134).
-// us: [16384,4096] of rank 16 33 (134 MB, 4.1 TB/s), of rank 64 two such sides 90 (3.0; and 67 MB of sums of tiles, written and read); with
+// us: [16384,4096] of rank 16 36 (134 MB, 3.7 TB/s), of rank 64 two such sides 90 (3.0; and 67 MB of sums of tiles, written and read); with
 // ALSO_H [16384,11008] 97 (361 MB, 3.7 TB/s) where both by themselves take 177.
 template <int RT, int TOKENS, bool ALSO_H>
 __global__ __launch_bounds__(kOuterWaves * 64, 2) void lowrank_outer_kernel(const OuterArgs p) {
