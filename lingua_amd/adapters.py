@@ -137,11 +137,12 @@ class Requests:
     The order of the tokens is written to the same memory for every batch of one shape, so that a captured forward pass that is replayed
     after a ``set`` sees it.  That memory is kept for the shapes that a capture asked for and the last 64 others."""
 
+    _read = None   # what the last forward pass went by: a plan and its version
+
     def __init__(self, n: int):
         self.n, self._plan = n, None
         self._plans = {}        # of each shape of tokens, the latest last
         self._captured = set()  # those that a graph goes on reading
-        self._read = None       # what the last forward pass went by: a plan and its version
 
     @property
     def plan(self) -> Optional[Plan]:

@@ -108,10 +108,11 @@ class Dropout(torch.nn.Module):
     activation checkpointing computes again has to call the module once: of several calls nothing says which one is repeated, an error; and
     ``numbers`` that changed since the last forward pass are one too."""
 
+    _pass, _calls, _several, _version = None, 0, False, None   # (here, so that a module that was pickled without them has them)
+
     def __init__(self, p: float, numbers: torch.Tensor, site: int = 0):
         super().__init__()
         self.p, self.numbers, self.site = p, numbers, site
-        self._pass, self._calls, self._several, self._version = None, 0, False, None
 
     def drop(self):
         """What a fused sum takes: the ``Drop`` of this module in training, else None."""

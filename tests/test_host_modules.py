@@ -143,3 +143,12 @@ def test_a_fused_feed_forward_at_several_places_is_refused():
         with pytest.raises(RuntimeError, match="fused feed-forward"):
             adapters.add_adapters(model, adapters.Requests(2), 8, match)
     assert type(fused.w2) is torch.nn.Linear
+
+
+def test_modules_that_were_pickled_before_their_calls_were_counted():
+    model = dropout.convert_dropouts(Twice(), dropout.numbers(1, "cpu"))
+    requests = adapters.Requests(2)
+    for thing in (model.drop, requests):
+        for name in ("_pass", "_calls", "_several", "_version", "_read"):
+            thing.__dict__.pop(name, None)
+    assert model.drop.drop().site == 0 and requests.plan is None
